@@ -45,6 +45,7 @@ struct MergeArgs {
   float* lse;
   int lse_base2;
   int num_q_heads, head_dim;
+  int keep_nan;  // a row whose sum is NaN stays NaN (else it counts as a row that sees nothing)
 };
 
 // Validate a rotation description and turn it into its device form.
@@ -61,6 +62,16 @@ inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<unsigned 
   if (e == hipSuccess) devices.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
+
+// Checks a launch against its plan's header `h` and fills the argument blocks of the attention and the merge kernels.
+int plan_arguments(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, const void* v_pool_dev,
+                   int64_t pool_row_stride, const int32_t* plan_dev, const int32_t* h, const int32_t* kv_indices_dev,
+                   const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride, void* out_dev,
+                   float* lse_dev, int32_t lse_base2, void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
+                   const VaRope* rope, AttnArgs* attn, MergeArgs* merge);
+
+// The merge of partial states (viewattn.hip); `waves`: the plan header's word.
+int launch_merge_typed(const MergeArgs& m, int dtype, int n_rows, int waves, hipStream_t stream);
 
 // Matrix-core attention (launched from va_mfma.hip).
 // `n_wide` leading items are wide tiles (va_mfma_wide.hip: `n_wide_slots` workgroups per kv head, each

@@ -465,6 +465,7 @@ __global__ __launch_bounds__(kGenThreads) void attn_generic_kernel(AttnArgs a) {
 // was waited for together with the requests of the states before it: a round was a chain of a trip per state.)  16
 // heads of 256 dims, 4 rows 6.2 -> 4.6 us, 333 rows 10.4 -> 8.7, 633 rows of 8 heads of 128 dims 7.8 -> 6.0; 8 rows of
 // 32 heads and sixteen waves 4.6 either way.
+__device__ __forceinline__ bool sees_any(const MergeArgs& a, float sum) { return sum > 0.f || (a.keep_nan && sum != sum); }
 using PlanTable = const __attribute__((address_space(4))) int32_t*;  // read only while a launch runs
 template <typename E, int kMergeWaves>
 __device__ __forceinline__ void merge_row_head(const MergeArgs& a, long long row, int hq, int begin, int end) {
@@ -540,10 +541,10 @@ __device__ __forceinline__ void merge_row_head(const MergeArgs& a, long long row
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int d = lane + 64 * k;
-    if (d < a.head_dim) o[d] = E::store(ll > 0.f ? av[k] / ll : 0.f);
+    if (d < a.head_dim) o[d] = E::store(sees_any(a, ll) ? av[k] / ll : 0.f);
   }
   if (lane == 0 && a.lse) {
-    const float lse2 = ll > 0.f ? mm + log2f(ll) : -INFINITY;
+    const float lse2 = sees_any(a, ll) ? mm + log2f(ll) : -INFINITY;
     a.lse[row * a.num_q_heads + hq] = a.lse_base2 ? lse2 : lse2 * kLn2;
   }
 }
@@ -679,7 +680,7 @@ __global__ __launch_bounds__(256, 4) void merge_rows_kernel(MergeArgs a, int n_r
 #pragma unroll
     for (int k = 0; k < kRuns; ++k) {
       if (base + 1024 * k >= width) continue;
-      const bool any = l[k] > 0.f;
+      const bool any = sees_any(a, l[k]);
       S y[4] = {E::store(any ? v[k].x / l[k] : 0.f), E::store(any ? v[k].y / l[k] : 0.f),
                 E::store(any ? v[k].z / l[k] : 0.f), E::store(any ? v[k].w / l[k] : 0.f)};
       if constexpr (sizeof(S) == 2) {
@@ -807,20 +808,20 @@ extern "C" int va_store_kv_rope(const void* k_dev, const void* v_dev, int64_t k_
   return rc;
 }
 
-// Both attention entry points: `workspace_dev` is the caller's buffer (va_attention) or this
-// device's copy of the library's own scratch array (va_attention_static).
-static int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev,
-                              const void* v_pool_dev, int64_t pool_row_stride, const int32_t* plan_dev,
-                              const int32_t* plan_header_host, const int32_t* kv_indices_dev,
-                              const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
-                              int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2,
-                              void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
-                              const VaRope* rope, void* stream) {
-  if (!shape || !plan_header_host || !plan_dev) return va_fail(VA_ERR_ARG, "null plan or shape");
-  const int32_t* h = plan_header_host;
-  if (h[VA_H_MAGIC] != VA_PLAN_MAGIC) return va_fail(VA_ERR_ARG, "plan header has no magic word");
-  const int n_rows = h[VA_H_N_ROWS], n_items = h[VA_H_N_ITEMS], n_partials = h[VA_H_N_PARTIALS];
-  if (n_rows == 0) return VA_OK;
+namespace va {
+
+int launch_merge_typed(const MergeArgs& m, int dtype, int n_rows, int waves, hipStream_t stream) {
+  int rc = VA_OK;
+  VA_DISPATCH_DTYPE(dtype, rc = launch_merge<E>(m, n_rows, waves, stream));
+  return rc;
+}
+
+int plan_arguments(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, const void* v_pool_dev,
+                   int64_t pool_row_stride, const int32_t* plan_dev, const int32_t* h, const int32_t* kv_indices_dev,
+                   const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride, void* out_dev,
+                   float* lse_dev, int32_t lse_base2, void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
+                   const VaRope* rope, AttnArgs* attn, MergeArgs* merge) {
+  const int n_items = h[VA_H_N_ITEMS], n_partials = h[VA_H_N_PARTIALS];
   // the kernels map workgroup -> (item, head) assuming each launch covers a multiple of 8 items
   if (n_items % 8 || h[VA_H_N_WIDE] % 8 || h[VA_H_N_WIDE] < 0 || h[VA_H_N_WIDE] > n_items)
     return va_fail(VA_ERR_ARG, "plan header: item counts (%d, %d wide) are not padded to the 8 dies", n_items,
@@ -835,17 +836,18 @@ static int attention_launches(const void* q_dev, int64_t q_row_stride, const voi
   const int64_t need = va_workspace_bytes_for(n_partials, shape->num_q_heads, shape->head_dim);
   if (need > 0 && (!workspace_dev || workspace_bytes < need))
     return va_fail(VA_ERR_CAPACITY, "workspace needs %lld bytes, got %lld", (long long)need, (long long)workspace_bytes);
-  va::RopeDev r;
-  int rc = va::make_rope(rope, shape->head_dim, &r);
+  RopeDev r;
+  const int rc = make_rope(rope, shape->head_dim, &r);
   if (rc) return rc;
 
-  va::AttnArgs a;
+  AttnArgs& a = *attn;
   a.q = q_dev;
   a.q_row_stride = q_row_stride;
   a.k_pool = k_pool_dev;
   a.v_pool = v_pool_dev;
   a.pool_row_stride = pool_row_stride;
   a.items = plan_dev + h[VA_H_OFF_ITEMS];
+  a.narrow_items = a.items + (long long)h[VA_H_N_WIDE] * VA_ITEM_WORDS;
   a.links = plan_dev + h[VA_H_OFF_LINKS];
   a.qrefs = plan_dev + h[VA_H_OFF_QREFS];
   a.qref_rows = plan_dev + h[VA_H_OFF_QREF_ROWS];
@@ -864,7 +866,45 @@ static int attention_launches(const void* q_dev, int64_t q_row_stride, const voi
   a.head_dim = shape->head_dim;
   a.page_size = shape->page_size;
   a.rope = r;
-  a.scale_log2 = va::kLog2e / sqrtf((float)shape->head_dim);
+  a.scale_log2 = kLog2e / sqrtf((float)shape->head_dim);
+
+  MergeArgs& m = *merge;
+  m.row_indptr = plan_dev + h[VA_H_OFF_ROW_INDPTR];
+  m.row_ids = plan_dev + h[VA_H_OFF_ROW_IDS];
+  m.row_flags = plan_dev + h[VA_H_OFF_ROW_FLAGS];
+  m.part_acc = a.part_acc;
+  m.part_ml = a.part_ml;
+  m.out = out_dev;
+  m.lse = lse_dev;
+  m.lse_base2 = lse_base2;
+  m.num_q_heads = shape->num_q_heads;
+  m.head_dim = shape->head_dim;
+  m.keep_nan = 0;
+  return VA_OK;
+}
+
+}  // namespace va
+
+// Both attention entry points: `workspace_dev` is the caller's buffer (va_attention) or this
+// device's copy of the library's own scratch array (va_attention_static).
+static int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev,
+                              const void* v_pool_dev, int64_t pool_row_stride, const int32_t* plan_dev,
+                              const int32_t* plan_header_host, const int32_t* kv_indices_dev,
+                              const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
+                              int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2,
+                              void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
+                              const VaRope* rope, void* stream) {
+  if (!shape || !plan_header_host || !plan_dev) return va_fail(VA_ERR_ARG, "null plan or shape");
+  const int32_t* h = plan_header_host;
+  if (h[VA_H_MAGIC] != VA_PLAN_MAGIC) return va_fail(VA_ERR_ARG, "plan header has no magic word");
+  const int n_rows = h[VA_H_N_ROWS], n_items = h[VA_H_N_ITEMS];
+  if (n_rows == 0) return VA_OK;
+  va::AttnArgs a;
+  va::MergeArgs m;
+  int rc = va::plan_arguments(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, h, kv_indices_dev,
+                              sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev, lse_base2,
+                              workspace_dev, workspace_bytes, shape, rope, &a, &m);
+  if (rc) return rc;
   hipStream_t s = (hipStream_t)stream;
 
   if (n_items > 0) {
@@ -877,20 +917,8 @@ static int attention_launches(const void* q_dev, int64_t q_row_stride, const voi
     }
     if (rc) return rc;
   }
-  if (n_partials > 0 || h[VA_H_N_EMPTY_ROWS] > 0) {
-    va::MergeArgs m;
-    m.row_indptr = plan_dev + h[VA_H_OFF_ROW_INDPTR];
-    m.row_ids = plan_dev + h[VA_H_OFF_ROW_IDS];
-    m.row_flags = plan_dev + h[VA_H_OFF_ROW_FLAGS];
-    m.part_acc = a.part_acc;
-    m.part_ml = a.part_ml;
-    m.out = out_dev;
-    m.lse = lse_dev;
-    m.lse_base2 = lse_base2;
-    m.num_q_heads = shape->num_q_heads;
-    m.head_dim = shape->head_dim;
-    VA_DISPATCH_DTYPE(shape->dtype, rc = va::launch_merge<E>(m, n_rows, h[VA_H_MERGE_WAVES], s));
-  }
+  if (h[VA_H_N_PARTIALS] > 0 || h[VA_H_N_EMPTY_ROWS] > 0)
+    rc = va::launch_merge_typed(m, shape->dtype, n_rows, h[VA_H_MERGE_WAVES], s);
   return rc;
 }
 

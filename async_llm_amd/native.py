@@ -23,10 +23,12 @@ VA_SUB_CAUSAL, VA_SUB_SLOTS = 1, 2
 PLAN_HEADER_WORDS = 24
 PLAN_FLAGS_WORD = 3  # of a header: the chunk, with flags in its low bits
 PLAN_SHORT_ITEMS = 1  # narrow items are short: several workgroups share a CU
+VA_CODE_E4M3, VA_CODE_INT8 = 0, 1
 VA_ERR_ARG, VA_ERR_CAPACITY = -1, -2
 STATIC_SCRATCH_BYTES = 32 << 20  # VA_STATIC_SCRATCH_BYTES: the array va_attention_static keeps on every GPU
 
 _DTYPES = {torch.float32: VA_F32, torch.float16: VA_F16, torch.bfloat16: VA_BF16}
+_CODES = {torch.float8_e4m3fn: VA_CODE_E4M3, torch.int8: VA_CODE_INT8}
 
 EXPORTED_SYMBOLS = (
     "va_last_error",
@@ -42,6 +44,10 @@ EXPORTED_SYMBOLS = (
     "va_plan_build_fixed",
     "va_attention",
     "va_attention_static",
+    "va_store_kv_rope_q8",
+    "va_load_kv_q8",
+    "va_copy_shift_kv_q8",
+    "va_attention_q8",
 )
 
 
@@ -64,6 +70,17 @@ class VaRope(C.Structure):
         ("section_h", C.c_int32),
         ("section_w", C.c_int32),
         ("inv_freq_dev", C.c_void_p),
+    ]
+
+
+class VaQuantPool(C.Structure):
+    _fields_ = [
+        ("k_codes_dev", C.c_void_p),
+        ("v_codes_dev", C.c_void_p),
+        ("k_scales_dev", C.c_void_p),
+        ("v_scales_dev", C.c_void_p),
+        ("code_type", C.c_int32),
+        ("num_pages", C.c_int32),
     ]
 
 
@@ -167,6 +184,17 @@ def _load() -> C.CDLL:
     lib.va_attention_static.restype = C.c_int
     lib.va_attention_static.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, i64, vp, vp, i32,
                                         C.POINTER(VaShape), C.POINTER(VaRope), vp]
+    pool = C.POINTER(VaQuantPool)
+    lib.va_store_kv_rope_q8.restype = C.c_int
+    lib.va_store_kv_rope_q8.argtypes = [vp, vp, i64, i64, pool, vp, i32, vp, i64, i64, C.POINTER(VaShape),
+                                        C.POINTER(VaRope), vp]
+    lib.va_load_kv_q8.restype = C.c_int
+    lib.va_load_kv_q8.argtypes = [pool, vp, i64, vp, vp, i64, C.POINTER(VaShape), vp]
+    lib.va_copy_shift_kv_q8.restype = C.c_int
+    lib.va_copy_shift_kv_q8.argtypes = [pool, i64, i64, i32, vp, vp, i64, i64, C.POINTER(VaShape), C.POINTER(VaRope), vp]
+    lib.va_attention_q8.restype = C.c_int
+    lib.va_attention_q8.argtypes = [vp, i64, pool, vp, vp, vp, vp, vp, i64, vp, vp, i32, vp, i64,
+                                    C.POINTER(VaShape), C.POINTER(VaRope), vp]
     return lib
 
 
@@ -189,6 +217,13 @@ def dtype_id(dtype: torch.dtype) -> int:
         raise ViewAttnError(f"unsupported element type {dtype}") from None
 
 
+def code_id(dtype: torch.dtype) -> int:
+    try:
+        return _CODES[dtype]
+    except KeyError:
+        raise ViewAttnError(f"unsupported code type {dtype} (torch.float8_e4m3fn or torch.int8)") from None
+
+
 def require_device(t: torch.Tensor, name: str) -> None:
     if t.device.type != "cuda":
         raise ViewAttnError(
@@ -206,6 +241,16 @@ def current_stream_ptr(device: torch.device) -> int:
         return torch.cuda.current_stream(device).cuda_stream
     index = device.index
     return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+def call_on(device: torch.device, function, *args) -> None:
+    """Call a launching function of the library with ``device`` current (a launch belongs to the current device,
+    whatever stream it names) and check its result."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        check(function(*args))
+        return
+    with torch.cuda.device(device):
+        check(function(*args))
 
 
 def make_shape(hq: int, hkv: int, d: int, page: int, dtype: torch.dtype) -> VaShape:

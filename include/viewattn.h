@@ -336,6 +336,88 @@ VA_API int va_attention_static(const void* q_dev, int64_t q_row_stride, const vo
                         int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2,
                         const VaShape* shape, const VaRope* rope, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The same path over a pool of 8-bit codes.  It has no counterpart in the
+ * reference.  A row (one token of one kv head, K or V) is stored as head_dim
+ * codes and one scale: element = code * 2^(scale - 127), where the scale byte is
+ * the exponent of a power of two (255: the row reads back as NaN).  Quantising
+ * a row x takes the smallest power of two for which max|x| <= largest code *
+ * 2^e (448 for e4m3, 127 for int8; scale bytes below 1 become 1) and rounds
+ * x / 2^e to the nearest code, ties to even (magnitudes over 1.875 * 2^127 for e4m3,
+ * 127 * 2^121 for int8, whose codes would stand for 2^128, count as those).  A row that holds a NaN or an
+ * infinity gets scale 255 and codes of zero.  As the scale is a power of two,
+ * reading a row back is exact in any element type whose range holds it, and
+ * quantising what was read back gives the same values.
+ *
+ * Layout of a layer: codes [num_pages, num_kv_heads, page_size, head_dim],
+ * scales [num_pages, num_kv_heads, page_size], one byte each, contiguous: the
+ * rows that one kv head reads of a page are one run.  head_dim is 16, 32, 64,
+ * 128 or 256; code arrays start on 16-byte boundaries.  Token slot s lies in
+ * page s / page_size at s % page_size.  shape->dtype is the type of the
+ * activations (k, v, q, out), not of the pool.
+ * ------------------------------------------------------------------------- */
+#define VA_CODE_E4M3 0 /* OCP float8 e4m3 (no infinities, largest 448) */
+#define VA_CODE_INT8 1 /* -127 .. 127 */
+
+typedef struct VaQuantPool {
+  void* k_codes_dev;      /* of one layer (the first one, for va_copy_shift_kv_q8) */
+  void* v_codes_dev;
+  uint8_t* k_scales_dev;
+  uint8_t* v_scales_dev;
+  int32_t code_type;      /* VA_CODE_* */
+  int32_t num_pages;
+} VaQuantPool;
+
+/*
+ * va_store_kv_rope_q8: for every row i whose slot out_loc[i] lies in the pool
+ *   k[out_loc[i]] <- quantise(R(pos[i]) k[i])   and   v[out_loc[i]] <- quantise(v[i])
+ * (other rows are skipped, negative slots among them).  The rotation is taken in
+ * fp32 and not rounded before it is quantised.  Slots must be distinct.  Any
+ * alignment and row stride of k and v (16-byte aligned rows and rotary_dim a
+ * multiple of 16 are fast).
+ */
+VA_API int va_store_kv_rope_q8(const void* k_dev, const void* v_dev, int64_t k_row_stride, int64_t v_row_stride,
+                        const VaQuantPool* pool, const void* out_loc_dev, int32_t out_loc_is_i64,
+                        const int64_t* pos_dev, int64_t pos_axis_stride, int64_t n_rows,
+                        const VaShape* shape, const VaRope* rope, void* stream);
+
+/*
+ * va_load_kv_q8: out_k[i] = k[slots[i]], out_v[i] = v[slots[i]] in shape->dtype,
+ * rounded to nearest even where the type has fewer bits; rows are
+ * num_kv_heads * head_dim elements, out_row_stride elements apart.  Slots outside
+ * the pool (negative ones) give rows of zeros.  Either output may be NULL.
+ */
+VA_API int va_load_kv_q8(const VaQuantPool* pool, const int64_t* slots_dev, int64_t n_rows, void* out_k_dev,
+                  void* out_v_dev, int64_t out_row_stride, const VaShape* shape, void* stream);
+
+/*
+ * va_copy_shift_kv_q8: va_copy_shift_kv over a quantised pool.  For every layer
+ * and token i
+ *   k[dst[i]] <- quantise(R(position_shift) k[src[i]])   and   v[dst[i]] <- v[src[i]],
+ * code for code where nothing rotates.  Layer l's arrays start l * code_layer_stride
+ * (scale_layer_stride) bytes after the pool's.  Tokens with a slot outside the
+ * pool are skipped.  Destination slots must be distinct, and disjoint from the
+ * source slots or equal to them row by row.
+ */
+VA_API int va_copy_shift_kv_q8(const VaQuantPool* pool, int64_t code_layer_stride, int64_t scale_layer_stride,
+                        int32_t num_layers, const int64_t* src_slots_dev, const int64_t* dst_slots_dev,
+                        int64_t n_tokens, int64_t position_shift, const VaShape* shape, const VaRope* rope,
+                        void* stream);
+
+/*
+ * va_attention_q8: va_attention over a quantised pool, with the plans of
+ * va_plan_build* for the same shape and params->wide_tile < 0 (no wide items).
+ * kv_indices of VA_SUB_SLOTS sub-requests are token slots of the pool.  Queries
+ * are rotated in fp32 and enter the products unrounded (vector-ALU kernel) or as
+ * sums of two bf16 numbers (matrix-core kernel: error 2^-17 of each element), and
+ * so do the weights of the second product.
+ */
+VA_API int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
+                    const int32_t* plan_header_host, const int32_t* kv_indices_dev,
+                    const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
+                    void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
+                    int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
