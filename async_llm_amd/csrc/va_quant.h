@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include "va_device.h"
+#include "va_mfma_common.h"
 
 namespace va {
 
@@ -27,6 +28,13 @@ struct E4M3 {
     const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     out[0] = lo[0], out[1] = lo[1], out[2] = hi[0], out[3] = hi[1];
   }
+  // Eight codes as bf16, exactly (four instructions, each at the full rate).
+  static __device__ __forceinline__ va_u32x4 bf16x8(va_u32x2 w) {
+    return va_u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.f, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.f, true)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.f, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.f, true))};
+  }
 };
 struct INT8 {
   static constexpr int kId = VA_CODE_INT8;
@@ -40,6 +48,11 @@ struct INT8 {
   static __device__ __forceinline__ void unpack4(uint32_t w, float* out) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = (float)(int8_t)(w >> (8 * i));
+  }
+  static __device__ __forceinline__ va_u32x4 bf16x8(va_u32x2 w) {  // (bf16 has the eight bits of a code)
+    float x[8];
+    unpack4(w[0], x), unpack4(w[1], x + 4);
+    return va_u32x4{Mma<BF16>::pack(x[0], x[1]), Mma<BF16>::pack(x[2], x[3]), Mma<BF16>::pack(x[4], x[5]), Mma<BF16>::pack(x[6], x[7])};
   }
 };
 
@@ -79,6 +92,36 @@ __device__ __forceinline__ long long quant_row(const PageMap& p, uint32_t slot, 
   uint32_t page, place;
   p.split(slot, page, place);
   return ((long long)page * num_kv_heads + head) * p.size + place;
+}
+
+// Eight cosines and sines of pairs [i0, i0 + 8) at position p.
+__device__ __forceinline__ void turns8(const RopeDev& rope, const Pos3& p, int i0, float* c, float* s) {
+  if (rope.mode == VA_ROPE_TABLE) {
+    long long a = p.t < 0 ? -p.t : p.t;
+    if (a > rope.max_pos - 1) a = rope.max_pos - 1;
+    const float* row = rope.cos_sin + a * (long long)rope.rotary_dim + i0;
+    const float4 c0 = *(const float4*)row, c1 = *(const float4*)(row + 4);
+    const float4 s0 = *(const float4*)(row + rope.half), s1 = *(const float4*)(row + rope.half + 4);
+    c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+    s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+    if (p.t < 0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k] = -s[k];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) rope_cos_sin(rope, p, i0 + k, c[k], s[k]);
+  }
+}
+
+// Pairs (a, b) rotated in place in fp32, every product and sum rounded by itself (the definition's arithmetic).
+__device__ __forceinline__ void turn8(const float* c, const float* s, float* a, float* b) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float x1 = a[k], x2 = b[k];
+    a[k] = mul_rounded(c[k], x1) - mul_rounded(s[k], x2);
+    b[k] = mul_rounded(c[k], x2) + mul_rounded(s[k], x1);
+  }
 }
 
 // Host: refuses a pool that the kernels cannot address.

@@ -46,4 +46,7 @@ __device__ __forceinline__ long long quant_token_row(const QuantAttnArgs& qa, in
   return ((long long)qa.a.kv_indices[kv_begin + (int)page] * qa.a.num_kv_heads + hk) * qa.pages.size + place;
 }
 
+// The matrix-core kernel (va_quant_stream.hip): narrow items of 16-bit activations, head_dim 64, 128 or 256.
+int launch_quant_stream(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream);
+
 }  // namespace va

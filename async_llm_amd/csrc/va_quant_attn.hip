@@ -235,8 +235,11 @@ extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const Va
   hipStream_t s = (hipStream_t)stream;
   const int n_items = h[VA_H_N_ITEMS];
   if (n_items > 0) {
-    rc = pool->code_type == VA_CODE_E4M3 ? va::launch_quant_any<va::E4M3>(qa, shape->dtype, n_items, s)
-                                         : va::launch_quant_any<va::INT8>(qa, shape->dtype, n_items, s);
+    if (h[VA_H_KERNEL] == VA_KERNEL_MFMA)
+      rc = va::launch_quant_stream(qa, shape->dtype, pool->code_type, n_items, h[VA_H_Q_TILE], s);
+    else
+      rc = pool->code_type == VA_CODE_E4M3 ? va::launch_quant_any<va::E4M3>(qa, shape->dtype, n_items, s)
+                                           : va::launch_quant_any<va::INT8>(qa, shape->dtype, n_items, s);
     if (rc) return rc;
   }
   if (h[VA_H_N_PARTIALS] > 0 || h[VA_H_N_EMPTY_ROWS] > 0)

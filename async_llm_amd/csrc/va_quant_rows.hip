@@ -54,36 +54,6 @@ __device__ __forceinline__ void load8(const typename E::storage* p, float* x) {
   for (int i = 0; i < 8; ++i) x[i] = E::load(u.e[i]);
 }
 
-// Eight cosines and sines of pairs [i0, i0 + 8) at position p.
-__device__ __forceinline__ void turns8(const RopeDev& rope, const Pos3& p, int i0, float* c, float* s) {
-  if (rope.mode == VA_ROPE_TABLE) {
-    long long a = p.t < 0 ? -p.t : p.t;
-    if (a > rope.max_pos - 1) a = rope.max_pos - 1;
-    const float* row = rope.cos_sin + a * (long long)rope.rotary_dim + i0;
-    const float4 c0 = *(const float4*)row, c1 = *(const float4*)(row + 4);
-    const float4 s0 = *(const float4*)(row + rope.half), s1 = *(const float4*)(row + rope.half + 4);
-    c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
-    s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
-    if (p.t < 0) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] = -s[k];
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) rope_cos_sin(rope, p, i0 + k, c[k], s[k]);
-  }
-}
-
-// Pairs (a, b) rotated in place in fp32, every product and sum rounded by itself (the definition's arithmetic).
-__device__ __forceinline__ void turn8(const float* c, const float* s, float* a, float* b) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float x1 = a[k], x2 = b[k];
-    a[k] = mul_rounded(c[k], x1) - mul_rounded(s[k], x2);
-    b[k] = mul_rounded(c[k], x2) + mul_rounded(s[k], x1);
-  }
-}
-
 __device__ __forceinline__ uint32_t top8(const float* x) {
   uint32_t top = 0;
 #pragma unroll
