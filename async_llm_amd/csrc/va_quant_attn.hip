@@ -236,7 +236,7 @@ extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const Va
   const int n_items = h[VA_H_N_ITEMS];
   if (n_items > 0) {
     if (h[VA_H_KERNEL] == VA_KERNEL_MFMA)
-      rc = va::launch_quant_stream(qa, shape->dtype, pool->code_type, n_items, h[VA_H_Q_TILE], s);
+      rc = va::launch_quant_mfma(qa, shape->dtype, pool->code_type, n_items, h[VA_H_Q_TILE], s);
     else
       rc = pool->code_type == VA_CODE_E4M3 ? va::launch_quant_any<va::E4M3>(qa, shape->dtype, n_items, s)
                                            : va::launch_quant_any<va::INT8>(qa, shape->dtype, n_items, s);

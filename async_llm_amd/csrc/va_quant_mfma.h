@@ -1,0 +1,185 @@
+// Matrix-core pieces of view attention over a quantised pool, shared by the kernels for whole and for scattered tiles.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "va_mfma_common.h"
+#include "va_quant.h"
+#include "va_quant_attn.h"
+
+namespace va {
+
+constexpr int kQuantThreads = 256;
+constexpr int kQuantWaves = 4;
+constexpr int kQuantTokens = 32;  // tokens per tile
+
+__device__ __forceinline__ va_u32x2 lds_read_tr8(uint32_t lds_byte_address) {
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  // Within 16 lanes, lane s supplies the address of eight bytes; lane i receives byte i of every 16: byte i % 8 of what
+  // lanes i / 8, i / 8 + 2, ... pointed at.
+  const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)lds_byte_address);
+  return __builtin_bit_cast(va_u32x2, r);
+}
+
+// x as the sum of two bf16 numbers, pairs packed.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = Mma<BF16>::pack(a, b);
+  lo = Mma<BF16>::pack(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+
+__device__ __forceinline__ float quant_group_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Eight activations from `at` on as fp32; `pieces`: rows lie on 16-byte boundaries.
+__device__ __forceinline__ void activations8(const void* x, long long at, int dtype, bool pieces, float* y) {
+  if (pieces) {
+    const va_u32x4 w = *(const va_u32x4*)((const uint16_t*)x + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t a = (uint16_t)w[i], b = (uint16_t)(w[i] >> 16);
+      y[2 * i] = dtype == VA_BF16 ? BF16::load(a) : __half2float(__builtin_bit_cast(__half, a));
+      y[2 * i + 1] = dtype == VA_BF16 ? BF16::load(b) : __half2float(__builtin_bit_cast(__half, b));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = activation(x, at + i, dtype);
+  }
+}
+
+// Wait until at most n of the wave's vector memory operations are outstanding.
+template <int n>
+__device__ __forceinline__ void wave_wait_loads() {
+  static_assert(n < kAnyInFlight, "the counter holds no more");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
+}
+
+// The query rows of a tile for a link, rotated in fp32 and split into two bf16 numbers, in LDS: sixteen rows of high parts,
+// then of low parts, piece c of row r at position c ^ (r & 7).
+template <int kD>
+__device__ __forceinline__ void stage_query(const AttnArgs& a, int n_q, int lflags, int qref, int hk, int dtype, bool pieces,
+                                            char* query) {
+  const int G = a.num_q_heads / a.num_kv_heads;
+  for (int idx = threadIdx.x; idx < 16 * (kD / 16); idx += kQuantThreads) {
+    const int r = idx / (kD / 16), x = idx - r * (kD / 16), iq = r / G, g = r - iq * G;
+    const int pairs = a.rope.rotary_dim / 16;
+    const int d0 = x < pairs ? 8 * x : 16 * x, d1 = x < pairs ? 8 * x + a.rope.half : 16 * x + 8;
+    float y0[8], y1[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y0[e] = y1[e] = 0.f;
+    if (iq < n_q) {
+      const bool indirect = lflags & VA_LINK_INDIRECT;
+      const int subrow = indirect ? a.qrefs[qref + iq] : qref + iq;
+      const long long src = indirect ? (long long)a.qref_rows[qref + iq] : a.sub_worker[subrow];
+      const long long at = src * a.q_row_stride + (long long)(hk * G + g) * kD;
+      activations8(a.q, at + d0, dtype, pieces, y0);
+      activations8(a.q, at + d1, dtype, pieces, y1);
+      if (x < pairs) {
+        float c[8], s[8];
+        turns8(a.rope, load_pos(a.sub_loc, a.sub_loc_axis_stride, subrow), d0, c, s);
+        turn8(c, s, y0, y1);
+      }
+    }
+    va_u32x4 h0, l0, h1, l1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t hi, lo;
+      split_pair(y0[2 * e], y0[2 * e + 1], hi, lo);
+      h0[e] = hi, l0[e] = lo;
+      split_pair(y1[2 * e], y1[2 * e + 1], hi, lo);
+      h1[e] = hi, l1[e] = lo;
+    }
+    char* q_row = query + r * (2 * kD);
+    const int c0 = 16 * ((d0 / 8) ^ (r & 7)), c1 = 16 * ((d1 / 8) ^ (r & 7));
+    *(va_u32x4*)(q_row + c0) = h0;
+    *(va_u32x4*)(q_row + c1) = h1;
+    *(va_u32x4*)(q_row + 32 * kD + c0) = l0;
+    *(va_u32x4*)(q_row + 32 * kD + c1) = l1;
+  }
+}
+// B operands of K.Q^T: step 2 s + b holds dims [64 s + 16 kg + 8 b, + 8) of row j; part 0 the high, 1 the low ones.
+template <int kD>
+__device__ __forceinline__ va_u32x4 staged_query(const char* query, int step, int part) {
+  const int j = threadIdx.x % 16, kg = (threadIdx.x % kWave) / 16;
+  return *(const va_u32x4*)(query + j * (2 * kD) + 16 * ((8 * (step / 2) + 2 * kg + step % 2) ^ (j & 7)) + part * 32 * kD);
+}
+
+// The state of a tile at the end: four waves', folded through LDS, then the result or the partial state.  o[t][r] is dim
+// 16 t + 4 kg + r of row j, l_run a sum spread over the four contraction groups.
+template <int kD>
+struct QuantFold {
+  static constexpr int kRowBytes = kD * 4 + 16;  // (padded, so that the sixteen rows of a write spread over the banks)
+  static constexpr int kBytes = 16 * (kRowBytes + 8);
+};
+template <int kD>
+__device__ __forceinline__ void fold_and_finish(const AttnArgs& a, const va_f32x4 (&o)[kD / 16], float m_run, float l_run, char* lds,
+                                                int n_q, int part_base, int qref0, int flags0, int hk, int dtype, bool pieces) {
+  using F = QuantFold<kD>;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, j = lane % 16, kg = lane / 16;
+  const int G = a.num_q_heads / a.num_kv_heads;
+  l_run += __shfl_xor(l_run, 16, kWave);
+  l_run += __shfl_xor(l_run, 32, kWave);
+  {
+    char* state = lds + wave * F::kBytes;
+#pragma unroll
+    for (int t = 0; t < kD / 16; ++t) *(va_f32x4*)(state + j * F::kRowBytes + 16 * kg + 64 * t) = o[t];
+    if (kg == 0) *(float2*)(state + 16 * F::kRowBytes + 8 * j) = make_float2(m_run, l_run);
+  }
+  __syncthreads();
+  const int r = tid / 16, seg = tid % 16, iq = r / G;
+  if (iq >= n_q) return;
+  float weight[kQuantWaves], m = kNegBig, l = 0.f;
+  float2 ml[kQuantWaves];
+#pragma unroll
+  for (int w = 0; w < kQuantWaves; ++w) {
+    ml[w] = *(const float2*)(lds + w * F::kBytes + 16 * F::kRowBytes + 8 * r);
+    m = fmaxf(m, ml[w].x);
+  }
+#pragma unroll
+  for (int w = 0; w < kQuantWaves; ++w) {
+    weight[w] = __builtin_amdgcn_exp2f(ml[w].x - m);
+    l += ml[w].y * weight[w];
+  }
+  const int hq = hk * G + r - iq * G;
+  va_f32x4 sum[kD / 64];
+#pragma unroll
+  for (int x = 0; x < kD / 64; ++x) {
+    sum[x] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kQuantWaves; ++w)
+      sum[x] += *(const va_f32x4*)(lds + w * F::kBytes + r * F::kRowBytes + 16 * (seg + 16 * x)) * weight[w];
+  }
+  if (part_base < 0) {
+    const long long out_row = (flags0 & VA_LINK_INDIRECT) ? (long long)a.qref_rows[qref0 + iq] : a.sub_worker[qref0 + iq];
+    const long long at = (out_row * a.num_q_heads + hq) * (long long)kD;
+#pragma unroll
+    for (int x = 0; x < kD / 64; ++x) {
+      const int d = 4 * (seg + 16 * x);
+      float y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[k] = normalised(sum[x][k], l);
+      if (pieces) {
+        const bool bf = dtype == VA_BF16;
+        *(uint2*)((uint16_t*)a.out + at + d) = make_uint2(bf ? Mma<BF16>::pack(y[0], y[1]) : Mma<F16>::pack(y[0], y[1]),
+                                                          bf ? Mma<BF16>::pack(y[2], y[3]) : Mma<F16>::pack(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store_activation(a.out, at + d + k, y[k], dtype);
+      }
+    }
+    if (seg == 0 && a.lse) a.lse[out_row * a.num_q_heads + hq] = log_sum(m, l, a.lse_base2);
+  } else {
+    const long long slot = (long long)(part_base + iq) * a.num_q_heads + hq;
+    float* prow = a.part_acc + slot * kD;
+#pragma unroll
+    for (int x = 0; x < kD / 64; ++x) *(va_f32x4*)(prow + 4 * (seg + 16 * x)) = sum[x];
+    if (seg == 0) {
+      a.part_ml[slot * 2 + 0] = m;
+      a.part_ml[slot * 2 + 1] = l;
+    }
+  }
+}
+
+}  // namespace va

@@ -1,8 +1,7 @@
 // Matrix-core view attention over a quantised pool: query tiles of up to 16 MFMA rows (decode tiles of 16 / G requests that
 // read the same tokens, and prefill tiles of 16 / G new tokens), row = tile row R / G, head R % G.
 //
-//   S^T[32 tokens, 16 rows] = K . Q^T      v_mfma_f32_16x16x32_bf16; the codes of K as the A operand, converted to bf16
-//                                          (exact) in the registers they were loaded to
+//   S^T[32 tokens, 16 rows] = K . Q^T      v_mfma_f32_16x16x32_bf16, the codes of K as the A operand, converted to bf16 (exact)
 //   p = exp2(S * 2^e_k * scale - max),     w = p * 2^e_v
 //   O^T[D, 16 rows] += V^T . W^T           the same product; V^T from transposing LDS reads of the codes
 //
@@ -11,11 +10,12 @@
 // float16 result would lose three bits).  The range of bf16 is why no scale has to be normalised: w is whatever p * 2^e_v is.
 // The matrix pipe has the time, the kernel is bound by HBM.
 //
-// Four independent waves a workgroup, each takes every fourth 32-token tile of the walk with loads of its own: no barrier in
-// the tile loop.  K goes from memory straight to the registers that feed the products: lane (j, kg) of a 16-token half
-// takes bytes [64 s + 16 kg, + 16) of token j, which are the contraction elements of steps 2 s and 2 s + 1 when the query is
-// laid out by the same order.  V passes through LDS (eight tokens of a dim in one ds_read_b64_tr_b8).  Both are requested a
-// tile ahead, V while the tile before is taken apart, K behind its last product; page entries two tiles ahead.
+// Four independent waves a workgroup, each takes every fourth 32-token tile of the walk and brings it global -> LDS
+// (global_load_lds) into a ring of its own: no barrier in the tile loop.  A tile is two halves of sixteen tokens, each one run
+// of 16 * D bytes of a page, for K and for V: whole lines, requested non-temporally where no other tile reads them (6.8 TB/s for
+// loads alone; as half lines straight to registers, which the products of K would take, 5.7).  A tile goes from LDS to
+// registers at once and its buffer is requested anew before the first product.  Two items that walk the same tokens (the
+// tiles of one run's many readers) share a workgroup, which converts each code once for both.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -25,377 +25,365 @@
 #include "va_mfma_common.h"
 #include "va_quant.h"
 #include "va_quant_attn.h"
+#include "va_quant_mfma.h"
 
 namespace va {
 
-constexpr int kQuantThreads = 256;
-constexpr int kQuantWaves = 4;
-constexpr int kQuantTokens = 32;  // tokens per tile
-
 template <int kD>
-struct QuantShape {
-  static constexpr int kPieces = kD / 64;    // 16-byte pieces of a token's row that a lane takes
-  static constexpr int kSteps = kD / 32;     // contraction steps of K.Q^T
-  static constexpr int kDimTiles = kD / 16;  // 16-dim tiles of the output
-  static constexpr int kTileBytes = kQuantTokens * kD;         // V of a tile
-  static constexpr int kWaveBytes = kTileBytes + 2 * kQuantTokens * 4;  // and its scales, K then V
-  static constexpr int kQueryBytes = 2 * 16 * kD * 2;          // hi and lo rows
-  static constexpr int kLoopBytes = kQuantWaves * kWaveBytes + kQueryBytes;
-  // The waves' states at the end: accumulators (rows padded by 16 bytes), maxima and sums.
-  static constexpr int kFoldRowBytes = kD * 4 + 16;
-  static constexpr int kFoldBytes = 16 * (kFoldRowBytes + 8);
-  static constexpr int kLdsBytes = kLoopBytes > kQuantWaves * kFoldBytes ? kLoopBytes : kQuantWaves * kFoldBytes;
+struct QuantRing {
+  static constexpr int kPieces = kD / 64;       // 16-byte pieces of a token's row that a lane takes
+  static constexpr int kSteps = kD / 32;        // contraction steps of K.Q^T
+  static constexpr int kDimTiles = kD / 16;     // 16-dim tiles of the output
+  static constexpr int kHalfBytes = 16 * kD;    // sixteen tokens of K (or V)
+  static constexpr int kLoads = kHalfBytes / 1024;      // wave-level loads of a half
+  static constexpr int kTileBytes = 4 * kHalfBytes;     // K, then V
+  static constexpr int kScaleBytes = 64 * 4;            // a word per scale: 32 keys', 32 values'
+  static constexpr int kBuffers = kD == 64 ? 4 : 2;     // ring depth of a wave, in tiles
+  static constexpr int kScaleSlots = 2 * kBuffers;      // scales stay in LDS while their tile is in registers
+  static constexpr int kMinBlocks = kD == 256 ? 1 : 2;  // workgroups per CU
+  static constexpr int kScaleOffset = kBuffers * kTileBytes;
+  static constexpr int kWaveBytes = kScaleOffset + kScaleSlots * kScaleBytes;
+  static constexpr int kQueryOffset = kQuantWaves * kWaveBytes;
+  static constexpr int kQueryBytes = 2 * 16 * kD * 2;  // of one tile: staged one after the other
+  static constexpr int kLdsBytes = kQueryOffset + kQueryBytes;
+  static_assert(kQuantWaves * QuantFold<kD>::kBytes <= kLdsBytes, "room for the waves' states");
+  static_assert(kMinBlocks * kLdsBytes <= 160 * 1024, "the LDS of a CU");
+  static constexpr int kLoadsPerTile = 4 * kLoads + 1;  // what the counter of outstanding loads sees of a tile
 };
 
-// Piece c of token t of a V tile lies at position c ^ quant_swz(t): the sixteen tokens that a write covers spread over the
-// banks, and so do the eight that a transposing read takes of one piece.
+// Piece c of token t of a tile lies at position c ^ ring_swz(t).  Sixteen tokens' pieces c (a fragment of K), and the piece
+// that a transposing read takes of tokens 4 k .. + 3 and 16 + 4 k .. + 3 (V), then lie in different banks.
 template <int kD>
-__device__ __forceinline__ int quant_swz(int t) {
-  if constexpr (kD == 256) return (t & 3) | (((t >> 4) & 1) << 2) | (((t >> 2) & 1) << 3);
-  if constexpr (kD == 128) return ((t >> 1) & 3) | (((t >> 4) & 1) << 2);
+__device__ __forceinline__ int ring_swz(int t) {
+  if constexpr (kD == 256) return (t & 15) ^ (((t >> 4) & 1) << 2);
+  if constexpr (kD == 128) return ((t >> 1) & 7) ^ (((t >> 4) & 1) << 1);
   return ((t >> 2) & 3) ^ ((t >> 4) & 1);
 }
 
-__device__ __forceinline__ va_u32x2 lds_read_tr8(uint32_t lds_byte_address) {
-  typedef int v2i __attribute__((ext_vector_type(2)));
-  // Within 16 lanes, lane s supplies the address of eight bytes; lane i receives byte i of every 16: byte i % 8 of what
-  // lanes i / 8, i / 8 + 2, ... pointed at.
-  const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)lds_byte_address);
-  return __builtin_bit_cast(va_u32x2, r);
+// One wave-level load of 1 KB with a cache policy (load_to_lds has none).
+template <bool kOnce>
+__device__ __forceinline__ void load_run_to_lds(const void* base, uint32_t lane_offset, uint32_t lds_base) {
+  uint32_t saved;
+#define VA_ONE_LOAD(policy)                                                                                              \
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" policy "\n\ts_mov_b32 m0, %0" \
+               : "=&s"(saved)                                                                                            \
+               : "v"(lane_offset), "s"(base), "s"(lds_base)                                                              \
+               : "memory")
+  if constexpr (kOnce) VA_ONE_LOAD(" nt"); else VA_ONE_LOAD("");
+#undef VA_ONE_LOAD
+}
+// A byte per lane, each a word in LDS: lane l's lands at lds_base + 4 l.
+__device__ __forceinline__ void load_bytes_to_lds(unsigned long long at, uint32_t lds_base) {
+  uint32_t saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved)
+               : "v"(at), "s"(lds_base)
+               : "memory");
 }
 
-// x as the sum of two bf16 numbers, pairs packed.
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = Mma<BF16>::pack(a, b);
-  lo = Mma<BF16>::pack(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
-}
-
-__device__ __forceinline__ float quant_group_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-// Eight activations from `at` on as fp32; `pieces`: rows lie on 16-byte boundaries.
-__device__ __forceinline__ void activations8(const void* x, long long at, int dtype, bool pieces, float* y) {
-  if (pieces) {
-    const va_u32x4 w = *(const va_u32x4*)((const uint16_t*)x + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint16_t a = (uint16_t)w[i], b = (uint16_t)(w[i] >> 16);
-      y[2 * i] = dtype == VA_BF16 ? BF16::load(a) : __half2float(__builtin_bit_cast(__half, a));
-      y[2 * i + 1] = dtype == VA_BF16 ? BF16::load(b) : __half2float(__builtin_bit_cast(__half, b));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = activation(x, at + i, dtype);
-  }
-}
-
-template <int kD, typename C>
-__global__ __launch_bounds__(kQuantThreads, kD == 256 ? 1 : 2) void attn_quant_stream_kernel(QuantAttnArgs qa, int dtype, int pieces) {
+// kB items that walk the same tokens, for one kv head.
+template <int kD, typename C, int kB>
+__device__ __forceinline__ void quant_stream_items(const QuantAttnArgs& qa, const int (&item)[kB], int hk, int dtype, bool pieces) {
   const AttnArgs& a = qa.a;
-  using Sh = QuantShape<kD>;
-  constexpr int kPieces = Sh::kPieces, kSteps = Sh::kSteps, kDimTiles = Sh::kDimTiles;
+  using Sh = QuantRing<kD>;
+  using Words = const __attribute__((address_space(4))) int32_t*;
+  constexpr int kPieces = Sh::kPieces, kSteps = Sh::kSteps, kDimTiles = Sh::kDimTiles, kLoads = Sh::kLoads, kBuffers = Sh::kBuffers;
 
   extern __shared__ va_u32x4 smem[];
   char* lds = (char*)smem;
 
-  const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
-  using Words = const __attribute__((address_space(4))) int32_t*;
-  const Words item = (Words)a.items + (long long)where.item * VA_ITEM_WORDS;
-  const int n_q = item[VA_I_N_Q], n_links = item[VA_I_N_LINKS], part_base = item[VA_I_PART_BASE];
-  if (n_q == 0) return;  // padding item: keeps the launch order aligned with the die round-robin
-  const int hk = where.head, G = a.num_q_heads / a.num_kv_heads;
-  const int tid = threadIdx.x, lane = tid % kWave;
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int j = lane % 16, kg = lane / 16;  // MFMA row (token of a half tile, query row), contraction group
+  Words words[kB];
+  int n_q[kB];
+#pragma unroll
+  for (int b = 0; b < kB; ++b) {
+    words[b] = (Words)a.items + (long long)item[b] * VA_ITEM_WORDS;
+    n_q[b] = words[b][VA_I_N_Q];
+  }
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int j = lane % 16, kg = lane / 16;  // MFMA row (token of a half, query row), contraction group
   const int row_iq = j / G;
   const uint8_t* kp = (const uint8_t*)a.k_pool;
   const uint8_t* vp = (const uint8_t*)a.v_pool;
+  const int P = a.page_size, p_shift = qa.pages.shift;
 
-  char* mine = lds + wave * Sh::kWaveBytes;
-  float* scales = (float*)(mine + Sh::kTileBytes);  // [2][32]: K, V
-  char* query = lds + kQuantWaves * Sh::kWaveBytes;
-  // where this lane's pieces of V go, and where it reads them transposed
-  int v_write[2][kPieces];
+  // This lane's part of wave-level load u of a half: row and piece, the piece that belongs at its LDS position; the
+  // halves' swizzles differ by a bit of the position.  Loads of a group share one setting of M0, whose immediate offsets move
+  // the pool address as well (grouped_lane_offset; the base gives the bias back).
+  constexpr int kRowPieces = kD / 16;
+  constexpr int kBias = 1024 * (kLoads - 1);
+  auto ld_row = [&](int u) __attribute__((always_inline)) { return u * (64 / kRowPieces) + lane / kRowPieces; };
+  auto ld_piece = [&](int u, int half) __attribute__((always_inline)) {
+    return (lane % kRowPieces) ^ ring_swz<kD>(16 * half + ld_row(u));
+  };
+  uint32_t ld_off[2][kLoads];
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int s = 0; s < kPieces; ++s) v_write[u][s] = (16 * u + j) * kD + 16 * ((4 * s + kg) ^ quant_swz<kD>(16 * u + j));
+    for (int u = 0; u < kLoads; ++u)
+      ld_off[h][u] = grouped_lane_offset((uint32_t)(ld_row(u) * kD + 16 * ld_piece(u, h) + kBias), u);
+  // What it reads of a tile.  K: pieces 4 s + kg of token j of each half.  V: piece t of eight tokens, transposed.
+  int k_at[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) k_at[h] = 16 * (kg ^ ring_swz<kD>(16 * h + j));
   const int v_token = (j / 2 < 4 ? 0 : 12) + 4 * kg + j / 2;  // tokens 4 kg .. + 3, then 16 + 4 kg .. + 3
-  const uint32_t v_read = lds_address(mine) + v_token * kD + 8 * (j % 2);
-  const int v_swz = quant_swz<kD>(v_token);
+  const int v_at = 2 * Sh::kHalfBytes + v_token * kD + 8 * (j % 2), v_swz = 16 * ring_swz<kD>(v_token);
+  const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_address(lds)) + (uint32_t)wave * Sh::kWaveBytes;
+  char* query = lds + Sh::kQueryOffset;
 
-  float m_run = kNegBig, l_run = 0.f;  // running maximum (log2 units) and sum, of this wave's tokens
-  va_f32x4 o[kDimTiles];
+  float m_run[kB], l_run[kB];  // running maximum (log2 units) and sum, of this wave's tokens
+  va_f32x4 o[kB][kDimTiles];
 #pragma unroll
-  for (int t = 0; t < kDimTiles; ++t) o[t] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int b = 0; b < kB; ++b) {
+    m_run[b] = kNegBig;
+    l_run[b] = 0.f;
+#pragma unroll
+    for (int t = 0; t < kDimTiles; ++t) o[b][t] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 
+  const int n_links = words[0][VA_I_N_LINKS];
   for (int li = 0; li < n_links; ++li) {
-    const Words link = li == 0 ? item + VA_I_LINK0 : (Words)a.links + (long long)(item[VA_I_LINK_BEGIN] + li) * VA_LINK_WORDS;
+    const Words link = li == 0 ? words[0] + VA_I_LINK0 : (Words)a.links + (long long)(words[0][VA_I_LINK_BEGIN] + li) * VA_LINK_WORDS;
     const int lflags = link[VA_L_FLAGS], kv_begin = link[VA_L_KV_BEGIN], tok_begin = link[VA_L_TOK_BEGIN];
-    const int tok_end = link[VA_L_TOK_END], causal_base = link[VA_L_CAUSAL_BASE], qref = link[VA_L_QREF];
+    const int tok_end = link[VA_L_TOK_END], causal_base = link[VA_L_CAUSAL_BASE];
     const bool slots = lflags & VA_LINK_SLOTS;
-    const int t_stop = min(tok_end, causal_base + n_q);      // tokens any row of the tile sees
-    const int t_row = min(tok_end, causal_base + row_iq + 1);  // tokens this lane's row sees
+    const bool read_once = lflags & VA_LINK_ONCE;  // no other tile reads these rows: lines to evict first
+    const bool whole = !slots && tok_begin % 16 == 0;  // halves lie inside a page
+    const int t_stop = min(tok_end, causal_base + n_q[0]);   // tokens any row of the tile sees
+    const int t_row = min(tok_end, causal_base + row_iq + 1);  // tokens this lane's row sees (partners are not causal)
     const int t_last = t_stop - 1;
     const int n_all = t_stop > tok_begin ? (t_stop - tok_begin + kQuantTokens - 1) / kQuantTokens : 0;
     const int n_tiles = n_all > wave ? (n_all - wave + kQuantWaves - 1) / kQuantWaves : 0;  // this wave's
     auto first_token = [&](int i) __attribute__((always_inline)) { return tok_begin + (i * kQuantWaves + wave) * kQuantTokens; };
-
-    // Tokens of a half tile, past the visible range the last visible one (masked): its entry of the index, then its row.
-    auto token_of = [&](int i, int u) __attribute__((always_inline)) { return min(first_token(i) + 16 * u + j, t_last); };
-    int entry[2];
-    auto read_entries = [&](int i) __attribute__((always_inline)) {
+    auto page_entry = [&](int t) __attribute__((always_inline)) {  // (a scalar load: a vector one would be waited for with all others)
+      return ((Words)a.kv_indices)[kv_begin + t];
+    };
+    // pages of tile i, read a tile ahead of its request
+    auto read_pages = [&](int i, int (&page)[2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t t = (uint32_t)token_of(i, u);
-        uint32_t page = t, place;
-        if (!slots) qa.pages.split(t, page, place);
-        entry[u] = a.kv_indices[kv_begin + (int)page];
+      for (int h = 0; h < 2; ++h) page[h] = page_entry(min(first_token(i) + 16 * h, t_last) >> p_shift);
+    };
+    // Request tile i into buffer i % kBuffers.  Rows past the visible range repeat the last visible token (masked).
+    auto request_half = [&](const uint8_t* pool, long long base, const uint32_t* off, uint32_t dst, auto once) __attribute__((always_inline)) {
+      const void* from = pool + (base - kBias);
+      if constexpr (kLoads == 1) {
+        load_run_to_lds<decltype(once)::value>(from, off[0], dst);
+      } else {
+        load_group_to_lds<kLoads, decltype(once)::value>(from, off, dst);
       }
     };
-    long long row[2];
-    auto rows_of = [&](int i) __attribute__((always_inline)) {
+    auto request = [&](int i, const int (&page)[2]) __attribute__((always_inline)) {
+      const uint32_t dst = ring + (uint32_t)(i % kBuffers) * Sh::kTileBytes;
+      const uint32_t scales = ring + Sh::kScaleOffset + (uint32_t)(i % Sh::kScaleSlots) * Sh::kScaleBytes;
+      const int t0 = first_token(i);
+      long long row[2];  // of a half's first token
+      if (whole) {
+        uint32_t off[2][kLoads];
+        const bool full = t0 + kQuantTokens - 1 <= t_last;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t page = (uint32_t)entry[u], place;
-        if (slots) {
-          qa.pages.split((uint32_t)entry[u], page, place);
+        for (int h = 0; h < 2; ++h) {
+          const int t = min(t0 + 16 * h, t_last);
+          row[h] = ((long long)page[h] * a.num_kv_heads + hk) * P + (t & (P - 1));
+          const int most = max(0, t_last - (t0 + 16 * h));  // last row of the half that is visible
+#pragma unroll
+          for (int u = 0; u < kLoads; ++u)
+            off[h][u] = full ? ld_off[h][u] : ld_off[h][u] - (uint32_t)(max(0, ld_row(u) - most) * kD);
+        }
+        auto both = [&](auto once) __attribute__((always_inline)) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) request_half(kp, row[h] * kD, off[h], dst + h * Sh::kHalfBytes, once);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) request_half(vp, row[h] * kD, off[h], dst + (2 + h) * Sh::kHalfBytes, once);
+        };
+        if (read_once && full) {
+          both(std::true_type{});
         } else {
-          uint32_t ahead;
-          qa.pages.split((uint32_t)token_of(i, u), ahead, place);
+          both(std::false_type{});
         }
-        row[u] = ((long long)page * a.num_kv_heads + hk) * qa.pages.size + place;
+        const int h = kg & 1, place = min(j, max(0, t_last - (t0 + 16 * h)));
+        const unsigned long long scale = (unsigned long long)(lane < 32 ? qa.k_scales : qa.v_scales) + (h ? row[1] : row[0]) + place;
+        load_bytes_to_lds(scale, scales);
+      } else {  // every lane looks its tokens up, in vector loads
+        auto row_of = [&](int t) __attribute__((always_inline)) { return quant_token_row(qa, kv_begin, min(t, t_last), slots, hk); };
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int u = 0; u < kLoads; ++u) {
+            const long long at = row_of(t0 + 16 * h + ld_row(u)) * kD + 16 * ld_piece(u, h);
+            load_to_lds(kp + at, dst + h * Sh::kHalfBytes + 1024 * u);
+            load_to_lds(vp + at, dst + (2 + h) * Sh::kHalfBytes + 1024 * u);
+          }
+        load_bytes_to_lds((unsigned long long)(lane < 32 ? qa.k_scales : qa.v_scales) + row_of(t0 + lane % 32), scales);
       }
     };
-    va_u32x4 kraw[2][kPieces], vraw[2][kPieces];
-    uint32_t scale_byte;
-    auto load_v = [&]() __attribute__((always_inline)) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int s = 0; s < kPieces; ++s) vraw[u][s] = *(const va_u32x4*)(vp + row[u] * kD + 64 * s + 16 * kg);
-      // lanes 0 .. 31 the scales of the 32 keys, the others those of the values
-      scale_byte = (lane < 32 ? qa.k_scales : qa.v_scales)[row[kg & 1]];
-    };
-    auto load_k = [&]() __attribute__((always_inline)) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int s = 0; s < kPieces; ++s) kraw[u][s] = *(const va_u32x4*)(kp + row[u] * kD + 64 * s + 16 * kg);
-    };
-    if (n_tiles > 0) {
-      read_entries(0);
-      rows_of(0);
-      read_entries(1);
-      load_v();
-      load_k();
-      rows_of(1);
-    }
 
-    // ---- the query rows, rotated in fp32 and split, in LDS: piece c of row r at position c ^ (r & 7) ----
-    if (li > 0) __syncthreads();  // every wave has read the previous link's
-    for (int idx = tid; idx < 16 * (kD / 16); idx += kQuantThreads) {
-      const int r = idx / (kD / 16), x = idx - r * (kD / 16), iq = r / G, g = r - iq * G;
-      const int pairs = a.rope.rotary_dim / 16;
-      const int d0 = x < pairs ? 8 * x : 16 * x, d1 = x < pairs ? 8 * x + a.rope.half : 16 * x + 8;
-      float y0[8], y1[8];
+    // ---- set-up: first tiles on their way, then the query tiles ----
+    // (no barrier: a wave's ring is its own, and it has read the previous link's tiles)
+    int next_page[2] = {0, 0};
+    if (n_tiles > 0) {
+      int page[kBuffers][2] = {};
+      if (whole) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y0[e] = y1[e] = 0.f;
-      if (iq < n_q) {
-        const bool indirect = lflags & VA_LINK_INDIRECT;
-        const int subrow = indirect ? a.qrefs[qref + iq] : qref + iq;
-        const long long src = indirect ? (long long)a.qref_rows[qref + iq] : a.sub_worker[subrow];
-        const long long at = src * a.q_row_stride + (long long)(hk * G + g) * kD;
-        activations8(a.q, at + d0, dtype, pieces, y0);
-        activations8(a.q, at + d1, dtype, pieces, y1);
-        if (x < pairs) {
-          float c[8], s[8];
-          turns8(a.rope, load_pos(a.sub_loc, a.sub_loc_axis_stride, subrow), d0, c, s);
-          turn8(c, s, y0, y1);
-        }
+        for (int i = 0; i < kBuffers; ++i) read_pages(i, page[i]);
+        read_pages(kBuffers, next_page);
       }
-      va_u32x4 h0, l0, h1, l1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t hi, lo;
-        split_pair(y0[2 * e], y0[2 * e + 1], hi, lo);
-        h0[e] = hi, l0[e] = lo;
-        split_pair(y1[2 * e], y1[2 * e + 1], hi, lo);
-        h1[e] = hi, l1[e] = lo;
-      }
-      char* q_row = query + r * (2 * kD);
-      const int c0 = 16 * ((d0 / 8) ^ (r & 7)), c1 = 16 * ((d1 / 8) ^ (r & 7));
-      *(va_u32x4*)(q_row + c0) = h0;
-      *(va_u32x4*)(q_row + c1) = h1;
-      *(va_u32x4*)(q_row + 32 * kD + c0) = l0;
-      *(va_u32x4*)(q_row + 32 * kD + c1) = l1;
+      for (int i = 0; i < kBuffers; ++i)
+        if (i < n_tiles) request(i, page[i]);
     }
-    __syncthreads();
-    // B operands: step 2 s + b holds dims [64 s + 16 kg + 8 b, + 8) of row j
-    va_u32x4 q_hi[kSteps], q_lo[kSteps];
+    va_u32x4 q_hi[kB][kSteps], q_lo[kB][kSteps];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const char* at = query + j * (2 * kD) + 16 * ((8 * (s / 2) + 2 * kg + s % 2) ^ (j & 7));
-      q_hi[s] = *(const va_u32x4*)at;
-      q_lo[s] = *(const va_u32x4*)(at + 32 * kD);
+    for (int b = 0; b < kB; ++b) {
+      if (li > 0 || b > 0) ring_barrier<kAnyInFlight>();  // every wave has read the query tile before
+      stage_query<kD>(a, n_q[b], lflags, b == 0 ? link[VA_L_QREF] : words[b][VA_I_LINK0 + VA_L_QREF], hk, dtype, pieces, query);
+      ring_barrier<kAnyInFlight>();
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        q_hi[b][s] = staged_query<kD>(query, s, 0);
+        q_lo[b][s] = staged_query<kD>(query, s, 1);
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q_hi[b][s]), "+v"(q_lo[b][s]));
     }
 
     // ---- the tile loop ----
     for (int i = 0; i < n_tiles; ++i) {
-      // V and the scales to LDS, and the next ones on their way
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int s = 0; s < kPieces; ++s) *(va_u32x4*)(mine + v_write[u][s]) = vraw[u][s];
-      scales[lane] = scale_value(scale_byte);
-      asm volatile("" ::: "memory");
-      if (i + 1 < n_tiles) {
-        load_v();
-        read_entries(i + 2);
+      // The tile has landed once at most the loads of the kBuffers - 1 tiles requested after it are outstanding.
+      if (i + kBuffers - 1 < n_tiles) {
+        wave_wait_loads<(kBuffers - 1) * Sh::kLoadsPerTile>();
+      } else {
+        wave_wait_loads<0>();
       }
-
-      va_f32x4 hi[2], lo[2];
+      const uint32_t buffer = (uint32_t)(i % kBuffers) * Sh::kTileBytes;
+      const char* tile = lds + wave * Sh::kWaveBytes + buffer;
+      va_u32x4 kraw[2][kPieces];
+      va_u32x2 vraw[kDimTiles];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) hi[u] = lo[u] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int s = 0; s < kPieces; ++s) kraw[h][s] = *(const va_u32x4*)(tile + h * Sh::kHalfBytes + j * kD + (k_at[h] ^ (64 * s)));
+#pragma unroll
+      for (int t = 0; t < kDimTiles; ++t) vraw[t] = lds_read_tr8(ring + buffer + v_at + ((16 * t) ^ v_swz));
+      __builtin_amdgcn_sched_barrier(0);
+      // the buffer is requested anew as soon as its tile is in registers
+      if (i + kBuffers < n_tiles) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        request(i + kBuffers, next_page);
+        if (whole) read_pages(i + 1 + kBuffers, next_page);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+
+      va_f32x4 hi[kB][2], lo[kB][2];
+#pragma unroll
+      for (int b = 0; b < kB; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) hi[b][h] = lo[b][h] = va_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const va_u32x4 raw = kraw[u][s / 2];
+        for (int h = 0; h < 2; ++h) {
+          const va_u32x4 raw = kraw[h][s / 2];
           const va_u32x4 k8 = C::bf16x8(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]});
-          hi[u] = Mma<BF16>::run(k8, q_hi[s], hi[u]);
-          lo[u] = Mma<BF16>::run(k8, q_lo[s], lo[u]);
+#pragma unroll
+          for (int b = 0; b < kB; ++b) {
+            hi[b][h] = Mma<BF16>::run(k8, q_hi[b][s], hi[b][h]);
+            lo[b][h] = Mma<BF16>::run(k8, q_lo[b][s], lo[b][h]);
+          }
         }
       }
-      if (i + 1 < n_tiles) load_k();
 
-      // online softmax; this lane holds tokens 16 u + 4 kg + r of row j
+      // online softmax; this lane holds tokens 16 h + 4 kg + r of row j
       const int t0 = first_token(i);
-      float sc[2][4], vs[2][4], most = -INFINITY;
+      const char* scales = lds + wave * Sh::kWaveBytes + Sh::kScaleOffset + (i % Sh::kScaleSlots) * Sh::kScaleBytes + 16 * kg;
+      va_u32x4 kscale[2], vscale[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const va_f32x4 ks = *(const va_f32x4*)(scales + 16 * u + 4 * kg), v4 = *(const va_f32x4*)(scales + 32 + 16 * u + 4 * kg);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool seen = t0 + 16 * u + 4 * kg + r < t_row;
-          sc[u][r] = seen ? (hi[u][r] + lo[u][r]) * (ks[r] * a.scale_log2) : -INFINITY;
-          vs[u][r] = seen ? v4[r] : 0.f;
-          most = fmaxf(most, sc[u][r]);
-        }
+      for (int h = 0; h < 2; ++h) {
+        kscale[h] = *(const va_u32x4*)(scales + 64 * h);
+        vscale[h] = *(const va_u32x4*)(scales + 128 + 64 * h);
       }
-      if (__any(most > m_run)) {
-        const float m_new = fmaxf(m_run, quant_group_max(most));
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-        m_run = m_new;
-        l_run *= alpha;
+      va_u32x4 w_hi[kB], w_lo[kB];
 #pragma unroll
-        for (int t = 0; t < kDimTiles; ++t) o[t] *= alpha;
-      }
-      va_u32x4 w_hi, w_lo;
+      for (int b = 0; b < kB; ++b) {
+        float sc[2][4], most = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float w[4];
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(sc[u][r] - m_run);
-          l_run += p;
-          w[r] = p * vs[u][r];
+          for (int r = 0; r < 4; ++r) {
+            const bool seen = t0 + 16 * h + 4 * kg + r < t_row;
+            sc[h][r] = seen ? (hi[b][h][r] + lo[b][h][r]) * (scale_value(kscale[h][r]) * a.scale_log2) : -INFINITY;
+            most = fmaxf(most, sc[h][r]);
+          }
+        if (__any(most > m_run[b])) {
+          const float m_new = fmaxf(m_run[b], quant_group_max(most));
+          const float alpha = __builtin_amdgcn_exp2f(m_run[b] - m_new);
+          m_run[b] = m_new;
+          l_run[b] *= alpha;
+#pragma unroll
+          for (int t = 0; t < kDimTiles; ++t) o[b][t] *= alpha;
         }
-        uint32_t h, l;
-        split_pair(w[0], w[1], h, l);
-        w_hi[2 * u] = h, w_lo[2 * u] = l;
-        split_pair(w[2], w[3], h, l);
-        w_hi[2 * u + 1] = h, w_lo[2 * u + 1] = l;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float w[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(sc[h][r] - m_run[b]);
+            l_run[b] += p;
+            // (a token that the row does not see may have any scale)
+            w[r] = t0 + 16 * h + 4 * kg + r < t_row ? p * scale_value(vscale[h][r]) : 0.f;
+          }
+          uint32_t x, y;
+          split_pair(w[0], w[1], x, y);
+          w_hi[b][2 * h] = x, w_lo[b][2 * h] = y;
+          split_pair(w[2], w[3], x, y);
+          w_hi[b][2 * h + 1] = x, w_lo[b][2 * h + 1] = y;
+        }
       }
 
       // O^T += V^T . W^T, the lane's contraction elements being tokens 4 kg .. + 3 and 16 + 4 kg .. + 3
 #pragma unroll
       for (int t = 0; t < kDimTiles; ++t) {
-        const va_u32x4 v8 = C::bf16x8(lds_read_tr8(v_read + 16 * (t ^ v_swz)));
-        o[t] = Mma<BF16>::run(v8, w_hi, o[t]);
-        o[t] = Mma<BF16>::run(v8, w_lo, o[t]);
+        const va_u32x4 v8 = C::bf16x8(vraw[t]);
+#pragma unroll
+        for (int b = 0; b < kB; ++b) {
+          o[b][t] = Mma<BF16>::run(v8, w_hi[b], o[b][t]);
+          o[b][t] = Mma<BF16>::run(v8, w_lo[b], o[b][t]);
+        }
       }
-      asm volatile("" ::: "memory");
-      if (i + 1 < n_tiles) rows_of(i + 2);
     }
   }
 
-  // ---- the four waves' states are folded through LDS: o[t][r] is dim 16 t + 4 kg + r of row j ----
-  l_run += __shfl_xor(l_run, 16, kWave);
-  l_run += __shfl_xor(l_run, 32, kWave);
-  __syncthreads();  // every wave is done with its tiles and the query
-  {
-    char* state = lds + wave * Sh::kFoldBytes;
 #pragma unroll
-    for (int t = 0; t < kDimTiles; ++t) *(va_f32x4*)(state + j * Sh::kFoldRowBytes + 16 * kg + 64 * t) = o[t];
-    if (kg == 0) *(float2*)(state + 16 * Sh::kFoldRowBytes + 8 * j) = make_float2(m_run, l_run);
+  for (int b = 0; b < kB; ++b) {
+    __syncthreads();  // every wave is done with its tiles and the query, or has read the block before
+    fold_and_finish<kD>(a, o[b], m_run[b], l_run[b], lds, n_q[b], words[b][VA_I_PART_BASE], words[b][VA_I_LINK0 + VA_L_QREF],
+                        words[b][VA_I_LINK0 + VA_L_FLAGS], hk, dtype, pieces);
   }
-  __syncthreads();
-  const int r = tid / 16, seg = tid % 16, iq = r / G;
-  if (iq >= n_q) return;
-  float weight[kQuantWaves], m = kNegBig, l = 0.f;
-  float2 ml[kQuantWaves];
-#pragma unroll
-  for (int w = 0; w < kQuantWaves; ++w) {
-    ml[w] = *(const float2*)(lds + w * Sh::kFoldBytes + 16 * Sh::kFoldRowBytes + 8 * r);
-    m = fmaxf(m, ml[w].x);
-  }
-#pragma unroll
-  for (int w = 0; w < kQuantWaves; ++w) {
-    weight[w] = __builtin_amdgcn_exp2f(ml[w].x - m);
-    l += ml[w].y * weight[w];
-  }
-  const int hq = hk * G + r - iq * G;
-  va_f32x4 sum[kD / 64];
-#pragma unroll
-  for (int x = 0; x < kD / 64; ++x) {
-    sum[x] = va_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kQuantWaves; ++w)
-      sum[x] += *(const va_f32x4*)(lds + w * Sh::kFoldBytes + r * Sh::kFoldRowBytes + 16 * (seg + 16 * x)) * weight[w];
-  }
-  if (part_base < 0) {
-    const Words link0 = item + VA_I_LINK0;
-    const int qref0 = link0[VA_L_QREF];
-    const long long out_row = (link0[VA_L_FLAGS] & VA_LINK_INDIRECT) ? (long long)a.qref_rows[qref0 + iq] : a.sub_worker[qref0 + iq];
-    const long long at = (out_row * a.num_q_heads + hq) * (long long)kD;
-#pragma unroll
-    for (int x = 0; x < kD / 64; ++x) {
-      const int d = 4 * (seg + 16 * x);
-      float y[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) y[k] = normalised(sum[x][k], l);
-      if (pieces) {
-        const bool bf = dtype == VA_BF16;
-        const uint2 w = make_uint2(bf ? Mma<BF16>::pack(y[0], y[1]) : Mma<F16>::pack(y[0], y[1]),
-                                   bf ? Mma<BF16>::pack(y[2], y[3]) : Mma<F16>::pack(y[2], y[3]));
-        *(uint2*)((uint16_t*)a.out + at + d) = w;
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) store_activation(a.out, at + d + k, y[k], dtype);
-      }
-    }
-    if (seg == 0 && a.lse) a.lse[out_row * a.num_q_heads + hq] = log_sum(m, l, a.lse_base2);
+}
+
+template <int kD, typename C>
+__global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn_quant_stream_kernel(QuantAttnArgs qa, int dtype, int pieces) {
+  using Words = const __attribute__((address_space(4))) int32_t*;
+  const ItemHead where = item_and_head(blockIdx.x, qa.a.num_kv_heads);
+  const Words items = (Words)qa.a.items;
+  auto word = [&](int item, int w) __attribute__((always_inline)) { return items[(long long)item * VA_ITEM_WORDS + w]; };
+  if (word(where.item, VA_I_N_Q) == 0) return;  // padding item: keeps the launch order aligned with the die round-robin
+  // A run of partners lies eight items apart, the first of them with the number of the others: they are served in twos,
+  // by the first, the third, ...
+  int first = where.item, ahead = 0;
+  while (word(first, VA_I_PARTNERS) < 0 && first >= 8) first -= 8, ++ahead;
+  if (ahead % 2) return;
+  if (ahead < word(first, VA_I_PARTNERS)) {
+    quant_stream_items<kD, C, 2>(qa, {where.item, where.item + 8}, where.head, dtype, pieces);
   } else {
-    const long long slot = (long long)(part_base + iq) * a.num_q_heads + hq;
-    float* prow = a.part_acc + slot * kD;
-#pragma unroll
-    for (int x = 0; x < kD / 64; ++x) *(va_f32x4*)(prow + 4 * (seg + 16 * x)) = sum[x];
-    if (seg == 0) {
-      a.part_ml[slot * 2 + 0] = m;
-      a.part_ml[slot * 2 + 1] = l;
-    }
+    quant_stream_items<kD, C, 1>(qa, {where.item}, where.head, dtype, pieces);
   }
 }
 
 template <int kD, typename C>
 static int launch_quant_stream_one(const QuantAttnArgs& qa, int dtype, int n_items, int pieces, hipStream_t stream) {
   const dim3 grid((unsigned)n_items * (unsigned)qa.a.num_kv_heads), block(kQuantThreads);
-  constexpr int bytes = QuantShape<kD>::kLdsBytes;
+  constexpr int bytes = QuantRing<kD>::kLdsBytes;
   static std::atomic<unsigned long long> devices{0};
   hipError_t e = allow_lds(reinterpret_cast<const void*>(&attn_quant_stream_kernel<kD, C>), bytes, devices);
   if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
@@ -416,7 +404,7 @@ static int launch_quant_stream_coded(const QuantAttnArgs& qa, int dtype, int n_i
   }
 }
 
-int launch_quant_stream(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream) {
+int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream) {
   const AttnArgs& a = qa.a;
   const int g = a.num_q_heads / a.num_kv_heads;
   if (!va_mfma_supported(dtype, a.head_dim, g))
@@ -428,6 +416,8 @@ int launch_quant_stream(const QuantAttnArgs& qa, int dtype, int code_type, int n
   if ((uintptr_t)a.part_acc % 16) return va_fail(VA_ERR_ARG, "matrix-core path needs a 16-byte aligned workspace");
   // queries and results in 16-byte (8-byte) accesses where their addresses allow it
   const int pieces = a.q_row_stride % 8 == 0 && (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.out % 8 == 0;
+  // The choice hangs on the page size alone, so that a recorded launch keeps its kernel.
+  if (qa.pages.shift < 4) return launch_quant_scattered(qa, dtype, code_type, n_items, pieces, stream);
   return code_type == VA_CODE_E4M3 ? launch_quant_stream_coded<E4M3>(qa, dtype, n_items, pieces, stream)
                                    : launch_quant_stream_coded<INT8>(qa, dtype, n_items, pieces, stream);
 }
