@@ -56,54 +56,72 @@ __device__ __forceinline__ void wave_wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
 }
 
-// The query rows of a tile for a link, rotated in fp32 and split into two bf16 numbers, in LDS: sixteen rows of high parts,
-// then of low parts, piece c of row r at position c ^ (r & 7).
+// The query rows of a tile for a link, rotated in fp32 and split into two bf16 numbers: this thread's two pieces of eight
+// dims of a row, high parts and low parts.  (16 rows of kD / 16 units: at 64 and 128 dims some threads have none.)
+struct QueryPieces {
+  va_u32x4 part[2][2];  // [high, low][piece]
+  int row, d[2];        // row -1: no unit
+};
+// Where a thread's query row lies and what it is turned by: asked for ahead of its use.
+struct QuerySource {
+  int row, unit, g;  // row of the tile (-1: no unit), unit of the row, q head of the kv head
+  long long at;      // query row, or -1
+  Pos3 pos;
+};
 template <int kD>
-__device__ __forceinline__ void stage_query(const AttnArgs& a, int n_q, int lflags, int qref, int hk, int dtype, bool pieces,
-                                            char* query) {
-  const int G = a.num_q_heads / a.num_kv_heads;
-  for (int idx = threadIdx.x; idx < 16 * (kD / 16); idx += kQuantThreads) {
-    const int r = idx / (kD / 16), x = idx - r * (kD / 16), iq = r / G, g = r - iq * G;
-    const int pairs = a.rope.rotary_dim / 16;
-    const int d0 = x < pairs ? 8 * x : 16 * x, d1 = x < pairs ? 8 * x + a.rope.half : 16 * x + 8;
-    float y0[8], y1[8];
+__device__ __forceinline__ QuerySource query_source(const AttnArgs& a, int n_q, int lflags, int qref) {
+  static_assert(16 * (kD / 16) <= kQuantThreads, "a unit a thread");
+  const int G = a.num_q_heads / a.num_kv_heads, r = threadIdx.x / (kD / 16), iq = r / G;
+  QuerySource s{r < 16 ? r : -1, (int)(threadIdx.x % (kD / 16)), r - iq * G, -1, Pos3{0, 0, 0}};
+  if (r < 16 && iq < n_q) {
+    const bool indirect = lflags & VA_LINK_INDIRECT;
+    const int subrow = indirect ? a.qrefs[qref + iq] : qref + iq;
+    s.at = indirect ? (long long)a.qref_rows[qref + iq] : a.sub_worker[subrow];
+    if (a.rope.rotary_dim) s.pos = load_pos(a.sub_loc, a.sub_loc_axis_stride, subrow);
+  }
+  return s;
+}
+template <int kD>
+__device__ __forceinline__ QueryPieces turned_query(const AttnArgs& a, const QuerySource& from, int hk, int dtype, bool pieces) {
+  const int G = a.num_q_heads / a.num_kv_heads, x = from.unit, pairs = a.rope.rotary_dim / 16;
+  QueryPieces q;
+  q.row = from.row;
+  q.d[0] = x < pairs ? 8 * x : 16 * x;
+  q.d[1] = x < pairs ? 8 * x + a.rope.half : 16 * x + 8;
+  float y[2][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y0[e] = y1[e] = 0.f;
-    if (iq < n_q) {
-      const bool indirect = lflags & VA_LINK_INDIRECT;
-      const int subrow = indirect ? a.qrefs[qref + iq] : qref + iq;
-      const long long src = indirect ? (long long)a.qref_rows[qref + iq] : a.sub_worker[subrow];
-      const long long at = src * a.q_row_stride + (long long)(hk * G + g) * kD;
-      activations8(a.q, at + d0, dtype, pieces, y0);
-      activations8(a.q, at + d1, dtype, pieces, y1);
-      if (x < pairs) {
-        float c[8], s[8];
-        turns8(a.rope, load_pos(a.sub_loc, a.sub_loc_axis_stride, subrow), d0, c, s);
-        turn8(c, s, y0, y1);
-      }
-    }
-    va_u32x4 h0, l0, h1, l1;
+  for (int e = 0; e < 8; ++e) y[0][e] = y[1][e] = 0.f;
+  if (from.at >= 0) {
+    const long long at = from.at * a.q_row_stride + (long long)(hk * G + from.g) * kD;
+    float c[8], s[8];
+    if (x < pairs) turns8(a.rope, from.pos, q.d[0], c, s);
+    activations8(a.q, at + q.d[0], dtype, pieces, y[0]);
+    activations8(a.q, at + q.d[1], dtype, pieces, y[1]);
+    if (x < pairs) turn8(c, s, y[0], y[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       uint32_t hi, lo;
-      split_pair(y0[2 * e], y0[2 * e + 1], hi, lo);
-      h0[e] = hi, l0[e] = lo;
-      split_pair(y1[2 * e], y1[2 * e + 1], hi, lo);
-      h1[e] = hi, l1[e] = lo;
+      split_pair(y[i][2 * e], y[i][2 * e + 1], hi, lo);
+      q.part[0][i][e] = hi, q.part[1][i][e] = lo;
     }
-    char* q_row = query + r * (2 * kD);
-    const int c0 = 16 * ((d0 / 8) ^ (r & 7)), c1 = 16 * ((d1 / 8) ^ (r & 7));
-    *(va_u32x4*)(q_row + c0) = h0;
-    *(va_u32x4*)(q_row + c1) = h1;
-    *(va_u32x4*)(q_row + 32 * kD + c0) = l0;
-    *(va_u32x4*)(q_row + 32 * kD + c1) = l1;
-  }
+  return q;
 }
-// B operands of K.Q^T: step 2 s + b holds dims [64 s + 16 kg + 8 b, + 8) of row j; part 0 the high, 1 the low ones.
+// High or low parts in LDS (kD * 32 bytes): piece c of row r at position c ^ (r & 7).
 template <int kD>
-__device__ __forceinline__ va_u32x4 staged_query(const char* query, int step, int part) {
+__device__ __forceinline__ void stage_query(const QueryPieces& q, int part, char* query) {
+  if (q.row < 0) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *(va_u32x4*)(query + q.row * (2 * kD) + 16 * ((q.d[i] / 8) ^ (q.row & 7))) = part == 0 ? q.part[0][i] : q.part[1][i];
+}
+// B operands of K.Q^T: step 2 s + b holds dims [64 s + 16 kg + 8 b, + 8) of row j.
+template <int kD>
+__device__ __forceinline__ va_u32x4 staged_query(const char* query, int step) {
   const int j = threadIdx.x % 16, kg = (threadIdx.x % kWave) / 16;
-  return *(const va_u32x4*)(query + j * (2 * kD) + 16 * ((8 * (step / 2) + 2 * kg + step % 2) ^ (j & 7)) + part * 32 * kD);
+  return *(const va_u32x4*)(query + j * (2 * kD) + 16 * ((8 * (step / 2) + 2 * kg + step % 2) ^ (j & 7)));
 }
 
 // The state of a tile at the end: four waves', folded through LDS, then the result or the partial state.  o[t][r] is dim

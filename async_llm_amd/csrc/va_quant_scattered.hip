@@ -149,7 +149,11 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
 
     // ---- the query rows, rotated in fp32 and split, in LDS: piece c of row r at position c ^ (r & 7) ----
     if (li > 0) __syncthreads();  // every wave has read the previous link's
-    stage_query<kD>(a, n_q, lflags, qref, hk, dtype, pieces, query);
+    {
+      const QueryPieces own = turned_query<kD>(a, query_source<kD>(a, n_q, lflags, qref), hk, dtype, pieces);
+      stage_query<kD>(own, 0, query);
+      stage_query<kD>(own, 1, query + 32 * kD);
+    }
     __syncthreads();
     // B operands: step 2 s + b holds dims [64 s + 16 kg + 8 b, + 8) of row j
     // (at 256 dims they are read anew for every tile: held in registers they take the kernel over half of them, and one
@@ -158,7 +162,7 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
     va_u32x4 q_hi[kKeepQuery ? kSteps : 1], q_lo[kKeepQuery ? kSteps : 1];
     if constexpr (kKeepQuery) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) q_hi[s] = staged_query<kD>(query, s, 0), q_lo[s] = staged_query<kD>(query, s, 1);
+      for (int s = 0; s < kSteps; ++s) q_hi[s] = staged_query<kD>(query, s), q_lo[s] = staged_query<kD>(query + 32 * kD, s);
     }
 
     // ---- the tile loop ----
@@ -184,7 +188,7 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
         if constexpr (kKeepQuery) {
           high = q_hi[s], low = q_lo[s];
         } else {
-          high = staged_query<kD>(query, s, 0), low = staged_query<kD>(query, s, 1);
+          high = staged_query<kD>(query, s), low = staged_query<kD>(query + 32 * kD, s);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {

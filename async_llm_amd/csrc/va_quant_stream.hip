@@ -14,8 +14,11 @@
 // (global_load_lds) into a ring of its own: no barrier in the tile loop.  A tile is two halves of sixteen tokens, each one run
 // of 16 * D bytes of a page, for K and for V: whole lines, requested non-temporally where no other tile reads them (6.8 TB/s for
 // loads alone; as half lines straight to registers, which the products of K would take, 5.7).  A tile goes from LDS to
-// registers at once and its buffer is requested anew before the first product.  Two items that walk the same tokens (the
-// tiles of one run's many readers) share a workgroup, which converts each code once for both.
+// registers at once, K before its products and V behind them, and its half of the buffer is requested anew: one buffer is
+// enough, and two workgroups (three at 128, four at 64 dims) share a CU, so that an item's set-up and fold, about 5 us, run beside the
+// walks of others.  (One workgroup with two buffers and two tiles that walk the same tokens, as the 16-bit kernel has them:
+// 64 requests over a shared prompt 204 -> 247 us, 16 of short blocks 26 -> 36, a chunk of 333 tokens 97 -> 149; eight of 131072
+// tokens 340 either way.)
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -38,13 +41,14 @@ struct QuantRing {
   static constexpr int kLoads = kHalfBytes / 1024;      // wave-level loads of a half
   static constexpr int kTileBytes = 4 * kHalfBytes;     // K, then V
   static constexpr int kScaleBytes = 64 * 4;            // a word per scale: 32 keys', 32 values'
-  static constexpr int kBuffers = kD == 64 ? 4 : 2;     // ring depth of a wave, in tiles
+  static constexpr int kBuffers = kD == 64 ? 2 : 1;    // ring depth of a wave, in tiles
   static constexpr int kScaleSlots = 2 * kBuffers;      // scales stay in LDS while their tile is in registers
-  static constexpr int kMinBlocks = kD == 256 ? 1 : 2;  // workgroups per CU
+  static constexpr int kMinBlocks = kD == 64 ? 4 : kD == 128 ? 3 : 2;  // workgroups per CU
   static constexpr int kScaleOffset = kBuffers * kTileBytes;
   static constexpr int kWaveBytes = kScaleOffset + kScaleSlots * kScaleBytes;
   static constexpr int kQueryOffset = kQuantWaves * kWaveBytes;
-  static constexpr int kQueryBytes = 2 * 16 * kD * 2;  // of one tile: staged one after the other
+  static constexpr bool kKeepLow = kD < 128;  // low parts of the query in registers
+  static constexpr int kQueryBytes = 16 * kD * 2;       // high or low parts of a tile's query: staged one after the other
   static constexpr int kLdsBytes = kQueryOffset + kQueryBytes;
   static_assert(kQuantWaves * QuantFold<kD>::kBytes <= kLdsBytes, "room for the waves' states");
   static_assert(kMinBlocks * kLdsBytes <= 160 * 1024, "the LDS of a CU");
@@ -81,9 +85,8 @@ __device__ __forceinline__ void load_bytes_to_lds(unsigned long long at, uint32_
                : "memory");
 }
 
-// kB items that walk the same tokens, for one kv head.
-template <int kD, typename C, int kB>
-__device__ __forceinline__ void quant_stream_items(const QuantAttnArgs& qa, const int (&item)[kB], int hk, int dtype, bool pieces) {
+template <int kD, typename C>
+__global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn_quant_stream_kernel(QuantAttnArgs qa, int dtype, int pieces) {
   const AttnArgs& a = qa.a;
   using Sh = QuantRing<kD>;
   using Words = const __attribute__((address_space(4))) int32_t*;
@@ -92,14 +95,11 @@ __device__ __forceinline__ void quant_stream_items(const QuantAttnArgs& qa, cons
   extern __shared__ va_u32x4 smem[];
   char* lds = (char*)smem;
 
-  Words words[kB];
-  int n_q[kB];
-#pragma unroll
-  for (int b = 0; b < kB; ++b) {
-    words[b] = (Words)a.items + (long long)item[b] * VA_ITEM_WORDS;
-    n_q[b] = words[b][VA_I_N_Q];
-  }
-  const int G = a.num_q_heads / a.num_kv_heads;
+  const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
+  const Words item = (Words)a.items + (long long)where.item * VA_ITEM_WORDS;
+  const int n_q = item[VA_I_N_Q], n_links = item[VA_I_N_LINKS], link_begin = item[VA_I_LINK_BEGIN], part_base = item[VA_I_PART_BASE];
+  if (n_q == 0) return;  // padding item: keeps the launch order aligned with the die round-robin
+  const int hk = where.head, G = a.num_q_heads / a.num_kv_heads;
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int j = lane % 16, kg = lane / 16;  // MFMA row (token of a half, query row), contraction group
@@ -132,39 +132,29 @@ __device__ __forceinline__ void quant_stream_items(const QuantAttnArgs& qa, cons
   const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_address(lds)) + (uint32_t)wave * Sh::kWaveBytes;
   char* query = lds + Sh::kQueryOffset;
 
-  float m_run[kB], l_run[kB];  // running maximum (log2 units) and sum, of this wave's tokens
-  va_f32x4 o[kB][kDimTiles];
+  float m_run = kNegBig, l_run = 0.f;  // running maximum (log2 units) and sum, of this wave's tokens
+  va_f32x4 o[kDimTiles];
 #pragma unroll
-  for (int b = 0; b < kB; ++b) {
-    m_run[b] = kNegBig;
-    l_run[b] = 0.f;
-#pragma unroll
-    for (int t = 0; t < kDimTiles; ++t) o[b][t] = va_f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int t = 0; t < kDimTiles; ++t) o[t] = va_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const int n_links = words[0][VA_I_N_LINKS];
   for (int li = 0; li < n_links; ++li) {
-    const Words link = li == 0 ? words[0] + VA_I_LINK0 : (Words)a.links + (long long)(words[0][VA_I_LINK_BEGIN] + li) * VA_LINK_WORDS;
+    const Words link = li == 0 ? item + VA_I_LINK0 : (Words)a.links + (long long)(link_begin + li) * VA_LINK_WORDS;
     const int lflags = link[VA_L_FLAGS], kv_begin = link[VA_L_KV_BEGIN], tok_begin = link[VA_L_TOK_BEGIN];
-    const int tok_end = link[VA_L_TOK_END], causal_base = link[VA_L_CAUSAL_BASE];
+    const int tok_end = link[VA_L_TOK_END], causal_base = link[VA_L_CAUSAL_BASE], qref = link[VA_L_QREF];
     const bool slots = lflags & VA_LINK_SLOTS;
     const bool read_once = lflags & VA_LINK_ONCE;  // no other tile reads these rows: lines to evict first
     const bool whole = !slots && tok_begin % 16 == 0;  // halves lie inside a page
-    const int t_stop = min(tok_end, causal_base + n_q[0]);   // tokens any row of the tile sees
-    const int t_row = min(tok_end, causal_base + row_iq + 1);  // tokens this lane's row sees (partners are not causal)
+    const int t_stop = min(tok_end, causal_base + n_q);        // tokens any row of the tile sees
+    const int t_row = min(tok_end, causal_base + row_iq + 1);  // tokens this lane's row sees
     const int t_last = t_stop - 1;
     const int n_all = t_stop > tok_begin ? (t_stop - tok_begin + kQuantTokens - 1) / kQuantTokens : 0;
     const int n_tiles = n_all > wave ? (n_all - wave + kQuantWaves - 1) / kQuantWaves : 0;  // this wave's
     auto first_token = [&](int i) __attribute__((always_inline)) { return tok_begin + (i * kQuantWaves + wave) * kQuantTokens; };
-    auto page_entry = [&](int t) __attribute__((always_inline)) {  // (a scalar load: a vector one would be waited for with all others)
-      return ((Words)a.kv_indices)[kv_begin + t];
-    };
-    // pages of tile i, read a tile ahead of its request
+    // pages of tile i, read a tile ahead of its request (in scalar loads: a vector one would be waited for with all others)
     auto read_pages = [&](int i, int (&page)[2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) page[h] = page_entry(min(first_token(i) + 16 * h, t_last) >> p_shift);
+      for (int h = 0; h < 2; ++h) page[h] = ((Words)a.kv_indices)[kv_begin + (min(first_token(i) + 16 * h, t_last) >> p_shift)];
     };
-    // Request tile i into buffer i % kBuffers.  Rows past the visible range repeat the last visible token (masked).
     auto request_half = [&](const uint8_t* pool, long long base, const uint32_t* off, uint32_t dst, auto once) __attribute__((always_inline)) {
       const void* from = pool + (base - kBias);
       if constexpr (kLoads == 1) {
@@ -173,78 +163,88 @@ __device__ __forceinline__ void quant_stream_items(const QuantAttnArgs& qa, cons
         load_group_to_lds<kLoads, decltype(once)::value>(from, off, dst);
       }
     };
-    auto request = [&](int i, const int (&page)[2]) __attribute__((always_inline)) {
-      const uint32_t dst = ring + (uint32_t)(i % kBuffers) * Sh::kTileBytes;
+    // Request K (kind 0), or V and the scales (1), of tile i into buffer i % kBuffers.  Rows past the visible range repeat
+    // the last visible token (masked).
+    auto request = [&](int i, const int (&page)[2], auto kind) __attribute__((always_inline)) {
+      constexpr int v = decltype(kind)::value;
+      const uint8_t* pool = v ? vp : kp;
+      const uint32_t dst = ring + (uint32_t)(i % kBuffers) * Sh::kTileBytes + v * 2 * Sh::kHalfBytes;
       const uint32_t scales = ring + Sh::kScaleOffset + (uint32_t)(i % Sh::kScaleSlots) * Sh::kScaleBytes;
+      const uint8_t* of_scales = lane < 32 ? qa.k_scales : qa.v_scales;
       const int t0 = first_token(i);
-      long long row[2];  // of a half's first token
       if (whole) {
-        uint32_t off[2][kLoads];
         const bool full = t0 + kQuantTokens - 1 <= t_last;
+        long long row[2];  // of a half's first token
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int t = min(t0 + 16 * h, t_last);
-          row[h] = ((long long)page[h] * a.num_kv_heads + hk) * P + (t & (P - 1));
-          const int most = max(0, t_last - (t0 + 16 * h));  // last row of the half that is visible
+        for (int h = 0; h < 2; ++h) row[h] = ((long long)page[h] * a.num_kv_heads + hk) * P + (min(t0 + 16 * h, t_last) & (P - 1));
+        int place = j;
+        if (full && read_once) {
 #pragma unroll
-          for (int u = 0; u < kLoads; ++u)
-            off[h][u] = full ? ld_off[h][u] : ld_off[h][u] - (uint32_t)(max(0, ld_row(u) - most) * kD);
-        }
-        auto both = [&](auto once) __attribute__((always_inline)) {
+          for (int h = 0; h < 2; ++h) request_half(pool, row[h] * kD, ld_off[h], dst + h * Sh::kHalfBytes, std::true_type{});
+        } else if (full) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) request_half(kp, row[h] * kD, off[h], dst + h * Sh::kHalfBytes, once);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) request_half(vp, row[h] * kD, off[h], dst + (2 + h) * Sh::kHalfBytes, once);
-        };
-        if (read_once && full) {
-          both(std::true_type{});
+          for (int h = 0; h < 2; ++h) request_half(pool, row[h] * kD, ld_off[h], dst + h * Sh::kHalfBytes, std::false_type{});
         } else {
-          both(std::false_type{});
-        }
-        const int h = kg & 1, place = min(j, max(0, t_last - (t0 + 16 * h)));
-        const unsigned long long scale = (unsigned long long)(lane < 32 ? qa.k_scales : qa.v_scales) + (h ? row[1] : row[0]) + place;
-        load_bytes_to_lds(scale, scales);
-      } else {  // every lane looks its tokens up, in vector loads
-        auto row_of = [&](int t) __attribute__((always_inline)) { return quant_token_row(qa, kv_begin, min(t, t_last), slots, hk); };
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            const int most = max(0, t_last - (t0 + 16 * h));  // last row of the half that is visible
+            uint32_t off[kLoads];
 #pragma unroll
-          for (int u = 0; u < kLoads; ++u) {
-            const long long at = row_of(t0 + 16 * h + ld_row(u)) * kD + 16 * ld_piece(u, h);
-            load_to_lds(kp + at, dst + h * Sh::kHalfBytes + 1024 * u);
-            load_to_lds(vp + at, dst + (2 + h) * Sh::kHalfBytes + 1024 * u);
+            for (int u = 0; u < kLoads; ++u) off[u] = ld_off[h][u] - (uint32_t)(max(0, ld_row(u) - most) * kD);
+            request_half(pool, row[h] * kD, off, dst + h * Sh::kHalfBytes, std::false_type{});
           }
-        load_bytes_to_lds((unsigned long long)(lane < 32 ? qa.k_scales : qa.v_scales) + row_of(t0 + lane % 32), scales);
+          place = min(j, max(0, t_last - (t0 + 16 * (kg & 1))));
+        }
+        if constexpr (v) load_bytes_to_lds((unsigned long long)of_scales + (kg & 1 ? row[1] : row[0]) + place, scales);
+      } else {  // every lane looks its tokens up, in vector loads (one after the other: few tokens come this way)
+        auto row_of = [&](int t) __attribute__((always_inline)) {
+          const int at = min(t, t_last), entry = a.kv_indices[kv_begin + (slots ? at : at >> p_shift)];
+          const int page = slots ? entry >> p_shift : entry, place = (slots ? entry : at) & (P - 1);
+          return ((long long)page * a.num_kv_heads + hk) * P + place;
+        };
+#pragma unroll 1
+        for (int x = 0; x < 2 * kLoads; ++x) {
+          const int h = x / kLoads, u = x % kLoads;
+          load_to_lds(pool + row_of(t0 + 16 * h + ld_row(u)) * kD + 16 * ld_piece(u, h), dst + 1024 * x);
+        }
+        if constexpr (v) load_bytes_to_lds((unsigned long long)of_scales + row_of(t0 + lane % 32), scales);
       }
     };
+    constexpr std::integral_constant<int, 0> kKeys{};
+    constexpr std::integral_constant<int, 1> kValues{};
 
-    // ---- set-up: first tiles on their way, then the query tiles ----
+    // ---- set-up: first tiles on their way, then the query tile ----
     // (no barrier: a wave's ring is its own, and it has read the previous link's tiles)
-    int next_page[2] = {0, 0};
-    if (n_tiles > 0) {
-      int page[kBuffers][2] = {};
-      if (whole) {
+    int next_page[2] = {0, 0}, page[kBuffers][2] = {};
+    if (whole && n_tiles > 0) {
 #pragma unroll
-        for (int i = 0; i < kBuffers; ++i) read_pages(i, page[i]);
-        read_pages(kBuffers, next_page);
-      }
-#pragma unroll
-      for (int i = 0; i < kBuffers; ++i)
-        if (i < n_tiles) request(i, page[i]);
+      for (int i = 0; i < kBuffers; ++i) read_pages(i, page[i]);
+      read_pages(kBuffers, next_page);
     }
-    va_u32x4 q_hi[kB][kSteps], q_lo[kB][kSteps];
+    const QuerySource source = query_source<kD>(a, n_q, lflags, qref);
 #pragma unroll
-    for (int b = 0; b < kB; ++b) {
-      if (li > 0 || b > 0) ring_barrier<kAnyInFlight>();  // every wave has read the query tile before
-      stage_query<kD>(a, n_q[b], lflags, b == 0 ? link[VA_L_QREF] : words[b][VA_I_LINK0 + VA_L_QREF], hk, dtype, pieces, query);
-      ring_barrier<kAnyInFlight>();
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        q_hi[b][s] = staged_query<kD>(query, s, 0);
-        q_lo[b][s] = staged_query<kD>(query, s, 1);
+    for (int i = 0; i < kBuffers; ++i)
+      if (i < n_tiles) {
+        request(i, page[i], kKeys);
+        request(i, page[i], kValues);
       }
+    const QueryPieces mine = turned_query<kD>(a, source, hk, dtype, pieces);
+    if (li > 0) ring_barrier<kAnyInFlight>();  // every wave has read what lay there
+    stage_query<kD>(mine, 0, query);
+    ring_barrier<kAnyInFlight>();
+    va_u32x4 q_hi[kSteps], q_lo[Sh::kKeepLow ? kSteps : 1];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q_hi[b][s]), "+v"(q_lo[b][s]));
+    for (int s = 0; s < kSteps; ++s) q_hi[s] = staged_query<kD>(query, s);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q_hi[s]));
+    ring_barrier<kAnyInFlight>();
+    stage_query<kD>(mine, 1, query);
+    ring_barrier<kAnyInFlight>();
+    if constexpr (Sh::kKeepLow) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) q_lo[s] = staged_query<kD>(query, s);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q_lo[s]));
     }
 
     // ---- the tile loop ----
@@ -257,41 +257,45 @@ __device__ __forceinline__ void quant_stream_items(const QuantAttnArgs& qa, cons
       }
       const uint32_t buffer = (uint32_t)(i % kBuffers) * Sh::kTileBytes;
       const char* tile = lds + wave * Sh::kWaveBytes + buffer;
+      const bool more = i + kBuffers < n_tiles;
       va_u32x4 kraw[2][kPieces];
-      va_u32x2 vraw[kDimTiles];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int s = 0; s < kPieces; ++s) kraw[h][s] = *(const va_u32x4*)(tile + h * Sh::kHalfBytes + j * kD + (k_at[h] ^ (64 * s)));
-#pragma unroll
-      for (int t = 0; t < kDimTiles; ++t) vraw[t] = lds_read_tr8(ring + buffer + v_at + ((16 * t) ^ v_swz));
       __builtin_amdgcn_sched_barrier(0);
-      // the buffer is requested anew as soon as its tile is in registers
-      if (i + kBuffers < n_tiles) {
+      if (more) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        request(i + kBuffers, next_page);
-        if (whole) read_pages(i + 1 + kBuffers, next_page);
+        request(i + kBuffers, next_page, kKeys);
       }
       __builtin_amdgcn_sched_barrier(0);
 
-      va_f32x4 hi[kB][2], lo[kB][2];
+      va_f32x4 hi[2], lo[2];
 #pragma unroll
-      for (int b = 0; b < kB; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) hi[b][h] = lo[b][h] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2; ++h) hi[h] = lo[h] = va_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
+        va_u32x4 low;
+        if constexpr (Sh::kKeepLow) low = q_lo[s]; else low = staged_query<kD>(query, s);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const va_u32x4 raw = kraw[h][s / 2];
           const va_u32x4 k8 = C::bf16x8(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]});
-#pragma unroll
-          for (int b = 0; b < kB; ++b) {
-            hi[b][h] = Mma<BF16>::run(k8, q_hi[b][s], hi[b][h]);
-            lo[b][h] = Mma<BF16>::run(k8, q_lo[b][s], lo[b][h]);
-          }
+          hi[h] = Mma<BF16>::run(k8, q_hi[s], hi[h]);
+          lo[h] = Mma<BF16>::run(k8, low, lo[h]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      va_u32x2 vraw[kDimTiles];
+#pragma unroll
+      for (int t = 0; t < kDimTiles; ++t) vraw[t] = lds_read_tr8(ring + buffer + v_at + ((16 * t) ^ v_swz));
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        request(i + kBuffers, next_page, kValues);
+        if (whole) read_pages(i + 1 + kBuffers, next_page);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 
       // online softmax; this lane holds tokens 16 h + 4 kg + r of row j
       const int t0 = first_token(i);
@@ -302,82 +306,53 @@ __device__ __forceinline__ void quant_stream_items(const QuantAttnArgs& qa, cons
         kscale[h] = *(const va_u32x4*)(scales + 64 * h);
         vscale[h] = *(const va_u32x4*)(scales + 128 + 64 * h);
       }
-      va_u32x4 w_hi[kB], w_lo[kB];
+      float sc[2][4], most = -INFINITY;
 #pragma unroll
-      for (int b = 0; b < kB; ++b) {
-        float sc[2][4], most = -INFINITY;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool seen = t0 + 16 * h + 4 * kg + r < t_row;
-            sc[h][r] = seen ? (hi[b][h][r] + lo[b][h][r]) * (scale_value(kscale[h][r]) * a.scale_log2) : -INFINITY;
-            most = fmaxf(most, sc[h][r]);
-          }
-        if (__any(most > m_run[b])) {
-          const float m_new = fmaxf(m_run[b], quant_group_max(most));
-          const float alpha = __builtin_amdgcn_exp2f(m_run[b] - m_new);
-          m_run[b] = m_new;
-          l_run[b] *= alpha;
-#pragma unroll
-          for (int t = 0; t < kDimTiles; ++t) o[b][t] *= alpha;
+        for (int r = 0; r < 4; ++r) {
+          const bool seen = t0 + 16 * h + 4 * kg + r < t_row;
+          sc[h][r] = seen ? (hi[h][r] + lo[h][r]) * (scale_value(kscale[h][r]) * a.scale_log2) : -INFINITY;
+          most = fmaxf(most, sc[h][r]);
         }
+      if (__any(most > m_run)) {
+        const float m_new = fmaxf(m_run, quant_group_max(most));
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float w[4];
+        for (int t = 0; t < kDimTiles; ++t) o[t] *= alpha;
+      }
+      va_u32x4 w_hi, w_lo;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f(sc[h][r] - m_run[b]);
-            l_run[b] += p;
-            // (a token that the row does not see may have any scale)
-            w[r] = t0 + 16 * h + 4 * kg + r < t_row ? p * scale_value(vscale[h][r]) : 0.f;
-          }
-          uint32_t x, y;
-          split_pair(w[0], w[1], x, y);
-          w_hi[b][2 * h] = x, w_lo[b][2 * h] = y;
-          split_pair(w[2], w[3], x, y);
-          w_hi[b][2 * h + 1] = x, w_lo[b][2 * h + 1] = y;
+      for (int h = 0; h < 2; ++h) {
+        float w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(sc[h][r] - m_run);
+          l_run += p;
+          // (a token that the row does not see may have any scale)
+          w[r] = t0 + 16 * h + 4 * kg + r < t_row ? p * scale_value(vscale[h][r]) : 0.f;
         }
+        uint32_t x, y;
+        split_pair(w[0], w[1], x, y);
+        w_hi[2 * h] = x, w_lo[2 * h] = y;
+        split_pair(w[2], w[3], x, y);
+        w_hi[2 * h + 1] = x, w_lo[2 * h + 1] = y;
       }
 
       // O^T += V^T . W^T, the lane's contraction elements being tokens 4 kg .. + 3 and 16 + 4 kg .. + 3
 #pragma unroll
       for (int t = 0; t < kDimTiles; ++t) {
         const va_u32x4 v8 = C::bf16x8(vraw[t]);
-#pragma unroll
-        for (int b = 0; b < kB; ++b) {
-          o[b][t] = Mma<BF16>::run(v8, w_hi[b], o[b][t]);
-          o[b][t] = Mma<BF16>::run(v8, w_lo[b], o[b][t]);
-        }
+        o[t] = Mma<BF16>::run(v8, w_hi, o[t]);
+        o[t] = Mma<BF16>::run(v8, w_lo, o[t]);
       }
     }
   }
 
-#pragma unroll
-  for (int b = 0; b < kB; ++b) {
-    __syncthreads();  // every wave is done with its tiles and the query, or has read the block before
-    fold_and_finish<kD>(a, o[b], m_run[b], l_run[b], lds, n_q[b], words[b][VA_I_PART_BASE], words[b][VA_I_LINK0 + VA_L_QREF],
-                        words[b][VA_I_LINK0 + VA_L_FLAGS], hk, dtype, pieces);
-  }
-}
-
-template <int kD, typename C>
-__global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn_quant_stream_kernel(QuantAttnArgs qa, int dtype, int pieces) {
-  using Words = const __attribute__((address_space(4))) int32_t*;
-  const ItemHead where = item_and_head(blockIdx.x, qa.a.num_kv_heads);
-  const Words items = (Words)qa.a.items;
-  auto word = [&](int item, int w) __attribute__((always_inline)) { return items[(long long)item * VA_ITEM_WORDS + w]; };
-  if (word(where.item, VA_I_N_Q) == 0) return;  // padding item: keeps the launch order aligned with the die round-robin
-  // A run of partners lies eight items apart, the first of them with the number of the others: they are served in twos,
-  // by the first, the third, ...
-  int first = where.item, ahead = 0;
-  while (word(first, VA_I_PARTNERS) < 0 && first >= 8) first -= 8, ++ahead;
-  if (ahead % 2) return;
-  if (ahead < word(first, VA_I_PARTNERS)) {
-    quant_stream_items<kD, C, 2>(qa, {where.item, where.item + 8}, where.head, dtype, pieces);
-  } else {
-    quant_stream_items<kD, C, 1>(qa, {where.item}, where.head, dtype, pieces);
-  }
+  __syncthreads();  // every wave is done with its tiles and the query
+  fold_and_finish<kD>(a, o, m_run, l_run, lds, n_q, part_base, item[VA_I_LINK0 + VA_L_QREF], item[VA_I_LINK0 + VA_L_FLAGS], hk, dtype, pieces);
 }
 
 template <int kD, typename C>
