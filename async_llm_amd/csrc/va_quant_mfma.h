@@ -49,6 +49,24 @@ __device__ __forceinline__ void activations8(const void* x, long long at, int dt
   }
 }
 
+// Piece c of token t of a tile lies at position c ^ ring_swz(t).  Sixteen tokens' pieces c (a fragment of K), and the piece
+// that a transposing read takes of tokens 4 k .. + 3 and 16 + 4 k .. + 3 (V), then lie in different banks.
+template <int kD>
+__device__ __forceinline__ int ring_swz(int t) {
+  if constexpr (kD == 256) return (t & 15) ^ (((t >> 4) & 1) << 2);
+  if constexpr (kD == 128) return ((t >> 1) & 7) ^ (((t >> 4) & 1) << 1);
+  return ((t >> 2) & 3) ^ ((t >> 4) & 1);
+}
+
+// A byte per lane, each a word in LDS: lane l's lands at lds_base + 4 l.
+__device__ __forceinline__ void load_bytes_to_lds(unsigned long long at, uint32_t lds_base) {
+  uint32_t saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved)
+               : "v"(at), "s"(lds_base)
+               : "memory");
+}
+
 // Wait until at most n of the wave's vector memory operations are outstanding.
 template <int n>
 __device__ __forceinline__ void wave_wait_loads() {
@@ -124,6 +142,18 @@ __device__ __forceinline__ va_u32x4 staged_query(const char* query, int step) {
   return *(const va_u32x4*)(query + j * (2 * kD) + 16 * ((8 * (step / 2) + 2 * kg + step % 2) ^ (j & 7)));
 }
 
+// Four neighbouring results at `at`.
+__device__ __forceinline__ void store_results4(void* out, long long at, const float* y, int dtype, bool pieces) {
+  if (pieces) {
+    const bool bf = dtype == VA_BF16;
+    *(uint2*)((uint16_t*)out + at) = make_uint2(bf ? Mma<BF16>::pack(y[0], y[1]) : Mma<F16>::pack(y[0], y[1]),
+                                                bf ? Mma<BF16>::pack(y[2], y[3]) : Mma<F16>::pack(y[2], y[3]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) store_activation(out, at + k, y[k], dtype);
+  }
+}
+
 // The state of a tile at the end: four waves', folded through LDS, then the result or the partial state.  o[t][r] is dim
 // 16 t + 4 kg + r of row j, l_run a sum spread over the four contraction groups.
 template <int kD>
@@ -178,14 +208,7 @@ __device__ __forceinline__ void fold_and_finish(const AttnArgs& a, const va_f32x
       float y[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) y[k] = normalised(sum[x][k], l);
-      if (pieces) {
-        const bool bf = dtype == VA_BF16;
-        *(uint2*)((uint16_t*)a.out + at + d) = make_uint2(bf ? Mma<BF16>::pack(y[0], y[1]) : Mma<F16>::pack(y[0], y[1]),
-                                                          bf ? Mma<BF16>::pack(y[2], y[3]) : Mma<F16>::pack(y[2], y[3]));
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) store_activation(a.out, at + d + k, y[k], dtype);
-      }
+      store_results4(a.out, at + d, y, dtype, pieces);
     }
     if (seg == 0 && a.lse) a.lse[out_row * a.num_q_heads + hq] = log_sum(m, l, a.lse_base2);
   } else {

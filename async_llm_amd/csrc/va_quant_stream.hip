@@ -55,15 +55,6 @@ struct QuantRing {
   static constexpr int kLoadsPerTile = 4 * kLoads + 1;  // what the counter of outstanding loads sees of a tile
 };
 
-// Piece c of token t of a tile lies at position c ^ ring_swz(t).  Sixteen tokens' pieces c (a fragment of K), and the piece
-// that a transposing read takes of tokens 4 k .. + 3 and 16 + 4 k .. + 3 (V), then lie in different banks.
-template <int kD>
-__device__ __forceinline__ int ring_swz(int t) {
-  if constexpr (kD == 256) return (t & 15) ^ (((t >> 4) & 1) << 2);
-  if constexpr (kD == 128) return ((t >> 1) & 7) ^ (((t >> 4) & 1) << 1);
-  return ((t >> 2) & 3) ^ ((t >> 4) & 1);
-}
-
 // One wave-level load of 1 KB with a cache policy (load_to_lds has none).
 template <bool kOnce>
 __device__ __forceinline__ void load_run_to_lds(const void* base, uint32_t lane_offset, uint32_t lds_base) {
@@ -76,15 +67,6 @@ __device__ __forceinline__ void load_run_to_lds(const void* base, uint32_t lane_
   if constexpr (kOnce) VA_ONE_LOAD(" nt"); else VA_ONE_LOAD("");
 #undef VA_ONE_LOAD
 }
-// A byte per lane, each a word in LDS: lane l's lands at lds_base + 4 l.
-__device__ __forceinline__ void load_bytes_to_lds(unsigned long long at, uint32_t lds_base) {
-  uint32_t saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(at), "s"(lds_base)
-               : "memory");
-}
-
 template <int kD, typename C>
 __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn_quant_stream_kernel(QuantAttnArgs qa, int dtype, int pieces) {
   const AttnArgs& a = qa.a;
@@ -96,7 +78,7 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
   char* lds = (char*)smem;
 
   const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
-  const Words item = (Words)a.items + (long long)where.item * VA_ITEM_WORDS;
+  const Words item = (Words)a.narrow_items + (long long)where.item * VA_ITEM_WORDS;
   const int n_q = item[VA_I_N_Q], n_links = item[VA_I_N_LINKS], link_begin = item[VA_I_LINK_BEGIN], part_base = item[VA_I_PART_BASE];
   if (n_q == 0) return;  // padding item: keeps the launch order aligned with the die round-robin
   const int hk = where.head, G = a.num_q_heads / a.num_kv_heads;
@@ -379,7 +361,8 @@ static int launch_quant_stream_coded(const QuantAttnArgs& qa, int dtype, int n_i
   }
 }
 
-int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream) {
+int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int n_wide, int n_wide_slots, int q_tile,
+                      hipStream_t stream) {
   const AttnArgs& a = qa.a;
   const int g = a.num_q_heads / a.num_kv_heads;
   if (!va_mfma_supported(dtype, a.head_dim, g))
@@ -392,7 +375,14 @@ int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_i
   // queries and results in 16-byte (8-byte) accesses where their addresses allow it
   const int pieces = a.q_row_stride % 8 == 0 && (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.out % 8 == 0;
   // The choice hangs on the page size alone, so that a recorded launch keeps its kernel.
-  if (qa.pages.shift < 4) return launch_quant_scattered(qa, dtype, code_type, n_items, pieces, stream);
+  if (qa.pages.shift < 4) {
+    if (n_wide > 0) return va_fail(VA_ERR_ARG, "a plan over pages of %d tokens has no wide items (wide_tile < 0)", a.page_size);
+    return launch_quant_scattered(qa, dtype, code_type, n_items, pieces, stream);
+  }
+  if (n_wide > 0 && n_wide_slots > 0) {
+    const int rc = launch_quant_wide(qa, dtype, code_type, n_wide_slots, pieces, stream);
+    if (rc || n_items == 0) return rc;
+  }
   return code_type == VA_CODE_E4M3 ? launch_quant_stream_coded<E4M3>(qa, dtype, n_items, pieces, stream)
                                    : launch_quant_stream_coded<INT8>(qa, dtype, n_items, pieces, stream);
 }

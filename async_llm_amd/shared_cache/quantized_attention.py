@@ -46,7 +46,8 @@ class QuantizedCacheAttention(SharedCacheAttention):
         device = torch.device(device)
         if device.type != self.device.type or device.index not in (None, self.device.index):
             raise ValueError(f"kv_cache lives on {self.device}, the op is to run on {device}")
-        self.plan_params.wide_tile = -1  # the codes are read by tiles of up to 16 rows
+        if page_size < 16 or page_size & (page_size - 1):
+            self.plan_params.wide_tile = -1  # wide tiles take their tokens in halves of sixteen that lie inside a page
 
     # ------------------------------------------------------------------
     # planning

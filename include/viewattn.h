@@ -406,11 +406,13 @@ VA_API int va_copy_shift_kv_q8(const VaQuantPool* pool, int64_t code_layer_strid
 
 /*
  * va_attention_q8: va_attention over a quantised pool, with the plans of
- * va_plan_build* for the same shape and params->wide_tile < 0 (no wide items).
+ * va_plan_build* for the same shape; pages of fewer than 16 tokens or of a number
+ * that no power of two is need params->wide_tile < 0 (no wide items).
  * kv_indices of VA_SUB_SLOTS sub-requests are token slots of the pool.  Queries
- * are rotated in fp32 and enter the products unrounded (vector-ALU kernel) or as
- * sums of two bf16 numbers (matrix-core kernel: error 2^-17 of each element), and
- * so do the weights of the second product.
+ * are rotated in fp32 and enter the products unrounded (vector-ALU kernel), as
+ * sums of two bf16 numbers (narrow items of the matrix-core plans: an error of 2^-17
+ * of each element) or as float16 numbers (wide items: 2^-11), and so do the weights
+ * of the second product.
  */
 VA_API int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
                     const int32_t* plan_header_host, const int32_t* kv_indices_dev,

@@ -156,10 +156,10 @@ def slots_of(block, tokens=None):
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
-def attention64(op, q: torch.Tensor, segments, layer=0):
+def attention64(op, q: torch.Tensor, segments, layer=0, operand=2.0**-17):
     """One request: ``q [rows, Hq, D]``; ``segments``: ``(slots, positions [rows] or [3, rows], first)`` where token t of
     a segment is visible to row i iff t <= first + i.  Returns out ``[rows, Hq * D]``, lse ``[rows, Hq]`` and the bound of
-    |out| errors that 32-bit arithmetic over 16-bit-exact splits allows (see ``bounds``)."""
+    score errors where an operand that is no code is off by ``operand`` of itself, and the weighted values."""
     S, Hq, D = q.shape
     Hkv = op.num_kv_heads
     G = Hq // Hkv
@@ -178,18 +178,18 @@ def attention64(op, q: torch.Tensor, segments, layer=0):
     p = torch.where(torch.isinf(lse)[..., None], 0.0, torch.exp(x - torch.where(torch.isinf(lse), 0.0, lse)[..., None]))
     out = torch.einsum("hsgt,thd->shgd", p, v).reshape(S, Hq * D)
     weight = torch.einsum("hsgt,thd->shgd", p, v.abs()).reshape(S, Hq * D)
-    # A score is off by its operands' 2^-17 (two bf16 numbers hold 16 bits, rounded to half a step: 2^-17 of q; scores
-    # of D products in 32 bits: D * 2^-24, all of the magnitudes' sum), its exponent by 2^-23 of itself.
-    off = (size.amax(-1) * (2.0**-17 + D * 2.0**-24) + x.abs().masked_fill(torch.isinf(x), 0.0).amax(-1) * 2.0**-22) if x.shape[-1] else torch.zeros_like(lse)
+    # A score is off by its query's rounding (two bf16 numbers hold 16 bits: 2^-17; float16 for many new tokens: 2^-11) and
+    # that of D products in 32 bits (D * 2^-24), both of the magnitudes' sum, its exponent by 2^-23 of itself.
+    off = (size.amax(-1) * (operand + D * 2.0**-24) + x.abs().masked_fill(torch.isinf(x), 0.0).amax(-1) * 2.0**-22) if x.shape[-1] else torch.zeros_like(lse)
     off = off.permute(1, 0, 2).reshape(S, Hq)
     return out, lse.permute(1, 0, 2).reshape(S, Hq), off, weight
 
 
-def assert_attends(out, lse, expected, dtype, tokens):
-    """|out - out64| <= rounding of the result + (2 * score error + 2^-17 of a weight + sums of 32 bits) * sum p|v|."""
+def assert_attends(out, lse, expected, dtype, tokens, operand=2.0**-17):
+    """|out - out64| <= rounding of the result + (2 * score error + rounding of a weight + sums of 32 bits) * sum p|v|."""
     o, l, off, weight = expected
     got = out.detach().cpu().double()
-    relative = (2 * off + 2.0**-17 + (tokens + 64) * 2.0**-24).repeat_interleave(o.shape[1] // off.shape[1], dim=1)
+    relative = (2 * off + operand + (tokens + 64) * 2.0**-24).repeat_interleave(o.shape[1] // off.shape[1], dim=1)
     room = EPS[dtype] * o.abs() + weight * relative * (1 + EPS[dtype]) + 2.0**-24
     assert got.shape == o.shape
     worst = ((got - o).abs() - room).max().item()

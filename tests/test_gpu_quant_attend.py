@@ -16,11 +16,13 @@ BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 def check(op, step, q, first, rows, out, lse, layer=0):
     Hq, D = op.num_qo_heads, op.head_dim
     parts = []
+    # (tiles of many rows take queries and weights as single float16 numbers)
+    operand = 2.0**-11 if step.meta.launch.counts.n_wide_items else 2.0**-17
     for segments, at, n in zip(step.segments, first, rows):
-        parts.append(Q.attention64(op, q[at: at + n].cpu().view(n, Hq, D), segments, layer))
+        parts.append(Q.attention64(op, q[at: at + n].cpu().view(n, Hq, D), segments, layer, operand))
     expected = tuple(torch.cat(x) for x in zip(*parts))
     tokens = max(sum(len(s[0]) for s in segments) for segments in step.segments)
-    Q.assert_attends(out, lse, expected, op.dtype, tokens)
+    Q.assert_attends(out, lse, expected, op.dtype, tokens, operand)
 
 
 DECODES = [
@@ -79,13 +81,18 @@ PREFILLS = [
     ((6, 2, 64), 8, BF16, INT8, None, [50], [(3, 11)]),
     ((8, 2, 64), 1, F16, E4M3, None, [50], [(3, 41)]),
     ((16, 4, 256), 16, BF16, E4M3, (24, 20, 20), [200], [(40, 45), (0, 7)]),
+    ((16, 4, 256), 32, F16, INT8, None, [777, 40], [(90, 301), (0, 33)]),
+    ((32, 8, 128), 64, BF16, E4M3, None, [400], [(0, 200), (77, 1), (100, 65)]),
+    ((8, 8, 128), 16, F16, E4M3, None, [100], [(7, 290)]),
+    ((16, 1, 64), 16, BF16, INT8, None, [300], [(20, 100)]),
+    ((64, 16, 64), 16, F16, E4M3, (12, 10, 10), [120], [(3, 140)]),
 ]
 
 
 @pytest.mark.parametrize("heads,page,dtype,codes,mrope,context,requests", PREFILLS)
 def test_prefill(heads, page, dtype, codes, mrope, context, requests):
     num_pages = -(-(sum(context) + sum(h + n for h, n in requests)) // page) + 12
-    op, pool, g = Q.make(DEV, heads, page, num_pages, dtype, codes, 128 if mrope else None, mrope)
+    op, pool, g = Q.make(DEV, heads, page, num_pages, dtype, codes, min(heads[2], 128) if mrope else None, mrope)
     pages = Q.Pages(num_pages, page)
     blocks = [pages.block(DEV, n, span=n - n // 4 if mrope else None) for n in context]
     step = Q.prefill_step(op, [(blocks, pages.block(DEV, h, room=n), n) for h, n in requests], three=mrope is not None)
