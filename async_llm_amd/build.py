@@ -23,7 +23,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "libviewattn.so")
 HIP_SOURCES = ["viewattn.hip", "va_mfma.hip", "va_mfma_wide.hip", "va_mfma_stream.hip", "va_block_copy.hip",
                "va_quant_rows.hip", "va_quant_attn.hip", "va_quant_stream.hip",
-               "va_quant_scattered.hip", "va_quant_wide.hip"]
+               "va_quant_scattered.hip", "va_quant_back.hip"]
 HOST_SOURCES = ["va_plan.cpp"]
 
 COMMON_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-function", "-DVA_BUILDING=1"]
@@ -41,8 +41,7 @@ HOST_FLAGS = ["--offload-arch=gfx950", "--cuda-host-only"]
 SOURCE_DEVICE_FLAGS = {"va_mfma_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                        "va_mfma_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                        "va_quant_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-                       "va_quant_scattered.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-                       "va_quant_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+                       "va_quant_scattered.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _run(cmd, verbose):

@@ -71,6 +71,12 @@ int plan_arguments(const void* q_dev, int64_t q_row_stride, const void* k_pool_d
                    const VaRope* rope, AttnArgs* attn, MergeArgs* merge);
 
 // The merge of partial states (viewattn.hip); `waves`: the plan header's word.
+// A planned attention's launches; keep_nan as in MergeArgs.
+int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, const void* v_pool_dev,
+                       int64_t pool_row_stride, const int32_t* plan_dev, const int32_t* plan_header_host,
+                       const int32_t* kv_indices_dev, const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
+                       int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
+                       int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, int keep_nan, void* stream);
 int launch_merge_typed(const MergeArgs& m, int dtype, int n_rows, int waves, hipStream_t stream);
 
 // Matrix-core attention (launched from va_mfma.hip).

@@ -46,13 +46,10 @@ __device__ __forceinline__ long long quant_token_row(const QuantAttnArgs& qa, in
   return ((long long)qa.a.kv_indices[kv_begin + (int)page] * qa.a.num_kv_heads + hk) * qa.pages.size + place;
 }
 
-// The matrix-core kernels, for 16-bit activations and head_dim 64, 128 or 256: wide items (va_quant_wide.hip), narrow items
-// over tiles of whole pages (va_quant_stream.hip), and narrow items whose tokens are looked up one by one
-// (va_quant_scattered.hip: pages of fewer than 16 tokens or of a number that no power of two is).  `pieces`: q rows start on
-// 16-byte boundaries, out on 8-byte ones.  n_items: the narrow ones.
-int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int n_wide, int n_wide_slots, int q_tile,
-                      hipStream_t stream);
+// The matrix-core kernels: 16-bit activations, head_dim 64, 128 or 256.  Tiles of whole pages (va_quant_stream.hip), or tokens
+// looked up one by one (va_quant_scattered.hip: pages of fewer than 16 tokens or of a number that no power of two is).
+// `pieces`: q rows start on 16-byte boundaries, out on 8-byte ones.
+int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream);
 int launch_quant_scattered(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int pieces, hipStream_t stream);
-int launch_quant_wide(const QuantAttnArgs& qa, int dtype, int code_type, int n_slots, int pieces, hipStream_t stream);
 
 }  // namespace va

@@ -221,6 +221,7 @@ extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const Va
   const int32_t* h = plan_header_host;
   if (h[VA_H_MAGIC] != VA_PLAN_MAGIC) return va_fail(VA_ERR_ARG, "plan header has no magic word");
   if (h[VA_H_N_ROWS] == 0) return VA_OK;
+  if (h[VA_H_N_WIDE] != 0) return va_fail(VA_ERR_ARG, "a plan over a quantised pool has no wide items (wide_tile < 0)");
   va::QuantAttnArgs qa;
   va::MergeArgs m;
   rc = va::plan_arguments(q_dev, q_row_stride, pool->k_codes_dev, pool->v_codes_dev, 0, plan_dev, h, kv_indices_dev,
@@ -235,8 +236,7 @@ extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const Va
   const int n_items = h[VA_H_N_ITEMS];
   if (n_items > 0) {
     if (h[VA_H_KERNEL] == VA_KERNEL_MFMA)
-      rc = va::launch_quant_mfma(qa, shape->dtype, pool->code_type, n_items - h[VA_H_N_WIDE], h[VA_H_N_WIDE],
-                                 h[VA_H_N_WIDE_SLOTS], h[VA_H_Q_TILE], s);
+      rc = va::launch_quant_mfma(qa, shape->dtype, pool->code_type, n_items, h[VA_H_Q_TILE], s);
     else
       rc = pool->code_type == VA_CODE_E4M3 ? va::launch_quant_any<va::E4M3>(qa, shape->dtype, n_items, s)
                                            : va::launch_quant_any<va::INT8>(qa, shape->dtype, n_items, s);

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
 
   const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
   using Words = const __attribute__((address_space(4))) int32_t*;
-  const Words item = (Words)a.narrow_items + (long long)where.item * VA_ITEM_WORDS;
+  const Words item = (Words)a.items + (long long)where.item * VA_ITEM_WORDS;
   const int n_q = item[VA_I_N_Q], n_links = item[VA_I_N_LINKS], part_base = item[VA_I_PART_BASE];
   if (n_q == 0) return;  // padding item: keeps the launch order aligned with the die round-robin
   const int hk = where.head, G = a.num_q_heads / a.num_kv_heads;

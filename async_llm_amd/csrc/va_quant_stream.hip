@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
   char* lds = (char*)smem;
 
   const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
-  const Words item = (Words)a.narrow_items + (long long)where.item * VA_ITEM_WORDS;
+  const Words item = (Words)a.items + (long long)where.item * VA_ITEM_WORDS;
   const int n_q = item[VA_I_N_Q], n_links = item[VA_I_N_LINKS], link_begin = item[VA_I_LINK_BEGIN], part_base = item[VA_I_PART_BASE];
   if (n_q == 0) return;  // padding item: keeps the launch order aligned with the die round-robin
   const int hk = where.head, G = a.num_q_heads / a.num_kv_heads;
@@ -361,8 +361,7 @@ static int launch_quant_stream_coded(const QuantAttnArgs& qa, int dtype, int n_i
   }
 }
 
-int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int n_wide, int n_wide_slots, int q_tile,
-                      hipStream_t stream) {
+int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream) {
   const AttnArgs& a = qa.a;
   const int g = a.num_q_heads / a.num_kv_heads;
   if (!va_mfma_supported(dtype, a.head_dim, g))
@@ -375,14 +374,7 @@ int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_i
   // queries and results in 16-byte (8-byte) accesses where their addresses allow it
   const int pieces = a.q_row_stride % 8 == 0 && (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.out % 8 == 0;
   // The choice hangs on the page size alone, so that a recorded launch keeps its kernel.
-  if (qa.pages.shift < 4) {
-    if (n_wide > 0) return va_fail(VA_ERR_ARG, "a plan over pages of %d tokens has no wide items (wide_tile < 0)", a.page_size);
-    return launch_quant_scattered(qa, dtype, code_type, n_items, pieces, stream);
-  }
-  if (n_wide > 0 && n_wide_slots > 0) {
-    const int rc = launch_quant_wide(qa, dtype, code_type, n_wide_slots, pieces, stream);
-    if (rc || n_items == 0) return rc;
-  }
+  if (qa.pages.shift < 4) return launch_quant_scattered(qa, dtype, code_type, n_items, pieces, stream);
   return code_type == VA_CODE_E4M3 ? launch_quant_stream_coded<E4M3>(qa, dtype, n_items, pieces, stream)
                                    : launch_quant_stream_coded<INT8>(qa, dtype, n_items, pieces, stream);
 }

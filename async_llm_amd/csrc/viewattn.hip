@@ -847,7 +847,6 @@ int plan_arguments(const void* q_dev, int64_t q_row_stride, const void* k_pool_d
   a.v_pool = v_pool_dev;
   a.pool_row_stride = pool_row_stride;
   a.items = plan_dev + h[VA_H_OFF_ITEMS];
-  a.narrow_items = a.items + (long long)h[VA_H_N_WIDE] * VA_ITEM_WORDS;
   a.links = plan_dev + h[VA_H_OFF_LINKS];
   a.qrefs = plan_dev + h[VA_H_OFF_QREFS];
   a.qref_rows = plan_dev + h[VA_H_OFF_QREF_ROWS];
@@ -887,13 +886,14 @@ int plan_arguments(const void* q_dev, int64_t q_row_stride, const void* k_pool_d
 
 // Both attention entry points: `workspace_dev` is the caller's buffer (va_attention) or this
 // device's copy of the library's own scratch array (va_attention_static).
-static int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev,
+namespace va {
+int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev,
                               const void* v_pool_dev, int64_t pool_row_stride, const int32_t* plan_dev,
                               const int32_t* plan_header_host, const int32_t* kv_indices_dev,
                               const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
                               int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2,
                               void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
-                              const VaRope* rope, void* stream) {
+                              const VaRope* rope, int keep_nan, void* stream) {
   if (!shape || !plan_header_host || !plan_dev) return va_fail(VA_ERR_ARG, "null plan or shape");
   const int32_t* h = plan_header_host;
   if (h[VA_H_MAGIC] != VA_PLAN_MAGIC) return va_fail(VA_ERR_ARG, "plan header has no magic word");
@@ -905,6 +905,7 @@ static int attention_launches(const void* q_dev, int64_t q_row_stride, const voi
                               sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev, lse_base2,
                               workspace_dev, workspace_bytes, shape, rope, &a, &m);
   if (rc) return rc;
+  m.keep_nan = keep_nan;
   hipStream_t s = (hipStream_t)stream;
 
   if (n_items > 0) {
@@ -921,6 +922,7 @@ static int attention_launches(const void* q_dev, int64_t q_row_stride, const voi
     rc = va::launch_merge_typed(m, shape->dtype, n_rows, h[VA_H_MERGE_WAVES], s);
   return rc;
 }
+}  // namespace va
 
 extern "C" int va_attention(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev,
                             const void* v_pool_dev, int64_t pool_row_stride, const int32_t* plan_dev,
@@ -929,9 +931,9 @@ extern "C" int va_attention(const void* q_dev, int64_t q_row_stride, const void*
                             int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2,
                             void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
                             const VaRope* rope, void* stream) {
-  return attention_launches(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, plan_header_host,
+  return va::attention_launches(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, plan_header_host,
                             kv_indices_dev, sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev,
-                            lse_base2, workspace_dev, workspace_bytes, shape, rope, stream);
+                            lse_base2, workspace_dev, workspace_bytes, shape, rope, 0, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -987,7 +989,7 @@ extern "C" int va_attention_static(const void* q_dev, int64_t q_row_stride, cons
                    plan_header_host[VA_H_N_PARTIALS], (long long)need, (long long)VA_STATIC_SCRATCH_BYTES);
   void* ptr = static_scratch_of_current_device();
   if (!ptr) return VA_ERR_HIP;
-  return attention_launches(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, plan_header_host,
+  return va::attention_launches(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, plan_header_host,
                             kv_indices_dev, sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev,
-                            lse_base2, ptr, (int64_t)VA_STATIC_SCRATCH_BYTES, shape, rope, stream);
+                            lse_base2, ptr, (int64_t)VA_STATIC_SCRATCH_BYTES, shape, rope, 0, stream);
 }

@@ -294,27 +294,28 @@ class SharedCacheAttention:
     # ------------------------------------------------------------------
     # planning
     # ------------------------------------------------------------------
-    def _plan_into_scratch(self, subs, counts, params=None) -> np.ndarray:
+    def _plan_into_scratch(self, subs, counts, params=None, shape=None) -> np.ndarray:
         """Plan into the op's host scratch (grown on demand), within the workspace once that is fixed.  The caller
         gives the scratch back (``_plan_scratch``) when it has copied the plan; without one at hand, as where another
         thread is planning, it is a new one."""
         params = self.plan_params if params is None else params
+        shape = self._shape if shape is None else shape
         limit = self._workspace.numel() if self._workspace_prepared else -1  # (an arena of no bytes is a limit too)
         try:
             scratch = self._plan_scratch.pop()
         except IndexError:
             scratch = np.empty(1 << 16, dtype=np.int32)
-        rc = native.lib.va_plan_build_within(subs, self._shape, params, limit, scratch.ctypes.data,
+        rc = native.lib.va_plan_build_within(subs, shape, params, limit, scratch.ctypes.data,
                                              scratch.size, counts)
         if rc == native.VA_ERR_CAPACITY and counts.plan_words > scratch.size:
             scratch = np.empty(2 * counts.plan_words, dtype=np.int32)
-            rc = native.lib.va_plan_build_within(subs, self._shape, params, limit, scratch.ctypes.data,
+            rc = native.lib.va_plan_build_within(subs, shape, params, limit, scratch.ctypes.data,
                                                  scratch.size, counts)
         native.check(rc)
         return scratch
 
     def _build_launch(self, qo_indptr, kv_indptr, kv_indices_host, seq_lens, flags, chain, sub_worker_host,
-                      n_rows: int, tables: Sequence, refs: list, params=None):
+                      n_rows: int, tables: Sequence, refs: list, params=None, shape=None):
         """Run the native work decomposition over the planned tables and upload the resulting plan blob
         together with ``kv_indices`` and ``tables`` (int64 arrays); returns the launch and the device tables."""
         kv_indices = np.ascontiguousarray(kv_indices_host, dtype=np.int32)
@@ -328,19 +329,20 @@ class SharedCacheAttention:
             arrays[3].ctypes.data, arrays[4].ctypes.data, arrays[5].ctypes.data,
             sw.ctypes.data if sw.size else None)
         subs._keepalive = (arrays, sw)
-        launch, (dev_indices, *dev_tables) = self._upload_plan(subs, None, refs, (kv_indices, *tables), params)
+        launch, (dev_indices, *dev_tables) = self._upload_plan(subs, None, refs, (kv_indices, *tables), params,
+                                                              shape)
         launch.kv_indices = dev_indices
         return launch, dev_tables
 
     def _upload_plan(self, subs, kv_indices_dev: Optional[torch.Tensor], refs: list, tables: Sequence,
-                     params=None):
+                     params=None, shape=None):
         """One pass of the planner: build into a scratch that is normally large enough, then copy the blob
         and ``tables`` (int32 or int64), each on a 256-byte boundary, to one pinned staging tensor and from there
         in one transfer (apart, each of three to seven tables cost a pinned allocation and a copy command).
         Plans that ``attend`` may need a second time get a tensor of their own, with room for both.  Returns the
         launch and the device copies of ``tables``."""
         counts = native.VaPlanCounts()
-        scratch = self._plan_into_scratch(subs, counts, params)
+        scratch = self._plan_into_scratch(subs, counts, params, shape)
         words = counts.plan_words
         roomy = counts.workspace_bytes > native.STATIC_SCRATCH_BYTES
         pinned = self.device.type == "cuda"

@@ -4,13 +4,19 @@
 same constructor, planners, metadata and calls.  New keys are rotated to their
 block-relative position in fp32 and quantised with their values as they are written;
 attention reads the codes and takes each row's scale into the score (K) or the weight
-(V), so nothing is read back on the way:
+(V):
 
     score(row, t) = (R(loc) q . code_k[t]) * 2^e_k[t] / sqrt(head_dim)
     out(row)      = sum_t softmax(score)(t) * 2^e_v[t] * code_v[t]
 
-Queries and weights are not rounded to the activations' type in between: a step over an
-8-bit cache differs from one over its read-back values by the rounding of the result.
+Queries and weights are not rounded to the activations' type in between: such a step
+differs from one over the read-back values by the rounding of the result.
+
+Chunks of many new tokens read a token so often that it is converted once: their pages
+are read back as float16, within range by powers of two, and the 16-bit attention's
+matrix-core kernels run over that, in float16 for bf16 activations as well (its eleven bits
+keep the operands' roundings under the result's).  Plans over a workspace reserved by
+``prepare_workspace`` never do.
 
 The reference has no such cache; its path over 16-bit pools is
 ``python/minisgl/shared_cache/attention.py:624-752``.
@@ -18,12 +24,28 @@ The reference has no such cache; its path over 16-bit pools is
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+from typing import Optional
+
 import numpy as np
 import torch
 
 from .. import native
 from ..kvcache.quantized_pool import QuantizedKVCache, store_quantized
-from .attention import SharedCacheAttention, SharedCacheAttnMetadata
+from .attention import LaunchPlan, SharedCacheAttention, SharedCacheAttnMetadata
+
+
+@dataclass
+class ReadBack:
+    """The part of a step that runs over rows read back as float16: its plan, which knows the pages by their place in the
+    scratch, and the slots that fill it."""
+
+    launch: LaunchPlan
+    first_row: int  # rows in front of it are the codes' launch
+    sub_worker: torch.Tensor
+    first_subrow: int
+    slots: torch.Tensor  # int64, of every token of every page that it reads, -1 behind the last token of a page
+    scratch: torch.Tensor
 
 
 class QuantizedCacheAttention(SharedCacheAttention):
@@ -46,8 +68,13 @@ class QuantizedCacheAttention(SharedCacheAttention):
         device = torch.device(device)
         if device.type != self.device.type or device.index not in (None, self.device.index):
             raise ValueError(f"kv_cache lives on {self.device}, the op is to run on {device}")
-        if page_size < 16 or page_size & (page_size - 1):
-            self.plan_params.wide_tile = -1  # wide tiles take their tokens in halves of sixteen that lie inside a page
+        p = self.plan_params
+        self._read_back_params = native.VaPlanParams(p.kernel, p.q_tile, p.kv_chunk, p.target_items, p.wide_tile)
+        p.wide_tile = -1  # codes are read by tiles of up to 16 rows
+        self._read_back_shape = native.make_shape(num_qo_heads, num_kv_heads, head_dim, page_size, torch.float16)
+        self._matrix_core = p.kernel != native.VA_KERNEL_GENERIC and dtype != torch.float32 and head_dim in (64, 128, 256) \
+            and num_qo_heads // num_kv_heads in (1, 2, 4, 8, 16)
+        self._scratch: Optional[torch.Tensor] = None
 
     # ------------------------------------------------------------------
     # planning
@@ -63,8 +90,60 @@ class QuantizedCacheAttention(SharedCacheAttention):
             if bad.size:
                 raise ValueError(f"{'slot' if slots[bad[0]] else 'page'} {int(kv[bad[0]])} lies outside the pool of "
                                  f"{self.kv_cache.num_pages} pages of {self.page_size} tokens")
-        return super()._build_launch(qo_indptr, kv_indptr, kv_indices_host, seq_lens, flags, chain, sub_worker_host, n_rows,
-                                     tables, refs)
+        qo, kvp = np.asarray(qo_indptr), np.asarray(kv_indptr)
+        # chains stand behind the decodes; their pages count by their place among the distinct ones
+        n_codes = int(np.argmax(np.asarray(chain) >= 0)) if len(chain) and chain[-1] >= 0 else len(chain)
+        first_entry, first_subrow = int(kvp[n_codes]), int(qo[n_codes])
+        held = np.zeros(self.kv_cache.num_pages, dtype=np.int64)  # tokens of every page that someone sees
+        if n_codes < len(chain) and self._matrix_core and not self._workspace_prepared:
+            lengths = np.asarray(seq_lens)[n_codes:]
+            for begin, end, length in zip(kvp[n_codes:], kvp[n_codes + 1:], lengths):
+                if end > begin:
+                    held[kv[begin: end - 1]] = self.page_size
+                    held[kv[end - 1]] = max(held[kv[end - 1]], length - (end - 1 - begin) * self.page_size)
+        pages = np.flatnonzero(held)
+        if not len(pages) or not self._reads_back(int((np.diff(qo[n_codes:]) * lengths).sum()), len(pages)):
+            return super()._build_launch(qo_indptr, kv_indptr, kv_indices_host, seq_lens, flags, chain, sub_worker_host,
+                                         n_rows, tables, refs)
+        places = np.cumsum(held > 0)[kv[first_entry:]] - 1
+        within = np.arange(self.page_size, dtype=np.int64)
+        slots = np.where(within < held[pages, None], pages[:, None] * self.page_size + within, -1).reshape(-1)
+        rows = np.asarray(sub_worker_host)[first_subrow:]
+        first_row = int(rows.min())
+        scratch = self._ensure_scratch(int(native.lib.va_read_back_bytes(len(slots), n_rows - first_row, self._shape)))
+        more = () if n_codes else tuple(tables)
+        wide, (dev_rows, dev_slots, *dev_tables) = super()._build_launch(
+            qo[n_codes:] - first_subrow, kvp[n_codes:] - first_entry, places, seq_lens[n_codes:], flags[n_codes:],
+            chain[n_codes:], rows - first_row, n_rows - first_row, (rows - first_row, slots, *more), refs,
+            self._read_back_params, self._read_back_shape)
+        back = ReadBack(wide, first_row, dev_rows, first_subrow, dev_slots, scratch)
+        if n_codes:
+            launch, dev_tables = super()._build_launch(qo[: n_codes + 1], kvp[: n_codes + 1], kv[:first_entry],
+                                                       seq_lens[:n_codes], flags[:n_codes], chain[:n_codes],
+                                                       np.asarray(sub_worker_host)[:first_subrow], first_row, tables, refs)
+        else:
+            launch = LaunchPlan(wide.header, wide.blob, wide.kv_indices, wide.counts, wide.workspace)
+        launch.readback = back
+        return launch, dev_tables
+
+    def _reads_back(self, pairs: int, pages: int) -> bool:
+        """Whether the chains of a step, ``pairs`` of a row and a token that it may see, run over rows read back.
+
+        Reading back costs four launches more and 2 ns a token of 1024 elements, and takes two thirds off the products.  One
+        chunk, 32 q and 8 kv heads of 128: 256 rows over 3000 tokens 60.5 us against 58.6 over codes, 32 (48) rows over 20000
+        78 (83) against 67 (91), 8 rows over 20000 74 against 27; 8 and 8 heads: 128 (256) rows over 20000 79 (92) against 69
+        (123); 16 and 4 heads of 256: 64 rows over 20000 84 against 85; 64 and 16 heads of 64: 24 rows over 20000 82 against
+        79, 256 rows over 3000 63 against 69.  All of them change sides near 3.2e9 products, and near 128 query rows a token
+        and kv head where the tokens are many.
+        """
+        products = pairs * self.num_qo_heads * self.head_dim
+        return products >= 3 << 30 and products >= 128 * pages * self.page_size * self.num_kv_heads * self.head_dim
+
+    def _ensure_scratch(self, nbytes: int) -> torch.Tensor:
+        """Room for rows read back, shared by the op's steps like their workspace; a plan keeps the tensor it was given."""
+        if self._scratch is None or self._scratch.numel() < nbytes:
+            self._scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return self._scratch
 
     # ------------------------------------------------------------------
     # execution
@@ -98,13 +177,27 @@ class QuantizedCacheAttention(SharedCacheAttention):
             lse = torch.empty((W, Hq), dtype=torch.float32, device=self.device) if return_lse else None
         elif lse.shape != (W, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != self.device:
             raise ValueError(f"lse must be a contiguous float32 tensor [{W}, {Hq}] on {self.device}")
-        ws = launch.workspace
-        native.call_on(self.device, native.lib.va_attention_q8, q2.data_ptr(), q_stride, self.kv_cache.layer(layer_id),
-                       launch.blob.data_ptr(), launch.header_ptr, launch.kv_indices.data_ptr(), meta.sub_worker.data_ptr(),
-                       meta.sub_loc.data_ptr(), meta.sub_loc.stride(0) if meta.sub_loc.dim() == 2 else 0, out.data_ptr(),
-                       None if lse is None else lse.data_ptr(), int(lse_base2), None if ws is None else ws.data_ptr(),
-                       0 if ws is None else ws.numel(), self._shape, self._rope_descriptor(),
-                       native.current_stream_ptr(self.device))
+        stream, rope = native.current_stream_ptr(self.device), self._rope_descriptor()
+        lse_ptr = None if lse is None else lse.data_ptr()
+        axis_stride = meta.sub_loc.stride(0) if meta.sub_loc.dim() == 2 else 0
+        pool, back = self.kv_cache.layer(layer_id), launch.readback
+        if back is None or back.first_row:
+            ws = launch.workspace
+            native.call_on(self.device, native.lib.va_attention_q8, q2.data_ptr(), q_stride, pool, launch.blob.data_ptr(),
+                           launch.header_ptr, launch.kv_indices.data_ptr(), meta.sub_worker.data_ptr(),
+                           meta.sub_loc.data_ptr(), axis_stride, out.data_ptr(), lse_ptr, int(lse_base2),
+                           None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), self._shape, rope, stream)
+        if back is not None:
+            plan, item = back.launch, q2.element_size()
+            ws = plan.workspace
+            native.call_on(self.device, native.lib.va_attention_read_back_q8, q2.data_ptr() + back.first_row * q_stride * item,
+                           q_stride, pool, back.slots.data_ptr(), back.slots.numel(), plan.blob.data_ptr(), plan.header_ptr,
+                           plan.kv_indices.data_ptr(), back.sub_worker.data_ptr(),
+                           meta.sub_loc.data_ptr() + 8 * back.first_subrow, axis_stride,
+                           out.data_ptr() + back.first_row * Hq * D * item,
+                           None if lse is None else lse_ptr + 4 * back.first_row * Hq, int(lse_base2),
+                           None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), back.scratch.data_ptr(),
+                           back.scratch.numel(), self._shape, rope, stream)
         return (out, lse) if return_lse else out
 
     # ------------------------------------------------------------------

@@ -406,19 +406,42 @@ VA_API int va_copy_shift_kv_q8(const VaQuantPool* pool, int64_t code_layer_strid
 
 /*
  * va_attention_q8: va_attention over a quantised pool, with the plans of
- * va_plan_build* for the same shape; pages of fewer than 16 tokens or of a number
- * that no power of two is need params->wide_tile < 0 (no wide items).
+ * va_plan_build* for the same shape and params->wide_tile < 0 (no wide items).
  * kv_indices of VA_SUB_SLOTS sub-requests are token slots of the pool.  Queries
- * are rotated in fp32 and enter the products unrounded (vector-ALU kernel), as
- * sums of two bf16 numbers (narrow items of the matrix-core plans: an error of 2^-17
- * of each element) or as float16 numbers (wide items: 2^-11), and so do the weights
- * of the second product.
+ * are rotated in fp32 and enter the products unrounded (vector-ALU kernel) or as
+ * sums of two bf16 numbers (matrix-core kernel: error 2^-17 of each element), and
+ * so do the weights of the second product.
  */
 VA_API int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
                     const int32_t* plan_header_host, const int32_t* kv_indices_dev,
                     const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
                     void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
                     int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream);
+
+/*
+ * va_attention_read_back_q8: the same for many new tokens, which read a token so
+ * often that it is converted once: the rows of slots_dev[0 .. n_slots) are read
+ * back as float16 into a scratch pool, and va_attention runs over that with wide
+ * items.  The plan and kv_indices count pages (slots) of the scratch: its slot i
+ * holds the pool's slot slots_dev[i]; slots outside the pool (those behind the
+ * last token of a page) hold zeros.  Keys and values are scaled by powers of two that
+ * bring the largest row near the upper end of float16, queries by the inverse of the
+ * keys' and results by that of the values'.  Queries (rotated), weights and results are
+ * rounded to float16, with absolute errors of 2^-39 of the largest value for results;
+ * a key or value row of NaN makes NaN of the results and the lse of those that see it;
+ * query elements of |q_i| max|K| > 1.0e7 are held at that.  16-bit activations, head_dim
+ * 64, 128 or 256, and the matrix-core plans only (the plan is built for VA_F16).
+ * scratch_dev, on a 256-byte
+ * boundary, must hold va_read_back_bytes(n_slots, rows of the plan, shape).
+ */
+VA_API int64_t va_read_back_bytes(int64_t n_slots, int64_t n_rows, const VaShape* shape);
+VA_API int va_attention_read_back_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool,
+                              const int64_t* slots_dev, int64_t n_slots, const int32_t* plan_dev,
+                              const int32_t* plan_header_host, const int32_t* kv_indices_dev,
+                              const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
+                              int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2,
+                              void* workspace_dev, int64_t workspace_bytes, void* scratch_dev,
+                              int64_t scratch_bytes, const VaShape* shape, const VaRope* rope, void* stream);
 
 #ifdef __cplusplus
 }

@@ -13,6 +13,8 @@ from async_llm_amd.shared_cache import CacheBlock, QuantizedCacheAttention
 LIMIT = {torch.float8_e4m3fn: 1.875 * 2.0**127, torch.int8: 127 * 2.0**121}  # what a code may stand for in 32 bits
 LARGEST = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
 EPS = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}  # half a step, of the value
+OPERAND = {False: 2.0**-17, True: 2.0**-11}  # of queries and weights: sums of two bf16 numbers, or float16
+HALF_KEY = {torch.float8_e4m3fn: -1, torch.int8: 1}  # log2 of what a code of the largest scale counts as float16 key
 
 
 # ---------------------------------------------------------------------------
@@ -39,6 +41,23 @@ def values64(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     b = scales.view(torch.uint8).double()
     v = codes.float().double() * torch.pow(2.0, b - 127)[..., None]
     return torch.where((b == 255)[..., None], math.nan, v)
+
+
+def write(pool: QuantizedKVCache, which: int, layer: int, slots, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """Put ``codes [n, kv_heads, head_dim]`` and their scale bytes into slots."""
+    s = torch.as_tensor(slots, dtype=torch.int64)
+    page, place = s // pool.page_size, s % pool.page_size
+    for tensor, x in (((pool.k_codes, pool.v_codes)[which](layer), codes), ((pool.k_scales, pool.v_scales)[which](layer), scales)):
+        held = tensor.view(torch.uint8).cpu()
+        held[page, :, place] = x.view(torch.uint8)
+        tensor.view(torch.uint8).copy_(held)
+
+
+def scales_of(pool: QuantizedKVCache, which: int, layer: int, slots) -> torch.Tensor:
+    scales = (pool.k_scales, pool.v_scales)[which](layer).cpu().view(torch.uint8)
+    s = torch.as_tensor(slots, dtype=torch.int64)
+    page, place = s // pool.page_size, s % pool.page_size
+    return scales[page, :, place]
 
 
 def rows64(pool: QuantizedKVCache, which: int, layer: int, slots) -> torch.Tensor:
@@ -156,19 +175,27 @@ def slots_of(block, tokens=None):
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
-def attention64(op, q: torch.Tensor, segments, layer=0, operand=2.0**-17):
+def attention64(op, q: torch.Tensor, segments, layer=0, half=False):
     """One request: ``q [rows, Hq, D]``; ``segments``: ``(slots, positions [rows] or [3, rows], first)`` where token t of
     a segment is visible to row i iff t <= first + i.  Returns out ``[rows, Hq * D]``, lse ``[rows, Hq]`` and the bound of
-    score errors where an operand that is no code is off by ``operand`` of itself, and the weighted values."""
+    score errors, where a query element is off by 2^-17 of itself or, ``half``, by a rounding to float16, and the weighted
+    values."""
     S, Hq, D = q.shape
     Hkv = op.num_kv_heads
     G = Hq // Hkv
+    operand, least = OPERAND[half], 0.0
+    if half:
+        # q' = q 2^(top - 127 - shift) with the largest scale byte of the keys among the rows; below 2^-14 its steps are
+        # even, and it is rounded twice (as it is, and rotated)
+        sizes_of = torch.cat([scales_of(op.kv_cache, 0, layer, slots).flatten() for slots, _, _ in segments]).int()
+        top = max([1] + sizes_of[sizes_of != 255].tolist())
+        least = 2.0 ** (-13 - (top - 127 - HALF_KEY[op.kv_cache.code_dtype]))
     scores, sizes, values = [], [], []
     for slots, where, first in segments:
         k, v = rows64(op.kv_cache, 0, layer, slots), rows64(op.kv_cache, 1, layer, slots)
         r = rotated(op, q, where).view(S, Hkv, G, D)
         x = torch.einsum("shgd,thd->hsgt", r, k) / math.sqrt(D)
-        size = torch.einsum("shgd,thd->hsgt", r.abs(), k.abs()) / math.sqrt(D)
+        size = torch.einsum("shgd,thd->hsgt", r.abs().clamp(min=least), k.abs()) / math.sqrt(D)
         hidden = torch.arange(len(slots))[None, :] > first + torch.arange(S)[:, None]
         scores.append(x.masked_fill(hidden[None, :, None], -math.inf))
         sizes.append(size.masked_fill(hidden[None, :, None], 0.0))
@@ -185,12 +212,18 @@ def attention64(op, q: torch.Tensor, segments, layer=0, operand=2.0**-17):
     return out, lse.permute(1, 0, 2).reshape(S, Hq), off, weight
 
 
-def assert_attends(out, lse, expected, dtype, tokens, operand=2.0**-17):
-    """|out - out64| <= rounding of the result + (2 * score error + rounding of a weight + sums of 32 bits) * sum p|v|."""
+def assert_attends(out, lse, expected, dtype, tokens, half=None):
+    """|out - out64| <= rounding of the result + (2 * score error + rounding of a weight + sums of 32 bits) * sum p|v|.
+
+    ``half`` marks the rows [rows] that ran in float16 (a number: the largest value's magnitude; 0 others): results are
+    rounded to that first, by 2^-11 of themselves or 2^-39 of that, and weights by 2^-11 of themselves or 2^-25 each."""
     o, l, off, weight = expected
+    half = (torch.zeros(o.shape[0]) if half is None else half)[:, None]
+    operand = torch.where(half > 0, OPERAND[True], OPERAND[False])
     got = out.detach().cpu().double()
     relative = (2 * off + operand + (tokens + 64) * 2.0**-24).repeat_interleave(o.shape[1] // off.shape[1], dim=1)
-    room = EPS[dtype] * o.abs() + weight * relative * (1 + EPS[dtype]) + 2.0**-24
+    room = EPS[dtype] * o.abs() + weight * relative * (1 + EPS[dtype]) + (2.0**-24 if dtype == torch.float16 else 2.0**-126)
+    room = room + (half > 0) * 2.0**-11 * o.abs() * (1 + EPS[dtype]) + half * (2.0**-39 + tokens * 2.0**-25)
     assert got.shape == o.shape
     worst = ((got - o).abs() - room).max().item()
     assert worst <= 0, f"out is {worst:.3e} further off than rounding explains"

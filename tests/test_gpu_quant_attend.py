@@ -16,13 +16,17 @@ BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 def check(op, step, q, first, rows, out, lse, layer=0):
     Hq, D = op.num_qo_heads, op.head_dim
     parts = []
-    # (tiles of many rows take queries and weights as single float16 numbers)
-    operand = 2.0**-11 if step.meta.launch.counts.n_wide_items else 2.0**-17
+    back = step.meta.launch.readback  # rows from there on ran over float16
+    half = torch.zeros(out.shape[0], dtype=torch.float64)
+    largest = max([Q.rows64(op.kv_cache, 1, layer, s[0]).abs().max().item() for segments in step.segments for s in segments if len(s[0])])
     for segments, at, n in zip(step.segments, first, rows):
-        parts.append(Q.attention64(op, q[at: at + n].cpu().view(n, Hq, D), segments, layer, operand))
+        in_half = back is not None and at >= back.first_row
+        parts.append(Q.attention64(op, q[at: at + n].cpu().view(n, Hq, D), segments, layer, in_half))
+        if in_half:
+            half[at: at + n] = largest
     expected = tuple(torch.cat(x) for x in zip(*parts))
     tokens = max(sum(len(s[0]) for s in segments) for segments in step.segments)
-    Q.assert_attends(out, lse, expected, op.dtype, tokens, operand)
+    Q.assert_attends(out, lse, expected, op.dtype, tokens, half)
 
 
 DECODES = [
@@ -89,17 +93,55 @@ PREFILLS = [
 ]
 
 
-@pytest.mark.parametrize("heads,page,dtype,codes,mrope,context,requests", PREFILLS)
-def test_prefill(heads, page, dtype, codes, mrope, context, requests):
+@pytest.mark.parametrize("heads,page,dtype,codes,mrope,context,requests,back",
+                         [(*p, back) for p in PREFILLS for back in (False, True)
+                          if not back or (p[2] != F32 and p[0][0] // p[0][1] != 3)])  # (no matrix-core kernel for these)
+def test_prefill(heads, page, dtype, codes, mrope, context, requests, back, monkeypatch):
     num_pages = -(-(sum(context) + sum(h + n for h, n in requests)) // page) + 12
     op, pool, g = Q.make(DEV, heads, page, num_pages, dtype, codes, min(heads[2], 128) if mrope else None, mrope)
     pages = Q.Pages(num_pages, page)
     blocks = [pages.block(DEV, n, span=n - n // 4 if mrope else None) for n in context]
+    monkeypatch.setattr(op, "_reads_back", lambda pairs, pages: back)
     step = Q.prefill_step(op, [(blocks, pages.block(DEV, h, room=n), n) for h, n in requests], three=mrope is not None)
+    assert (step.meta.launch.readback is not None) == back
     new = [n for _, n in requests]
     q = torch.randn(sum(new), heads[0] * heads[2], generator=g).to(dtype).to(DEV)
     out, lse = op.attend(q, 0, step.meta, return_lse=True)
     check(op, step, q, [sum(new[:r]) for r in range(len(new))], new, out, lse)
+
+
+def test_large_chunks_are_read_back_and_small_ones_are_not():
+    op, pool, g = Q.make(DEV, (32, 8, 128), 16, 260, BF16, E4M3)
+    pages = Q.Pages(260, 16)
+    context = [pages.block(DEV, 3210)]
+    for new, back in ((16, False), (300, True)):
+        step = Q.prefill_step(op, [(context, pages.block(DEV, 5, room=new), new)])
+        assert (step.meta.launch.readback is not None) == back
+        q = torch.randn(new, 32 * 128, generator=g).to(BF16).to(DEV)
+        out, lse = op.attend(q, 0, step.meta, return_lse=True)
+        check(op, step, q, [0], [new], out, lse)
+
+
+@pytest.mark.parametrize("codes", [E4M3, INT8])
+def test_rows_read_back_over_a_wide_range(codes):
+    """Keys and values far from one, and among them rows that are far smaller: float16 alone would lose them."""
+    op, pool, g = Q.make(DEV, (8, 2, 64), 16, 40, BF16, codes)
+    pages = Q.Pages(40, 16)
+    op._reads_back = lambda pairs, pages: True
+    for k_size, v_size, q_size in ((2.0**20, 2.0**-40, 2.0**-20), (2.0**-60, 2.0**50, 2.0**55), (2.0**10, 2.0**-100, 2.0**-9)):
+        block, own = pages.block(DEV, 100), pages.block(DEV, 3, room=20)
+        slots = torch.cat([Q.slots_of(block), Q.slots_of(own, 23)])
+        spread = 2.0 ** -torch.randint(0, 12, (123, 1, 1), generator=g)
+        k = torch.randn(123, 2, 64, generator=g) * k_size * spread
+        v = torch.randn(123, 2, 64, generator=g) * v_size * spread
+        for which, x in enumerate((k, v)):
+            c, s = Q.quantised32(x, codes)
+            Q.write(pool, which, 0, slots, c, s)
+        step = Q.prefill_step(op, [([block], own, 20)])
+        q = (torch.randn(20, 8 * 64, generator=g) * q_size).to(BF16).to(DEV)
+        out, lse = op.attend(q, 0, step.meta, return_lse=True)
+        check(op, step, q, [0], [20], out, lse)
+        pages = Q.Pages(40, 16)
 
 
 def test_queries_on_rows_apart_and_given_outputs():
@@ -142,6 +184,28 @@ def test_a_row_that_is_not_finite_reaches_those_that_see_it(which, dtype):
     assert torch.isnan(out[0, 4:]).all() and torch.isfinite(out[0, :4]).all() and torch.isfinite(out[1:]).all()
     assert torch.isnan(lse[0, 4:]).all() if which == 0 else torch.isfinite(lse).all()
     assert torch.isfinite(lse[0, :4]).all() and torch.isfinite(lse[1:]).all()
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_row_that_is_not_finite_in_a_chunk(which, back):
+    """Rows of the chunk in front of it and other requests never see it; those behind it do, in its kv head."""
+    op, pool, g = Q.make(DEV, (8, 2, 128), 16, 400, BF16, E4M3)
+    op._reads_back = lambda pairs, pages: back
+    pages = Q.Pages(400, 16)
+    context = [pages.block(DEV, 1500)]
+    own, other = pages.block(DEV, 7, room=90), pages.block(DEV, 0, room=33)
+    step = Q.prefill_step(op, [(context, own, 90), (context, other, 33)])
+    at = Q.slots_of(own, 97)[50].item()  # row 43 of the first chunk
+    codes, scales = (pool.k_codes, pool.v_codes)[which](0), (pool.k_scales, pool.v_scales)[which](0)
+    codes.view(torch.uint8)[at // 16, 1, at % 16] = 0
+    scales.view(torch.uint8)[at // 16, 1, at % 16] = 255
+    q = torch.randn(123, 1024, generator=g).to(BF16).to(DEV)
+    out, lse = op.attend(q, 0, step.meta, return_lse=True)
+    out, seen = out.view(123, 8, 128), torch.zeros(123, 8, dtype=torch.bool, device=DEV)
+    seen[43:90, 4:] = True
+    assert torch.equal(torch.isnan(out), seen[..., None].expand(out.shape)) and not torch.isinf(out).any()
+    assert torch.equal(torch.isnan(lse), seen if which == 0 or back else torch.zeros_like(seen))
 
 
 def test_a_step_stores_and_attends():
