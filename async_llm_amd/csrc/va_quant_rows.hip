@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256) void quant_load_kernel(LoadArgs a, int per_hea
   S* out = (S*)(which ? a.out[1] : a.out[0]) + row * a.out_stride + (long long)h * a.head_dim + d0;
   if (((uintptr_t)out & 15) == 0) {
 #pragma unroll
-    for (int i = 0; i < (int)(8 * sizeof(S) / 16); ++i) ((uint4*)out)[i] = y.raw[i];
+    for (int i = 0; i < (int)(8 * sizeof(S) / 16); ++i) __builtin_nontemporal_store(__builtin_bit_cast(va_u32x4, y.raw[i]), (va_u32x4*)out + i);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) out[k] = y.e[k];
@@ -276,7 +276,7 @@ static int launch_quant_load(const LoadArgs& a_in, hipStream_t stream) {
 // copy with a shift
 // ---------------------------------------------------------------------------
 constexpr int kQuantCopyTokens = 16;  // tokens per workgroup
-constexpr int kQuantCopyBatch = 4;    // tokens whose loads are in flight together
+constexpr int kQuantCopyBatch = 4;    // heads whose loads are in flight together
 
 struct QuantCopyArgs {
   uint8_t* codes[2];
@@ -292,62 +292,73 @@ struct QuantCopyArgs {
   RopeDev rope;
 };
 
-// A workgroup moves kQuantCopyTokens tokens of a layer.  As in the store a row is kD / 16 neighbouring lanes; a thread
-// keeps its place in the row and walks the tokens with it, so the turns of its pairs, the same for every token, stay in
-// registers.  kTurn: keys are rotated (rotary_dim a multiple of 16); otherwise they move code for code like the values.
+// A workgroup moves the keys (blockIdx.z 0) or values (1) of kQuantCopyTokens tokens of a layer.  As in the store a row is
+// kD / 16 neighbouring lanes; a thread keeps its token and its place in the row, so the slots and the turns of its pairs
+// are looked up once, and walks the heads: neighbouring rows of a wave are neighbouring tokens of a page, one run of
+// memory.  kTurn: keys are rotated (rotary_dim a multiple of 16); otherwise they move code for code like the values.
 template <typename C, int kD, bool kTurn>
 __global__ __launch_bounds__(256) void quant_copy_kernel(QuantCopyArgs a) {
-  constexpr int kLanes = kD / 16;
-  const long long layer = blockIdx.y, t0 = (long long)blockIdx.x * kQuantCopyTokens;
-  const int n_tok = (int)min((long long)kQuantCopyTokens, a.n_tokens - t0);
-  const int tasks = 2 * a.num_kv_heads * kLanes;
-  for (int task = threadIdx.x; task < tasks; task += blockDim.x) {
-    const int which = task >= a.num_kv_heads * kLanes, h = task / kLanes - (which ? a.num_kv_heads : 0), x = task % kLanes;
-    uint8_t* codes = (which ? a.codes[1] : a.codes[0]) + layer * a.code_layer_stride;
-    uint8_t* scales = (which ? a.scales[1] : a.scales[0]) + layer * a.scale_layer_stride;
-    const bool turns = kTurn && !which && x < a.rope.rotary_dim / 16;
-    const int d0 = turns ? 8 * x : 16 * x, d1 = turns ? 8 * x + a.rope.half : 16 * x + 8;
-    float c[8], s[8];
-    if (turns) turns8(a.rope, Pos3{a.shift, a.shift, a.shift}, d0, c, s);
-    for (int b = 0; b < n_tok; b += kQuantCopyBatch) {
-      long long from[kQuantCopyBatch], to[kQuantCopyBatch];
-      uint2 lo[kQuantCopyBatch], hi[kQuantCopyBatch];
-      uint32_t e[kQuantCopyBatch];
+  constexpr int kLanes = kD / 16, kHeads = 256 / kLanes / kQuantCopyTokens;  // heads side by side
+  const int x = threadIdx.x % kLanes, which = blockIdx.z;
+  const long long layer = blockIdx.y, i = (long long)blockIdx.x * kQuantCopyTokens + threadIdx.x / kLanes % kQuantCopyTokens;
+  if (i >= a.n_tokens) return;  // (whole rows leave)
+  const long long src = a.src[i], dst = a.dst[i];
+  if (src < 0 || src >= (long long)a.num_slots || dst < 0 || dst >= (long long)a.num_slots) return;
+  uint8_t* codes = (which ? a.codes[1] : a.codes[0]) + layer * a.code_layer_stride;
+  uint8_t* scales = (which ? a.scales[1] : a.scales[0]) + layer * a.scale_layer_stride;
+  const long long from = quant_row(a.pages, (uint32_t)src, 0, a.num_kv_heads), to = quant_row(a.pages, (uint32_t)dst, 0, a.num_kv_heads);
+  const int first = threadIdx.x / (kLanes * kQuantCopyTokens);
+  if (!kTurn || which) {
+    for (int h0 = first; h0 < a.num_kv_heads; h0 += kQuantCopyBatch * kHeads) {
+      uint4 row[kQuantCopyBatch];
+      uint8_t e[kQuantCopyBatch];
 #pragma unroll
       for (int u = 0; u < kQuantCopyBatch; ++u) {
-        const long long i = t0 + min(b + u, n_tok - 1), src = a.src[i], dst = a.dst[i];
-        const bool live = b + u < n_tok && src >= 0 && src < (long long)a.num_slots && dst >= 0 && dst < (long long)a.num_slots;
-        from[u] = live ? quant_row(a.pages, (uint32_t)src, h, a.num_kv_heads) : -1;
-        to[u] = live ? quant_row(a.pages, (uint32_t)dst, h, a.num_kv_heads) : -1;
+        const long long r = from + (long long)min(h0 + u * kHeads, a.num_kv_heads - 1) * a.pages.size;
+        row[u] = *(const uint4*)(codes + r * kD + 16 * x);
+        e[u] = scales[r];
       }
 #pragma unroll
       for (int u = 0; u < kQuantCopyBatch; ++u) {
-        lo[u] = hi[u] = make_uint2(0, 0);
-        e[u] = 1;
-        if (from[u] >= 0) {
-          lo[u] = *(const uint2*)(codes + from[u] * kD + d0);
-          hi[u] = *(const uint2*)(codes + from[u] * kD + d1);
-          e[u] = scales[from[u]];
-        }
+        if (h0 + u * kHeads >= a.num_kv_heads) break;
+        const long long r = to + (long long)(h0 + u * kHeads) * a.pages.size;
+        *(uint4*)(codes + r * kD + 16 * x) = row[u];
+        if (x == 0) scales[r] = e[u];
       }
+    }
+    return;
+  }
+  const bool turns = x < a.rope.rotary_dim / 16;
+  const int d0 = turns ? 8 * x : 16 * x, d1 = turns ? 8 * x + a.rope.half : 16 * x + 8;
+  float c[8], s[8];
+  if (turns) turns8(a.rope, Pos3{a.shift, a.shift, a.shift}, d0, c, s);
+  for (int h0 = first; h0 < a.num_kv_heads; h0 += kQuantCopyBatch * kHeads) {
+    uint2 lo[kQuantCopyBatch], hi[kQuantCopyBatch];
+    uint32_t e[kQuantCopyBatch];
 #pragma unroll
-      for (int u = 0; u < kQuantCopyBatch; ++u) {
-        if (kTurn && !which) {
-          float p[8], q[8];
-          const float f = scale_value(e[u]);
-          C::unpack4(lo[u].x, p), C::unpack4(lo[u].y, p + 4), C::unpack4(hi[u].x, q), C::unpack4(hi[u].y, q + 4);
+    for (int u = 0; u < kQuantCopyBatch; ++u) {
+      const long long r = from + (long long)min(h0 + u * kHeads, a.num_kv_heads - 1) * a.pages.size;
+      lo[u] = *(const uint2*)(codes + r * kD + d0);
+      hi[u] = *(const uint2*)(codes + r * kD + d1);
+      e[u] = scales[r];
+    }
 #pragma unroll
-          for (int k = 0; k < 8; ++k) p[k] *= f, q[k] *= f;
-          if (turns) turn8(c, s, p, q);
-          e[u] = scale_of<C>(top_of_row<kLanes>(max(top8(p), top8(q))));
-          lo[u] = codes8<C>(p, e[u]);
-          hi[u] = codes8<C>(q, e[u]);
-        }
-        if (to[u] >= 0) {
-          *(uint2*)(codes + to[u] * kD + d0) = lo[u];
-          *(uint2*)(codes + to[u] * kD + d1) = hi[u];
-          if (x == 0) scales[to[u]] = (uint8_t)e[u];
-        }
+    for (int u = 0; u < kQuantCopyBatch; ++u) {
+      const int h = h0 + u * kHeads;
+      float p[8], q[8];
+      const float f = scale_value(e[u]);
+      C::unpack4(lo[u].x, p), C::unpack4(lo[u].y, p + 4), C::unpack4(hi[u].x, q), C::unpack4(hi[u].y, q + 4);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) p[k] *= f, q[k] *= f;
+      if (turns) turn8(c, s, p, q);
+      e[u] = scale_of<C>(top_of_row<kLanes>(max(top8(p), top8(q))));
+      lo[u] = codes8<C>(p, e[u]);
+      hi[u] = codes8<C>(q, e[u]);
+      if (h < a.num_kv_heads) {
+        const long long r = to + (long long)h * a.pages.size;
+        *(uint2*)(codes + r * kD + d0) = lo[u];
+        *(uint2*)(codes + r * kD + d1) = hi[u];
+        if (x == 0) scales[r] = (uint8_t)e[u];
       }
     }
   }
@@ -419,8 +430,7 @@ static int launch_quant_copy(const QuantCopyArgs& a, int head_dim, int num_layer
   }
   const long long groups = (a.n_tokens + kQuantCopyTokens - 1) / kQuantCopyTokens;
   if (groups > 0x7fffffffLL) return va_fail(VA_ERR_ARG, "too many tokens for one launch");
-  const int tasks = 2 * a.num_kv_heads * (head_dim / 16);
-  const dim3 grid((unsigned)groups, (unsigned)num_layers), block((unsigned)(tasks < 256 ? (tasks + 63) / 64 * 64 : 256));
+  const dim3 grid((unsigned)groups, (unsigned)num_layers, 2), block(256);
   switch (head_dim) {
 #define VA_CASE(D)                                                                            \
   case D:                                                                                     \
