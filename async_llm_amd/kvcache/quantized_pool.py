@@ -57,6 +57,7 @@ class QuantizedKVCache:
             raise ValueError("codes must start on a 16-byte boundary")
         self._codes, self._scales, self._dtype = codes, scales.view(torch.uint8), dtype
         self._shape = native.make_shape(self._num_kv_heads, self._num_kv_heads, self._head_dim, self._page_size, dtype)
+        self._device = codes.device  # (asking the tensor costs a launch's arguments their time)
         # the descriptions of the layers' arrays, made once: addresses do not change
         c, s = codes.data_ptr(), scales.data_ptr()
         self.code_layer_bytes = self._num_pages * self._num_kv_heads * self._page_size * self._head_dim
@@ -121,7 +122,7 @@ class QuantizedKVCache:
 
     @property
     def device(self) -> torch.device:
-        return self._codes.device
+        return self._device
 
     @property
     def dtype(self) -> torch.dtype:
@@ -158,32 +159,36 @@ _NO_ROPE = native.VaRope(native.VA_ROPE_TABLE, 0, None, 0, 0, 0, None)
 def store_quantized(pool: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, layer_id: int,
                     positions: Optional[torch.Tensor], rope: Optional[native.VaRope]) -> None:
     """Rotate the keys to ``positions`` (``[n]`` or ``[3, n]`` int64; ``None``: as they are), quantise and scatter."""
-    width = pool.num_kv_heads * pool.head_dim
+    width, device, dtype = pool._num_kv_heads * pool._head_dim, pool._device, pool._dtype
     n = k.shape[0]
     rows = []
     for name, x in (("k", k), ("v", v)):
-        native.require_device(x, name)
-        if x.dtype != pool.dtype or x.device != pool.device or x.shape[0] != n or x.numel() != n * width:
-            raise ValueError(f"{name} must be {n} rows of {width} {pool.dtype} elements on {pool.device}, got {x.dtype} "
+        if x.dtype != dtype or x.device != device or x.shape[0] != n or x.numel() != n * width:
+            native.require_device(x, name)
+            raise ValueError(f"{name} must be {n} rows of {width} {dtype} elements on {device}, got {x.dtype} "
                              f"{tuple(x.shape)} on {x.device}")
         if x.dim() != 2:
             x = x.reshape(n, width)
         rows.append(x if x.stride(1) == 1 else x.contiguous())
-    if out_loc.dtype not in (torch.int32, torch.int64) or out_loc.numel() != n or out_loc.device != pool.device:
-        raise ValueError(f"out_loc must be {n} int32 or int64 slots on {pool.device}, got {out_loc.numel()} {out_loc.dtype} "
+    k, v = rows
+    wide = out_loc.dtype == torch.int64
+    if not (wide or out_loc.dtype == torch.int32) or out_loc.numel() != n or out_loc.device != device:
+        raise ValueError(f"out_loc must be {n} int32 or int64 slots on {device}, got {out_loc.numel()} {out_loc.dtype} "
                          f"on {out_loc.device}")
+    native.require_device(k, "k")
     if n == 0:
         return
     out_loc = out_loc.contiguous()
-    axis_stride = 0
+    where, axis_stride = None, 0
     if positions is not None:
-        if positions.dtype != torch.int64 or positions.device != pool.device:
-            positions = positions.to(device=pool.device, dtype=torch.int64)
+        if positions.dtype != torch.int64 or positions.device != device:
+            positions = positions.to(device=device, dtype=torch.int64)
         positions = positions.contiguous()
-        if tuple(positions.shape) not in ((n,), (3, n)):
-            raise ValueError(f"positions must be [{n}] or [3, {n}], got {tuple(positions.shape)}")
-        axis_stride = n if positions.dim() == 2 else 0
-    native.call_on(pool.device, native.lib.va_store_kv_rope_q8, rows[0].data_ptr(), rows[1].data_ptr(), rows[0].stride(0),
-                   rows[1].stride(0), pool.layer(layer_id), out_loc.data_ptr(), out_loc.dtype == torch.int64,
-                   None if positions is None else positions.data_ptr(), axis_stride, n, pool._shape,
-                   _NO_ROPE if rope is None else rope, native.current_stream_ptr(pool.device))
+        if positions.numel() != n or positions.dim() != 1:
+            if tuple(positions.shape) != (3, n):
+                raise ValueError(f"positions must be [{n}] or [3, {n}], got {tuple(positions.shape)}")
+            axis_stride = n
+        where = positions.data_ptr()
+    native.call_on(device, native.lib.va_store_kv_rope_q8, k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0),
+                   pool.layer(layer_id), out_loc.data_ptr(), wide, where, axis_stride, n, pool._shape,
+                   _NO_ROPE if rope is None else rope, native.current_stream_ptr(device))
