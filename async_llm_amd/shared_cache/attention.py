@@ -34,6 +34,7 @@ import numpy as np
 import torch
 
 from .. import native
+from ..kvcache.quantized_pool import QuantizedKVCache
 from .attention_metadata import join_page_indices, page_numbers_array
 from .rope_correction import rope_rows
 
@@ -146,6 +147,8 @@ class SharedCacheAttention:
     tensors on ``device``; ``cos_sin_cache`` is the fp32 ``[max_pos, rotary_dim]``
     cos|sin table (unused when ``mrope_section`` is set)."""
 
+    _over_codes = False  # whether kv_cache is a pool of 8-bit codes
+
     def __init__(
         self,
         kv_cache,
@@ -162,6 +165,8 @@ class SharedCacheAttention:
         kernel: str | None = None,
         fused_store: bool = True,
     ) -> None:
+        if isinstance(kv_cache, QuantizedKVCache) and not self._over_codes:
+            raise TypeError("a QuantizedKVCache holds codes: attention over it is QuantizedCacheAttention")
         self.kv_cache = kv_cache
         # False: new rows reach the pool through ``kv_cache.store_kv`` as in the reference
         # (``attention.py:645-649``: rotate, then store), one launch more per step -- for a pool whose
@@ -294,6 +299,9 @@ class SharedCacheAttention:
     # ------------------------------------------------------------------
     # planning
     # ------------------------------------------------------------------
+    def _check_entries(self, kv_indices: np.ndarray, kv_indptr: np.ndarray, flags: np.ndarray) -> None:
+        """Refuse pages and slots outside the pool, where the pool says how many it has."""
+
     def _plan_into_scratch(self, subs, counts, params=None, shape=None) -> np.ndarray:
         """Plan into the op's host scratch (grown on demand), within the workspace once that is fixed.  The caller
         gives the scratch back (``_plan_scratch``) when it has copied the plan; without one at hand, as where another

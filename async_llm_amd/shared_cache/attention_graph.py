@@ -84,6 +84,7 @@ class _FixedPlanBuffers:
         indices, positions and the valid mask to their device buffers."""
         tables = [np.ascontiguousarray(a, dtype=np.int32) for a in (qo_indptr, kv_indptr, seq_lens, flags, chain)]
         sw = np.ascontiguousarray(sub_worker, dtype=np.int64)
+        self.attention._check_entries(self._kv_host.numpy()[: tables[1][-1]], tables[1], tables[3])
         subs = native.VaSubRequests(
             len(tables[2]), len(sw), n_rows, tables[0].ctypes.data, tables[1].ctypes.data,
             self._kv_host.data_ptr(), tables[2].ctypes.data, tables[3].ctypes.data, tables[4].ctypes.data,

@@ -25,6 +25,7 @@ import numpy as np
 import torch
 
 from .. import native
+from ..kvcache.quantized_pool import QuantizedKVCache
 from .shared_block import CacheBlock
 
 
@@ -54,12 +55,15 @@ class BlockKVOps:
 
     ``kv_cache`` offers ``num_layers``, ``k_cache(layer)`` and ``v_cache(layer)``
     (contiguous ``[num_pages, page_size, kv_heads, head_dim]`` tensors on the
-    GPU); ``sc_attn`` is the ``SharedCacheAttention`` whose rotation the keys were
+    GPU), or is the ``QuantizedKVCache`` of a ``QuantizedCacheAttention``, whose
+    shifted keys are quantised anew; ``sc_attn`` is the ``SharedCacheAttention`` whose rotation the keys were
     stored with; ``page_allocator`` offers ``alloc_pages(n)``.
     """
 
     def __init__(self, kv_cache, sc_attn, page_allocator,
                  compose_affines: Optional[Callable[..., Tuple[torch.Tensor, torch.Tensor]]] = None) -> None:
+        if isinstance(kv_cache, QuantizedKVCache) and getattr(sc_attn, "kv_cache", None) is not kv_cache:
+            raise ValueError("blocks of a QuantizedKVCache are moved by the QuantizedCacheAttention over it")
         self.kv_cache = kv_cache
         self.sc_attn = sc_attn
         self.page_allocator = page_allocator
@@ -192,6 +196,9 @@ class BlockKVOps:
         host = host.pin_memory()
         dev = host.to(self.device, non_blocking=True)
         self._refs = (host, dev)  # alive until the next copy on this stream has been queued
+        if isinstance(self.kv_cache, QuantizedKVCache):
+            att.copy_shifted(dev[0], dev[1], position_shift)
+            return
         L = self.kv_cache.num_layers
         k0, v0 = self.kv_cache.k_cache(0), self.kv_cache.v_cache(0)
         assert k0.is_contiguous() and v0.is_contiguous(), "pool layers must be contiguous"

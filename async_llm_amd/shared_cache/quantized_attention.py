@@ -51,6 +51,8 @@ class ReadBack:
 class QuantizedCacheAttention(SharedCacheAttention):
     """View attention over a :class:`QuantizedKVCache` whose ``dtype`` is the op's."""
 
+    _over_codes = True
+
     def __init__(self, kv_cache: QuantizedKVCache, cos_sin_cache: torch.Tensor, num_qo_heads: int, num_kv_heads: int,
                  head_dim: int, page_size: int, dtype: torch.dtype, device: torch.device, rotary_dim: int | None = None,
                  mrope_section: tuple | None = None, rope_base: float | None = None, kernel: str | None = None) -> None:
@@ -79,17 +81,21 @@ class QuantizedCacheAttention(SharedCacheAttention):
     # ------------------------------------------------------------------
     # planning
     # ------------------------------------------------------------------
+    def _check_entries(self, kv_indices, kv_indptr, flags) -> None:
+        if not kv_indices.size:
+            return
+        # page numbers, and token slots of sub-requests that list those
+        pages = self.kv_cache.num_pages
+        slots = np.repeat(flags & native.VA_SUB_SLOTS, np.diff(kv_indptr)) != 0
+        bad = np.flatnonzero((kv_indices < 0) | (kv_indices >= np.where(slots, pages * self.page_size, pages)))
+        if bad.size:
+            raise ValueError(f"{'slot' if slots[bad[0]] else 'page'} {int(kv_indices[bad[0]])} lies outside the pool of "
+                             f"{pages} pages of {self.page_size} tokens")
+
     def _build_launch(self, qo_indptr, kv_indptr, kv_indices_host, seq_lens, flags, chain, sub_worker_host, n_rows,
                       tables, refs):
         kv = np.asarray(kv_indices_host)
-        if kv.size:
-            # page numbers, and token slots of sub-requests that list those
-            slots = np.repeat(np.asarray(flags) & native.VA_SUB_SLOTS, np.diff(np.asarray(kv_indptr))) != 0
-            limit = np.where(slots, self.kv_cache.num_pages * self.page_size, self.kv_cache.num_pages)
-            bad = np.nonzero((kv < 0) | (kv >= limit))[0]
-            if bad.size:
-                raise ValueError(f"{'slot' if slots[bad[0]] else 'page'} {int(kv[bad[0]])} lies outside the pool of "
-                                 f"{self.kv_cache.num_pages} pages of {self.page_size} tokens")
+        self._check_entries(kv, np.asarray(kv_indptr), np.asarray(flags))
         qo, kvp = np.asarray(qo_indptr), np.asarray(kv_indptr)
         # chains stand behind the decodes; their pages count by their place among the distinct ones
         n_codes = int(np.argmax(np.asarray(chain) >= 0)) if len(chain) and chain[-1] >= 0 else len(chain)

@@ -235,7 +235,7 @@ def assert_attends(out, lse, expected, dtype, tokens, half=None):
         assert ((have - l).abs()[seen] <= slack[seen]).all(), "lse"
 
 
-def decode_step(op, pages, views, writers, gen, outside=()):
+def decode_step(op, pages, views, writers, gen, buffers=None):
     """Plan a decode step over ``views`` (lists of blocks) whose requests write ``writers``: metadata, and each
     request's segments for :func:`attention64`."""
     from async_llm_amd.shared_cache import WorkerGroup
@@ -248,7 +248,7 @@ def decode_step(op, pages, views, writers, gen, outside=()):
         pending[id(b)] = opened
         slots.append((b.page_starts[-1] if opened is None else opened) + b.num_tokens % P)
     slots = torch.tensor(slots, dtype=torch.int32, device=op.device)
-    meta = op.prepare(group, pending, slots)
+    meta = op.prepare(group, pending, slots, **({} if buffers is None else {"graph_buffers": buffers}))
     segments = []
     for w, view in enumerate(views):
         grown = [b.num_tokens + (id(b) in pending) for b in view]
@@ -264,7 +264,7 @@ def decode_step(op, pages, views, writers, gen, outside=()):
     return SimpleNamespace(meta=meta, segments=segments, slots=slots, positions=positions, group=group, pending=pending)
 
 
-def prefill_step(op, requests, three=False):
+def prefill_step(op, requests, three=False, buffers=None):
     """``requests``: ``(context blocks, own block with room, new)``."""
     from async_llm_amd.shared_cache import PrefillSpec
 
@@ -281,6 +281,6 @@ def prefill_step(op, requests, three=False):
         segments.append(rows)
         slots.append(slots_of(own, own.num_tokens + new)[own.num_tokens:])
         positions.append(rel + own.mrope_span)
-    meta = op.prepare_prefill_batch(specs)
+    meta = op.prepare_prefill_batch(specs, **({} if buffers is None else {"graph_buffers": buffers}))
     return SimpleNamespace(meta=meta, segments=segments, specs=specs, slots=torch.cat(slots).to(op.device),
                            positions=torch.cat(positions, dim=-1).to(op.device), new=[n for _, _, n in requests])
