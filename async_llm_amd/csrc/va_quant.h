@@ -35,12 +35,6 @@ struct E4M3 {
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.f, false)),
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.f, true))};
   }
-  static __device__ __forceinline__ va_u32x4 f16x8(va_u32x2 w) {
-    return va_u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 1.f, false)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 1.f, true)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], 1.f, false)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], 1.f, true))};
-  }
 };
 struct INT8 {
   static constexpr int kId = VA_CODE_INT8;
@@ -59,19 +53,6 @@ struct INT8 {
     float x[8];
     unpack4(w[0], x), unpack4(w[1], x + 4);
     return va_u32x4{Mma<BF16>::pack(x[0], x[1]), Mma<BF16>::pack(x[2], x[3]), Mma<BF16>::pack(x[4], x[5]), Mma<BF16>::pack(x[6], x[7])};
-  }
-  // Code + 128 as the low bits of a float16 from 1024 on, less 1152: exact, and 1.25 instructions a code.
-  static __device__ __forceinline__ va_u32x4 f16x8(va_u32x2 w) {
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    const f16x2 less = {(_Float16)1152.f, (_Float16)1152.f};
-    va_u32x4 out;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t u = w[i] ^ 0x80808080u;
-      out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - less);
-      out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - less);
-    }
-    return out;
   }
 };
 
