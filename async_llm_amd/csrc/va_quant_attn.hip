@@ -15,34 +15,75 @@ namespace va {
 // Any activation type, head_dim a power of two from 16 to 256, any number of q heads per kv head: float32 activations and
 // what the matrix-core kernel rejects.  One workgroup of four waves per (work item, kv head), tile rows one after another,
 // four q heads a pass.  A token's K (and V) row is sixteen codes for each of kD / 16 adjacent lanes, a wave takes
-// 1024 / kD tokens a step, kAhead steps are in flight together.  Every lane group keeps a softmax state of its own; they are
-// folded by shuffles and through LDS at the end of the chain.
+// 1024 / kD tokens a step and two steps together; the next two are requested before their products, the first ones before the
+// queries are rotated.  Every lane group keeps sums of its own under the wave's maxima, joined at the end of the chain.
+//
+// Small steps are a chain of trips (item, link, page, codes; row, query, turns) and a fold, so what counts is their number:
+// one row, 2 kv heads of 128 dims, 1900 tokens 8.1 us (12.7 where codes were requested behind the query, lane groups kept
+// maxima of their own and joined by shuffles); eight rows of 3000 tokens, 4 heads of 256 dims 26 (32 for the step), 32 rows
+// of 12000, 8 heads of 128 dims 320 (399): the vector ALU's products.
 constexpr int kAnyHeads = 4;
 constexpr int kAnyThreads = 256;
 constexpr int kAnyWaves = kAnyThreads / kWave;
 constexpr int kAnyAhead = 2;
 
+// Lane exchanges on the vector ALU (a shuffle is a trip through LDS).
+template <int kCtrl>
+__device__ __forceinline__ float lane_of_row(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), kCtrl, 0xf, 0xf, true));
+}
+// Sum over kLanes neighbouring lanes, in all of them: neighbours, pairs, then mirrored halves of 8 and of 16.
+template <int kLanes>
+__device__ __forceinline__ float neighbour_sum(float x) {
+  if constexpr (kLanes >= 2) x += lane_of_row<0xB1>(x);
+  if constexpr (kLanes >= 4) x += lane_of_row<0x4E>(x);
+  if constexpr (kLanes >= 8) x += lane_of_row<0x141>(x);
+  if constexpr (kLanes >= 16) x += lane_of_row<0x140>(x);
+  return x;
+}
+// f over the lanes of a row of 16 that lie a multiple of kStep apart, in all of them: rotations by kStep, twice it, ...
+template <int kStep, typename F>
+__device__ __forceinline__ float over_row(float x, F f) {
+  if constexpr (kStep <= 1) x = f(x, lane_of_row<0x121>(x));
+  if constexpr (kStep <= 2) x = f(x, lane_of_row<0x122>(x));
+  if constexpr (kStep <= 4) x = f(x, lane_of_row<0x124>(x));
+  if constexpr (kStep <= 8) x = f(x, lane_of_row<0x128>(x));
+  return x;
+}
+template <typename F>
+__device__ __forceinline__ float over_rows16(float x, F f) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
 template <int kD, typename C>
 __global__ __launch_bounds__(kAnyThreads) void attn_quant_any_kernel(QuantAttnArgs qa, int dtype) {
   const AttnArgs& a = qa.a;
+  using Words = const __attribute__((address_space(4))) int32_t*;  // read only while a launch runs
+  using Longs = const __attribute__((address_space(4))) int64_t*;
   constexpr int kVec = 16;
   constexpr int kLPT = kD / kVec;  // lanes per token
   constexpr int kTPW = kWave / kLPT;
+  static_assert(kAnyHeads == kWave / 16, "a head for each row of 16 lanes");
 
   __shared__ float q_s[kAnyHeads][kD];
-  __shared__ float acc_s[kAnyWaves][kAnyHeads][kD];
-  __shared__ float ml_s[kAnyWaves][kAnyHeads][2];
+  __shared__ __align__(16) float acc_s[kAnyWaves][kAnyHeads][kD];
+  __shared__ float m_s[kAnyWaves][kAnyHeads], l_s[kAnyWaves][kAnyHeads];
 
   const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
-  const int32_t* item = a.items + (long long)where.item * VA_ITEM_WORDS;
+  const Words item = (Words)a.items + (long long)where.item * VA_ITEM_WORDS;
   const int hk = where.head, G = a.num_q_heads / a.num_kv_heads;
   const int n_q = item[VA_I_N_Q];
   if (n_q == 0) return;  // padding item: keeps the launch order aligned with the die round-robin
-  const int part_base = item[VA_I_PART_BASE];
+  const int part_base = item[VA_I_PART_BASE], link_begin = item[VA_I_LINK_BEGIN], n_links = item[VA_I_N_LINKS];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int li = lane % kLPT, lg = lane / kLPT;
   const uint8_t* kp = (const uint8_t*)a.k_pool;
   const uint8_t* vp = (const uint8_t*)a.v_pool;
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  const auto sum = [](float x, float y) { return x + y; };
 
   for (int iq = 0; iq < n_q; ++iq) {
     long long out_row = -1;
@@ -55,15 +96,33 @@ __global__ __launch_bounds__(kAnyThreads) void attn_quant_any_kernel(QuantAttnAr
 #pragma unroll
         for (int e = 0; e < kVec; ++e) acc[g][e] = 0.f;
       }
-      for (int lk = 0; lk < item[VA_I_N_LINKS]; ++lk) {
-        const int32_t* link = a.links + (long long)(item[VA_I_LINK_BEGIN] + lk) * VA_LINK_WORDS;
-        const int lflags = link[VA_L_FLAGS];
-        const int subrow = (lflags & VA_LINK_INDIRECT) ? a.qrefs[link[VA_L_QREF] + iq] : link[VA_L_QREF] + iq;
-        const long long src_row = a.sub_worker[subrow];
-        out_row = src_row;
-        const Pos3 p = load_pos(a.sub_loc, a.sub_loc_axis_stride, subrow);
+      for (int lk = 0; lk < n_links; ++lk) {
+        const Words link = (Words)a.links + (long long)(link_begin + lk) * VA_LINK_WORDS;
+        const int lflags = link[VA_L_FLAGS], qref = link[VA_L_QREF], kv_begin = link[VA_L_KV_BEGIN];
+        const int t_end = min(link[VA_L_TOK_END], link[VA_L_CAUSAL_BASE] + iq + 1);
+        const bool slots = lflags & VA_LINK_SLOTS;
+        int t0 = link[VA_L_TOK_BEGIN] + wave * kTPW;
+        constexpr int kStep = kAnyAhead * kAnyWaves * kTPW;
+        uint4 kraw[kAnyAhead], vraw[kAnyAhead];
+        uint8_t ks[kAnyAhead], vs[kAnyAhead];
+        // (past the range the last token's rows, whose products are masked)
+        const auto request = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+          for (int u = 0; u < kAnyAhead; ++u) {
+            const long long row = quant_token_row(qa, kv_begin, min(t0 + u * kAnyWaves * kTPW + lg, t_end - 1), slots, hk);
+            kraw[u] = *(const uint4*)(kp + row * kD + li * kVec);
+            vraw[u] = *(const uint4*)(vp + row * kD + li * kVec);
+            ks[u] = qa.k_scales[row];
+            vs[u] = qa.v_scales[row];
+          }
+        };
+        if (t0 < t_end) request(t0);
 
         // this row's query for the link, rotated in fp32
+        const int subrow = (lflags & VA_LINK_INDIRECT) ? ((Words)a.qrefs)[qref + iq] : qref + iq;
+        const long long src_row = ((Longs)a.sub_worker)[subrow];
+        out_row = src_row;
+        const Pos3 p = load_pos(a.sub_loc, a.sub_loc_axis_stride, subrow);
         __syncthreads();
         for (int e = threadIdx.x; e < kAnyHeads * kD; e += kAnyThreads) {
           const int g = e / kD, d = e - g * kD;
@@ -88,91 +147,101 @@ __global__ __launch_bounds__(kAnyThreads) void attn_quant_any_kernel(QuantAttnAr
 #pragma unroll
           for (int e = 0; e < kVec; ++e) qr[g][e] = q_s[g][li * kVec + e];
 
-        const int t_end = min(link[VA_L_TOK_END], link[VA_L_CAUSAL_BASE] + iq + 1);
-        const int kv_begin = link[VA_L_KV_BEGIN];
-        const bool slots = lflags & VA_LINK_SLOTS;
-        for (int t0 = link[VA_L_TOK_BEGIN] + wave * kTPW; t0 < t_end; t0 += kAnyAhead * kAnyWaves * kTPW) {
+        for (; t0 < t_end; t0 += kStep) {
+          float sc[kAnyAhead][kAnyHeads], vscale[kAnyAhead];
+          uint4 v[kAnyAhead];
           bool live[kAnyAhead];
-          uint4 kraw[kAnyAhead], vraw[kAnyAhead];
-          float ks[kAnyAhead], vs[kAnyAhead];
 #pragma unroll
           for (int u = 0; u < kAnyAhead; ++u) {
-            const int t = t0 + u * kAnyWaves * kTPW + lg;
-            live[u] = t < t_end;
-            const long long row = quant_token_row(qa, kv_begin, live[u] ? t : t_end - 1, slots, hk);
-            kraw[u] = *(const uint4*)(kp + row * kD + li * kVec);
-            vraw[u] = *(const uint4*)(vp + row * kD + li * kVec);
-            ks[u] = scale_value(qa.k_scales[row]);
-            vs[u] = scale_value(qa.v_scales[row]);
-          }
-#pragma unroll
-          for (int u = 0; u < kAnyAhead; ++u) {
-            if (t0 + u * kAnyWaves * kTPW >= t_end) break;  // (wave-uniform: the step lies past the range)
-            float kf[kVec], vf[kVec], sc[kAnyHeads];
+            live[u] = t0 + u * kAnyWaves * kTPW + lg < t_end;
+            float kf[kVec];
             C::unpack4(kraw[u].x, kf), C::unpack4(kraw[u].y, kf + 4), C::unpack4(kraw[u].z, kf + 8), C::unpack4(kraw[u].w, kf + 12);
-            C::unpack4(vraw[u].x, vf), C::unpack4(vraw[u].y, vf + 4), C::unpack4(vraw[u].z, vf + 8), C::unpack4(vraw[u].w, vf + 12);
+            const float kscale = scale_value(ks[u]) * a.scale_log2;
 #pragma unroll
             for (int g = 0; g < kAnyHeads; ++g) {
               float d = 0.f;
 #pragma unroll
               for (int e = 0; e < kVec; ++e) d = fmaf(qr[g][e], kf[e], d);
-              d = group_sum<kLPT>(d);
-              sc[g] = live[u] ? d * (ks[u] * a.scale_log2) : -INFINITY;
+              sc[u][g] = live[u] ? neighbour_sum<kLPT>(d) * kscale : -INFINITY;
             }
+            v[u] = vraw[u];
+            vscale[u] = live[u] ? scale_value(vs[u]) : 0.f;  // (a token that the row does not see may have any scale)
+          }
+          if (t0 + kStep < t_end) request(t0 + kStep);
+          float pr[kAnyAhead][kAnyHeads];
+#pragma unroll
+          for (int g = 0; g < kAnyHeads; ++g) {
+            const float m_new = fmaxf(m[g], fmaxf(sc[0][g], sc[1][g]));
+            const float alpha = exp2f(m[g] - m_new);
+            m[g] = m_new;
+#pragma unroll
+            for (int u = 0; u < kAnyAhead; ++u) pr[u][g] = exp2f(sc[u][g] - m_new);
+            l[g] = fmaf(l[g], alpha, pr[0][g] + pr[1][g]);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) acc[g][e] *= alpha;
+          }
+#pragma unroll
+          for (int u = 0; u < kAnyAhead; ++u) {
+            float vf[kVec];
+            C::unpack4(v[u].x, vf), C::unpack4(v[u].y, vf + 4), C::unpack4(v[u].z, vf + 8), C::unpack4(v[u].w, vf + 12);
 #pragma unroll
             for (int g = 0; g < kAnyHeads; ++g) {
-              const float m_new = fmaxf(m[g], sc[g]);
-              const float alpha = exp2f(m[g] - m_new);
-              const float pr = exp2f(sc[g] - m_new), weight = live[u] ? pr * vs[u] : 0.f;
-              m[g] = m_new;
-              l[g] = l[g] * alpha + pr;
+              const float weight = pr[u][g] * vscale[u];
 #pragma unroll
-              for (int e = 0; e < kVec; ++e) acc[g][e] = fmaf(weight, vf[e], acc[g][e] * alpha);
+              for (int e = 0; e < kVec; ++e) acc[g][e] = fmaf(weight, vf[e], acc[g][e]);
             }
           }
         }
       }
 
-      // the lane groups of the wave
+      // One maximum for the workgroup, then plain sums: over the lane groups of a row of 16, then over the rows, whose
+      // swaps leave row r with head r.
 #pragma unroll
-      for (int off = kLPT; off < kWave; off <<= 1) {
-#pragma unroll
-        for (int g = 0; g < kAnyHeads; ++g) {
-          const float m_o = __shfl_xor(m[g], off, kWave), l_o = __shfl_xor(l[g], off, kWave);
-          const float m_new = fmaxf(m[g], m_o);
-          const float sa = exp2f(m[g] - m_new), sb = exp2f(m_o - m_new);
-          l[g] = l[g] * sa + l_o * sb;
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) acc[g][e] = acc[g][e] * sa + __shfl_xor(acc[g][e], off, kWave) * sb;
-          m[g] = m_new;
-        }
+      for (int g = 0; g < kAnyHeads; ++g) {
+        const float top = over_rows16(over_row<kLPT>(m[g], larger), larger);
+        if (lane == 0) m_s[wave][g] = top;
       }
       __syncthreads();
-      if (lg == 0) {
+      float top[kAnyHeads];
 #pragma unroll
-        for (int g = 0; g < kAnyHeads; ++g) {
+      for (int g = 0; g < kAnyHeads; ++g) {
+        top[g] = m_s[0][g];
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) acc_s[wave][g][li * kVec + e] = acc[g][e];
-          if (li == 0) {
-            ml_s[wave][g][0] = m[g];
-            ml_s[wave][g][1] = l[g];
-          }
+        for (int w = 1; w < kAnyWaves; ++w) top[g] = fmaxf(top[g], m_s[w][g]);
+        const float s = exp2f(m[g] - top[g]);
+        const float ll = over_rows16(over_row<kLPT>(l[g] * s, sum), sum);
+        if (lane == 0) l_s[wave][g] = ll;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) acc[g][e] *= s;
+      }
+      float mine[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        float pair[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[g][e]), __float_as_uint(acc[g + 2][e]), false, false);
+          pair[g] = __uint_as_float(r[0]) + __uint_as_float(r[1]);  // low half: head g, high half: g + 2
         }
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(pair[0]), __float_as_uint(pair[1]), false, false);
+        mine[e] = over_row<kLPT>(__uint_as_float(r[0]) + __uint_as_float(r[1]), sum);
+      }
+      if (lane % 16 < kLPT) {
+#pragma unroll
+        for (int e = 0; e < kVec; e += 4)
+          *(float4*)&acc_s[wave][lane / 16][li * kVec + e] = make_float4(mine[e], mine[e + 1], mine[e + 2], mine[e + 3]);
       }
       __syncthreads();
       // the waves
       for (int e = threadIdx.x; e < kAnyHeads * kD; e += kAnyThreads) {
         const int g = e / kD, d = e - g * kD;
         if (hb + g >= G) continue;
-        float mm = kNegBig;
-#pragma unroll
-        for (int w = 0; w < kAnyWaves; ++w) mm = fmaxf(mm, ml_s[w][g][0]);
-        float ll = 0.f, av = 0.f;
+        float ll = 0.f, av = 0.f, mm = m_s[0][g];
 #pragma unroll
         for (int w = 0; w < kAnyWaves; ++w) {
-          const float sw = exp2f(ml_s[w][g][0] - mm);
-          ll += ml_s[w][g][1] * sw;
-          av += acc_s[w][g][d] * sw;
+          mm = fmaxf(mm, m_s[w][g]);
+          ll += l_s[w][g];
+          av += acc_s[w][g][d];
         }
         const int hq = hk * G + hb + g;
         if (part_base < 0) {

@@ -167,40 +167,43 @@ class QuantizedCacheAttention(SharedCacheAttention):
         fp32 on request).  ``static_scratch`` is refused: partial states go to the op's workspace."""
         if static_scratch:
             raise ValueError("attention over a quantised pool has no static scratch: reserve a workspace with prepare_workspace")
-        native.require_device(q, "q")
-        launch = meta.launch
-        assert launch is not None, "metadata carries no launch plan"
-        W, Hq, D = meta.num_workers, self.num_qo_heads, self.head_dim
+        launch, device = meta.launch, self.device
+        W, Hq = meta.num_workers, self.num_qo_heads
+        width = Hq * self.head_dim
         q2, q_stride = self._rows(q, Hq)
-        if q2.shape[0] < W or q2.dtype != self.dtype or q2.device != self.device:
-            raise ValueError(f"q must be {W} rows of {Hq * D} {self.dtype} elements on {self.device}, got {q2.dtype} "
+        if q2.dtype != self.dtype or q2.device != device or q2.shape[0] < W:
+            native.require_device(q, "q")
+            raise ValueError(f"q must be {W} rows of {width} {self.dtype} elements on {device}, got {q2.dtype} "
                              f"{tuple(q2.shape)} on {q2.device}")
+        native.require_device(q2, "q")
+        assert launch is not None, "metadata carries no launch plan"
         if out is None:
-            out = torch.empty((W, Hq * D), dtype=self.dtype, device=self.device)
-        elif out.shape != (W, Hq * D) or out.dtype != self.dtype or not out.is_contiguous() or out.device != self.device:
-            raise ValueError(f"out must be a contiguous {self.dtype} tensor [{W}, {Hq * D}] on {self.device}")
+            out = torch.empty((W, width), dtype=self.dtype, device=device)
+        elif out.shape != (W, width) or out.dtype != self.dtype or not out.is_contiguous() or out.device != device:
+            raise ValueError(f"out must be a contiguous {self.dtype} tensor [{W}, {width}] on {device}")
         if lse is None:
-            lse = torch.empty((W, Hq), dtype=torch.float32, device=self.device) if return_lse else None
-        elif lse.shape != (W, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != self.device:
-            raise ValueError(f"lse must be a contiguous float32 tensor [{W}, {Hq}] on {self.device}")
-        stream, rope = native.current_stream_ptr(self.device), self._rope_descriptor()
+            lse = torch.empty((W, Hq), dtype=torch.float32, device=device) if return_lse else None
+        elif lse.shape != (W, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != device:
+            raise ValueError(f"lse must be a contiguous float32 tensor [{W}, {Hq}] on {device}")
+        stream, rope = native.current_stream_ptr(device), self._rope_descriptor()
         lse_ptr = None if lse is None else lse.data_ptr()
-        axis_stride = meta.sub_loc.stride(0) if meta.sub_loc.dim() == 2 else 0
+        sub_loc = meta.sub_loc
+        axis_stride = sub_loc.stride(0) if sub_loc.dim() == 2 else 0
         pool, back = self.kv_cache.layer(layer_id), launch.readback
         if back is None or back.first_row:
             ws = launch.workspace
-            native.call_on(self.device, native.lib.va_attention_q8, q2.data_ptr(), q_stride, pool, launch.blob.data_ptr(),
+            native.call_on(device, native.lib.va_attention_q8, q2.data_ptr(), q_stride, pool, launch.blob.data_ptr(),
                            launch.header_ptr, launch.kv_indices.data_ptr(), meta.sub_worker.data_ptr(),
-                           meta.sub_loc.data_ptr(), axis_stride, out.data_ptr(), lse_ptr, int(lse_base2),
+                           sub_loc.data_ptr(), axis_stride, out.data_ptr(), lse_ptr, int(lse_base2),
                            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), self._shape, rope, stream)
         if back is not None:
             plan, item = back.launch, q2.element_size()
             ws = plan.workspace
-            native.call_on(self.device, native.lib.va_attention_read_back_q8, q2.data_ptr() + back.first_row * q_stride * item,
+            native.call_on(device, native.lib.va_attention_read_back_q8, q2.data_ptr() + back.first_row * q_stride * item,
                            q_stride, pool, back.slots.data_ptr(), back.slots.numel(), plan.blob.data_ptr(), plan.header_ptr,
                            plan.kv_indices.data_ptr(), back.sub_worker.data_ptr(),
-                           meta.sub_loc.data_ptr() + 8 * back.first_subrow, axis_stride,
-                           out.data_ptr() + back.first_row * Hq * D * item,
+                           sub_loc.data_ptr() + 8 * back.first_subrow, axis_stride,
+                           out.data_ptr() + back.first_row * width * item,
                            None if lse is None else lse_ptr + 4 * back.first_row * Hq, int(lse_base2),
                            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), back.scratch.data_ptr(),
                            back.scratch.numel(), self._shape, rope, stream)
