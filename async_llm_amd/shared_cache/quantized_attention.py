@@ -86,6 +86,8 @@ class QuantizedCacheAttention(SharedCacheAttention):
             return
         # page numbers, and token slots of sub-requests that list those
         pages = self.kv_cache.num_pages
+        if kv_indices.min() >= 0 and kv_indices.max() < pages:
+            return
         slots = np.repeat(flags & native.VA_SUB_SLOTS, np.diff(kv_indptr)) != 0
         bad = np.flatnonzero((kv_indices < 0) | (kv_indices >= np.where(slots, pages * self.page_size, pages)))
         if bad.size:
