@@ -261,8 +261,8 @@ extern "C" int va_attention_read_back_q8(const void* q_dev, int64_t q_row_stride
   VaShape half = *shape;
   half.dtype = VA_F16;
   rc = va::attention_launches(a.q16, width, a.rows[0], a.rows[1], (int64_t)shape->num_kv_heads * shape->head_dim, plan_dev, h,
-                    kv_indices_dev, sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, scratch + l.out, lse_dev, lse_base2,
-                    workspace_dev, workspace_bytes, &half, rope, 1, stream);
+                              kv_indices_dev, sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, scratch + l.out, lse_dev,
+                              lse_base2, workspace_dev, workspace_bytes, &half, rope, 1, stream);
   if (rc) return rc;
   const __half* from = (const __half*)(scratch + l.out);
   return e4m3 ? va::launch_quant_results<va::E4M3>(from, out_dev, lse_dev, a.tops, n_rows * width, shape->head_dim, shape->dtype, s)

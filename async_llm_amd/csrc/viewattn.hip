@@ -882,28 +882,23 @@ int plan_arguments(const void* q_dev, int64_t q_row_stride, const void* k_pool_d
   return VA_OK;
 }
 
-}  // namespace va
-
 // Both attention entry points: `workspace_dev` is the caller's buffer (va_attention) or this
 // device's copy of the library's own scratch array (va_attention_static).
-namespace va {
-int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev,
-                              const void* v_pool_dev, int64_t pool_row_stride, const int32_t* plan_dev,
-                              const int32_t* plan_header_host, const int32_t* kv_indices_dev,
-                              const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
-                              int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2,
-                              void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
-                              const VaRope* rope, int keep_nan, void* stream) {
+int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, const void* v_pool_dev,
+                       int64_t pool_row_stride, const int32_t* plan_dev, const int32_t* plan_header_host,
+                       const int32_t* kv_indices_dev, const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
+                       int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
+                       int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, int keep_nan, void* stream) {
   if (!shape || !plan_header_host || !plan_dev) return va_fail(VA_ERR_ARG, "null plan or shape");
   const int32_t* h = plan_header_host;
   if (h[VA_H_MAGIC] != VA_PLAN_MAGIC) return va_fail(VA_ERR_ARG, "plan header has no magic word");
   const int n_rows = h[VA_H_N_ROWS], n_items = h[VA_H_N_ITEMS];
   if (n_rows == 0) return VA_OK;
-  va::AttnArgs a;
-  va::MergeArgs m;
-  int rc = va::plan_arguments(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, h, kv_indices_dev,
-                              sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev, lse_base2,
-                              workspace_dev, workspace_bytes, shape, rope, &a, &m);
+  AttnArgs a;
+  MergeArgs m;
+  int rc = plan_arguments(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, h, kv_indices_dev,
+                          sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev, lse_base2,
+                          workspace_dev, workspace_bytes, shape, rope, &a, &m);
   if (rc) return rc;
   m.keep_nan = keep_nan;
   hipStream_t s = (hipStream_t)stream;
@@ -932,8 +927,8 @@ extern "C" int va_attention(const void* q_dev, int64_t q_row_stride, const void*
                             void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
                             const VaRope* rope, void* stream) {
   return va::attention_launches(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, plan_header_host,
-                            kv_indices_dev, sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev,
-                            lse_base2, workspace_dev, workspace_bytes, shape, rope, 0, stream);
+                                kv_indices_dev, sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev,
+                                lse_base2, workspace_dev, workspace_bytes, shape, rope, 0, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -990,6 +985,6 @@ extern "C" int va_attention_static(const void* q_dev, int64_t q_row_stride, cons
   void* ptr = static_scratch_of_current_device();
   if (!ptr) return VA_ERR_HIP;
   return va::attention_launches(q_dev, q_row_stride, k_pool_dev, v_pool_dev, pool_row_stride, plan_dev, plan_header_host,
-                            kv_indices_dev, sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev,
-                            lse_base2, ptr, (int64_t)VA_STATIC_SCRATCH_BYTES, shape, rope, 0, stream);
+                                kv_indices_dev, sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev,
+                                lse_base2, ptr, (int64_t)VA_STATIC_SCRATCH_BYTES, shape, rope, 0, stream);
 }

@@ -101,19 +101,22 @@ class QuantizedCacheAttention(SharedCacheAttention):
         qo, kvp = np.asarray(qo_indptr), np.asarray(kv_indptr)
         # chains stand behind the decodes; their pages count by their place among the distinct ones
         n_codes = int(np.argmax(np.asarray(chain) >= 0)) if len(chain) and chain[-1] >= 0 else len(chain)
-        first_entry, first_subrow = int(kvp[n_codes]), int(qo[n_codes])
-        held = np.zeros(self.kv_cache.num_pages, dtype=np.int64)  # tokens of every page that someone sees
-        if n_codes < len(chain) and self._matrix_core and not self._workspace_prepared:
-            lengths = np.asarray(seq_lens)[n_codes:]
-            for begin, end, length in zip(kvp[n_codes:], kvp[n_codes + 1:], lengths):
-                if end > begin:
-                    held[kv[begin: end - 1]] = self.page_size
-                    held[kv[end - 1]] = max(held[kv[end - 1]], length - (end - 1 - begin) * self.page_size)
-        pages = np.flatnonzero(held)
+        pages = np.empty(0, dtype=np.int64)
+        if n_codes < len(chain) and self._matrix_core and not self._workspace_prepared \
+                and not (np.asarray(flags[n_codes:]) & native.VA_SUB_SLOTS).any():
+            held = np.zeros(self.kv_cache.num_pages, dtype=np.int64)  # tokens of every page that someone sees
+            lengths = np.asarray(seq_lens[n_codes:], dtype=np.int64)
+            for begin, end, length in zip(kvp[n_codes:].tolist(), kvp[n_codes + 1:].tolist(), lengths.tolist()):
+                full, rest = divmod(length, self.page_size)
+                held[kv[begin: min(begin + full, end)]] = self.page_size
+                if rest and begin + full < end:
+                    held[kv[begin + full]] = max(held[kv[begin + full]], rest)
+            pages = np.flatnonzero(held)
         if not len(pages) or not self._reads_back(int((np.diff(qo[n_codes:]) * lengths).sum()), len(pages)):
             return super()._build_launch(qo_indptr, kv_indptr, kv_indices_host, seq_lens, flags, chain, sub_worker_host,
                                          n_rows, tables, refs)
-        places = np.cumsum(held > 0)[kv[first_entry:]] - 1
+        first_entry, first_subrow = int(kvp[n_codes]), int(qo[n_codes])
+        places = np.maximum(np.cumsum(held > 0)[kv[first_entry:]] - 1, 0)  # (a listed page that nobody sees: any of them)
         within = np.arange(self.page_size, dtype=np.int64)
         slots = np.where(within < held[pages, None], pages[:, None] * self.page_size + within, -1).reshape(-1)
         rows = np.asarray(sub_worker_host)[first_subrow:]

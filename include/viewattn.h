@@ -345,7 +345,8 @@ VA_API int va_attention_static(const void* q_dev, int64_t q_row_stride, const vo
  * 2^e (448 for e4m3, 127 for int8; scale bytes below 1 become 1) and rounds
  * x / 2^e to the nearest code, ties to even (magnitudes over 1.875 * 2^127 for e4m3,
  * 127 * 2^121 for int8, whose codes would stand for 2^128, count as those).  A row that holds a NaN or an
- * infinity gets scale 255 and codes of zero.  As the scale is a power of two,
+ * infinity gets scale 255 and codes of zero; scale 0 and NaN codes are never written
+ * (in a pool from elsewhere a scale of 0 makes zeros, a NaN code may reach rows that do not see it).  As the scale is a power of two,
  * reading a row back is exact in any element type whose range holds it, and
  * quantising what was read back gives the same values.
  *
@@ -431,8 +432,8 @@ VA_API int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuan
  * a key or value row of NaN makes NaN of the results and the lse of those that see it;
  * query elements of |q_i| max|K| > 1.0e7 are held at that.  16-bit activations, head_dim
  * 64, 128 or 256, and the matrix-core plans only (the plan is built for VA_F16).
- * scratch_dev, on a 256-byte
- * boundary, must hold va_read_back_bytes(n_slots, rows of the plan, shape).
+ * scratch_dev, on a 256-byte boundary, must hold va_read_back_bytes(n_slots, rows of
+ * the plan, shape).
  */
 VA_API int64_t va_read_back_bytes(int64_t n_slots, int64_t n_rows, const VaShape* shape);
 VA_API int va_attention_read_back_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool,

@@ -263,6 +263,18 @@ def test_a_read_back_plan_names_every_visible_token_once(dtype):
     assert back.launch.header is launch.header
 
 
+def test_pages_that_nobody_sees_are_not_read_back():
+    """Lists may name more pages than their tokens fill."""
+    op, pool = make(pages=60)
+    op._reads_back = lambda pairs, pages: True
+    shared = block([7, 3, 50, 1], 32)
+    spec = PrefillSpec([shared], torch.tensor([16 * 20, 16 * 2, 16 * 59], dtype=torch.int32), 14, 0)
+    back = op.prepare_prefill_batch([spec]).launch.readback
+    assert back.slots.tolist() == [*range(48, 64), *range(112, 128), *range(320, 334), -1, -1]  # pages 3, 7 and 20
+    seen = back.launch.kv_indices.tolist()
+    assert seen[:2] == [1, 0] and 2 in seen and all(0 <= i < 3 for i in seen)
+
+
 def test_a_mixed_plan_keeps_decodes_on_codes():
     op, pool = make(pages=60)
     op._reads_back = lambda pairs, pages: True
