@@ -97,14 +97,16 @@ class QuantizedKVCache:
         """The K and V rows of ``slots`` (int64 on the device) as ``[n, kv_heads, head_dim]`` tensors of ``dtype``:
         new ones, or ``out``, whose rows may lie apart.  Negative slots give rows of zeros."""
         native.require_device(slots, "slots")
-        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != self._codes.device:
-            raise ValueError(f"slots must be one row of int64 on {self._codes.device}, got {slots.dtype} "
+        device = self._device
+        if slots.dim() != 1 or slots.dtype is not torch.int64 or slots.device != device:
+            raise ValueError(f"slots must be one row of int64 on {device}, got {slots.dtype} "
                              f"{tuple(slots.shape)} on {slots.device}")
         slots = slots.contiguous()
         shape = (slots.numel(), self._num_kv_heads, self._head_dim)
         width = self._num_kv_heads * self._head_dim
         if out is None:
-            k, v = (torch.empty(shape, dtype=self._dtype, device=self._codes.device) for _ in range(2))
+            k = torch.empty(shape, dtype=self._dtype, device=device)
+            v = torch.empty_like(k)
             stride = width
         else:
             k, v = out
@@ -116,8 +118,8 @@ class QuantizedKVCache:
             stride = k.stride(0) if shape[0] > 1 else width
             if stride < width:
                 raise ValueError("the rows of out overlap")
-        native.call_on(slots.device, native.lib.va_load_kv_q8, self.layer(layer_id), slots.data_ptr(), shape[0], k.data_ptr(),
-                       v.data_ptr(), stride, self._shape, native.current_stream_ptr(slots.device))
+        native.call_on(device, native.lib.va_load_kv_q8, self.layer(layer_id), slots.data_ptr(), shape[0], k.data_ptr(),
+                       v.data_ptr(), stride, self._shape, native.current_stream_ptr(device))
         return k, v
 
     @property
@@ -156,23 +158,28 @@ class QuantizedKVCache:
 _NO_ROPE = native.VaRope(native.VA_ROPE_TABLE, 0, None, 0, 0, 0, None)
 
 
+def _rows(pool: QuantizedKVCache, x: torch.Tensor, n: int, width: int, name: str):
+    """``x`` as ``n`` rows of ``width`` adjacent elements, and how far apart they are."""
+    shape = x.shape
+    if x.dtype is not pool._dtype or x.device != pool._device or shape[0] != n or x.numel() != n * width:
+        native.require_device(x, name)
+        raise ValueError(f"{name} must be {n} rows of {width} {pool._dtype} elements on {pool._device}, got {x.dtype} "
+                         f"{tuple(shape)} on {x.device}")
+    if len(shape) != 2:
+        x = x.reshape(n, width)
+    stride, element = x.stride()
+    return (x, stride) if element == 1 else (x.contiguous(), width)
+
+
 def store_quantized(pool: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, layer_id: int,
                     positions: Optional[torch.Tensor], rope: Optional[native.VaRope]) -> None:
     """Rotate the keys to ``positions`` (``[n]`` or ``[3, n]`` int64; ``None``: as they are), quantise and scatter."""
-    width, device, dtype = pool._num_kv_heads * pool._head_dim, pool._device, pool._dtype
+    width, device = pool._num_kv_heads * pool._head_dim, pool._device
     n = k.shape[0]
-    rows = []
-    for name, x in (("k", k), ("v", v)):
-        if x.dtype != dtype or x.device != device or x.shape[0] != n or x.numel() != n * width:
-            native.require_device(x, name)
-            raise ValueError(f"{name} must be {n} rows of {width} {dtype} elements on {device}, got {x.dtype} "
-                             f"{tuple(x.shape)} on {x.device}")
-        if x.dim() != 2:
-            x = x.reshape(n, width)
-        rows.append(x if x.stride(1) == 1 else x.contiguous())
-    k, v = rows
-    wide = out_loc.dtype == torch.int64
-    if not (wide or out_loc.dtype == torch.int32) or out_loc.numel() != n or out_loc.device != device:
+    k, k_stride = _rows(pool, k, n, width, "k")
+    v, v_stride = _rows(pool, v, n, width, "v")
+    wide = out_loc.dtype is torch.int64
+    if not (wide or out_loc.dtype is torch.int32) or out_loc.numel() != n or out_loc.device != device:
         raise ValueError(f"out_loc must be {n} int32 or int64 slots on {device}, got {out_loc.numel()} {out_loc.dtype} "
                          f"on {out_loc.device}")
     native.require_device(k, "k")
@@ -181,7 +188,7 @@ def store_quantized(pool: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, ou
     out_loc = out_loc.contiguous()
     where, axis_stride = None, 0
     if positions is not None:
-        if positions.dtype != torch.int64 or positions.device != device:
+        if positions.dtype is not torch.int64 or positions.device != device:
             positions = positions.to(device=device, dtype=torch.int64)
         positions = positions.contiguous()
         if positions.numel() != n or positions.dim() != 1:
@@ -189,6 +196,6 @@ def store_quantized(pool: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, ou
                 raise ValueError(f"positions must be [{n}] or [3, {n}], got {tuple(positions.shape)}")
             axis_stride = n
         where = positions.data_ptr()
-    native.call_on(device, native.lib.va_store_kv_rope_q8, k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0),
+    native.call_on(device, native.lib.va_store_kv_rope_q8, k.data_ptr(), v.data_ptr(), k_stride, v_stride,
                    pool.layer(layer_id), out_loc.data_ptr(), wide, where, axis_stride, n, pool._shape,
                    _NO_ROPE if rope is None else rope, native.current_stream_ptr(device))

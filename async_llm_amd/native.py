@@ -250,11 +250,17 @@ def current_stream_ptr(device: torch.device) -> int:
     return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def call_on(device: torch.device, function, *args) -> None:
     """Call a launching function of the library with ``device`` current (a launch belongs to the current device,
     whatever stream it names) and check its result."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(function(*args))
+    index = device.index
+    if index is None or index == _current_device():
+        rc = function(*args)
+        if rc:
+            check(rc)
         return
     with torch.cuda.device(device):
         check(function(*args))
