@@ -74,7 +74,8 @@ __device__ __forceinline__ void wave_wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
 }
 
-// The query rows of a tile for a link, rotated in fp32 and split into two bf16 numbers: this thread's two pieces of eight
+// The query rows of a tile for a link, rotated in fp32, scaled (scores are powers of two from here on) and split into two
+// bf16 numbers: this thread's two pieces of eight
 // dims of a row, high parts and low parts.  (16 rows of kD / 16 units: at 64 and 128 dims some threads have none.)
 struct QueryPieces {
   va_u32x4 part[2][2];  // [high, low][piece]
@@ -116,6 +117,8 @@ __device__ __forceinline__ QueryPieces turned_query(const AttnArgs& a, const Que
     activations8(a.q, at + q.d[0], dtype, pieces, y[0]);
     activations8(a.q, at + q.d[1], dtype, pieces, y[1]);
     if (x < pairs) turn8(c, s, y[0], y[1]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[0][e] *= a.scale_log2, y[1][e] *= a.scale_log2;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i)

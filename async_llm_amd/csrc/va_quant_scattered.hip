@@ -209,7 +209,7 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const bool seen = t0 + 16 * u + 4 * kg + r < t_row;
-          sc[u][r] = seen ? (hi[u][r] + lo[u][r]) * (ks[r] * a.scale_log2) : -INFINITY;
+          sc[u][r] = seen ? (hi[u][r] + lo[u][r]) * ks[r] : -INFINITY;
           vs[u][r] = seen ? v4[r] : 0.f;
           most = fmaxf(most, sc[u][r]);
         }

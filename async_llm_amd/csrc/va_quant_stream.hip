@@ -2,7 +2,7 @@
 // read the same tokens, and prefill tiles of 16 / G new tokens), row = tile row R / G, head R % G.
 //
 //   S^T[32 tokens, 16 rows] = K . Q^T      v_mfma_f32_16x16x32_bf16, the codes of K as the A operand, converted to bf16 (exact)
-//   p = exp2(S * 2^e_k * scale - max),     w = p * 2^e_v
+//   p = exp2(S * 2^e_k - max),     w = p * 2^e_v          (Q scaled by log2(e) / sqrt(D))
 //   O^T[D, 16 rows] += V^T . W^T           the same product; V^T from transposing LDS reads of the codes
 //
 // Operands that are not codes are split into two bf16 numbers, x = hi + lo with an error of 2^-17 of x, and each product is
@@ -128,6 +128,7 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
     const bool whole = !slots && tok_begin % 16 == 0;  // halves lie inside a page
     const int t_stop = min(tok_end, causal_base + n_q);        // tokens any row of the tile sees
     const int t_row = min(tok_end, causal_base + row_iq + 1);  // tokens this lane's row sees
+    const int t_all = min(tok_end, causal_base + 1);           // tokens every row sees
     const int t_last = t_stop - 1;
     const int n_all = t_stop > tok_begin ? (t_stop - tok_begin + kQuantTokens - 1) / kQuantTokens : 0;
     const int n_tiles = n_all > wave ? (n_all - wave + kQuantWaves - 1) / kQuantWaves : 0;  // this wave's
@@ -252,20 +253,22 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
       }
       __builtin_amdgcn_sched_barrier(0);
 
-      va_f32x4 hi[2], lo[2];
+      va_f32x4 dots[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) hi[h] = lo[h] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2; ++h) dots[h] = va_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         va_u32x4 low;
         if constexpr (Sh::kKeepLow) low = q_lo[s]; else low = staged_query<kD>(query, s);
+        va_u32x4 k8[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const va_u32x4 raw = kraw[h][s / 2];
-          const va_u32x4 k8 = C::bf16x8(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]});
-          hi[h] = Mma<BF16>::run(k8, q_hi[s], hi[h]);
-          lo[h] = Mma<BF16>::run(k8, low, lo[h]);
+          k8[h] = C::bf16x8(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]});
+          dots[h] = Mma<BF16>::run(k8[h], q_hi[s], dots[h]);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) dots[h] = Mma<BF16>::run(k8[h], low, dots[h]);
       }
       __builtin_amdgcn_sched_barrier(0);
       va_u32x2 vraw[kDimTiles];
@@ -292,11 +295,21 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool seen = t0 + 16 * h + 4 * kg + r < t_row;
-          sc[h][r] = seen ? (hi[h][r] + lo[h][r]) * (scale_value(kscale[h][r]) * a.scale_log2) : -INFINITY;
-          most = fmaxf(most, sc[h][r]);
-        }
+        for (int r = 0; r < 4; ++r) sc[h][r] = dots[h][r] * scale_value(kscale[h][r]);
+      if (t0 + kQuantTokens > t_all) {  // some row does not see some token, which may have any scale
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool seen = t0 + 16 * h + 4 * kg + r < t_row;
+            sc[h][r] = seen ? sc[h][r] : -INFINITY;
+            vscale[h][r] = seen ? vscale[h][r] : 0u;
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, sc[h][r]);
       if (__any(most > m_run)) {
         const float m_new = fmaxf(m_run, quant_group_max(most));
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
@@ -313,8 +326,7 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(sc[h][r] - m_run);
           l_run += p;
-          // (a token that the row does not see may have any scale)
-          w[r] = t0 + 16 * h + 4 * kg + r < t_row ? p * scale_value(vscale[h][r]) : 0.f;
+          w[r] = p * scale_value(vscale[h][r]);
         }
         uint32_t x, y;
         split_pair(w[0], w[1], x, y);
