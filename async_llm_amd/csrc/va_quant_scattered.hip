@@ -214,7 +214,7 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
           most = fmaxf(most, sc[u][r]);
         }
       }
-      if (__any(most > m_run)) {
+      if (__any(most > m_run + kQuantLeap)) {
         const float m_new = fmaxf(m_run, quant_group_max(most));
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
         m_run = m_new;

@@ -310,7 +310,7 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 4; ++r) most = fmaxf(most, sc[h][r]);
-      if (__any(most > m_run)) {
+      if (__any(most > m_run + kQuantLeap)) {
         const float m_new = fmaxf(m_run, quant_group_max(most));
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
         m_run = m_new;
