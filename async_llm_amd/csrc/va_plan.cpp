@@ -107,8 +107,8 @@ inline int32_t visible_end(int32_t len, int32_t nq, bool causal, int32_t b) {
 // shows: 48 readers of 512 tokens, 483 us in pairs, 494 in fours.  Where the line lies, us in pairs / in fours, 256 dims and
 // 2 kv heads of 128: 128 readers of 2048 tokens 270 / 281, 73 / 78; 48 of 3000 139 / 139, 45 / 45; 64 of 4096 166 / 163,
 // 49 / 46; 64 of 12000 349 / 308, 90 / 90 (at 64 dims 48 of 3000 142 / 139, 64 of 4096 170 / 166, 64 of 12000 330 / 307).
-int tiles_together(int kernel, int page_size, int64_t tokens) {
-  return kernel != VA_KERNEL_MFMA ? 1 : page_size < 16 ? VA_TOGETHER_SCATTERED : tokens < 4096 ? 2 : VA_TOGETHER;
+int tiles_together(int kernel, int page_size, int64_t tokens, bool apart) {
+  return kernel != VA_KERNEL_MFMA || apart ? 1 : page_size < 16 ? VA_TOGETHER_SCATTERED : tokens < 4096 ? 2 : VA_TOGETHER;
 }
 
 // Work items wanted per kv head.  The streaming kernel: 512 workgroups, but not so few items that their ends leave the
@@ -191,6 +191,9 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
   // group once the groups are known (group_is_wide below); narrow tiles are emitted chunk-major, so the
   // tiles that stream the same chunk run side by side and share it in L2.
   const bool wide_on_request = params && params->wide_tile > 0;
+  // A workgroup for every tile: 64 rows over 65536 shared tokens, counted together / apart, 173 / 159 us over codes, over 8192 alone
+  // 48.6 / 41.9, beside private blocks 193.8 / 189.8.
+  const bool tiles_apart = params && params->wide_tile < -1;
   const int target = params && params->target_items > 0 ? params->target_items : default_target(kernel, shape->num_kv_heads);
   const int gran = 64;  // chunk boundaries are multiples of this many tokens
 
@@ -260,7 +263,7 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
     int64_t most_tiles = 0;                   // narrow ones of one of these groups
     for (size_t gi = 0; gi < groups.size(); ++gi) {
       const int64_t n = (int64_t)groups[gi].subrows.size(), len = s->seq_lens[groups[gi].rep];
-      const int64_t narrow = (n + q_tile - 1) / q_tile, at_once = tiles_together(kernel, shape->page_size, len);
+      const int64_t narrow = (n + q_tile - 1) / q_tile, at_once = tiles_together(kernel, shape->page_size, len, tiles_apart);
       cut_tiles(n, tiles, true);
       const int64_t bytes = (narrow - (int64_t)tiles.size()) * len * token_bytes;
       many[gi] = n > q_tile && bytes >= kFairShare;
@@ -326,7 +329,7 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
   std::vector<int64_t> walks[2];
   int64_t walked[2] = {0, 0};
   for (size_t gi = 0; gi < groups.size(); ++gi) {
-    const int64_t len = s->seq_lens[groups[gi].rep], at_once = group_is_wide[gi] ? 1 : tiles_together(kernel, shape->page_size, len);
+    const int64_t len = s->seq_lens[groups[gi].rep], at_once = group_is_wide[gi] ? 1 : tiles_together(kernel, shape->page_size, len, tiles_apart);
     cut_tiles((int64_t)groups[gi].subrows.size(), tiles, group_is_wide[gi]);
     for (int each = 0; each < 2; ++each) {
       walks[each].push_back(each ? (int64_t)tiles.size() : ((int64_t)tiles.size() + at_once - 1) / at_once);
@@ -350,14 +353,18 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
       // 256 dims, 60 / 43 / 35 / 29 items for 64 at once) 18.2 / 15.8 / 16.1 / 17.0 us; 256 / 320 / 384 / 512, 8 of
       // 1400..4000 (8 of 128 dims, 69 / 60 / 53 / 42 for 64) 21.4 / 19.6 / 20.1 / 19.6.  At 128 dims up to sixteen: 16
       // requests of 64..2048 behind 1500 shared tokens (8 kv heads), chunks of 512 / 896, 30.9 / 28.6 us.
-      const int64_t at_once = std::max(1, (shape->head_dim != 256 ? 384 : any_wide ? 192 : 208) / shape->num_kv_heads);
+      // Over codes (tiles apart), where two to four workgroups share a CU, 614 start at once under 256 dims (384 / 614, us: 4
+      // requests of 20 k tokens, 8 kv heads of 128 dims, 29.8 / 25.8; 24 of 7 k, 2 heads of 128, 22.0 / 20.3; at 256 dims one of 30 k
+      // tokens 19.6, with a third more items 22.8), and twelve granules where they do not (eight / twelve, 16 requests
+      // of 5 k at 256 dims 24.8 / 23.3, 19 of 900 25.9 / 23.8).
+      const int64_t at_once = std::max(1, (shape->head_dim != 256 ? (tiles_apart ? 614 : 384) : any_wide ? 192 : 208) / shape->num_kv_heads);
       for (least = gran; least < most; least += gran) {
         int64_t n = 0;
         for (size_t gi = 0; gi < groups.size(); ++gi) n += walks[each][gi] * ((s->seq_lens[groups[gi].rep] + least - 1) / least);
         one_round = n <= at_once;
         if (one_round) break;
       }
-      if (!one_round) least = 8 * gran;
+      if (!one_round) least = (tiles_apart ? 12 : 8) * gran;
     } else if (kernel != VA_KERNEL_MFMA) {
       const int64_t spread = (walked[each] + (256 / shape->num_kv_heads) - 1) / std::max(1, 256 / shape->num_kv_heads);
       least = std::min<int64_t>(least, std::max<int64_t>(gran, round_up(spread, gran)));
@@ -376,7 +383,7 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
   size_chunk(each);
   const bool tiles_short = kernel == VA_KERNEL_MFMA && !cap && !any_wide && kv_chunk <= kLongestShort &&
                            (walked[1] - walked[0]) * token_bytes <= kReadAgain;
-  if (kernel == VA_KERNEL_MFMA && !cap && each && !tiles_short) size_chunk(each = false);
+  if (kernel == VA_KERNEL_MFMA && !cap && each && !tiles_short && !tiles_apart) size_chunk(each = false);
 
   out.kernel = kernel;
   out.q_tile = q_tile;
@@ -433,7 +440,7 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
       const size_t a = tiles[ti].first, b = tiles[ti].second;
       emit((int32_t)(b - a), {Link{s->kv_indptr[rep], t0, t1, tile_qref[ti], VA_NO_CAUSAL, lflags}},
            [&](int32_t i) { return (int32_t)s->sub_worker[gr.subrows[a + i]]; }, unit);
-      out.items.back().together = tiles_together(kernel, shape->page_size, len);
+      out.items.back().together = tiles_together(kernel, shape->page_size, len, tiles_apart);
     };
     auto chunk_len = [&](int32_t chunk) {
       const int32_t n_chunks = (len + chunk - 1) / chunk;

@@ -72,7 +72,7 @@ class QuantizedCacheAttention(SharedCacheAttention):
             raise ValueError(f"kv_cache lives on {self.device}, the op is to run on {device}")
         p = self.plan_params
         self._read_back_params = native.VaPlanParams(p.kernel, p.q_tile, p.kv_chunk, p.target_items, p.wide_tile)
-        p.wide_tile = -1  # codes are read by tiles of up to 16 rows
+        p.wide_tile = -2  # codes are read by tiles of up to 16 rows, a workgroup each
         self._read_back_shape = native.make_shape(num_qo_heads, num_kv_heads, head_dim, page_size, torch.float16)
         self._matrix_core = p.kernel != native.VA_KERNEL_GENERIC and dtype != torch.float32 and head_dim in (64, 128, 256) \
             and num_qo_heads // num_kv_heads in (1, 2, 4, 8, 16)

@@ -14,6 +14,7 @@ from async_llm_amd.kvcache import MHAKVCache, QuantizedKVCache
 from async_llm_amd.shared_cache import BlockKVOps, CacheBlock, PrefillSpec, QuantizedCacheAttention, SharedCacheAttention, WorkerGroup
 from async_llm_amd.shared_cache.attention_graph import SharedDecodeAttentionBuffers, SharedPrefillAttentionBuffers
 from tests import quant_util as Q
+from tests.test_native_abi_cpu import decode_plan
 
 CPU = torch.device("cpu")
 E4M3, INT8 = torch.float8_e4m3fn, torch.int8
@@ -273,6 +274,27 @@ def test_pages_that_nobody_sees_are_not_read_back():
     assert back.slots.tolist() == [*range(48, 64), *range(112, 128), *range(320, 334), -1, -1]  # pages 3, 7 and 20
     seen = back.launch.kv_indices.tolist()
     assert seen[:2] == [1, 0] and 2 in seen and all(0 <= i < 3 for i in seen)
+
+
+@pytest.mark.parametrize("readers,tokens", [(64, 8192), (5, 300), (33, 70)])
+def test_tiles_of_a_plan_over_codes_walk_apart(readers, tokens):
+    """Every (row, token) pair once, and no item that another's workgroup would have to serve."""
+    op, pool = make(heads=(16, 4, 256), pages=6000)
+    shared = block(list(range(-(-tokens // 16))), tokens)
+    own = [block([1000 + 2 * i], 1 + i % 15) for i in range(readers)]
+    group = WorkerGroup(cache_structure=[[shared, b] for b in own], write_to=own)
+    slots = torch.tensor([(1000 + 2 * i) * 16 + 1 + i % 15 for i in range(readers)], dtype=torch.int32)
+    meta = op.prepare(group, {id(b): None for b in own}, slots)
+    pages, row_of = meta.launch.kv_indices.tolist(), meta.sub_worker.tolist()
+    _, items, links, qrefs, *_ = decode_plan(meta.launch.blob.numpy())
+    seen = np.zeros((readers, 2), dtype=np.int64)
+    for begin, n_links, n_q, _, _, _, partners in items[:, :7].tolist():
+        assert partners == 0 and n_q <= 4
+        for kv_begin, t0, t1, qref, _, flags in links[begin: begin + n_links, :6].tolist() if n_q else ():
+            for i in range(n_q):
+                row = row_of[qrefs[qref + i] if flags & 1 else qref + i]
+                seen[row, int(pages[kv_begin] >= 1000)] += t1 - t0
+    assert (seen[:, 0] == tokens).all() and seen[:, 1].tolist() == [b.num_tokens + 1 for b in own]
 
 
 def test_a_mixed_plan_keeps_decodes_on_codes():
