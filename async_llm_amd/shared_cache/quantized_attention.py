@@ -140,15 +140,15 @@ class QuantizedCacheAttention(SharedCacheAttention):
     def _reads_back(self, pairs: int, pages: int) -> bool:
         """Whether the chains of a step, ``pairs`` of a row and a token that it may see, run over rows read back.
 
-        Reading back costs four launches more and 2 ns a token of 1024 elements, and takes two thirds off the products.  One
-        chunk, 32 q and 8 kv heads of 128: 256 rows over 3000 tokens 60.5 us against 58.6 over codes, 32 (48) rows over 20000
-        78 (83) against 67 (91), 8 rows over 20000 74 against 27; 8 and 8 heads: 128 (256) rows over 20000 79 (92) against 69
-        (123); 16 and 4 heads of 256: 64 rows over 20000 84 against 85; 64 and 16 heads of 64: 24 rows over 20000 82 against
-        79, 256 rows over 3000 63 against 69.  All of them change sides near 3.2e9 products, and near 128 query rows a token
-        and kv head where the tokens are many.
+        Reading back costs four launches more and 2 ns a token of 1024 elements, and takes half to two thirds off the products.
+        Us read back / over codes, one chunk, 32 q and 8 kv heads of 128: 256 rows over 3000 tokens 61 / 52, 48 (64) rows over
+        20000 84 / 80 (89 / 106), 24 rows 80 / 48; 8 and 8 heads: 128 (256) rows over 20000 81 / 62 (92 / 108); 16 and 4
+        heads of 256: 64 (96) rows over 20000 86 / 78 (98 / 107), 256 rows over 3000 59 / 58; 64 and 16 heads of 64: 24 (32) rows
+        over 20000 83 / 68 (85 / 91), 256 rows over 3000 64 / 59. They change sides between 2.4e9 and 7e9 products, most near 4e9,
+        and at 120 to 350 query rows a token and kv head where the tokens are many.
         """
         products = pairs * self.num_qo_heads * self.head_dim
-        return products >= 3 << 30 and products >= 128 * pages * self.page_size * self.num_kv_heads * self.head_dim
+        return products >= 4 << 30 and products >= 160 * pages * self.page_size * self.num_kv_heads * self.head_dim
 
     def _ensure_scratch(self, nbytes: int) -> torch.Tensor:
         """Room for rows read back, shared by the op's steps like their workspace; a plan keeps the tensor it was given."""
