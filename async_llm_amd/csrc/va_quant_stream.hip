@@ -47,7 +47,7 @@ struct QuantRing {
   static constexpr int kScaleOffset = kBuffers * kTileBytes;
   static constexpr int kWaveBytes = kScaleOffset + kScaleSlots * kScaleBytes;
   static constexpr int kQueryOffset = kQuantWaves * kWaveBytes;
-  static constexpr bool kKeepLow = kD < 128;  // low parts of the query in registers
+  static constexpr bool kKeepLow = kD < 256;  // low parts of the query in registers
   static constexpr int kQueryBytes = 16 * kD * 2;       // high or low parts of a tile's query: staged one after the other
   static constexpr int kLdsBytes = kQueryOffset + kQueryBytes;
   static_assert(kQuantWaves * QuantFold<kD>::kBytes <= kLdsBytes, "room for the waves' states");
