@@ -2,7 +2,7 @@
 //
 // A prefill chunk reads every token of its view for hundreds of rows: the products are what it costs, and the 16-bit
 // kernel's wide tiles (va_mfma_wide.hip) run them at a rate that a kernel which converts codes beside them did not come
-// near: four chunks of 300 to 1500 tokens over 8000 at 128 dims 640 us, with tiles of 16 rows over codes 1605, with
+// near: four chunks of 300 to 1500 tokens over 8000 at 128 dims 675 us, with tiles of 16 rows over codes 1473, with
 // wide tiles over codes 960 to 1140.  Reading back is a tenth of it (47 k tokens, 94 MB of codes).
 //
 // It runs in float16 whatever the activations are: codes have four (eight) bits, so eleven hold them, and a bf16 query or
@@ -84,7 +84,8 @@ __global__ __launch_bounds__(256) void quant_top_kernel(BackArgs a) {
   }
   __syncthreads();
   if (threadIdx.x < 2)
-    a.tops[2 * blockIdx.x + threadIdx.x] = max(max(of_wave[0][threadIdx.x], of_wave[1][threadIdx.x]), max(of_wave[2][threadIdx.x], of_wave[3][threadIdx.x]));
+    a.tops[2 * blockIdx.x + threadIdx.x] = max(max(of_wave[0][threadIdx.x], of_wave[1][threadIdx.x]),
+                                               max(of_wave[2][threadIdx.x], of_wave[3][threadIdx.x]));
 }
 __device__ __forceinline__ int back_top(const uint32_t* tops, int which) {  // (by a whole wave)
   static_assert(kBackGroups == kWave, "a lane a group");
@@ -157,7 +158,8 @@ __global__ __launch_bounds__(256) void quant_back_kernel(BackArgs a, long long r
 // Results in the activations' type, eight elements a thread.  A row that a NaN reached has NaN for its lse (the attention's
 // kernels leave -inf where the sum of its weights is no number).
 template <typename C>
-__global__ __launch_bounds__(256) void quant_results_kernel(const __half* from, void* out, float* lse, const uint32_t* tops, long long threads, int head_dim, int dtype, int pieces) {
+__global__ __launch_bounds__(256) void quant_results_kernel(const __half* from, void* out, float* lse, const uint32_t* tops,
+                                                            long long threads, int head_dim, int dtype, int pieces) {
   const long long idx = blockIdx.x * 256ll + threadIdx.x;
   const float f = power_of_two(back_top(tops, 1) - 127 - BackScale<C>::kValue);
   if (idx >= threads) return;
@@ -208,10 +210,11 @@ static int launch_quant_back(const BackArgs& a, int pieces, hipStream_t stream) 
 }
 
 template <typename C>
-static int launch_quant_results(const __half* from, void* out, float* lse, const uint32_t* tops, long long n, int head_dim, int dtype, hipStream_t stream) {
+static int launch_quant_results(const __half* from, void* out, float* lse, const uint32_t* tops, long long n, int head_dim,
+                                int dtype, hipStream_t stream) {
   const int pieces = (uintptr_t)out % 16 == 0;
-  hipLaunchKernelGGL((quant_results_kernel<C>), dim3((unsigned)((n / 8 + 255) / 256)), dim3(256), 0, stream, from, out, lse, tops, n / 8,
-                     head_dim, dtype, pieces);
+  hipLaunchKernelGGL((quant_results_kernel<C>), dim3((unsigned)((n / 8 + 255) / 256)), dim3(256), 0, stream, from, out, lse,
+                     tops, n / 8, head_dim, dtype, pieces);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "results launch: %s", hipGetErrorString(e));
 }

@@ -104,7 +104,8 @@ __global__ __launch_bounds__(256) void quant_store_kernel(StoreArgs a) {
   const int h = (int)(unit - row * a.num_kv_heads), D = a.head_dim;
   uint32_t slot;
   if (!slot_of_row(a.dst, a.dst_is_i64, row, a.num_slots, slot)) return;
-  const typename E::storage* x = (const typename E::storage*)(which ? a.x[1] : a.x[0]) + row * (which ? a.x_stride[1] : a.x_stride[0]) + (long long)h * D;
+  const typename E::storage* x = (const typename E::storage*)(which ? a.x[1] : a.x[0]) +
+                                 row * (which ? a.x_stride[1] : a.x_stride[0]) + (long long)h * D;
   const int rotary = which ? 0 : a.rope.rotary_dim, half = rotary / 2;
   Pos3 p{0, 0, 0};
   if (rotary) p = load_pos(a.pos, a.pos_axis_stride, row);
@@ -245,7 +246,8 @@ __global__ __launch_bounds__(256) void quant_load_kernel(LoadArgs a, int per_hea
   S* out = (S*)(which ? a.out[1] : a.out[0]) + row * a.out_stride + (long long)h * a.head_dim + d0;
   if (((uintptr_t)out & 15) == 0) {
 #pragma unroll
-    for (int i = 0; i < (int)(8 * sizeof(S) / 16); ++i) __builtin_nontemporal_store(__builtin_bit_cast(va_u32x4, y.raw[i]), (va_u32x4*)out + i);
+    for (int i = 0; i < (int)(8 * sizeof(S) / 16); ++i)
+      __builtin_nontemporal_store(__builtin_bit_cast(va_u32x4, y.raw[i]), (va_u32x4*)out + i);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) out[k] = y.e[k];
@@ -298,7 +300,8 @@ struct QuantCopyArgs {
 // are looked up once, and walks the heads: neighbouring rows of a wave are neighbouring tokens of a page, one run of
 // memory.  Bound by HBM: 12556 tokens of 4 layers of 4 heads of 256 dims (207 MB read and written) 39 us, 5.3 TB/s; with a thread
 // walking sixteen tokens of its head 66 us, with stores that stay in the caches 49.  Small copies are bound by the trip
-// slot, scale and codes, store: 5.6 us for 4.3 MB (17 with walks).  kTurn: keys are rotated (rotary_dim a multiple of 16); otherwise they move code for code like the values.
+// slot, scale and codes, store: 5.6 us for 4.3 MB (17 with walks).  kTurn: keys are rotated (rotary_dim a multiple of 16);
+// otherwise they move code for code like the values.
 template <typename C, int kD, bool kTurn>
 __global__ __launch_bounds__(256) void quant_copy_kernel(QuantCopyArgs a) {
   constexpr int kLanes = kD / 16, kHeads = 256 / kLanes / kQuantCopyTokens;  // heads side by side
@@ -309,7 +312,8 @@ __global__ __launch_bounds__(256) void quant_copy_kernel(QuantCopyArgs a) {
   if (src < 0 || src >= (long long)a.num_slots || dst < 0 || dst >= (long long)a.num_slots) return;
   uint8_t* codes = (which ? a.codes[1] : a.codes[0]) + layer * a.code_layer_stride;
   uint8_t* scales = (which ? a.scales[1] : a.scales[0]) + layer * a.scale_layer_stride;
-  const long long from = quant_row(a.pages, (uint32_t)src, 0, a.num_kv_heads), to = quant_row(a.pages, (uint32_t)dst, 0, a.num_kv_heads);
+  const long long from = quant_row(a.pages, (uint32_t)src, 0, a.num_kv_heads);
+  const long long to = quant_row(a.pages, (uint32_t)dst, 0, a.num_kv_heads);
   const int first = threadIdx.x / (kLanes * kQuantCopyTokens);
   if (!kTurn || which) {
     for (int h0 = first; h0 < a.num_kv_heads; h0 += kQuantCopyBatch * kHeads) {
