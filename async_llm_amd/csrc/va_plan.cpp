@@ -329,7 +329,8 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
   std::vector<int64_t> walks[2];
   int64_t walked[2] = {0, 0};
   for (size_t gi = 0; gi < groups.size(); ++gi) {
-    const int64_t len = s->seq_lens[groups[gi].rep], at_once = group_is_wide[gi] ? 1 : tiles_together(kernel, shape->page_size, len, tiles_apart);
+    const int64_t len = s->seq_lens[groups[gi].rep];
+    const int64_t at_once = group_is_wide[gi] ? 1 : tiles_together(kernel, shape->page_size, len, tiles_apart);
     cut_tiles((int64_t)groups[gi].subrows.size(), tiles, group_is_wide[gi]);
     for (int each = 0; each < 2; ++each) {
       walks[each].push_back(each ? (int64_t)tiles.size() : ((int64_t)tiles.size() + at_once - 1) / at_once);
@@ -357,7 +358,8 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
       // requests of 20 k tokens, 8 kv heads of 128 dims, 29.8 / 25.8; 24 of 7 k, 2 heads of 128, 22.0 / 20.3; at 256 dims one of 30 k
       // tokens 19.6, with a third more items 22.8), and twelve granules where they do not (eight / twelve, 16 requests
       // of 5 k at 256 dims 24.8 / 23.3, 19 of 900 25.9 / 23.8).
-      const int64_t at_once = std::max(1, (shape->head_dim != 256 ? (tiles_apart ? 614 : 384) : any_wide ? 192 : 208) / shape->num_kv_heads);
+      const int start = shape->head_dim != 256 ? (tiles_apart ? 614 : 384) : any_wide ? 192 : 208;
+      const int64_t at_once = std::max(1, start / shape->num_kv_heads);
       for (least = gran; least < most; least += gran) {
         int64_t n = 0;
         for (size_t gi = 0; gi < groups.size(); ++gi) n += walks[each][gi] * ((s->seq_lens[groups[gi].rep] + least - 1) / least);

@@ -12,7 +12,8 @@ constexpr int kQuantThreads = 256;
 constexpr int kQuantWaves = 4;
 constexpr int kQuantTokens = 32;  // tokens per tile
 // How far (log2) a score may lie above the running reference before sums are rescaled to it.  Weights up to 2^8 lose nothing: they
-// are split into two bf16 numbers and summed in fp32, whose errors are relative.  Maxima of 16 rows rise in most tiles
+// are split into two bf16 numbers and summed in fp32, whose errors are relative (what they cost is range: sums overflow for
+// values over 2^119 instead of 2^127 divided by their number).  Maxima of 16 rows rise in most tiles
 // of a walk, and each time all of O^T is multiplied (64 of 400 vector instructions a tile at 256 dims).
 constexpr float kQuantLeap = 8.f;
 
