@@ -178,8 +178,8 @@ def slots_of(block, tokens=None):
 def attention64(op, q: torch.Tensor, segments, layer=0, half=False):
     """One request: ``q [rows, Hq, D]``; ``segments``: ``(slots, positions [rows] or [3, rows], first)`` where token t of
     a segment is visible to row i iff t <= first + i.  Returns out ``[rows, Hq * D]``, lse ``[rows, Hq]`` and the bound of
-    score errors, where a query element is off by 2^-17 of itself or, ``half``, by a rounding to float16, and the weighted
-    values."""
+    score errors, where a query element is off by 2^-17 of itself or, ``half``, by a rounding to float16, the weighted
+    values, and what underflow may lose."""
     S, Hq, D = q.shape
     Hkv = op.num_kv_heads
     G = Hq // Hkv
@@ -209,7 +209,10 @@ def attention64(op, q: torch.Tensor, segments, layer=0, half=False):
     # that of D products in 32 bits (D * 2^-24), both of the magnitudes' sum, its exponent by 2^-23 of itself.
     off = (size.amax(-1) * (operand + D * 2.0**-24) + x.abs().masked_fill(torch.isinf(x), 0.0).amax(-1) * 2.0**-22) if x.shape[-1] else torch.zeros_like(lse)
     off = off.permute(1, 0, 2).reshape(S, Hq)
-    return out, lse.permute(1, 0, 2).reshape(S, Hq), off, weight
+    # Weights under 2^-126, and low parts of weights under 2^-117, are no normal 32-bit (bf16) numbers and may become zero:
+    # less than 2^-125 of a value for each token.
+    lost = (v.abs().amax() * len(v) * 2.0**-125 if len(v) else torch.zeros(())).double().expand(S, 1)
+    return out, lse.permute(1, 0, 2).reshape(S, Hq), off, weight, lost
 
 
 def assert_attends(out, lse, expected, dtype, tokens, half=None):
@@ -217,12 +220,12 @@ def assert_attends(out, lse, expected, dtype, tokens, half=None):
 
     ``half`` marks the rows [rows] that ran in float16 (a number: the largest value's magnitude; 0 others): results are
     rounded to that first, by 2^-11 of themselves or 2^-39 of that, and weights by 2^-11 of themselves or 2^-25 each."""
-    o, l, off, weight = expected
+    o, l, off, weight, lost = expected
     half = (torch.zeros(o.shape[0]) if half is None else half)[:, None]
     operand = torch.where(half > 0, OPERAND[True], OPERAND[False])
     got = out.detach().cpu().double()
     relative = (2 * off + operand + (tokens + 64) * 2.0**-24).repeat_interleave(o.shape[1] // off.shape[1], dim=1)
-    room = EPS[dtype] * o.abs() + weight * relative * (1 + EPS[dtype]) + (2.0**-24 if dtype == torch.float16 else 2.0**-126)
+    room = EPS[dtype] * o.abs() + weight * relative * (1 + EPS[dtype]) + lost + (2.0**-24 if dtype == torch.float16 else 2.0**-126)
     room = room + (half > 0) * 2.0**-11 * o.abs() * (1 + EPS[dtype]) + half * (2.0**-39 + tokens * 2.0**-25)
     assert got.shape == o.shape
     worst = ((got - o).abs() - room).max().item()
