@@ -28,12 +28,13 @@ struct E4M3 {
     const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     out[0] = lo[0], out[1] = lo[1], out[2] = hi[0], out[3] = hi[1];
   }
-  // Eight codes as bf16, exactly (four instructions, each at the full rate).
-  static __device__ __forceinline__ va_u32x4 bf16x8(va_u32x2 w) {
-    return va_u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.f, false)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.f, true)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.f, false)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.f, true))};
+  // Eight codes as bf16, exactly, and times a power of two at no cost (four instructions, each at the full rate).
+  static constexpr bool kScales = true;
+  static __device__ __forceinline__ va_u32x4 bf16x8(va_u32x2 w, float scale = 1.f) {
+    return va_u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], scale, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], scale, true)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], scale, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], scale, true))};
   }
 };
 struct INT8 {
@@ -49,6 +50,7 @@ struct INT8 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = (float)(int8_t)(w >> (8 * i));
   }
+  static constexpr bool kScales = false;
   static __device__ __forceinline__ va_u32x4 bf16x8(va_u32x2 w) {  // (bf16 has the eight bits of a code)
     float x[8];
     unpack4(w[0], x), unpack4(w[1], x + 4);

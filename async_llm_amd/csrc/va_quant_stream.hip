@@ -1,7 +1,8 @@
 // Matrix-core view attention over a quantised pool: query tiles of up to 16 MFMA rows (decode tiles of 16 / G requests that
 // read the same tokens, and prefill tiles of 16 / G new tokens), row = tile row R / G, head R % G.
 //
-//   S^T[32 tokens, 16 rows] = K . Q^T      v_mfma_f32_16x16x32_bf16, the codes of K as the A operand, converted to bf16 (exact)
+//   S^T[32 tokens, 16 rows] = K . Q^T      v_mfma_f32_16x16x32_bf16, the codes of K as the A operand, converted to bf16 (exact;
+//                                          the conversion of e4m3 takes 2^e_k along)
 //   p = exp2(S * 2^e_k - max),     w = p * 2^e_v          (Q scaled by log2(e) / sqrt(D))
 //   O^T[D, 16 rows] += V^T . W^T           the same product; V^T from transposing LDS reads of the codes
 //
@@ -254,6 +255,11 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
       }
       __builtin_amdgcn_sched_barrier(0);
 
+      const char* scales = lds + wave * Sh::kWaveBytes + Sh::kScaleOffset + (i % Sh::kScaleSlots) * Sh::kScaleBytes;
+      float of_token[2] = {1.f, 1.f};  // of this lane's token of each half, where the conversion takes it
+      if constexpr (C::kScales)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) of_token[h] = scale_value(*(const uint32_t*)(scales + 64 * h + 4 * j));
       va_f32x4 dots[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) dots[h] = va_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -265,7 +271,8 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const va_u32x4 raw = kraw[h][s / 2];
-          k8[h] = C::bf16x8(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]});
+          const va_u32x2 codes = s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]};
+          if constexpr (C::kScales) k8[h] = C::bf16x8(codes, of_token[h]); else k8[h] = C::bf16x8(codes);
           dots[h] = Mma<BF16>::run(k8[h], q_hi[s], dots[h]);
         }
 #pragma unroll
@@ -285,18 +292,21 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
 
       // online softmax; this lane holds tokens 16 h + 4 kg + r of row j
       const int t0 = first_token(i);
-      const char* scales = lds + wave * Sh::kWaveBytes + Sh::kScaleOffset + (i % Sh::kScaleSlots) * Sh::kScaleBytes + 16 * kg;
-      va_u32x4 kscale[2], vscale[2];
+      va_u32x4 vscale[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        kscale[h] = *(const va_u32x4*)(scales + 64 * h);
-        vscale[h] = *(const va_u32x4*)(scales + 128 + 64 * h);
-      }
+      for (int h = 0; h < 2; ++h) vscale[h] = *(const va_u32x4*)(scales + 128 + 64 * h + 16 * kg);
       float sc[2][4], most = -INFINITY;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (C::kScales) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[h][r] = dots[h][r] * scale_value(kscale[h][r]);
+          for (int r = 0; r < 4; ++r) sc[h][r] = dots[h][r];
+        } else {
+          const va_u32x4 kscale = *(const va_u32x4*)(scales + 64 * h + 16 * kg);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[h][r] = dots[h][r] * scale_value(kscale[r]);
+        }
+      }
       if (t0 + kQuantTokens > t_all) {  // some row does not see some token, which may have any scale
 #pragma unroll
         for (int h = 0; h < 2; ++h)

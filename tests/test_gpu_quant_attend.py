@@ -122,12 +122,14 @@ def test_large_chunks_are_read_back_and_small_ones_are_not():
         check(op, step, q, [0], [new], out, lse)
 
 
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("page", [8, 16])
 @pytest.mark.parametrize("codes", [E4M3, INT8])
-def test_rows_read_back_over_a_wide_range(codes):
+def test_chunks_over_a_wide_range(codes, page, back):
     """Keys and values far from one, and among them rows that are far smaller: float16 alone would lose them."""
-    op, pool, g = Q.make(DEV, (8, 2, 64), 16, 40, BF16, codes)
-    pages = Q.Pages(40, 16)
-    op._reads_back = lambda pairs, pages: True
+    op, pool, g = Q.make(DEV, (8, 2, 64), page, 40, BF16, codes)
+    pages = Q.Pages(40, page)
+    op._reads_back = lambda pairs, pages: back
     for k_size, v_size, q_size in ((2.0**20, 2.0**-40, 2.0**-20), (2.0**-60, 2.0**50, 2.0**55), (2.0**10, 2.0**-100, 2.0**-9)):
         block, own = pages.block(DEV, 100), pages.block(DEV, 3, room=20)
         slots = torch.cat([Q.slots_of(block), Q.slots_of(own, 23)])
@@ -140,8 +142,9 @@ def test_rows_read_back_over_a_wide_range(codes):
         step = Q.prefill_step(op, [([block], own, 20)])
         q = (torch.randn(20, 8 * 64, generator=g) * q_size).to(BF16).to(DEV)
         out, lse = op.attend(q, 0, step.meta, return_lse=True)
+        assert (step.meta.launch.readback is not None) == back
         check(op, step, q, [0], [20], out, lse)
-        pages = Q.Pages(40, 16)
+        pages = Q.Pages(40, page)
 
 
 def test_queries_on_rows_apart_and_given_outputs():
