@@ -5,7 +5,10 @@
 //   K: lane (j, kg) of a 16-token half takes bytes [64 s + 16 kg, + 16) of token j: the contraction elements of steps
 //      2 s and 2 s + 1 of the products as they are.
 //   V: the same pieces go through LDS (eight tokens of a dim in one ds_read_b64_tr_b8).
-// Half lines a load cost it bandwidth (pages of 16 tokens: 5.7 TB/s, 6.8 in whole lines), which scattered rows do anyway.
+// Half lines a load cost it bandwidth (pages of 16 tokens: 5.7 TB/s, 6.8 in whole lines), which scattered rows do anyway: 8
+// requests of 40 k tokens (0.6 GB) 105 us in pages of 16, here 128 to 134 in pages of 8 or 48 and 151 / 169 / 205 at 256 / 128 / 64
+// dims in pages of one, whose scale bytes come in a line each.  Two, three and four workgroups a CU at these dims: 64 requests
+// over 8192 tokens and blocks of 256..8192, pages of 8, two / now, 233 / 215 at 128 dims, 244 / 220 at 64.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -27,6 +30,7 @@ struct ScatteredShape {
   static constexpr int kTileBytes = kQuantTokens * kD;         // V of a tile
   static constexpr int kWaveBytes = kTileBytes + 2 * kQuantTokens * 4;  // and its scales, K then V
   static constexpr int kQueryBytes = 2 * 16 * kD * 2;          // hi and lo rows
+  static constexpr int kMinBlocks = kD == 64 ? 4 : kD == 128 ? 3 : 2;  // workgroups per CU
   static constexpr int kLoopBytes = kQuantWaves * kWaveBytes + kQueryBytes;
   static constexpr int kFold = kQuantWaves * QuantFold<kD>::kBytes;
   static constexpr int kLdsBytes = kLoopBytes > kFold ? kLoopBytes : kFold;
@@ -42,7 +46,7 @@ __device__ __forceinline__ int quant_swz(int t) {
 }
 
 template <int kD, typename C>
-__global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(QuantAttnArgs qa, int dtype, int pieces) {
+__global__ __launch_bounds__(kQuantThreads, ScatteredShape<kD>::kMinBlocks) void attn_quant_scattered_kernel(QuantAttnArgs qa, int dtype, int pieces) {
   const AttnArgs& a = qa.a;
   using Sh = ScatteredShape<kD>;
   constexpr int kPieces = Sh::kPieces, kSteps = Sh::kSteps, kDimTiles = Sh::kDimTiles;
@@ -156,13 +160,13 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
     }
     __syncthreads();
     // B operands: step 2 s + b holds dims [64 s + 16 kg + 8 b, + 8) of row j
-    // (at 256 dims they are read anew for every tile: held in registers they take the kernel over half of them, and one
-    // workgroup a CU does not cover the latency of its loads; a tile's 32 KB of LDS traffic are a fifth of its time)
-    constexpr bool kKeepQuery = kD < 256;
-    va_u32x4 q_hi[kKeepQuery ? kSteps : 1], q_lo[kKeepQuery ? kSteps : 1];
+    // (but at 64 dims they are read anew for every tile, and low parts are everywhere: held in registers they cost workgroups a
+    // CU, which cover the latency of each other's loads)
+    constexpr bool kKeepQuery = kD < 128;
+    va_u32x4 q_hi[kKeepQuery ? kSteps : 1];
     if constexpr (kKeepQuery) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) q_hi[s] = staged_query<kD>(query, s), q_lo[s] = staged_query<kD>(query + 32 * kD, s);
+      for (int s = 0; s < kSteps; ++s) q_hi[s] = staged_query<kD>(query, s);
     }
 
     // ---- the tile loop ----
@@ -179,24 +183,22 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
         read_entries(i + 2);
       }
 
-      va_f32x4 hi[2], lo[2];
+      va_f32x4 dots[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) hi[u] = lo[u] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < 2; ++u) dots[u] = va_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        va_u32x4 high, low;
-        if constexpr (kKeepQuery) {
-          high = q_hi[s], low = q_lo[s];
-        } else {
-          high = staged_query<kD>(query, s), low = staged_query<kD>(query + 32 * kD, s);
-        }
+        const va_u32x4 high = kKeepQuery ? q_hi[kKeepQuery ? s : 0] : staged_query<kD>(query, s);
+        const va_u32x4 low = staged_query<kD>(query + 32 * kD, s);
+        va_u32x4 k8[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const va_u32x4 raw = kraw[u][s / 2];
-          const va_u32x4 k8 = C::bf16x8(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]});
-          hi[u] = Mma<BF16>::run(k8, high, hi[u]);
-          lo[u] = Mma<BF16>::run(k8, low, lo[u]);
+          k8[u] = C::bf16x8(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]});
+          dots[u] = Mma<BF16>::run(k8[u], high, dots[u]);
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) dots[u] = Mma<BF16>::run(k8[u], low, dots[u]);
       }
       if (i + 1 < n_tiles) load_k();
 
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(kQuantThreads, 2) void attn_quant_scattered_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const bool seen = t0 + 16 * u + 4 * kg + r < t_row;
-          sc[u][r] = seen ? (hi[u][r] + lo[u][r]) * ks[r] : -INFINITY;
+          sc[u][r] = seen ? dots[u][r] * ks[r] : -INFINITY;
           vs[u][r] = seen ? v4[r] : 0.f;
           most = fmaxf(most, sc[u][r]);
         }
