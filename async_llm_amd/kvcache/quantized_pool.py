@@ -105,7 +105,7 @@ class QuantizedKVCache:
         shape = (slots.numel(), self._num_kv_heads, self._head_dim)
         width = self._num_kv_heads * self._head_dim
         if out is None:
-            k = torch.empty(shape, dtype=self._dtype, device=device)
+            k = torch.empty_strided(shape, (width, self._head_dim, 1), dtype=self._dtype, device=device)
             v = torch.empty_like(k)
             stride = width
         else:
