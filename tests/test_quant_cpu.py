@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from async_llm_amd import native
+from async_llm_amd.attention_backend import ViewAttnBackend
 from async_llm_amd.kvcache import MHAKVCache, QuantizedKVCache
 from async_llm_amd.shared_cache import BlockKVOps, CacheBlock, PrefillSpec, QuantizedCacheAttention, SharedCacheAttention, WorkerGroup
 from async_llm_amd.shared_cache.attention_graph import SharedDecodeAttentionBuffers, SharedPrefillAttentionBuffers
@@ -95,6 +96,8 @@ def test_ops_that_do_not_fit_their_pool():
         QuantizedCacheAttention(pool, table, 8, 2, 64, 16, BF16, torch.device("meta"))
     with pytest.raises(ValueError):
         BlockKVOps(pool, make()[0], None)
+    with pytest.raises(TypeError):
+        ViewAttnBackend(SimpleNamespace(num_qo_heads=8, num_kv_heads=2, head_dim=64), pool, torch.zeros(1, 8, dtype=torch.int32))
     with pytest.raises(IndexError):
         pool.layer(2)
     with pytest.raises(IndexError):
