@@ -54,7 +54,7 @@ struct QuantRing {
   // Low parts of the query in registers, where there are any to spare (read from LDS for each tile at 128 dims: 28 rows of 7 k
   // shared and up to 16 k tokens 94.7 us instead of 92.5).
   static constexpr bool kKeepLow = kD < 256;
-  static constexpr int kQueryBytes = 16 * kD * 2;       // high or low parts of a tile's query: staged one after the other
+  static constexpr int kQueryBytes = (kKeepLow ? 2 : 1) * 16 * kD * 2;  // parts of a tile's query
   static constexpr int kLdsBytes = kQueryOffset + kQueryBytes;
   static_assert(kQuantWaves * QuantFold<kD>::kBytes <= kLdsBytes, "room for the waves' states");
   static_assert(kMinBlocks * kLdsBytes <= 160 * 1024, "the LDS of a CU");
@@ -219,21 +219,25 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
       }
     const QueryPieces mine = turned_query<kD>(a, source, hk, dtype, pieces);
     if (li > 0) ring_barrier<kAnyInFlight>();  // every wave has read what lay there
-    stage_query<kD>(mine, 0, query);
-    ring_barrier<kAnyInFlight>();
     va_u32x4 q_hi[kSteps], q_lo[Sh::kKeepLow ? kSteps : 1];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) q_hi[s] = staged_query<kD>(query, s);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q_hi[s]));
-    ring_barrier<kAnyInFlight>();
-    stage_query<kD>(mine, 1, query);
-    ring_barrier<kAnyInFlight>();
     if constexpr (Sh::kKeepLow) {
+      stage_query<kD>(mine, 0, query);
+      stage_query<kD>(mine, 1, query + 32 * kD);
+      ring_barrier<kAnyInFlight>();
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) q_lo[s] = staged_query<kD>(query, s);
+      for (int s = 0; s < kSteps; ++s) q_hi[s] = staged_query<kD>(query, s), q_lo[s] = staged_query<kD>(query + 32 * kD, s);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q_lo[s]));
+      for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q_hi[s]), "+v"(q_lo[s]));
+    } else {  // one after the other through the same room
+      stage_query<kD>(mine, 0, query);
+      ring_barrier<kAnyInFlight>();
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) q_hi[s] = staged_query<kD>(query, s);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q_hi[s]));
+      ring_barrier<kAnyInFlight>();
+      stage_query<kD>(mine, 1, query);
+      ring_barrier<kAnyInFlight>();
     }
 
     // ---- the tile loop ----
