@@ -19,6 +19,7 @@ struct E4M3 {
   static constexpr int kTopExponent = 8;
   // 1.875 * 2^127 (code 240): what a larger number would round to, 2^128, is no fp32 number
   static constexpr uint32_t kLimit = 0x7f700000u;
+  static constexpr uint32_t kNotZero = 0x7f7f7f7fu;  // bits of four codes of which one at least is set where not all are zero
   static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);  // round to nearest even; no value exceeds 448
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
@@ -42,6 +43,7 @@ struct INT8 {
   static constexpr uint32_t kTopMantissa = 0x7E0000u;  // largest code 127 = 1.984375 * 2^6
   static constexpr int kTopExponent = 6;
   static constexpr uint32_t kLimit = 0x7f7e0000u;  // 127 * 2^121, as above
+  static constexpr uint32_t kNotZero = 0xffffffffu;
   static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
     const uint32_t x = (uint8_t)(int)rintf(a), y = (uint8_t)(int)rintf(b), z = (uint8_t)(int)rintf(c), w = (uint8_t)(int)rintf(d);
     return x | (y << 8) | (z << 16) | (w << 24);

@@ -48,8 +48,10 @@ __device__ __forceinline__ long long quant_token_row(const QuantAttnArgs& qa, in
 
 // The matrix-core kernels: 16-bit activations, head_dim 64, 128 or 256.  Tiles of whole pages (va_quant_stream.hip), or tokens
 // looked up one by one (va_quant_scattered.hip: pages of fewer than 16 tokens or of a number that no power of two is).
-// `pieces`: q rows start on 16-byte boundaries, out on 8-byte ones.
-int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream);
-int launch_quant_scattered(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int pieces, hipStream_t stream);
+// `pieces`: q rows start on 16-byte boundaries, out on 8-byte ones.  `only_if`: where it is given and holds 0 when the launch
+// runs, all workgroups leave at once.  Such launches have kernels of their own: asked in the others, it takes 0.4 us of a
+// step of 13.5.
+int launch_quant_mfma(const QuantAttnArgs& qa, const int32_t* only_if, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream);
+int launch_quant_scattered(const QuantAttnArgs& qa, const int32_t* only_if, int dtype, int code_type, int n_items, int pieces, hipStream_t stream);
 
 }  // namespace va

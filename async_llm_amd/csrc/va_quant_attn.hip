@@ -277,11 +277,11 @@ static int launch_quant_any(const QuantAttnArgs& qa, int dtype, int n_items, hip
 
 }  // namespace va
 
-extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
-                               const int32_t* plan_header_host, const int32_t* kv_indices_dev,
-                               const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
-                               void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
-                               int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream) {
+static int attention_q8(const int32_t* only_if, const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool,
+                        const int32_t* plan_dev, const int32_t* plan_header_host, const int32_t* kv_indices_dev,
+                        const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
+                        void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
+                        int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream) {
   if (!shape || !plan_header_host || !plan_dev) return va_fail(VA_ERR_ARG, "null plan or shape");
   int rc = va::check_quant_pool(pool, shape);
   if (rc) return rc;
@@ -291,6 +291,9 @@ extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const Va
   if (h[VA_H_MAGIC] != VA_PLAN_MAGIC) return va_fail(VA_ERR_ARG, "plan header has no magic word");
   if (h[VA_H_N_ROWS] == 0) return VA_OK;
   if (h[VA_H_N_WIDE] != 0) return va_fail(VA_ERR_ARG, "a plan over a quantised pool has no wide items (wide_tile < 0)");
+  if (only_if && (h[VA_H_N_PARTIALS] > 0 || h[VA_H_N_EMPTY_ROWS] > 0))
+    return va_fail(VA_ERR_ARG, "a launch under a condition takes plans without partial states and empty rows");
+  if (only_if && h[VA_H_KERNEL] != VA_KERNEL_MFMA) return va_fail(VA_ERR_ARG, "a launch under a condition takes matrix-core plans");
   va::QuantAttnArgs qa;
   va::MergeArgs m;
   rc = va::plan_arguments(q_dev, q_row_stride, pool->k_codes_dev, pool->v_codes_dev, 0, plan_dev, h, kv_indices_dev,
@@ -305,7 +308,7 @@ extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const Va
   const int n_items = h[VA_H_N_ITEMS];
   if (n_items > 0) {
     if (h[VA_H_KERNEL] == VA_KERNEL_MFMA)
-      rc = va::launch_quant_mfma(qa, shape->dtype, pool->code_type, n_items, h[VA_H_Q_TILE], s);
+      rc = va::launch_quant_mfma(qa, only_if, shape->dtype, pool->code_type, n_items, h[VA_H_Q_TILE], s);
     else
       rc = pool->code_type == VA_CODE_E4M3 ? va::launch_quant_any<va::E4M3>(qa, shape->dtype, n_items, s)
                                            : va::launch_quant_any<va::INT8>(qa, shape->dtype, n_items, s);
@@ -314,4 +317,23 @@ extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const Va
   if (h[VA_H_N_PARTIALS] > 0 || h[VA_H_N_EMPTY_ROWS] > 0)
     rc = va::launch_merge_typed(m, shape->dtype, h[VA_H_N_ROWS], h[VA_H_MERGE_WAVES], s);
   return rc;
+}
+
+extern "C" int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
+                               const int32_t* plan_header_host, const int32_t* kv_indices_dev,
+                               const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
+                               void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
+                               int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream) {
+  return attention_q8(nullptr, q_dev, q_row_stride, pool, plan_dev, plan_header_host, kv_indices_dev, sub_worker_dev, sub_loc_dev,
+                      sub_loc_axis_stride, out_dev, lse_dev, lse_base2, workspace_dev, workspace_bytes, shape, rope, stream);
+}
+
+extern "C" int va_attention_if_q8(const int32_t* condition_dev, const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool,
+                                  const int32_t* plan_dev, const int32_t* plan_header_host, const int32_t* kv_indices_dev,
+                                  const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
+                                  void* out_dev, float* lse_dev, int32_t lse_base2, const VaShape* shape, const VaRope* rope,
+                                  void* stream) {
+  if (!condition_dev) return va_fail(VA_ERR_ARG, "null condition");
+  return attention_q8(condition_dev, q_dev, q_row_stride, pool, plan_dev, plan_header_host, kv_indices_dev, sub_worker_dev,
+                      sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev, lse_base2, nullptr, 0, shape, rope, stream);
 }

@@ -10,9 +10,16 @@
 // what float16 lacks; it is given by powers of two, exactly:
 //   K' = K 2^-b,  q' = q 2^b,  V' = V 2^-s,  out = out' 2^s
 // with b and s from the largest scales among the rows, found by a pass over the scale bytes.  Beside float16's relative
-// errors this leaves absolute ones of 2^-25, half of its smallest step: 2^-39 of the largest value for V' and out', and
-// 2^-17 / sqrt(D) of a score for each q' element below 2^-14.  Keys up to 2^8 leave queries of |q_i| max|K| < 1.0e7 within
-// float16 after their rotation; larger ones are held there (32 bits leave their scores a step of one).
+// errors this leaves absolute ones of 2^-25, half of its smallest step: 2^-39 of the largest value for V' and out', 2^-17 /
+// sqrt(D) of a score for each q' element below 2^-14 (K' is at most 2^8), and 2^-25 q' / sqrt(D) for each K' element below it.
+//
+// One b and one s serve all heads and requests of a launch, whose rows need not be of a size.  Where float16 would lose what
+// codes keep, the launch says so in the scratch's first word, and its results are taken from the codes (va_attention_if_q8):
+//   * a query element is over kMostQuery = 2^9 in front of its rotation, |q_i| max|K| > 1.1e5: below it the errors of all D
+//     elements of K' add up to 2^-12 of a score at most, whatever their size, and nothing overflows;
+//   * a value row's scale is more than kMostSpread = 16 powers of two under the largest one, and the row is not zero: above
+//     that its codes are exact in V' (e4m3 the multiples of 2^(6 - 9 - 16), int8 of 2^(7 - 16)), and the row's largest is over
+//     2^-4, 2^21 times the absolute error.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -45,7 +52,8 @@ struct BackArgs {
   uint32_t num_slots;
   int num_kv_heads, head_dim;
   PageMap pages;
-  uint32_t* tops;  // [kBackGroups][2]: largest scale bytes of keys and values
+  int32_t* beyond;  // whether float16 does not hold the launch's numbers
+  uint32_t* tops;   // [kBackGroups][2]: largest scale bytes of keys and values
   __half* rows[2];
   const void* q;
   long long q_row_stride;
@@ -62,6 +70,7 @@ __device__ __forceinline__ bool back_slot(const BackArgs& a, long long i, uint32
 
 // The largest scales of a stride of the slots (255 marks rows of NaN; 1 is the least there is).
 __global__ __launch_bounds__(256) void quant_top_kernel(BackArgs a) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.beyond = 0;
   uint32_t top[2] = {1, 1};
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < a.n_slots; i += kBackGroups * 256ll) {
     uint32_t slot;
@@ -95,12 +104,8 @@ __device__ __forceinline__ int back_top(const uint32_t* tops, int which) {  // (
   return (int)top;
 }
 
-// A query element for float16: a rotation makes it larger by sqrt(2) at most, and 46000 sqrt(2) < 65504.  Infinities and
-// NaN stay.
-__device__ __forceinline__ __half back_query(float x, float f) {
-  const float y = x * f;
-  return __float2half_rn(fabsf(x) < INFINITY ? fminf(46000.f, fmaxf(-46000.f, y)) : x);
-}
+constexpr float kMostQuery = 512.f;
+constexpr int kMostSpread = 16;
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)min(254, max(0, e + 127)) << 23); }
 
 // K (blockIdx.y 0), V (1) and the queries (2) as float16, eight elements a thread.
@@ -109,6 +114,7 @@ __global__ __launch_bounds__(256) void quant_back_kernel(BackArgs a, long long r
   const long long idx = blockIdx.x * 256ll + threadIdx.x;
   const int which = blockIdx.y;
   const int top = back_top(a.tops, which == 1 ? 1 : 0);
+  bool beyond = which == 2 && top - 127 - BackScale<C>::kKey > 127;  // (no scale of this library's stores)
   union {
     uint4 raw;
     __half e[8];
@@ -132,6 +138,7 @@ __global__ __launch_bounds__(256) void quant_back_kernel(BackArgs a, long long r
       C::unpack4(codes.y, x + 4);
 #pragma unroll
       for (int k = 0; k < 8; ++k) y.e[k] = nan && !which ? __float2half_rn(NAN) : __float2half_rn(x[k] * f);
+      beyond = which && !nan && (int)e < top - kMostSpread && ((codes.x | codes.y) & C::kNotZero) != 0;
     }
     *(uint4*)((which ? a.rows[1] : a.rows[0]) + idx * 8) = y.raw;
   } else {
@@ -139,20 +146,25 @@ __global__ __launch_bounds__(256) void quant_back_kernel(BackArgs a, long long r
     const int per_row = a.q_width / 8;
     const long long row = idx / per_row, at = row * a.q_row_stride + (idx - row * per_row) * 8;
     const float f = power_of_two(top - 127 - BackScale<C>::kKey);
+    auto query = [&](float x) __attribute__((always_inline)) {
+      beyond = beyond || fabsf(x * f) > kMostQuery;  // (a NaN makes one of its own row either way)
+      return __float2half_rn(x * f);
+    };
     if (pieces) {
       const uint4 w = *(const uint4*)((const uint16_t*)a.q + at);
       const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const uint16_t b = (uint16_t)(words[k / 2] >> (16 * (k % 2)));
-        y.e[k] = back_query(a.dtype == VA_BF16 ? BF16::load(b) : __half2float(__builtin_bit_cast(__half, b)), f);
+        y.e[k] = query(a.dtype == VA_BF16 ? BF16::load(b) : __half2float(__builtin_bit_cast(__half, b)));
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) y.e[k] = back_query(activation(a.q, at + k, a.dtype), f);
+      for (int k = 0; k < 8; ++k) y.e[k] = query(activation(a.q, at + k, a.dtype));
     }
     *(uint4*)(a.q16 + idx * 8) = y.raw;
   }
+  if (beyond) *a.beyond = 1;  // (all that write it write the same)
 }
 
 // Results in the activations' type, eight elements a thread.  A row that a NaN reached has NaN for its lse (the attention's
@@ -184,13 +196,14 @@ __global__ __launch_bounds__(256) void quant_results_kernel(const __half* from, 
 }
 
 struct BackLayout {
-  int64_t rows[2], q, out, bytes;
+  int64_t tops, rows[2], q, out, bytes;
 };
 static BackLayout back_layout(int64_t n_slots, int64_t n_rows, const VaShape* s) {
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   const int64_t kv = up(2 * n_slots * s->num_kv_heads * s->head_dim), q = up(2 * n_rows * s->num_q_heads * s->head_dim);
   BackLayout l;
-  l.rows[0] = up(kBackGroups * 2 * 4);
+  l.tops = 256;  // (behind the word that says whether float16 holds the launch)
+  l.rows[0] = l.tops + up(kBackGroups * 2 * 4);
   l.rows[1] = l.rows[0] + kv;
   l.q = l.rows[1] + kv;
   l.out = l.q + q;
@@ -255,7 +268,8 @@ extern "C" int va_attention_read_back_q8(const void* q_dev, int64_t q_row_stride
   va::BackArgs a{{(const uint8_t*)pool->k_codes_dev, (const uint8_t*)pool->v_codes_dev},
                  {pool->k_scales_dev, pool->v_scales_dev}, slots_dev, n_slots,
                  (uint32_t)pool->num_pages * (uint32_t)shape->page_size, shape->num_kv_heads, shape->head_dim,
-                 va::page_map(shape->page_size), (uint32_t*)scratch, {(__half*)(scratch + l.rows[0]), (__half*)(scratch + l.rows[1])},
+                 va::page_map(shape->page_size), (int32_t*)scratch, (uint32_t*)(scratch + l.tops),
+                 {(__half*)(scratch + l.rows[0]), (__half*)(scratch + l.rows[1])},
                  q_dev, q_row_stride, (__half*)(scratch + l.q), n_rows, width, shape->dtype};
   const int pieces = (uintptr_t)q_dev % 16 == 0 && q_row_stride % 8 == 0;
   const bool e4m3 = pool->code_type == VA_CODE_E4M3;

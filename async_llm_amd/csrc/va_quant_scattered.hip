@@ -46,7 +46,7 @@ __device__ __forceinline__ int quant_swz(int t) {
 }
 
 template <int kD, typename C>
-__global__ __launch_bounds__(kQuantThreads, ScatteredShape<kD>::kMinBlocks) void attn_quant_scattered_kernel(QuantAttnArgs qa, int dtype, int pieces) {
+__device__ __forceinline__ void quant_scattered_item(const QuantAttnArgs& qa, int dtype, int pieces) {
   const AttnArgs& a = qa.a;
   using Sh = ScatteredShape<kD>;
   constexpr int kPieces = Sh::kPieces, kSteps = Sh::kSteps, kDimTiles = Sh::kDimTiles;
@@ -258,32 +258,47 @@ __global__ __launch_bounds__(kQuantThreads, ScatteredShape<kD>::kMinBlocks) void
 }
 
 template <int kD, typename C>
-static int launch_quant_scattered_one(const QuantAttnArgs& qa, int dtype, int n_items, int pieces, hipStream_t stream) {
+__global__ __launch_bounds__(kQuantThreads, ScatteredShape<kD>::kMinBlocks) void attn_quant_scattered_kernel(QuantAttnArgs qa, int dtype, int pieces) {
+  quant_scattered_item<kD, C>(qa, dtype, pieces);
+}
+template <int kD, typename C>
+__global__ __launch_bounds__(kQuantThreads, ScatteredShape<kD>::kMinBlocks) void attn_quant_scattered_if_kernel(QuantAttnArgs qa, const int32_t* only_if, int dtype,
+    int pieces) {
+  if (*only_if) quant_scattered_item<kD, C>(qa, dtype, pieces);
+}
+
+template <int kD, typename C>
+static int launch_quant_scattered_one(const QuantAttnArgs& qa, const int32_t* only_if, int dtype, int n_items, int pieces, hipStream_t stream) {
   const dim3 grid((unsigned)n_items * (unsigned)qa.a.num_kv_heads), block(kQuantThreads);
   constexpr int bytes = ScatteredShape<kD>::kLdsBytes;
-  static std::atomic<unsigned long long> devices{0};
-  hipError_t e = allow_lds(reinterpret_cast<const void*>(&attn_quant_scattered_kernel<kD, C>), bytes, devices);
+  static std::atomic<unsigned long long> devices{0}, if_devices{0};
+  hipError_t e = only_if ? allow_lds(reinterpret_cast<const void*>(&attn_quant_scattered_if_kernel<kD, C>), bytes, if_devices)
+                         : allow_lds(reinterpret_cast<const void*>(&attn_quant_scattered_kernel<kD, C>), bytes, devices);
   if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
-  hipLaunchKernelGGL((attn_quant_scattered_kernel<kD, C>), grid, block, bytes, stream, qa, dtype, pieces);
+  if (only_if) {
+    hipLaunchKernelGGL((attn_quant_scattered_if_kernel<kD, C>), grid, block, bytes, stream, qa, only_if, dtype, pieces);
+  } else {
+    hipLaunchKernelGGL((attn_quant_scattered_kernel<kD, C>), grid, block, bytes, stream, qa, dtype, pieces);
+  }
   e = hipGetLastError();
   return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "quantised attention launch: %s", hipGetErrorString(e));
 }
 
 template <typename C>
-static int launch_quant_scattered_coded(const QuantAttnArgs& qa, int dtype, int n_items, int pieces, hipStream_t stream) {
+static int launch_quant_scattered_coded(const QuantAttnArgs& qa, const int32_t* only_if, int dtype, int n_items, int pieces, hipStream_t stream) {
   switch (qa.a.head_dim) {
     case 64:
-      return launch_quant_scattered_one<64, C>(qa, dtype, n_items, pieces, stream);
+      return launch_quant_scattered_one<64, C>(qa, only_if, dtype, n_items, pieces, stream);
     case 128:
-      return launch_quant_scattered_one<128, C>(qa, dtype, n_items, pieces, stream);
+      return launch_quant_scattered_one<128, C>(qa, only_if, dtype, n_items, pieces, stream);
     default:
-      return launch_quant_scattered_one<256, C>(qa, dtype, n_items, pieces, stream);
+      return launch_quant_scattered_one<256, C>(qa, only_if, dtype, n_items, pieces, stream);
   }
 }
 
-int launch_quant_scattered(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int pieces, hipStream_t stream) {
-  return code_type == VA_CODE_E4M3 ? launch_quant_scattered_coded<E4M3>(qa, dtype, n_items, pieces, stream)
-                                   : launch_quant_scattered_coded<INT8>(qa, dtype, n_items, pieces, stream);
+int launch_quant_scattered(const QuantAttnArgs& qa, const int32_t* only_if, int dtype, int code_type, int n_items, int pieces, hipStream_t stream) {
+  return code_type == VA_CODE_E4M3 ? launch_quant_scattered_coded<E4M3>(qa, only_if, dtype, n_items, pieces, stream)
+                                   : launch_quant_scattered_coded<INT8>(qa, only_if, dtype, n_items, pieces, stream);
 }
 
 }  // namespace va

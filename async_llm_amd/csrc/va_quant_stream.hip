@@ -74,7 +74,7 @@ __device__ __forceinline__ void load_run_to_lds(const void* base, uint32_t lane_
 #undef VA_ONE_LOAD
 }
 template <int kD, typename C>
-__global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn_quant_stream_kernel(QuantAttnArgs qa, int dtype, int pieces) {
+__device__ __forceinline__ void quant_stream_item(const QuantAttnArgs& qa, int dtype, int pieces) {
   const AttnArgs& a = qa.a;
   using Sh = QuantRing<kD>;
   using Words = const __attribute__((address_space(4))) int32_t*;
@@ -369,30 +369,45 @@ __global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn
 }
 
 template <int kD, typename C>
-static int launch_quant_stream_one(const QuantAttnArgs& qa, int dtype, int n_items, int pieces, hipStream_t stream) {
+__global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn_quant_stream_kernel(QuantAttnArgs qa, int dtype, int pieces) {
+  quant_stream_item<kD, C>(qa, dtype, pieces);
+}
+template <int kD, typename C>
+__global__ __launch_bounds__(kQuantThreads, QuantRing<kD>::kMinBlocks) void attn_quant_stream_if_kernel(QuantAttnArgs qa, const int32_t* only_if, int dtype,
+    int pieces) {
+  if (*only_if) quant_stream_item<kD, C>(qa, dtype, pieces);
+}
+
+template <int kD, typename C>
+static int launch_quant_stream_one(const QuantAttnArgs& qa, const int32_t* only_if, int dtype, int n_items, int pieces, hipStream_t stream) {
   const dim3 grid((unsigned)n_items * (unsigned)qa.a.num_kv_heads), block(kQuantThreads);
   constexpr int bytes = QuantRing<kD>::kLdsBytes;
-  static std::atomic<unsigned long long> devices{0};
-  hipError_t e = allow_lds(reinterpret_cast<const void*>(&attn_quant_stream_kernel<kD, C>), bytes, devices);
+  static std::atomic<unsigned long long> devices{0}, if_devices{0};
+  hipError_t e = only_if ? allow_lds(reinterpret_cast<const void*>(&attn_quant_stream_if_kernel<kD, C>), bytes, if_devices)
+                         : allow_lds(reinterpret_cast<const void*>(&attn_quant_stream_kernel<kD, C>), bytes, devices);
   if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
-  hipLaunchKernelGGL((attn_quant_stream_kernel<kD, C>), grid, block, bytes, stream, qa, dtype, pieces);
+  if (only_if) {
+    hipLaunchKernelGGL((attn_quant_stream_if_kernel<kD, C>), grid, block, bytes, stream, qa, only_if, dtype, pieces);
+  } else {
+    hipLaunchKernelGGL((attn_quant_stream_kernel<kD, C>), grid, block, bytes, stream, qa, dtype, pieces);
+  }
   e = hipGetLastError();
   return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "quantised attention launch: %s", hipGetErrorString(e));
 }
 
 template <typename C>
-static int launch_quant_stream_coded(const QuantAttnArgs& qa, int dtype, int n_items, int pieces, hipStream_t stream) {
+static int launch_quant_stream_coded(const QuantAttnArgs& qa, const int32_t* only_if, int dtype, int n_items, int pieces, hipStream_t stream) {
   switch (qa.a.head_dim) {
     case 64:
-      return launch_quant_stream_one<64, C>(qa, dtype, n_items, pieces, stream);
+      return launch_quant_stream_one<64, C>(qa, only_if, dtype, n_items, pieces, stream);
     case 128:
-      return launch_quant_stream_one<128, C>(qa, dtype, n_items, pieces, stream);
+      return launch_quant_stream_one<128, C>(qa, only_if, dtype, n_items, pieces, stream);
     default:
-      return launch_quant_stream_one<256, C>(qa, dtype, n_items, pieces, stream);
+      return launch_quant_stream_one<256, C>(qa, only_if, dtype, n_items, pieces, stream);
   }
 }
 
-int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream) {
+int launch_quant_mfma(const QuantAttnArgs& qa, const int32_t* only_if, int dtype, int code_type, int n_items, int q_tile, hipStream_t stream) {
   const AttnArgs& a = qa.a;
   const int g = a.num_q_heads / a.num_kv_heads;
   if (!va_mfma_supported(dtype, a.head_dim, g))
@@ -405,9 +420,9 @@ int launch_quant_mfma(const QuantAttnArgs& qa, int dtype, int code_type, int n_i
   // queries and results in 16-byte (8-byte) accesses where their addresses allow it
   const int pieces = a.q_row_stride % 8 == 0 && (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.out % 8 == 0;
   // The choice hangs on the page size alone, so that a recorded launch keeps its kernel.
-  if (qa.pages.shift < 4) return launch_quant_scattered(qa, dtype, code_type, n_items, pieces, stream);
-  return code_type == VA_CODE_E4M3 ? launch_quant_stream_coded<E4M3>(qa, dtype, n_items, pieces, stream)
-                                   : launch_quant_stream_coded<INT8>(qa, dtype, n_items, pieces, stream);
+  if (qa.pages.shift < 4) return launch_quant_scattered(qa, only_if, dtype, code_type, n_items, pieces, stream);
+  return code_type == VA_CODE_E4M3 ? launch_quant_stream_coded<E4M3>(qa, only_if, dtype, n_items, pieces, stream)
+                                   : launch_quant_stream_coded<INT8>(qa, only_if, dtype, n_items, pieces, stream);
 }
 
 }  // namespace va

@@ -48,6 +48,7 @@ EXPORTED_SYMBOLS = (
     "va_load_kv_q8",
     "va_copy_shift_kv_q8",
     "va_attention_q8",
+    "va_attention_if_q8",
     "va_read_back_bytes",
     "va_attention_read_back_q8",
 )
@@ -197,6 +198,9 @@ def _load() -> C.CDLL:
     lib.va_attention_q8.restype = C.c_int
     lib.va_attention_q8.argtypes = [vp, i64, pool, vp, vp, vp, vp, vp, i64, vp, vp, i32, vp, i64,
                                     C.POINTER(VaShape), C.POINTER(VaRope), vp]
+    lib.va_attention_if_q8.restype = C.c_int
+    lib.va_attention_if_q8.argtypes = [vp, vp, i64, pool, vp, vp, vp, vp, vp, i64, vp, vp, i32, C.POINTER(VaShape),
+                                       C.POINTER(VaRope), vp]
     lib.va_read_back_bytes.restype = C.c_int64
     lib.va_read_back_bytes.argtypes = [i64, i64, C.POINTER(VaShape)]
     lib.va_attention_read_back_q8.restype = C.c_int

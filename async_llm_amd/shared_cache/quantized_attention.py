@@ -15,8 +15,11 @@ differs from one over the read-back values by the rounding of the result.
 Chunks of many new tokens read a token so often that it is converted once: their pages
 are read back as float16, within range by powers of two, and the 16-bit attention's
 matrix-core kernels run over that, in float16 for bf16 activations as well (its eleven bits
-keep the operands' roundings under the result's).  Plans over a workspace reserved by
-``prepare_workspace`` never do.
+keep the operands' roundings under the result's).  One pair of powers serves a whole step, so
+one whose rows differ too much in size for float16 -- a key of 1e6 in any of its requests, a
+value 2^16 times as large as another -- is answered over the codes after all: the launch over
+them stands behind the others and runs where these found that.  Plans over a workspace reserved
+by ``prepare_workspace`` never read back.
 
 The reference has no such cache; its path over 16-bit pools is
 ``python/minisgl/shared_cache/attention.py:624-752``.
@@ -45,7 +48,8 @@ class ReadBack:
     sub_worker: torch.Tensor
     first_subrow: int
     slots: torch.Tensor  # int64, of every token of every page that it reads, -1 behind the last token of a page
-    scratch: torch.Tensor
+    scratch: torch.Tensor  # its first word: whether float16 did not hold the step
+    codes: LaunchPlan  # the same rows over the codes, for that case
 
 
 class QuantizedCacheAttention(SharedCacheAttention):
@@ -73,6 +77,8 @@ class QuantizedCacheAttention(SharedCacheAttention):
         p = self.plan_params
         self._read_back_params = native.VaPlanParams(p.kernel, p.q_tile, p.kv_chunk, p.target_items, p.wide_tile)
         p.wide_tile = -2  # codes are read by tiles of up to 16 rows, a workgroup each
+        # one work item a tile: nothing to merge, no workspace
+        self._uncut_params = native.VaPlanParams(p.kernel, p.q_tile, p.kv_chunk, 1, p.wide_tile)
         self._read_back_shape = native.make_shape(num_qo_heads, num_kv_heads, head_dim, page_size, torch.float16)
         self._matrix_core = p.kernel != native.VA_KERNEL_GENERIC and dtype != torch.float32 and head_dim in (64, 128, 256) \
             and num_qo_heads // num_kv_heads in (1, 2, 4, 8, 16)
@@ -121,13 +127,16 @@ class QuantizedCacheAttention(SharedCacheAttention):
         slots = np.where(within < held[pages, None], pages[:, None] * self.page_size + within, -1).reshape(-1)
         rows = np.asarray(sub_worker_host)[first_subrow:]
         first_row = int(rows.min())
+        relative = (qo[n_codes:] - first_subrow, kvp[n_codes:] - first_entry)
+        described = (seq_lens[n_codes:], flags[n_codes:], chain[n_codes:], rows - first_row, n_rows - first_row)
+        over_codes, _ = super()._build_launch(*relative, kv[first_entry:], *described, (), refs, self._uncut_params)
+        assert not over_codes.counts.n_partials
         scratch = self._ensure_scratch(int(native.lib.va_read_back_bytes(len(slots), n_rows - first_row, self._shape)))
         more = () if n_codes else tuple(tables)
         wide, (dev_rows, dev_slots, *dev_tables) = super()._build_launch(
-            qo[n_codes:] - first_subrow, kvp[n_codes:] - first_entry, places, seq_lens[n_codes:], flags[n_codes:],
-            chain[n_codes:], rows - first_row, n_rows - first_row, (rows - first_row, slots, *more), refs,
-            self._read_back_params, self._read_back_shape)
-        back = ReadBack(wide, first_row, dev_rows, first_subrow, dev_slots, scratch)
+            *relative, places, *described, (rows - first_row, slots, *more), refs, self._read_back_params,
+            self._read_back_shape)
+        back = ReadBack(wide, first_row, dev_rows, first_subrow, dev_slots, scratch, over_codes)
         if n_codes:
             launch, dev_tables = super()._build_launch(qo[: n_codes + 1], kvp[: n_codes + 1], kv[:first_entry],
                                                        seq_lens[:n_codes], flags[:n_codes], chain[:n_codes],
@@ -204,15 +213,18 @@ class QuantizedCacheAttention(SharedCacheAttention):
                            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), self._shape, rope, stream)
         if back is not None:
             plan, item = back.launch, q2.element_size()
-            ws = plan.workspace
-            native.call_on(device, native.lib.va_attention_read_back_q8, q2.data_ptr() + back.first_row * q_stride * item,
-                           q_stride, pool, back.slots.data_ptr(), back.slots.numel(), plan.blob.data_ptr(), plan.header_ptr,
-                           plan.kv_indices.data_ptr(), back.sub_worker.data_ptr(),
-                           sub_loc.data_ptr() + 8 * back.first_subrow, axis_stride,
-                           out.data_ptr() + back.first_row * width * item,
-                           None if lse is None else lse_ptr + 4 * back.first_row * Hq, int(lse_base2),
-                           None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), back.scratch.data_ptr(),
+            ws, scratch = plan.workspace, back.scratch.data_ptr()
+            q_ptr = q2.data_ptr() + back.first_row * q_stride * item
+            rows = (back.sub_worker.data_ptr(), sub_loc.data_ptr() + 8 * back.first_subrow, axis_stride,
+                    out.data_ptr() + back.first_row * width * item,
+                    None if lse is None else lse_ptr + 4 * back.first_row * Hq, int(lse_base2))
+            native.call_on(device, native.lib.va_attention_read_back_q8, q_ptr, q_stride, pool, back.slots.data_ptr(),
+                           back.slots.numel(), plan.blob.data_ptr(), plan.header_ptr, plan.kv_indices.data_ptr(), *rows,
+                           None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), scratch,
                            back.scratch.numel(), self._shape, rope, stream)
+            plan = back.codes
+            native.call_on(device, native.lib.va_attention_if_q8, scratch, q_ptr, q_stride, pool, plan.blob.data_ptr(),
+                           plan.header_ptr, plan.kv_indices.data_ptr(), *rows, self._shape, rope, stream)
         return (out, lse) if return_lse else out
 
     # ------------------------------------------------------------------

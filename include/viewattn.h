@@ -422,6 +422,17 @@ VA_API int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuan
                     int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream);
 
 /*
+ * va_attention_if_q8: va_attention_q8 where *condition_dev is not 0 when the launch runs; where it is 0, out and lse stay
+ * as they are.  Matrix-core plans without partial states and empty rows only (chains under params->target_items = 1 have
+ * none).
+ */
+VA_API int va_attention_if_q8(const int32_t* condition_dev, const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool,
+                       const int32_t* plan_dev, const int32_t* plan_header_host, const int32_t* kv_indices_dev,
+                       const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
+                       void* out_dev, float* lse_dev, int32_t lse_base2, const VaShape* shape, const VaRope* rope,
+                       void* stream);
+
+/*
  * va_attention_read_back_q8: the same for many new tokens, which read a token so
  * often that it is converted once: the rows of slots_dev[0 .. n_slots) are read
  * back as float16 into a scratch pool, and va_attention runs over that with wide
@@ -431,8 +442,13 @@ VA_API int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuan
  * bring the largest row near the upper end of float16, queries by the inverse of the
  * keys' and results by that of the values'.  Queries (rotated), weights and results are
  * rounded to float16, with absolute errors of 2^-39 of the largest value for results;
- * a key or value row of NaN makes NaN of the results and the lse of those that see it;
- * query elements of |q_i| max|K| > 1.0e7 are held at that.  16-bit activations, head_dim
+ * a key or value row of NaN makes NaN of the results and the lse of those that see it.
+ * One power serves all rows of the call, whatever requests they belong to.  Where
+ * float16 does not hold them (a query element of |q_i| max|K| > 1.1e5, or a value row, not
+ * zero, whose scale is more than 2^16 times smaller than the largest) the first word of
+ * scratch_dev, an int32, is 1 behind the call, otherwise 0: where it is 1 the results are not
+ * to be used, and va_attention_if_q8 under that word puts those of the codes in their
+ * place.  16-bit activations, head_dim
  * 64, 128 or 256, and the matrix-core plans only (the plan is built for VA_F16).
  * scratch_dev, on a 256-byte boundary, must hold va_read_back_bytes(n_slots, rows of
  * the plan, shape).
