@@ -44,6 +44,12 @@ struct BackScale<INT8> {
   static constexpr int kKey = 1, kValue = 7;
 };
 
+// The least of the largest scales: rows that are all smaller lie lower in float16, and the powers that undo it, 2^(scale - 127 -
+// kKey) and 2^(scale - 127 - kValue), stay normal numbers of 32 bits.
+constexpr uint32_t kLeastTop = 8;
+static_assert((int)kLeastTop - 127 - BackScale<INT8>::kValue >= -126 && (int)kLeastTop - 127 - BackScale<E4M3>::kValue >= -126 &&
+              (int)kLeastTop - 127 - BackScale<INT8>::kKey >= -126, "powers of two that are not normal numbers");
+
 struct BackArgs {
   const uint8_t* codes[2];
   const uint8_t* scales[2];
@@ -68,10 +74,10 @@ __device__ __forceinline__ bool back_slot(const BackArgs& a, long long i, uint32
   return s >= 0 && s < (long long)a.num_slots;
 }
 
-// The largest scales of a stride of the slots (255 marks rows of NaN; 1 is the least there is).
+// The largest scales of a stride of the slots (255 marks rows of NaN), or kLeastTop.
 __global__ __launch_bounds__(256) void quant_top_kernel(BackArgs a) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.beyond = 0;
-  uint32_t top[2] = {1, 1};
+  uint32_t top[2] = {kLeastTop, kLeastTop};
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < a.n_slots; i += kBackGroups * 256ll) {
     uint32_t slot;
     if (!back_slot(a, i, slot)) continue;
