@@ -14,8 +14,8 @@ differs from one over the read-back values by the rounding of the result.
 
 Chunks of many new tokens read a token so often that it is converted once: their pages
 are read back as float16, within range by powers of two, and the 16-bit attention's
-matrix-core kernels run over that, in float16 for bf16 activations as well (its eleven bits
-keep the operands' roundings under the result's).  One pair of powers serves a whole step, so
+matrix-core kernels run over that: for bf16 activations, whose results are rounded by more than
+float16's eleven bits cost the operands.  One pair of powers serves a whole step, so
 one whose rows differ too much in size for float16 -- a key of 1e6 in any of its requests, a
 value 2^16 times as large as another -- is answered over the codes after all: the launch over
 them stands behind the others and runs where these found that.  Plans over a workspace reserved
@@ -149,6 +149,10 @@ class QuantizedCacheAttention(SharedCacheAttention):
     def _reads_back(self, pairs: int, pages: int) -> bool:
         """Whether the chains of a step, ``pairs`` of a row and a token that it may see, run over rows read back.
 
+        Not those of float16 activations: operands of float16 put errors on the result that are larger than its own
+        rounding.  Relative to the result (2-norms), over codes / read back, 64 rows over 7800 tokens, 32 q and 8 kv heads of
+        128: float16 0.00021 / 0.00036, with scores up to +-100 0.00014 / 0.00063; bf16 0.00166 / 0.00172, 0.00106 / 0.00128.
+
         Reading back costs four launches more and 2 ns a token of 1024 elements, and takes half to two thirds off the products.
         Us read back / over codes, one chunk, 32 q and 8 kv heads of 128: 256 rows over 3000 tokens 61 / 52, 48 (64) rows over
         20000 84 / 80 (89 / 106), 24 rows 80 / 48; 8 and 8 heads: 128 (256) rows over 20000 81 / 62 (92 / 108); 16 and 4
@@ -157,7 +161,7 @@ class QuantizedCacheAttention(SharedCacheAttention):
         and at 120 to 350 query rows a token and kv head where the tokens are many.
         """
         products = pairs * self.num_qo_heads * self.head_dim
-        return products >= 4 << 30 and products >= 160 * pages * self.page_size * self.num_kv_heads * self.head_dim
+        return self.dtype == torch.bfloat16 and products >= 4 << 30 and products >= 160 * pages * self.page_size * self.num_kv_heads * self.head_dim
 
     def _ensure_scratch(self, nbytes: int) -> torch.Tensor:
         """Room for rows read back, shared by the op's steps like their workspace; a plan keeps the tensor it was given."""

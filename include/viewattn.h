@@ -441,7 +441,9 @@ VA_API int va_attention_if_q8(const int32_t* condition_dev, const void* q_dev, i
  * last token of a page) hold zeros.  Keys and values are scaled by powers of two that
  * bring the largest row near the upper end of float16, queries by the inverse of the
  * keys' and results by that of the values'.  Queries (rotated), weights and results are
- * rounded to float16, with absolute errors of 2^-39 of the largest value for results;
+ * rounded to float16, with absolute errors of 2^-39 of the largest value for results
+ * (what results of VA_F16 lose by that is more than their own rounding: va_attention_q8 is as
+ * exact as it);
  * a key or value row of NaN makes NaN of the results and the lse of those that see it.
  * One power serves all rows of the call, whatever requests they belong to.  Where
  * float16 does not hold them (a query element of |q_i| max|K| > 1.1e5, or a value row, not

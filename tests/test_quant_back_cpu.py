@@ -69,3 +69,10 @@ def test_a_condition_takes_plans_that_one_launch_answers():
     assert step.launch.counts.n_partials
     assert call(plan=step.launch.header) == native.VA_ERR_ARG and b"partial states" in native.lib.va_last_error()
     assert call(plan=back.launch.header) < 0 or not back.launch.counts.n_wide_items
+
+
+def test_float16_activations_are_not_read_back():
+    """Whatever the work: float16 operands would cost them as much as the rounding of the result."""
+    for dtype in (BF16, F16):
+        op, _ = make(heads=(32, 8, 128), dtype=dtype)
+        assert op._reads_back(300 * 20000, 20000 // 16) == (dtype == BF16)
