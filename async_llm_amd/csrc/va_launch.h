@@ -70,22 +70,23 @@ int plan_arguments(const void* q_dev, int64_t q_row_stride, const void* k_pool_d
                    float* lse_dev, int32_t lse_base2, void* workspace_dev, int64_t workspace_bytes, const VaShape* shape,
                    const VaRope* rope, AttnArgs* attn, MergeArgs* merge);
 
-// The merge of partial states (viewattn.hip); `waves`: the plan header's word.
-// A planned attention's launches; keep_nan as in MergeArgs.
+// A planned attention's launches.  `read_back`: over rows of a quantised pool read back as float16 -- NaN stays NaN, and
+// weights are those of F16Lifted.
 int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, const void* v_pool_dev,
                        int64_t pool_row_stride, const int32_t* plan_dev, const int32_t* plan_header_host,
                        const int32_t* kv_indices_dev, const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
                        int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
-                       int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, int keep_nan, void* stream);
+                       int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, int read_back, void* stream);
+// The merge of partial states (viewattn.hip); `waves`: the plan header's word.
 int launch_merge_typed(const MergeArgs& m, int dtype, int n_rows, int waves, hipStream_t stream);
 
 // Matrix-core attention (launched from va_mfma.hip).
 // `n_wide` leading items are wide tiles (va_mfma_wide.hip: `n_wide_slots` workgroups per kv head, each
 // running the items a.wide_slots gives it), the rest narrow ones: in the same launch behind the wide ones, or in
-// one of their own (va_mfma_stream.hip).
-int launch_mfma(const AttnArgs& a, int dtype, int n_items, int n_wide, int n_wide_slots, int q_tile, bool short_items,
+// one of their own (va_mfma_stream.hip).  `lifted`: the type is VA_F16, its weights those of F16Lifted (va_mfma_common.h).
+int launch_mfma(const AttnArgs& a, int dtype, bool lifted, int n_items, int n_wide, int n_wide_slots, int q_tile, bool short_items,
                 bool apart, hipStream_t stream);
-int launch_mfma_wide(const AttnArgs& a, int dtype, int n_slots, int n_narrow, hipStream_t stream);
-int launch_mfma_stream(const AttnArgs& a, int dtype, int n_items, bool short_items, hipStream_t stream);
+int launch_mfma_wide(const AttnArgs& a, int dtype, bool lifted, int n_slots, int n_narrow, hipStream_t stream);
+int launch_mfma_stream(const AttnArgs& a, int dtype, bool lifted, int n_items, bool short_items, hipStream_t stream);
 
 }  // namespace va

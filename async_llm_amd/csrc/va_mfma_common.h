@@ -82,6 +82,24 @@ struct Mma<F16> {
   }
 };
 
+// float16 with softmax weights under a reference 2^8 times as small as the largest: float16 loses bits of numbers under 2^-14
+// and all of those under 2^-25, so beside one key that has nearly all of the weight many thousands, whose sum counts, came to
+// nothing (65536 of 2^-26 each: 0 instead of 0.001 of their value).  What is lost now is at most 2^-33 of a value for each
+// token.  Products and sums are taken in 32 bits; weights themselves stay within float16 (the wide kernel's limit).
+struct F16Lifted : F16 {};
+template <>
+struct Mma<F16Lifted> : Mma<F16> {};
+
+// The reference (log2 units) of a row whose largest score is `most`.
+template <typename E>
+__device__ __forceinline__ float softmax_reference(float most) {
+  return most;
+}
+template <>
+__device__ __forceinline__ float softmax_reference<F16Lifted>(float most) {
+  return most - 8.f;
+}
+
 // One 16-byte piece (dims [d0, d0+8)) of a query head row, rotated for position `p` and
 // rounded to the element type; pieces beyond rotary_dim pass through.  rotary_dim is a
 // multiple of 16 here, so a piece never straddles the two rotary halves.

@@ -60,8 +60,9 @@ static int launch_stream_typed(const AttnArgs& a, int n_items, bool short_items,
   }
 }
 
-int launch_mfma_stream(const AttnArgs& a, int dtype, int n_items, bool short_items, hipStream_t stream) {
+int launch_mfma_stream(const AttnArgs& a, int dtype, bool lifted, int n_items, bool short_items, hipStream_t stream) {
   if (n_items == 0) return VA_OK;
+  if (lifted) return launch_stream_typed<F16Lifted>(a, n_items, short_items, stream);
   return dtype == VA_BF16 ? launch_stream_typed<BF16>(a, n_items, short_items, stream)
                           : launch_stream_typed<F16>(a, n_items, short_items, stream);
 }

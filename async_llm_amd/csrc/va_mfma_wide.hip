@@ -40,7 +40,13 @@
 namespace va {
 
 constexpr int kWideThreads = 256;
-constexpr float kWideRaise = 14.f;  // a tile maximum this far above the reference (log2 units) raises it
+// A tile maximum this far above the reference (log2 units) raises it.  Lifted weights: 2^15.5 is the most that a float16
+// weight may be, and leaves a row's maximum 2^7.5 to grow (by 2^4 it grows in many tiles: four chunks of 300..1500 tokens over 8 k 682
+// us without the lift, 730 with 2^10 and 14, 682 as it is).
+template <typename E>
+constexpr float kWideRaise = 14.f;
+template <>
+constexpr float kWideRaise<F16Lifted> = 15.5f;
 constexpr int kWideWaves = 4;
 constexpr int kWideTokens = 32;  // tokens per K/V tile
 #ifndef VA_WIDE_BUFFERS
@@ -237,7 +243,7 @@ __device__ __forceinline__ void wide_slot(const AttnArgs& a, unsigned workgroup,
   for (int b = 0; b < kB; ++b) {
     m_ref[b] = kNegBig;
     m_tile[b] = kNegBig;
-    raise_above[b] = kNegBig + kWideRaise;
+    raise_above[b] = kNegBig + kWideRaise<E>;
     l_run[b] = 0.f;
 #pragma unroll
     for (int t = 0; t < kDimTiles; ++t)
@@ -900,10 +906,10 @@ __device__ __forceinline__ void wide_slot(const AttnArgs& a, unsigned workgroup,
       accumulator_fence<kB * kDimTiles>(&o[0][0]);
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
-        const float m_new = fmaxf(m_ref[b], m_tile[b]);
+        const float m_new = fmaxf(m_ref[b], softmax_reference<E>(m_tile[b]));
         const float alpha = __builtin_amdgcn_exp2f(m_ref[b] - m_new);
         m_ref[b] = m_new;
-        raise_above[b] = m_new + kWideRaise;
+        raise_above[b] = m_new + kWideRaise<E>;
         l_run[b] *= alpha;
 #pragma unroll
         for (int t = 0; t < kDimTiles; ++t) o[b][t] *= alpha;
@@ -1110,7 +1116,8 @@ static int launch_wide_typed(const AttnArgs& a, int n_slots, int n_narrow, hipSt
   }
 }
 
-int launch_mfma_wide(const AttnArgs& a, int dtype, int n_slots, int n_narrow, hipStream_t stream) {
+int launch_mfma_wide(const AttnArgs& a, int dtype, bool lifted, int n_slots, int n_narrow, hipStream_t stream) {
+  if (lifted) return launch_wide_typed<F16Lifted>(a, n_slots, n_narrow, stream);
   return dtype == VA_BF16 ? launch_wide_typed<BF16>(a, n_slots, n_narrow, stream) : launch_wide_typed<F16>(a, n_slots, n_narrow, stream);
 }
 

@@ -10,8 +10,10 @@
 // what float16 lacks; it is given by powers of two, exactly:
 //   K' = K 2^-b,  q' = q 2^b,  V' = V 2^-s,  out = out' 2^s
 // with b and s from the largest scales among the rows, found by a pass over the scale bytes.  Beside float16's relative
-// errors this leaves absolute ones of 2^-25, half of its smallest step: 2^-39 of the largest value for V' and out', 2^-17 /
-// sqrt(D) of a score for each q' element below 2^-14 (K' is at most 2^8), and 2^-25 q' / sqrt(D) for each K' element below it.
+// errors (under mRoPE its kernels round cosines, sines, products and their sum to it, each) this leaves absolute ones of 2^-25,
+// half of its smallest step: 2^-39 of the largest value for V' and out'; 2^-17 / sqrt(D) of a score for each q' element below
+// 2^-14 (K' is at most 2^8) and 2^-25 q' / sqrt(D) for each K' element below it; and 2^-33 of a value for each token's weight,
+// whose largest is taken as 2^8 (F16Lifted in va_mfma_common.h).
 //
 // One b and one s serve all heads and requests of a launch, whose rows need not be of a size.  Where float16 would lose what
 // codes keep, the launch says so in the scratch's first word, and its results are taken from the codes (va_attention_if_q8):

@@ -175,7 +175,7 @@ __device__ __forceinline__ void stream_items(const AttnArgs& a, const int (&item
   const uint32_t wave_ring = lds_base + (uint32_t)wave * Sh::kWaveRingBytes;
   va_u32x4* q_stage = smem + Sh::kRingBytes / 16;
 
-  float m_run[kB], l_run[kB];  // running maximum (log2 units) and row sum, of this wave's tokens
+  float m_run[kB], l_run[kB];  // reference of the running maximum (log2 units) and row sum, of this wave's tokens
   va_f32x4 o[kB][kDimTiles];
 #pragma unroll
   for (int b = 0; b < kB; ++b) {
@@ -464,12 +464,12 @@ __device__ __forceinline__ void stream_items(const AttnArgs& a, const int (&item
             sc[b][r] = v;
             most[b] = fmaxf(most[b], v);
           }
-          raise = raise || most[b] > m_run[b];
+          raise = raise || softmax_reference<E>(most[b]) > m_run[b];
         }
         if (__any(raise)) {
 #pragma unroll
           for (int b = 0; b < kB; ++b) {
-            const float m_new = fmaxf(m_run[b], max_over_contraction_groups(most[b]));
+            const float m_new = fmaxf(m_run[b], softmax_reference<E>(max_over_contraction_groups(most[b])));
             // (the bare instruction: results below 2^-126 become 0 instead of denormal)
             const float alpha = __builtin_amdgcn_exp2f(m_run[b] - m_new);
             m_run[b] = m_new;

@@ -888,7 +888,7 @@ int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_po
                        int64_t pool_row_stride, const int32_t* plan_dev, const int32_t* plan_header_host,
                        const int32_t* kv_indices_dev, const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
                        int64_t sub_loc_axis_stride, void* out_dev, float* lse_dev, int32_t lse_base2, void* workspace_dev,
-                       int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, int keep_nan, void* stream) {
+                       int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, int read_back, void* stream) {
   if (!shape || !plan_header_host || !plan_dev) return va_fail(VA_ERR_ARG, "null plan or shape");
   const int32_t* h = plan_header_host;
   if (h[VA_H_MAGIC] != VA_PLAN_MAGIC) return va_fail(VA_ERR_ARG, "plan header has no magic word");
@@ -900,12 +900,12 @@ int attention_launches(const void* q_dev, int64_t q_row_stride, const void* k_po
                           sub_worker_dev, sub_loc_dev, sub_loc_axis_stride, out_dev, lse_dev, lse_base2,
                           workspace_dev, workspace_bytes, shape, rope, &a, &m);
   if (rc) return rc;
-  m.keep_nan = keep_nan;
+  m.keep_nan = read_back;
   hipStream_t s = (hipStream_t)stream;
 
   if (n_items > 0) {
     if (h[VA_H_KERNEL] == VA_KERNEL_MFMA) {
-      rc = va::launch_mfma(a, shape->dtype, n_items, h[VA_H_N_WIDE], h[VA_H_N_WIDE_SLOTS], h[VA_H_Q_TILE],
+      rc = va::launch_mfma(a, shape->dtype, read_back != 0, n_items, h[VA_H_N_WIDE], h[VA_H_N_WIDE_SLOTS], h[VA_H_Q_TILE],
                            (h[VA_H_KV_CHUNK] & VA_CHUNK_SHORT_ITEMS) != 0, (h[VA_H_KV_CHUNK] & VA_CHUNK_APART) != 0,
                            s);
     } else {

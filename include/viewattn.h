@@ -438,20 +438,24 @@ VA_API int va_attention_if_q8(const int32_t* condition_dev, const void* q_dev, i
  * back as float16 into a scratch pool, and va_attention runs over that with wide
  * items.  The plan and kv_indices count pages (slots) of the scratch: its slot i
  * holds the pool's slot slots_dev[i]; slots outside the pool (those behind the
- * last token of a page) hold zeros.  Keys and values are scaled by powers of two that
- * bring the largest row near the upper end of float16, queries by the inverse of the
- * keys' and results by that of the values'.  Queries (rotated), weights and results are
- * rounded to float16, with absolute errors of 2^-39 of the largest value for results
- * (what results of VA_F16 lose by that is more than their own rounding: va_attention_q8 is as
- * exact as it);
- * a key or value row of NaN makes NaN of the results and the lse of those that see it.
- * One power serves all rows of the call, whatever requests they belong to.  Where
- * float16 does not hold them (a query element of |q_i| max|K| > 1.1e5, or a value row, not
- * zero, whose scale is more than 2^16 times smaller than the largest) the first word of
- * scratch_dev, an int32, is 1 behind the call, otherwise 0: where it is 1 the results are not
- * to be used, and va_attention_if_q8 under that word puts those of the codes in their
- * place.  16-bit activations, head_dim
- * 64, 128 or 256, and the matrix-core plans only (the plan is built for VA_F16).
+ * last token of a page) hold zeros.  16-bit activations, head_dim 64, 128 or 256, and
+ * matrix-core plans only (the plan is built for VA_F16).
+ *
+ * Keys and values are scaled by powers of two that bring the largest row near the upper
+ * end of float16, queries by the inverse of the keys' and results by that of the values'.
+ * Rotated queries, weights and results are rounded to float16: by 2^-11 of themselves
+ * (under VA_ROPE_MROPE a query's cosines, sines, products and their sum each), scores by
+ * up to 2^-11, results by 2^-39 of the largest value and, as weights vanish that are far
+ * smaller than the largest, by 2^-33 of the largest value in sight for every token in
+ * sight.  Results of VA_F16 lose more by that than by their own rounding; those of
+ * va_attention_q8 do not.  A key or value row of NaN makes NaN of the results and the lse
+ * of those that see it (the lse of va_attention_q8 does not depend on values).
+ *
+ * One power serves all rows of the call, whatever requests they belong to.  Where float16
+ * does not hold them -- a query element of |q_i| max|K| > 1.1e5, or a value row, not zero,
+ * whose scale is more than 2^16 times smaller than the largest -- the first word of
+ * scratch_dev, an int32, is 1 behind the call, otherwise 0.  Where it is 1 the results are
+ * not to be used: va_attention_if_q8 under that word puts those of the codes in their place.
  * scratch_dev, on a 256-byte boundary, must hold va_read_back_bytes(n_slots, rows of
  * the plan, shape).
  */
