@@ -193,7 +193,7 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
   const bool wide_on_request = params && params->wide_tile > 0;
   // A workgroup for every tile: 64 rows over 65536 shared tokens, counted together / apart, 173 / 159 us over codes, over 8192 alone
   // 48.6 / 41.9, beside private blocks 193.8 / 189.8.
-  const bool tiles_apart = params && params->wide_tile < -1;
+  const bool tiles_apart = params && params->wide_tile == VA_TILES_APART;
   const int target = params && params->target_items > 0 ? params->target_items : default_target(kernel, shape->num_kv_heads);
   const int gran = 64;  // chunk boundaries are multiples of this many tokens
 

@@ -23,6 +23,7 @@ VA_SUB_CAUSAL, VA_SUB_SLOTS = 1, 2
 PLAN_HEADER_WORDS = 24
 PLAN_FLAGS_WORD = 3  # of a header: the chunk, with flags in its low bits
 PLAN_SHORT_ITEMS = 1  # narrow items are short: several workgroups share a CU
+VA_TILES_APART = -(2**31)  # of VaPlanParams.wide_tile: no wide tiles, nor several in a workgroup
 VA_CODE_E4M3, VA_CODE_INT8 = 0, 1
 VA_ERR_ARG, VA_ERR_CAPACITY = -1, -2
 STATIC_SCRATCH_BYTES = 32 << 20  # VA_STATIC_SCRATCH_BYTES: the array va_attention_static keeps on every GPU

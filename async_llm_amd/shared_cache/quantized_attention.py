@@ -76,7 +76,7 @@ class QuantizedCacheAttention(SharedCacheAttention):
             raise ValueError(f"kv_cache lives on {self.device}, the op is to run on {device}")
         p = self.plan_params
         self._read_back_params = native.VaPlanParams(p.kernel, p.q_tile, p.kv_chunk, p.target_items, p.wide_tile)
-        p.wide_tile = -2  # codes are read by tiles of up to 16 rows, a workgroup each
+        p.wide_tile = native.VA_TILES_APART  # codes are read by tiles of up to 16 rows, a workgroup each
         # one work item a tile: nothing to merge, no workspace
         self._uncut_params = native.VaPlanParams(p.kernel, p.q_tile, p.kv_chunk, 1, p.wide_tile)
         self._read_back_shape = native.make_shape(num_qo_heads, num_kv_heads, head_dim, page_size, torch.float16)

@@ -149,9 +149,10 @@ typedef struct VaPlanParams {
   int32_t target_items;  /* 0 = default (work items wanted per kv head)       */
   int32_t wide_tile;     /* rows of a wide query tile: 0 = default (prefill tiles; decode readers of one
                             block only where the re-reads saved outweigh what the others lose), >0 = this many
-                            rows, decode readers included, <0 = never (-1), nor several tiles in a workgroup
-                            (-2: plans for va_attention_q8) */
+                            rows, decode readers included, <0 = never, VA_TILES_APART = never, nor several
+                            tiles in a workgroup (plans for va_attention_q8) */
 } VaPlanParams;
+#define VA_TILES_APART (-0x7fffffff - 1) /* of VaPlanParams.wide_tile */
 
 typedef struct VaPlanCounts {
   int32_t kernel;        /* resolved kernel family */
@@ -408,8 +409,8 @@ VA_API int va_copy_shift_kv_q8(const VaQuantPool* pool, int64_t code_layer_strid
 
 /*
  * va_attention_q8: va_attention over a quantised pool, with the plans of
- * va_plan_build* for the same shape and params->wide_tile < 0 (no wide items; -2
- * counts its workgroups as they are).
+ * va_plan_build* for the same shape and params->wide_tile < 0 (no wide items;
+ * VA_TILES_APART counts its workgroups as they are).
  * kv_indices of VA_SUB_SLOTS sub-requests are token slots of the pool.  Queries
  * are rotated in fp32 and enter the products unrounded (vector-ALU kernel) or as
  * sums of two bf16 numbers (matrix-core kernel: error 2^-17 of each element), and

@@ -76,3 +76,22 @@ def test_float16_activations_are_not_read_back():
     for dtype in (BF16, F16):
         op, _ = make(heads=(32, 8, 128), dtype=dtype)
         assert op._reads_back(300 * 20000, 20000 // 16) == (dtype == BF16)
+
+
+def test_only_one_value_sets_the_tiles_of_a_plan_apart():
+    """Any other negative number of rows asks for no wide tiles and nothing else."""
+    plans = {}
+    for rows in (-1, -2, -3, -(2**31) + 1, native.VA_TILES_APART):
+        shape = native.make_shape(16, 4, 256, 16, BF16)
+        shared = np.arange(512, dtype=np.int32)
+        tables = [np.arange(65, dtype=np.int32), np.arange(65, dtype=np.int32) * 512, np.tile(shared, 64), np.full(64, 8192, dtype=np.int32),
+                  np.zeros(64, dtype=np.int32), np.full(64, -1, dtype=np.int32)]
+        row = np.arange(64, dtype=np.int64)
+        subs = native.VaSubRequests(64, 64, 64, *(t.ctypes.data for t in tables), row.ctypes.data)
+        params, counts = native.VaPlanParams(native.VA_KERNEL_MFMA, 0, 0, 0, rows), native.VaPlanCounts()
+        native.check(native.lib.va_plan_count(subs, shape, params, counts))
+        blob = np.zeros(counts.plan_words, dtype=np.int32)
+        native.check(native.lib.va_plan_build(subs, shape, params, blob.ctypes.data, blob.size, counts))
+        plans[rows] = blob.tobytes()
+    assert plans[-1] == plans[-2] == plans[-3] == plans[-(2**31) + 1] != plans[native.VA_TILES_APART]
+    assert make()[0].plan_params.wide_tile == native.VA_TILES_APART
