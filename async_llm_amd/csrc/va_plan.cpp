@@ -354,10 +354,11 @@ int build(const VaSubRequests* s, const VaShape* shape, const VaPlanParams* para
       // 256 dims, 60 / 43 / 35 / 29 items for 64 at once) 18.2 / 15.8 / 16.1 / 17.0 us; 256 / 320 / 384 / 512, 8 of
       // 1400..4000 (8 of 128 dims, 69 / 60 / 53 / 42 for 64) 21.4 / 19.6 / 20.1 / 19.6.  At 128 dims up to sixteen: 16
       // requests of 64..2048 behind 1500 shared tokens (8 kv heads), chunks of 512 / 896, 30.9 / 28.6 us.
-      // Over codes (tiles apart), where two to four workgroups share a CU, 614 start at once under 256 dims (384 / 614, us: 4
-      // requests of 20 k tokens, 8 kv heads of 128 dims, 29.8 / 25.8; 24 of 7 k, 2 heads of 128, 22.0 / 20.3; at 256 dims one of 30 k
-      // tokens 19.6, with a third more items 22.8), and twelve granules where they do not (eight / twelve, 16 requests
-      // of 5 k at 256 dims 24.8 / 23.3, 19 of 900 25.9 / 23.8).
+      // Over codes (tiles apart) 614 workgroups are taken for a round under 256 dims.  The CUs hold more, 1024 at 64 dims and 768
+      // at 128; the number is one from timing (384 / 614, us: 4 requests of 20 k tokens, 8 kv heads of 128 dims, 29.8 / 25.8; 24 of
+      // 7 k, 2 heads of 128, 22.0 / 20.3; at 256 dims, where it stays, one of 30 k tokens 19.6, with a third more items 22.8).  So are
+      // the twelve granules where one round does not do (eight / twelve, 16 requests of 5 k at 256 dims 24.8 / 23.3, 19 of 900
+      // 25.9 / 23.8).
       const int start = shape->head_dim != 256 ? (tiles_apart ? 614 : 384) : any_wide ? 192 : 208;
       const int64_t at_once = std::max(1, start / shape->num_kv_heads);
       for (least = gran; least < most; least += gran) {

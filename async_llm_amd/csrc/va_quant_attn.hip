@@ -16,11 +16,12 @@ namespace va {
 // what the matrix-core kernel rejects.  One workgroup of four waves per (work item, kv head), tile rows one after another,
 // four q heads a pass.  A token's K (and V) row is sixteen codes for each of kD / 16 adjacent lanes, a wave takes
 // 1024 / kD tokens a step and two steps together; the next two are requested before their products, the first ones before the
-// queries are rotated.  Every lane group keeps sums of its own under the wave's maxima, joined at the end of the chain.
+// queries are rotated.  Every lane group keeps maxima and sums of its own; the workgroup's maximum is found at the end of the
+// chain, and what is left are plain sums.
 //
 // Small steps are a chain of trips (item, link, page, codes; row, query, turns) and a fold, so what counts is their number:
-// one row, 2 kv heads of 128 dims, 1900 tokens 8.1 us (12.7 where codes were requested behind the query, lane groups kept
-// maxima of their own and joined by shuffles); eight rows of 3000 tokens, 4 heads of 256 dims 26 (32 for the step), 32 rows
+// one row, 2 kv heads of 128 dims, 1900 tokens 8.1 us (12.7 where codes were requested behind the query and lane groups joined
+// pair by pair, each with its rescaling, by shuffles); eight rows of 3000 tokens, 4 heads of 256 dims 26 (32 for the step), 32 rows
 // of 12000, 8 heads of 128 dims 320 (399): the vector ALU's products.
 constexpr int kAnyHeads = 4;
 constexpr int kAnyThreads = 256;

@@ -10,7 +10,11 @@ attention reads the codes and takes each row's scale into the score (K) or the w
     out(row)      = sum_t softmax(score)(t) * 2^e_v[t] * code_v[t]
 
 Queries and weights are not rounded to the activations' type in between: such a step
-differs from one over the read-back values by the rounding of the result.
+differs from one over the read-back values by the rounding of the result.  Values are summed
+in 32 bits under weights of up to 2^8: results are finite for |v| up to 2^119 divided by the
+tokens in sight.  A key or value row that is not finite makes NaN of the results that see it, and
+of no other; the lse of such results has no meaning (it is NaN for keys, and for values where the
+step was read back).
 
 Chunks of many new tokens read a token so often that it is converted once: their pages
 are read back as float16, within range by powers of two, and the 16-bit attention's
@@ -153,12 +157,13 @@ class QuantizedCacheAttention(SharedCacheAttention):
         rounding.  Relative to the result (2-norms), over codes / read back, 64 rows over 7800 tokens, 32 q and 8 kv heads of
         128: float16 0.00021 / 0.00036, with scores up to +-100 0.00014 / 0.00063; bf16 0.00166 / 0.00172, 0.00106 / 0.00128.
 
-        Reading back costs four launches more and 2 ns a token of 1024 elements, and takes half to two thirds off the products.
+        Reading back costs five launches more and 2 ns a token of 1024 elements, and takes half to two thirds off the products.
         Us read back / over codes, one chunk, 32 q and 8 kv heads of 128: 256 rows over 3000 tokens 61 / 52, 48 (64) rows over
         20000 84 / 80 (89 / 106), 24 rows 80 / 48; 8 and 8 heads: 128 (256) rows over 20000 81 / 62 (92 / 108); 16 and 4
         heads of 256: 64 (96) rows over 20000 86 / 78 (98 / 107), 256 rows over 3000 59 / 58; 64 and 16 heads of 64: 24 (32) rows
         over 20000 83 / 68 (85 / 91), 256 rows over 3000 64 / 59. They change sides between 2.4e9 and 7e9 products, most near 4e9,
-        and at 120 to 350 query rows a token and kv head where the tokens are many.
+        and at 120 to 350 query rows a token and kv head where the tokens are many.  One line for all of them is off by up to a
+        tenth beside it: 64 rows of 16 and 4 heads of 256 over 20000 tokens are read back, 32 rows of 64 and 16 heads of 64 are not.
         """
         products = pairs * self.num_qo_heads * self.head_dim
         return self.dtype == torch.bfloat16 and products >= 4 << 30 and products >= 160 * pages * self.page_size * self.num_kv_heads * self.head_dim

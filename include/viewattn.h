@@ -414,7 +414,9 @@ VA_API int va_copy_shift_kv_q8(const VaQuantPool* pool, int64_t code_layer_strid
  * kv_indices of VA_SUB_SLOTS sub-requests are token slots of the pool.  Queries
  * are rotated in fp32 and enter the products unrounded (vector-ALU kernel) or as
  * sums of two bf16 numbers (matrix-core kernel: error 2^-17 of each element), and
- * so do the weights of the second product.
+ * so do the weights of the second product.  Sums of weighted values are kept in 32 bits in
+ * front of their division: where |v| times the tokens in sight passes 2^119 (2^127 on the
+ * vector ALU) a result may be infinite or NaN.
  */
 VA_API int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
                     const int32_t* plan_header_host, const int32_t* kv_indices_dev,
