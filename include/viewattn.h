@@ -416,7 +416,9 @@ VA_API int va_copy_shift_kv_q8(const VaQuantPool* pool, int64_t code_layer_strid
  * sums of two bf16 numbers (matrix-core kernel: error 2^-17 of each element), and
  * so do the weights of the second product.  Sums of weighted values are kept in 32 bits in
  * front of their division: where |v| times the tokens in sight passes 2^119 (2^127 on the
- * vector ALU) a result may be infinite or NaN.
+ * vector ALU) a result may be infinite or NaN.  On the matrix cores a token's weight times
+ * its scale has steps of 2^-133: every token in sight may add an error of 2^-125, which
+ * values under 2^-108 feel.
  */
 VA_API int va_attention_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
                     const int32_t* plan_header_host, const int32_t* kv_indices_dev,
