@@ -6,7 +6,8 @@
 // wide tiles over codes 960 to 1140.  Reading back is a tenth of it (47 k tokens, 94 MB of codes).
 //
 // It runs in float16 whatever the activations are: codes have four (eight) bits, so eleven hold them, and a bf16 query or
-// weight would put an error on the result that is as large as its own rounding (0.0034 against 0.0017 of it, in bf16).  Range is
+// weight would put an error on the result that is as large as its own rounding (0.0034 against 0.0017 of it, in bf16).  A float16 one does
+// the same to float16 results (0.00036 against 0.00021), which the Python op therefore leaves to the codes.  Range is
 // what float16 lacks; it is given by powers of two, exactly:
 //   K' = K 2^-b,  q' = q 2^b,  V' = V 2^-s,  out = out' 2^s
 // with b and s from the largest scales among the rows, found by a pass over the scale bytes.  Beside float16's relative
