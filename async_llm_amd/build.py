@@ -23,8 +23,8 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "libviewattn.so")
 HIP_SOURCES = ["viewattn.hip", "va_mfma.hip", "va_mfma_wide.hip", "va_mfma_stream.hip", "va_block_copy.hip",
                "va_quant_rows.hip", "va_quant_attn.hip", "va_quant_stream.hip",
-               "va_quant_scattered.hip", "va_quant_back.hip"]
-HOST_SOURCES = ["va_plan.cpp"]
+               "va_quant_scattered.hip", "va_quant_back.hip", "va_rotary.hip", "va_select.hip", "va_move.hip", "va_weigh.hip"]
+HOST_SOURCES = ["va_plan.cpp", "va_weigh_plan.cpp"]
 
 COMMON_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-function", "-DVA_BUILDING=1"]
 DEVICE_FLAGS = ["--offload-arch=gfx950", "--cuda-device-only",

@@ -86,6 +86,7 @@ __device__ __forceinline__ float mul_rounded(float a, float b);
 // 2^(e - 53) units away from the nearest one (e: the angle's exponent), and what is left is reduced once
 // more.  An angle within 64 bits (any int64 position, frequencies up to 1) leaves 2^11 units then, and
 // an error of 2^-41 in them.
+__device__ __forceinline__ void sin_cos_of_quadrant(float r, int quadrant, float& s, float& c);
 __device__ __forceinline__ void sin_cos(float x, float& s, float& c) {
   const double k = rint((double)x * 0.63661977236758134308);
   double near = fma(-k, 1.57079632679489655800, (double)x), units = k;
@@ -95,9 +96,14 @@ __device__ __forceinline__ void sin_cos(float x, float& s, float& c) {
     near = fma(-more, 1.57079632679489655800, near);
     units = more;
   }
-  const float r = (float)fma(-units, 6.12323399573676603587e-17, near), z = r * r;
+  const float r = (float)fma(-units, 6.12323399573676603587e-17, near);
   int quadrant = (int)(k - 4.0 * floor(0.25 * k));
   if (fabsf(x) > 0x1p50f) quadrant += (int)units;
+  sin_cos_of_quadrant(r, quadrant, s, c);
+}
+// sin and cos of r + quadrant * pi / 2, |r| <= pi / 4.
+__device__ __forceinline__ void sin_cos_of_quadrant(float r, int quadrant, float& s, float& c) {
+  const float z = r * r;
   const float sp = fmaf(z, fmaf(z, fmaf(z, fmaf(z, -2.50521084e-8f, 2.75573192e-6f), -1.98412698e-4f), 8.33333333e-3f), -1.66666667e-1f);
   const float cp = fmaf(z, fmaf(z, fmaf(z, fmaf(z, -2.75573192e-7f, 2.48015873e-5f), -1.38888889e-3f), 4.16666667e-2f), -0.5f);
   const float sr = fmaf(r * z, sp, r), cr = fmaf(z, cp, 1.f);

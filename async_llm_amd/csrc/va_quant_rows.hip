@@ -5,6 +5,7 @@
 #include "va_internal.h"
 #include "va_launch.h"
 #include "va_quant.h"
+#include "va_token_weights.h"
 
 namespace va {
 
@@ -293,7 +294,10 @@ struct QuantCopyArgs {
   int num_kv_heads;
   PageMap pages;
   RopeDev rope;
+  const int64_t* shifts;  // a shift for every token, in the place of `shift`
+  TokenWeights weights;   // moved along (kOwnTurn only)
 };
+enum { kNoTurn, kOneTurn, kOwnTurn };  // keys: as they are, all by one shift, each token's by its own
 
 // A workgroup moves the keys (blockIdx.z 0) or values (1) of kQuantCopyTokens tokens of a layer.  As in the store a row is
 // kD / 16 neighbouring lanes; a thread keeps its token and its place in the row, so the slots and the turns of its pairs
@@ -301,8 +305,8 @@ struct QuantCopyArgs {
 // memory.  Bound by HBM: 12556 tokens of 4 layers of 4 heads of 256 dims (207 MB read and written) 39 us, 5.3 TB/s; with a thread
 // walking sixteen tokens of its head 66 us, with stores that stay in the caches 49.  Small copies are bound by the trip
 // slot, scale and codes, store: 5.6 us for 4.3 MB (17 with walks).  kTurn: keys are rotated (rotary_dim a multiple of 16);
-// otherwise they move code for code like the values.
-template <typename C, int kD, bool kTurn>
+// otherwise, and where a token's own shift is 0, they move code for code like the values.
+template <typename C, int kD, int kTurn>
 __global__ __launch_bounds__(256) void quant_copy_kernel(QuantCopyArgs a) {
   constexpr int kLanes = kD / 16, kHeads = 256 / kLanes / kQuantCopyTokens;  // heads side by side
   const int x = threadIdx.x % kLanes, which = blockIdx.z;
@@ -315,7 +319,10 @@ __global__ __launch_bounds__(256) void quant_copy_kernel(QuantCopyArgs a) {
   const long long from = quant_row(a.pages, (uint32_t)src, 0, a.num_kv_heads);
   const long long to = quant_row(a.pages, (uint32_t)dst, 0, a.num_kv_heads);
   const int first = threadIdx.x / (kLanes * kQuantCopyTokens);
-  if (!kTurn || which) {
+  const long long shift = kTurn == kOwnTurn ? (a.shifts ? a.shifts[i] : 0) : a.shift;
+  if constexpr (kTurn == kOwnTurn)
+    if (which && layer == 0) move_weights(a.weights, a.num_kv_heads, src, dst, first * kLanes + x, kHeads * kLanes);
+  if (kTurn == kNoTurn || which || (kTurn == kOwnTurn && shift == 0)) {
     for (int h0 = first; h0 < a.num_kv_heads; h0 += kQuantCopyBatch * kHeads) {
       va_u32x4 row[kQuantCopyBatch];
       uint8_t e[kQuantCopyBatch];
@@ -338,7 +345,7 @@ __global__ __launch_bounds__(256) void quant_copy_kernel(QuantCopyArgs a) {
   const bool turns = x < a.rope.rotary_dim / 16;
   const int d0 = turns ? 8 * x : 16 * x, d1 = turns ? 8 * x + a.rope.half : 16 * x + 8;
   float c[8], s[8];
-  if (turns) turns8(a.rope, Pos3{a.shift, a.shift, a.shift}, d0, c, s);
+  if (turns) turns8(a.rope, Pos3{shift, shift, shift}, d0, c, s);
   for (int h0 = first; h0 < a.num_kv_heads; h0 += kQuantCopyBatch * kHeads) {
     uint2 lo[kQuantCopyBatch], hi[kQuantCopyBatch];
     uint32_t e[kQuantCopyBatch];
@@ -383,9 +390,20 @@ __global__ __launch_bounds__(256) void quant_copy_any_kernel(QuantCopyArgs a, in
   const long long src = a.src[i], dst = a.dst[i];
   if (src < 0 || src >= (long long)a.num_slots || dst < 0 || dst >= (long long)a.num_slots) return;
   const long long from = quant_row(a.pages, (uint32_t)src, h, a.num_kv_heads), to = quant_row(a.pages, (uint32_t)dst, h, a.num_kv_heads);
-  const Pos3 p{a.shift, a.shift, a.shift};
+  const long long shift = a.shifts ? a.shifts[i] : a.shift;
+  const Pos3 p{shift, shift, shift};
   uint8_t* codes = a.codes[0] + layer * a.code_layer_stride;
   uint8_t* scales = a.scales[0] + layer * a.scale_layer_stride;
+  if (a.weights.sums && layer == 0 && lane == 0) move_weights(a.weights, h + 1, src, dst, h, 1);
+  const uint8_t* v_from = a.codes[1] + layer * a.code_layer_stride + from * D;
+  uint8_t* v_to = a.codes[1] + layer * a.code_layer_stride + to * D;
+  for (int d = lane; d < D; d += 64) v_to[d] = v_from[d];
+  if (lane == 0) a.scales[1][layer * a.scale_layer_stride + to] = a.scales[1][layer * a.scale_layer_stride + from];
+  if (shift == 0) {
+    for (int d = lane; d < D; d += 64) codes[to * D + d] = codes[from * D + d];
+    if (lane == 0) scales[to] = scales[from];
+    return;
+  }
   const float f = scale_value(scales[from]);
   auto element = [&](int d) __attribute__((always_inline)) {
     float x[4];
@@ -418,15 +436,11 @@ __global__ __launch_bounds__(256) void quant_copy_any_kernel(QuantCopyArgs a, in
     if (d < D) codes[to * D + d] = scale == 255 ? (uint8_t)0 : (uint8_t)C::pack4(limited<C>(y[k]) * inv, 0.f, 0.f, 0.f);
   }
   if (lane == 0) scales[to] = (uint8_t)scale;
-  const uint8_t* v_from = a.codes[1] + layer * a.code_layer_stride + from * D;
-  uint8_t* v_to = a.codes[1] + layer * a.code_layer_stride + to * D;
-  for (int d = lane; d < D; d += 64) v_to[d] = v_from[d];
-  if (lane == 0) a.scales[1][layer * a.scale_layer_stride + to] = a.scales[1][layer * a.scale_layer_stride + from];
 }
 
 template <typename C>
-static int launch_quant_copy(const QuantCopyArgs& a, int head_dim, int num_layers, hipStream_t stream) {
-  const bool turn = a.shift != 0 && a.rope.half > 0;
+static int launch_quant_copy(const QuantCopyArgs& a, bool own_turns, int head_dim, int num_layers, hipStream_t stream) {
+  const bool turn = (a.shift != 0 || a.shifts) && a.rope.half > 0;
   const bool pieces = !turn || (a.rope.rotary_dim % 16 == 0 && (a.rope.mode != VA_ROPE_TABLE || (uintptr_t)a.rope.cos_sin % 16 == 0));
   if (num_layers > 65535) return va_fail(VA_ERR_ARG, "too many layers for one launch");
   if (!pieces) {
@@ -441,10 +455,12 @@ static int launch_quant_copy(const QuantCopyArgs& a, int head_dim, int num_layer
   switch (head_dim) {
 #define VA_CASE(D)                                                                            \
   case D:                                                                                     \
-    if (turn) {                                                                               \
-      hipLaunchKernelGGL((quant_copy_kernel<C, D, true>), grid, block, 0, stream, a);         \
+    if (own_turns) {                                                                          \
+      hipLaunchKernelGGL((quant_copy_kernel<C, D, kOwnTurn>), grid, block, 0, stream, a);     \
+    } else if (turn) {                                                                        \
+      hipLaunchKernelGGL((quant_copy_kernel<C, D, kOneTurn>), grid, block, 0, stream, a);     \
     } else {                                                                                  \
-      hipLaunchKernelGGL((quant_copy_kernel<C, D, false>), grid, block, 0, stream, a);        \
+      hipLaunchKernelGGL((quant_copy_kernel<C, D, kNoTurn>), grid, block, 0, stream, a);      \
     }                                                                                         \
     break;
     VA_CASE(16) VA_CASE(32) VA_CASE(64) VA_CASE(128) VA_CASE(256)
@@ -514,11 +530,33 @@ extern "C" int va_copy_shift_kv_q8(const VaQuantPool* pool, int64_t code_layer_s
   va::QuantCopyArgs a{{(uint8_t*)pool->k_codes_dev, (uint8_t*)pool->v_codes_dev}, {pool->k_scales_dev, pool->v_scales_dev},
                       code_layer_stride, scale_layer_stride, src_slots_dev, dst_slots_dev, n_tokens, position_shift,
                       (uint32_t)pool->num_pages * (uint32_t)shape->page_size, shape->num_kv_heads,
-                      va::page_map(shape->page_size), va::RopeDev{}};
+                      va::page_map(shape->page_size), va::RopeDev{}, nullptr, va::TokenWeights{nullptr, 0}};
   if (position_shift != 0) {
     rc = va::make_rope(rope, shape->head_dim, &a.rope);
     if (rc) return rc;
   }
-  return pool->code_type == VA_CODE_E4M3 ? va::launch_quant_copy<va::E4M3>(a, shape->head_dim, num_layers, (hipStream_t)stream)
-                                         : va::launch_quant_copy<va::INT8>(a, shape->head_dim, num_layers, (hipStream_t)stream);
+  return pool->code_type == VA_CODE_E4M3 ? va::launch_quant_copy<va::E4M3>(a, false, shape->head_dim, num_layers, (hipStream_t)stream)
+                                         : va::launch_quant_copy<va::INT8>(a, false, shape->head_dim, num_layers, (hipStream_t)stream);
+}
+
+extern "C" int va_move_kv_q8(const VaQuantPool* pool, int64_t code_layer_stride, int64_t scale_layer_stride, int32_t num_layers,
+                             const int64_t* src_slots_dev, const int64_t* dst_slots_dev, const int64_t* shifts_dev, int64_t n_tokens,
+                             float* weights_dev, const VaShape* shape, const VaRope* rope, void* stream) {
+  int rc = va::check_quant_pool(pool, shape);
+  if (rc) return rc;
+  if (n_tokens < 0 || num_layers < 0) return va_fail(VA_ERR_ARG, "negative count");
+  if (n_tokens == 0 || num_layers == 0) return VA_OK;
+  if (!src_slots_dev || !dst_slots_dev) return va_fail(VA_ERR_ARG, "null pointer");
+  if (num_layers > 1 && code_layer_stride % 16) return va_fail(VA_ERR_ARG, "code arrays must start on 16-byte boundaries");
+  const uint32_t slots = (uint32_t)pool->num_pages * (uint32_t)shape->page_size;
+  va::QuantCopyArgs a{{(uint8_t*)pool->k_codes_dev, (uint8_t*)pool->v_codes_dev}, {pool->k_scales_dev, pool->v_scales_dev},
+                      code_layer_stride, scale_layer_stride, src_slots_dev, dst_slots_dev, n_tokens, 0, slots, shape->num_kv_heads,
+                      va::page_map(shape->page_size), va::RopeDev{}, nullptr, va::TokenWeights{weights_dev, (long long)slots}};
+  if (shifts_dev) {
+    rc = va::make_rope(rope, shape->head_dim, &a.rope);
+    if (rc) return rc;
+    if (a.rope.half > 0) a.shifts = shifts_dev;  // (nothing rotates: code for code)
+  }
+  return pool->code_type == VA_CODE_E4M3 ? va::launch_quant_copy<va::E4M3>(a, true, shape->head_dim, num_layers, (hipStream_t)stream)
+                                         : va::launch_quant_copy<va::INT8>(a, true, shape->head_dim, num_layers, (hipStream_t)stream);
 }

@@ -1,0 +1,239 @@
+// Host side of attention weights: the sub-request tables of a step, turned round (va_weigh.h).
+#include <algorithm>
+#include <climits>
+#include <numeric>
+#include <stdexcept>
+#include <vector>
+
+#include "../../include/viewattn.h"
+#include "va_internal.h"
+#include "va_weigh.h"
+
+namespace {
+
+struct Visitor {
+  int32_t sub;
+  int32_t entry;  // of its list
+  int32_t place;  // -1: the whole page; a token of it, for lists of slots
+  bool operator==(const Visitor& o) const { return sub == o.sub && entry == o.entry && place == o.place; }
+};
+
+struct Planner {
+  const VaSubRequests& in;
+  const VaShape& shape;
+  int num_pages, window;
+  std::vector<int64_t> first_visitor;  // by page, [num_pages + 1]
+  std::vector<Visitor> visitors;
+  std::vector<int32_t> pages, items, joins, sub_row, lo, hi;
+  int64_t n_partials = 0;
+
+  int rows_of(int s) const { return in.qo_indptr[s + 1] - in.qo_indptr[s]; }
+  int skipped(int s) const { return window > 0 ? std::max(0, rows_of(s) - window) : 0; }
+  // tokens of its list that row i of sub-request s sees
+  int64_t seen(int s, int i) const {
+    const int64_t len = in.seq_lens[s];
+    return in.flags[s] & VA_SUB_CAUSAL ? std::max<int64_t>(0, len - rows_of(s) + i + 1) : len;
+  }
+  bool slots(int s) const { return in.flags[s] & VA_SUB_SLOTS; }
+  int64_t entries(int s) const { return slots(s) ? in.seq_lens[s] : ((int64_t)in.seq_lens[s] + shape.page_size - 1) / shape.page_size; }
+
+  int check() const {
+    if (in.n_sub < 0 || in.n_subrows < 0) return va_fail(VA_ERR_ARG, "negative count");
+    if (in.n_sub == 0) return VA_OK;
+    if (!in.qo_indptr || !in.kv_indptr || !in.seq_lens || !in.flags) return va_fail(VA_ERR_ARG, "null table");
+    if (in.qo_indptr[0] != 0 || in.qo_indptr[in.n_sub] != in.n_subrows || in.kv_indptr[0] != 0)
+      return va_fail(VA_ERR_ARG, "tables do not start at 0 or end at n_subrows");
+    const int64_t pool = (int64_t)num_pages * shape.page_size;
+    for (int s = 0; s < in.n_sub; ++s) {
+      if (in.qo_indptr[s + 1] < in.qo_indptr[s] || in.kv_indptr[s + 1] < in.kv_indptr[s] || in.seq_lens[s] < 0)
+        return va_fail(VA_ERR_ARG, "sub-request %d: tables must not fall", s);
+      const int64_t n = entries(s);
+      if (n > in.kv_indptr[s + 1] - in.kv_indptr[s]) return va_fail(VA_ERR_ARG, "sub-request %d: %d tokens in %d entries", s, in.seq_lens[s], in.kv_indptr[s + 1] - in.kv_indptr[s]);
+      if (n && !in.kv_indices) return va_fail(VA_ERR_ARG, "null table");
+      for (int64_t e = 0; e < n; ++e) {
+        const int32_t x = in.kv_indices[in.kv_indptr[s] + e];
+        if (x < 0 || x >= (slots(s) ? pool : num_pages))
+          return va_fail(VA_ERR_ARG, "%s %d lies outside the pool of %d pages of %d tokens", slots(s) ? "slot" : "page", x, num_pages, shape.page_size);
+      }
+    }
+    return VA_OK;
+  }
+
+  void find_visitors() {
+    first_visitor.assign((size_t)num_pages + 1, 0);
+    const int P = shape.page_size;
+    auto each = [&](auto&& f) {
+      for (int s = 0; s < in.n_sub; ++s) {
+        if (rows_of(s) == 0) continue;
+        const int32_t* list = in.kv_indices + in.kv_indptr[s];
+        const bool by_slot = slots(s);
+        for (int64_t e = 0, n = entries(s); e < n; ++e) by_slot ? f(list[e] / P, Visitor{s, (int32_t)e, list[e] % P}) : f(list[e], Visitor{s, (int32_t)e, -1});
+      }
+    };
+    each([&](int32_t page, const Visitor&) { ++first_visitor[page + 1]; });
+    for (int p = 0; p < num_pages; ++p) first_visitor[p + 1] += first_visitor[p];
+    visitors.resize((size_t)first_visitor[num_pages]);
+    std::vector<int64_t> at(first_visitor.begin(), first_visitor.end() - 1);
+    each([&](int32_t page, const Visitor& v) { visitors[(size_t)at[page]++] = v; });
+  }
+
+  // Whether the sub-requests that read page a read page b as their next one, and nobody else does.
+  bool follows(int32_t a, int32_t b) const {
+    const int64_t n = first_visitor[a + 1] - first_visitor[a];
+    if (n != first_visitor[b + 1] - first_visitor[b]) return false;
+    const Visitor *x = &visitors[(size_t)first_visitor[a]], *y = &visitors[(size_t)first_visitor[b]];
+    for (int64_t i = 0; i < n; ++i)
+      if (x[i].place >= 0 || !(Visitor{x[i].sub, x[i].entry + 1, -1} == y[i])) return false;
+    return true;
+  }
+
+  struct Span {
+    int64_t page_begin;
+    int32_t first, end;  // tokens that anybody sees
+    int64_t row_begin, row_end;  // packed
+  };
+  std::vector<Span> spans;
+
+  int close(const std::vector<int32_t>& run) {
+    const int P = shape.page_size, G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G);
+    const int64_t room = (int64_t)run.size() * P;
+    const int64_t row_begin = (int64_t)sub_row.size();
+    int64_t first = INT64_MAX, end = 0;
+    for (int64_t k = first_visitor[run[0]]; k < first_visitor[run[0] + 1]; ++k) {
+      const Visitor& v = visitors[(size_t)k];
+      for (int i = skipped(v.sub); i < rows_of(v.sub); ++i) {
+        int64_t from = 0, to = std::min(room, seen(v.sub, i) - (int64_t)v.entry * P);
+        if (v.place >= 0) from = v.place, to = seen(v.sub, i) > v.entry ? v.place + 1 : 0;
+        if (to <= from) continue;
+        sub_row.push_back(in.qo_indptr[v.sub] + i);
+        lo.push_back((int32_t)from);
+        hi.push_back((int32_t)to);
+        first = std::min(first, from), end = std::max(end, to);
+      }
+    }
+    if ((int64_t)sub_row.size() == row_begin) return VA_OK;
+    while (sub_row.size() % unit) sub_row.push_back(-1), lo.push_back(0), hi.push_back(0);
+    if ((int64_t)sub_row.size() * G > INT32_MAX) return va_fail(VA_ERR_ARG, "too many query rows for one plan");
+    spans.push_back(Span{(int64_t)pages.size(), (int32_t)first, (int32_t)end, row_begin, (int64_t)sub_row.size()});
+    pages.insert(pages.end(), run.begin(), run.end());
+    return VA_OK;
+  }
+
+  int find_spans() {
+    std::vector<char> done((size_t)num_pages, 0);
+    std::vector<int32_t> run;
+    for (int s = 0; s < in.n_sub; ++s) {
+      if (rows_of(s) == 0) continue;
+      const int32_t* list = in.kv_indices + in.kv_indptr[s];
+      for (int64_t e = 0, n = entries(s); e < n; ++e) {
+        const int32_t page = slots(s) ? list[e] / shape.page_size : list[e];
+        if (done[page]) continue;
+        done[page] = 1;
+        // (tokens of a span are counted in 32 bits)
+        if (!run.empty() && !(follows(run.back(), page) && ((int64_t)run.size() + 1) * shape.page_size <= INT32_MAX)) {
+          if (const int rc = close(run)) return rc;
+          run.clear();
+        }
+        run.push_back(page);
+      }
+    }
+    if (run.empty()) return VA_OK;
+    return close(run);
+  }
+
+  // Rows of a chunk are split where the launch has too few workgroups otherwise.
+  int make_items() {
+    const int G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G), T = VA_WEIGH_CHUNK;
+    constexpr int64_t kWanted = 1024;
+    int64_t chunks = 0;
+    for (const Span& s : spans) chunks += ((int64_t)s.end - s.first + T - 1) / T;
+    const int64_t groups = chunks * shape.num_kv_heads, cuts = std::max<int64_t>(1, (kWanted + groups - 1) / std::max<int64_t>(1, groups));
+    for (const Span& s : spans) {
+      for (int64_t t = s.first; t < s.end; t += T) {
+        const int n_tok = (int)std::min<int64_t>(T, s.end - t);
+        // the rows that see any of it lie between these (a request's rows see ever more)
+        int64_t a = s.row_begin, b = s.row_end;
+        while (a < b && (hi[(size_t)a] <= t || lo[(size_t)a] >= t + n_tok)) ++a;
+        while (b > a && (hi[(size_t)b - 1] <= t || lo[(size_t)b - 1] >= t + n_tok)) --b;
+        if (a == b) continue;
+        const int64_t tile_a = a / unit * unit * G / 16, tile_b = ((b + unit - 1) / unit * unit) * G / 16;
+        const int64_t parts = std::min(cuts, tile_b - tile_a);
+        if (parts > 1) {
+          if (n_partials + parts * n_tok > INT32_MAX) return va_fail(VA_ERR_ARG, "too many partial sums for one plan");
+          const int32_t join[VA_WEIGH_JOIN_WORDS] = {(int32_t)s.page_begin, (int32_t)t, n_tok, (int32_t)n_partials, (int32_t)parts, 0, 0, 0};
+          joins.insert(joins.end(), join, join + VA_WEIGH_JOIN_WORDS);
+        }
+        for (int64_t p = 0; p < parts; ++p) {
+          const int32_t item[VA_WEIGH_ITEM_WORDS] = {(int32_t)s.page_begin, (int32_t)t, n_tok, (int32_t)(tile_a + (tile_b - tile_a) * p / parts),
+                                                     (int32_t)(tile_a + (tile_b - tile_a) * (p + 1) / parts),
+                                                     parts > 1 ? (int32_t)(n_partials + p * n_tok) : -1, 0, 0};
+          items.insert(items.end(), item, item + VA_WEIGH_ITEM_WORDS);
+        }
+        if (parts > 1) n_partials += parts * n_tok;
+      }
+    }
+    while (items.size() % (8 * VA_WEIGH_ITEM_WORDS)) items.push_back(0);
+    if (items.size() / VA_WEIGH_ITEM_WORDS * (size_t)shape.num_kv_heads > INT32_MAX) return va_fail(VA_ERR_ARG, "too many work items for one launch");
+    return VA_OK;
+  }
+};
+
+int build(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, int32_t window, int32_t* plan, int64_t capacity, VaWeighCounts* counts) {
+  if (!subs || !shape || !counts) return va_fail(VA_ERR_ARG, "null pointer");
+  if (shape->num_kv_heads <= 0 || shape->num_q_heads <= 0 || shape->num_q_heads % shape->num_kv_heads || shape->head_dim <= 0 || shape->page_size <= 0)
+    return va_fail(VA_ERR_ARG, "bad shape");
+  if (num_pages < 0 || (int64_t)num_pages * shape->page_size > INT32_MAX || window < 0)
+    return va_fail(VA_ERR_ARG, "%d pages of %d tokens, window %d", (int)num_pages, (int)shape->page_size, (int)window);
+  Planner p{*subs, *shape, num_pages, window, {}, {}, {}, {}, {}, {}, {}, {}, 0, {}};
+  int rc = p.check();
+  if (rc) return rc;
+  p.find_visitors();
+  if ((rc = p.find_spans()) || (rc = p.make_items())) return rc;
+  const int64_t n_rows = (int64_t)p.sub_row.size();
+  const int64_t words = VA_WEIGH_HEADER_WORDS + (int64_t)p.items.size() + (int64_t)p.joins.size() + (int64_t)p.pages.size() + 3 * n_rows;
+  if (words > INT32_MAX) return va_fail(VA_ERR_ARG, "too large a plan");
+  const int64_t pairs = n_rows * (shape->num_q_heads / shape->num_kv_heads);
+  counts->n_items = (int32_t)(p.items.size() / VA_WEIGH_ITEM_WORDS);
+  counts->n_rows = (int32_t)n_rows;
+  counts->n_joins = (int32_t)(p.joins.size() / VA_WEIGH_JOIN_WORDS);
+  counts->n_spans = (int32_t)p.spans.size();
+  counts->plan_words = (int32_t)words;
+  // queries as up to three 16-bit numbers an element (one 32-bit one on the vector ALU), 16 bytes a row beside them, partial sums
+  counts->workspace_bytes = shape->num_kv_heads * (pairs * (6 * (int64_t)shape->head_dim + 16) + 4 * p.n_partials);
+  if (!plan || capacity < words) return va_fail(VA_ERR_CAPACITY, "plan needs %lld words, %lld given", (long long)words, (long long)capacity);
+  int32_t* h = plan;
+  std::fill(h, h + VA_WEIGH_HEADER_WORDS, 0);
+  int64_t at = VA_WEIGH_HEADER_WORDS;
+  auto put = [&](const std::vector<int32_t>& x) {
+    std::copy(x.begin(), x.end(), plan + at);
+    const int32_t begin = (int32_t)at;
+    at += (int64_t)x.size();
+    return begin;
+  };
+  h[VA_WH_MAGIC] = VA_WEIGH_MAGIC;
+  h[VA_WH_N_ITEMS] = counts->n_items;
+  h[VA_WH_N_ROWS] = counts->n_rows;
+  h[VA_WH_N_JOINS] = counts->n_joins;
+  h[VA_WH_N_PARTIALS] = (int32_t)p.n_partials;
+  h[VA_WH_N_PAGES] = (int32_t)p.pages.size();
+  h[VA_WH_OFF_ITEMS] = put(p.items);
+  h[VA_WH_OFF_JOINS] = put(p.joins);
+  h[VA_WH_OFF_PAGES] = put(p.pages);
+  h[VA_WH_OFF_ROWS] = put(p.sub_row);
+  put(p.lo);
+  put(p.hi);
+  h[VA_WH_HQ] = shape->num_q_heads, h[VA_WH_HKV] = shape->num_kv_heads, h[VA_WH_D] = shape->head_dim;
+  h[VA_WH_PAGE] = shape->page_size, h[VA_WH_DTYPE] = shape->dtype, h[VA_WH_POOL_PAGES] = num_pages, h[VA_WH_N_SUBROWS] = subs->n_subrows;
+  return VA_OK;
+}
+
+}  // namespace
+
+extern "C" int va_weigh_plan(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, int32_t window, int32_t* plan_host,
+                             int64_t plan_capacity_words, VaWeighCounts* counts) {
+  try {
+    return build(subs, shape, num_pages, window, plan_host, plan_capacity_words, counts);
+  } catch (const std::exception& e) {  // (no memory: nothing may leave a C entry)
+    return va_fail(VA_ERR_CAPACITY, "planning weights: %s", e.what());
+  }
+}

@@ -48,6 +48,19 @@ class MHAKVCache:
         return self._num_layers
 
 
+def layer_runs(pool) -> list:
+    """A pool's layers as ``(first, layers, elements from one to the next)``: one run where they lie evenly apart."""
+    L = pool.num_layers
+    if L < 2:
+        return [(0, L, 0)]
+    k0, v0 = pool.k_cache(0), pool.v_cache(0)
+    item, k_step = k0.element_size(), pool.k_cache(1).data_ptr() - k0.data_ptr()
+    uniform = k_step % item == 0 and pool.v_cache(1).data_ptr() - v0.data_ptr() == k_step and all(
+        pool.k_cache(l).data_ptr() == k0.data_ptr() + l * k_step
+        and pool.v_cache(l).data_ptr() == v0.data_ptr() + l * k_step for l in range(2, L))
+    return [(0, L, k_step // item)] if uniform else [(l, 1, 0) for l in range(L)]
+
+
 def store_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, indices: torch.Tensor,
                k: torch.Tensor, v: torch.Tensor) -> None:
     """``cache[indices[i]] = row i`` for K and V (same argument order as the

@@ -21,6 +21,7 @@ VA_ROPE_TABLE, VA_ROPE_MROPE = 0, 1
 VA_KERNEL_AUTO, VA_KERNEL_GENERIC, VA_KERNEL_MFMA = 0, 1, 2
 VA_SUB_CAUSAL, VA_SUB_SLOTS = 1, 2
 PLAN_HEADER_WORDS = 24
+WEIGH_HEADER_WORDS = 24  # VA_WEIGH_HEADER_WORDS
 PLAN_FLAGS_WORD = 3  # of a header: the chunk, with flags in its low bits
 PLAN_SHORT_ITEMS = 1  # narrow items are short: several workgroups share a CU
 VA_TILES_APART = -(2**31)  # of VaPlanParams.wide_tile: no wide tiles, nor several in a workgroup
@@ -52,6 +53,15 @@ EXPORTED_SYMBOLS = (
     "va_attention_if_q8",
     "va_read_back_bytes",
     "va_attention_read_back_q8",
+    "va_rotate_qk",
+    "va_rotary_table",
+    "va_select_workspace_bytes",
+    "va_select_tokens",
+    "va_move_kv",
+    "va_move_kv_q8",
+    "va_weigh_plan",
+    "va_weigh",
+    "va_weigh_q8",
 )
 
 
@@ -85,6 +95,15 @@ class VaQuantPool(C.Structure):
         ("v_scales_dev", C.c_void_p),
         ("code_type", C.c_int32),
         ("num_pages", C.c_int32),
+    ]
+
+
+class VaTurns(C.Structure):
+    _fields_ = [
+        ("rotary_dim", C.c_int32),
+        ("neighbours", C.c_int32),
+        ("factor", C.c_float),
+        ("quarters_dev", C.c_void_p),
     ]
 
 
@@ -128,6 +147,17 @@ class VaPlanCounts(C.Structure):
         ("n_wide_items", C.c_int32),
         ("workspace_bytes", C.c_int64),
         ("n_wide_slots", C.c_int32),
+    ]
+
+
+class VaWeighCounts(C.Structure):
+    _fields_ = [
+        ("n_items", C.c_int32),
+        ("n_rows", C.c_int32),
+        ("n_joins", C.c_int32),
+        ("n_spans", C.c_int32),
+        ("plan_words", C.c_int32),
+        ("workspace_bytes", C.c_int64),
     ]
 
 
@@ -207,6 +237,26 @@ def _load() -> C.CDLL:
     lib.va_attention_read_back_q8.restype = C.c_int
     lib.va_attention_read_back_q8.argtypes = [vp, i64, pool, vp, i64, vp, vp, vp, vp, vp, i64, vp, vp, i32, vp, i64, vp, i64,
                                               C.POINTER(VaShape), C.POINTER(VaRope), vp]
+    turns = C.POINTER(VaTurns)
+    lib.va_rotate_qk.restype = C.c_int
+    lib.va_rotate_qk.argtypes = [vp, i64, i32, vp, i64, vp, i64, i32, vp, i64, vp, i32, i64, i32, i32, turns, vp]
+    lib.va_rotary_table.restype = C.c_int
+    lib.va_rotary_table.argtypes = [turns, i64, i64, vp, vp]
+    lib.va_select_workspace_bytes.restype = C.c_int64
+    lib.va_select_workspace_bytes.argtypes = [i32, vp]
+    lib.va_select_tokens.restype = C.c_int
+    lib.va_select_tokens.argtypes = [vp, i32, i64, vp, i32, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp]
+    lib.va_move_kv.restype = C.c_int
+    lib.va_move_kv.argtypes = [vp, vp, i64, i64, i32, i64, vp, vp, vp, i64, vp, C.POINTER(VaShape), C.POINTER(VaRope), vp]
+    lib.va_move_kv_q8.restype = C.c_int
+    lib.va_move_kv_q8.argtypes = [pool, i64, i64, i32, vp, vp, vp, i64, vp, C.POINTER(VaShape), C.POINTER(VaRope), vp]
+    lib.va_weigh_plan.restype = C.c_int
+    lib.va_weigh_plan.argtypes = [C.POINTER(VaSubRequests), C.POINTER(VaShape), i32, i32, vp, i64, C.POINTER(VaWeighCounts)]
+    tables = [vp, vp, vp, vp, i64, vp, i32, vp, vp, vp, i64, C.POINTER(VaShape), C.POINTER(VaRope), vp]
+    lib.va_weigh.restype = C.c_int
+    lib.va_weigh.argtypes = [vp, i64, vp, i64, *tables]
+    lib.va_weigh_q8.restype = C.c_int
+    lib.va_weigh_q8.argtypes = [vp, i64, pool, *tables]
     return lib
 
 

@@ -62,6 +62,8 @@ class LaunchPlan:
     staging: Optional[torch.Tensor] = None
     coarse: Optional["LaunchPlan"] = None
     readback: object = None  # what an op over a quantised pool reads back in front of the launch
+    # the sub-request tables that it was planned from (int32 arrays in VaSubRequests' order, sub_worker, rows): who sees what
+    host_tables: Optional[tuple] = None
 
     @property
     def header_ptr(self) -> int:
@@ -340,6 +342,7 @@ class SharedCacheAttention:
         launch, (dev_indices, *dev_tables) = self._upload_plan(subs, None, refs, (kv_indices, *tables), params,
                                                               shape)
         launch.kv_indices = dev_indices
+        launch.host_tables = (arrays, sw, n_rows)
         return launch, dev_tables
 
     def _upload_plan(self, subs, kv_indices_dev: Optional[torch.Tensor], refs: list, tables: Sequence,

@@ -25,7 +25,9 @@ import numpy as np
 import torch
 
 from .. import native
+from ..kvcache.mha_pool import layer_runs
 from ..kvcache.quantized_pool import QuantizedKVCache
+from .eviction import CacheEviction
 from .shared_block import CacheBlock
 
 
@@ -71,6 +73,7 @@ class BlockKVOps:
         self.device = sc_attn.device
         self.compose_affines = compose_affines
         self._refs: tuple = ()
+        self._eviction: Optional[CacheEviction] = None
 
     def create_block(self) -> CacheBlock:
         return CacheBlock(self.device, self.page_size)
@@ -116,6 +119,50 @@ class BlockKVOps:
         self._finish_block_merge(destination=left, left=left, right=right, left_span=left_span,
                                  right_span=right_span, keep_left_state=True)
         return left
+
+    def evict_tokens(self, block: CacheBlock, weights: torch.Tensor, keep: int, first: int = 0, last: int = 0,
+                     close_gaps: bool = False) -> CacheBlock:
+        """Copy what stays of ``block`` into a new compact block: ``keep`` tokens, the first ``first`` and the last ``last`` among
+        them and the others by ``weights`` (``CacheEviction``), which move along.  ``block`` stays valid and unchanged; its pages
+        are the caller's to hand back.
+
+        Keys keep their positions and the new block spans as many as the old one; with ``close_gaps`` they are turned to
+        the positions that the tokens have in the new block, which needs a block whose positions count its tokens.  A
+        recurrent state, which holds all tokens, goes along as it is."""
+        self._validate_block(block)
+        if getattr(self.sc_attn, "kv_cache", None) is not self.kv_cache:
+            raise ValueError("tokens are evicted with the attention over this pool")
+        if self.device.type != "cuda":
+            raise native.ViewAttnError("blocks are evicted from on the GPU only (HIP kernels, no CPU path)")
+        if keep < 0 or first < 0 or last < 0:
+            raise ValueError(f"keep, first and last must not be negative, got {keep}, {first} and {last}")
+        if close_gaps and block.mrope_span != block.num_tokens:
+            raise ValueError("close_gaps needs a block whose positions count its tokens")
+        if self._eviction is None:
+            self._eviction = CacheEviction(self.sc_attn)
+        eviction = self._eviction
+        eviction._check_weights(weights)
+        n = min(keep, block.num_tokens)
+        result = self.create_block()
+        if n:
+            source = token_slots(block)
+            result.page_starts = self.page_allocator.alloc_pages(-(-n // self.page_size)).tolist()
+            result.num_tokens = result.num_pages * self.page_size
+            room = token_slots(result)  # whole pages
+            result.num_tokens = n
+            host = torch.from_numpy(np.concatenate([source, room])).pin_memory()
+            dev = host.to(self.device, non_blocking=True)
+            self._refs = (host, dev)
+            eviction.clear(weights, dev[source.size:])
+            kept = eviction.select(weights, dev[: source.size], [source.size], n, first, last)
+            eviction.move(kept.slots, dev[source.size: source.size + n], kept.shifts if close_gaps else None, weights)
+            if len(block.token_ids) == block.num_tokens:
+                result.token_ids = [block.token_ids[i] for i in kept.positions.tolist()]
+        span = n if close_gaps else block.mrope_span
+        result.mrope_span_override = None if span == n else span
+        result._replace_linear_states({i: (a.clone(), b.clone()) for i, (a, b) in block.linear_affine.items()},
+                                      {i: s.clone() for i, s in block.linear_conv_state.items()})
+        return result
 
     # ------------------------------------------------------------------
     def _finish_block_merge(self, *, destination: CacheBlock, left: CacheBlock, right: CacheBlock, left_span: int,
@@ -199,22 +246,12 @@ class BlockKVOps:
         if isinstance(self.kv_cache, QuantizedKVCache):
             att.copy_shifted(dev[0], dev[1], position_shift)
             return
-        L = self.kv_cache.num_layers
         k0, v0 = self.kv_cache.k_cache(0), self.kv_cache.v_cache(0)
         assert k0.is_contiguous() and v0.is_contiguous(), "pool layers must be contiguous"
         width = att.num_kv_heads * att.head_dim
-        item = k0.element_size()
-        groups = [(0, L, 0)]
-        if L > 1:
-            k_step = self.kv_cache.k_cache(1).data_ptr() - k0.data_ptr()
-            v_step = self.kv_cache.v_cache(1).data_ptr() - v0.data_ptr()
-            uniform = k_step == v_step and k_step % item == 0 and all(
-                self.kv_cache.k_cache(l).data_ptr() == k0.data_ptr() + l * k_step
-                and self.kv_cache.v_cache(l).data_ptr() == v0.data_ptr() + l * k_step for l in range(2, L))
-            groups = [(0, L, k_step // item)] if uniform else [(l, 1, 0) for l in range(L)]
         rope = att._rope_descriptor() if position_shift else None
         stream = native.current_stream_ptr(self.device)
-        for first, count, stride in groups:
+        for first, count, stride in layer_runs(self.kv_cache):
             k_pool, v_pool = self.kv_cache.k_cache(first), self.kv_cache.v_cache(first)
             native.check(native.lib.va_copy_shift_kv(
                 k_pool.data_ptr(), v_pool.data_ptr(), width, stride, count, dev[0].data_ptr(), dev[1].data_ptr(),

@@ -1,0 +1,230 @@
+"""Eviction from a paged cache by accumulated attention weight.
+
+Blocks of a view live long and only ever grow.  ``CacheEviction`` keeps count of what
+attention looks at, chooses what stays of a block and moves that together:
+
+* ``accumulate`` adds, for every cached token and kv head, the softmax weight that a
+  step's queries gave the token (from the step's plan, its unrotated queries and its
+  log-sums) to ``weights [kv_heads, slots]``;
+* ``select`` keeps of each block the first and the last few tokens and the heaviest of
+  the others;
+* ``move`` copies tokens to other slots in all layers, each key turned by a shift of its
+  own, and their weights with them.
+
+``BlockKVOps.evict_tokens`` does the last two for a block.  The reference has no eviction;
+what this stands beside is its block merge and append
+(``python/minisgl/shared_cache/session.py:330-528``).
+
+Weights are by slot: whoever hands pages back and gets them again clears theirs (``clear``).
+A key keeps its position where it is moved without a shift: the block then spans as many
+positions as before.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import List, Optional, Sequence, Union
+
+import numpy as np
+import torch
+
+from .. import native
+from ..kvcache.mha_pool import layer_runs
+from ..kvcache.quantized_pool import QuantizedKVCache
+from .attention import SharedCacheAttention, SharedCacheAttnMetadata
+
+
+@dataclass
+class WeightPlan:
+    """Who sees which token in a step, by token; serves all layers of the step."""
+
+    header: np.ndarray  # int32, host
+    blob: torch.Tensor  # int32, device
+    counts: native.VaWeighCounts
+    sub_worker: torch.Tensor
+    sub_loc: torch.Tensor
+    rows: int  # query rows of the step
+    refs: tuple = ()
+
+
+@dataclass
+class KeptTokens:
+    """What stays of some blocks, one after the other: positions in each block in rising order, slots, new position minus
+    position (int64 on the device), and how many of each block (host)."""
+
+    positions: torch.Tensor
+    slots: torch.Tensor
+    shifts: torch.Tensor
+    counts: List[int]
+
+
+class CacheEviction:
+    """Eviction over the pool of ``op``, a ``SharedCacheAttention`` or ``QuantizedCacheAttention``."""
+
+    def __init__(self, op: SharedCacheAttention) -> None:
+        self.op = op
+        self.kv_cache = op.kv_cache
+        self.device = op.device
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        if op.num_qo_heads % op.num_kv_heads:
+            raise ValueError(f"{op.num_qo_heads} q heads are no multiple of {op.num_kv_heads} kv heads")
+        self._coded = isinstance(self.kv_cache, QuantizedKVCache)
+        if self._coded:
+            self.num_pages = self.kv_cache.num_pages
+        else:
+            op._check_pool_layout()
+            self.num_pages = self.kv_cache.k_cache(0).shape[0]
+        self.num_slots = self.num_pages * op.page_size
+        if self.num_slots > 2**31 - 1:
+            raise ValueError(f"{self.num_pages} pages of {op.page_size} tokens are more slots than 32 bits address")
+
+    # ------------------------------------------------------------------
+    # weights
+    # ------------------------------------------------------------------
+    def new_weights(self) -> torch.Tensor:
+        """Weights of a pool that nobody has looked at: float32 zeros ``[kv_heads, slots]``."""
+        return torch.zeros((self.op.num_kv_heads, self.num_slots), dtype=torch.float32, device=self.device)
+
+    def _check_weights(self, weights: torch.Tensor, name: str = "weights") -> None:
+        want = (self.op.num_kv_heads, self.num_slots)
+        if weights.shape != want or weights.dtype != torch.float32 or weights.device != self.device or not weights.is_contiguous():
+            native.require_device(weights, name)
+            raise ValueError(f"{name} must be a contiguous float32 tensor {list(want)} on {self.device}, got {weights.dtype} "
+                             f"{list(weights.shape)} on {weights.device}")
+
+    def clear(self, weights: torch.Tensor, slots: torch.Tensor) -> None:
+        """Forget what the tokens of ``slots`` (int64) were given."""
+        self._check_weights(weights)
+        weights.index_fill_(1, slots.to(device=self.device, dtype=torch.int64), 0.0)
+
+    def plan(self, meta: SharedCacheAttnMetadata, window: int = 0) -> WeightPlan:
+        """Turn a step's plan (of ``prepare``, ``prepare_prefill_batch`` or ``prepare_mixed``) round.  ``window > 0``: of many new
+        tokens of a request only the last ``window`` are counted."""
+        tables = None if meta.launch is None else meta.launch.host_tables
+        if meta.shared_cache_op is not self.op or tables is None:
+            raise ValueError("plan needs the metadata of a step that this op planned without fixed buffers")
+        if window < 0:
+            raise ValueError(f"window must not be negative, got {window}")
+        arrays, sub_worker, n_rows = tables
+        n_sub = len(arrays[3])
+        subs = native.VaSubRequests(n_sub, len(sub_worker), n_rows, arrays[0].ctypes.data, arrays[1].ctypes.data,
+                                    arrays[2].ctypes.data if arrays[2].size else None, arrays[3].ctypes.data,
+                                    arrays[4].ctypes.data, None, None)
+        counts = native.VaWeighCounts()
+        words = np.empty(1 << 14, dtype=np.int32)
+        for _ in range(2):
+            rc = native.lib.va_weigh_plan(subs, self.op._shape, self.num_pages, window, words.ctypes.data, words.size, counts)
+            if rc != native.VA_ERR_CAPACITY or counts.plan_words <= words.size:
+                break
+            words = np.empty(counts.plan_words, dtype=np.int32)
+        native.check(rc)
+        host = torch.empty(counts.plan_words, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        host.numpy()[:] = words[: counts.plan_words]
+        blob = host.to(self.device, non_blocking=True)
+        return WeightPlan(words[: native.WEIGH_HEADER_WORDS].copy(), blob, counts, meta.sub_worker, meta.sub_loc, meta.num_workers,
+                          (host,))
+
+    def accumulate(self, q: torch.Tensor, lse: torch.Tensor, layer_id: int, plan: WeightPlan, weights: torch.Tensor,
+                   out: Optional[torch.Tensor] = None, lse_base2: bool = False) -> torch.Tensor:
+        """Add what the step's queries ``q`` (unrotated rows, as ``forward`` takes them) gave the tokens of layer ``layer_id``
+        to ``weights``, and return it.  ``lse [rows, q_heads]``: the log-sums that ``forward_with_lse`` returned for the same
+        queries.  With ``out`` the sums of the tokens in sight go there instead, and ``weights`` and the other slots of
+        ``out`` stay as they are."""
+        op, device = self.op, self.device
+        native.require_device(q, "q")
+        q2, q_stride = op._rows(q, op.num_qo_heads)
+        if q2.dtype != op.dtype or q2.device != device or q2.shape[0] < plan.rows:
+            raise ValueError(f"q must be {plan.rows} rows of {op.dtype} on {device}, got {q2.dtype} {tuple(q2.shape)} on {q2.device}")
+        if lse.dim() != 2 or lse.shape[0] < plan.rows or lse.shape[1] != op.num_qo_heads or lse.dtype != torch.float32 \
+                or lse.device != device or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous float32 tensor [{plan.rows}, {op.num_qo_heads}] on {device}, got {lse.dtype} "
+                             f"{tuple(lse.shape)} on {lse.device}")
+        self._check_weights(weights)
+        if out is None:
+            out = weights
+        else:
+            self._check_weights(out, "out")
+        # (from the allocator, call by call: streams and graphs that share a plan have scratch of their own)
+        workspace = torch.empty(plan.counts.workspace_bytes, dtype=torch.uint8, device=device)
+        sub_loc = plan.sub_loc
+        tables = (plan.blob.data_ptr(), plan.header.ctypes.data, plan.sub_worker.data_ptr(), sub_loc.data_ptr(),
+                  sub_loc.stride(0) if sub_loc.dim() == 2 else 0, lse.data_ptr(), int(lse_base2), weights.data_ptr(),
+                  out.data_ptr(), workspace.data_ptr(), plan.counts.workspace_bytes, op._shape, op._rope_descriptor(),
+                  native.current_stream_ptr(device))
+        if self._coded:
+            native.call_on(device, native.lib.va_weigh_q8, q2.data_ptr(), q_stride, self.kv_cache.layer(layer_id), *tables)
+            return out
+        pool = self.kv_cache.k_cache(layer_id)
+        if pool.shape[0] != self.num_pages or pool.dtype != op.dtype or not pool.is_contiguous():
+            raise ValueError(f"kv_cache.k_cache({layer_id}) must be a contiguous {op.dtype} tensor of {self.num_pages} pages")
+        native.call_on(device, native.lib.va_weigh, q2.data_ptr(), q_stride, pool.data_ptr(), op.num_kv_heads * op.head_dim, *tables)
+        return out
+
+    # ------------------------------------------------------------------
+    # choosing
+    # ------------------------------------------------------------------
+    @staticmethod
+    def select(weights: torch.Tensor, slots: torch.Tensor, counts: Sequence[int], keep: Union[int, Sequence[int]],
+               first: int = 0, last: int = 0) -> KeptTokens:
+        """What stays of blocks whose token slots are ``counts[b]`` consecutive entries of ``slots`` (int64): ``keep[b]`` tokens (all of
+        a block with fewer), the first ``first`` and the last ``last`` among them (the lower positions where those are more), the
+        others by ``weights [heads, slots]``, heaviest first; ties go to the lower position."""
+        native.require_device(weights, "weights")
+        device = weights.device
+        if weights.dim() != 2 or weights.dtype != torch.float32 or not weights.is_contiguous():
+            raise ValueError(f"weights must be a contiguous float32 tensor [heads, slots], got {weights.dtype} {tuple(weights.shape)}")
+        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != device:
+            raise ValueError(f"slots must be one row of int64 on {device}, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
+        tokens = np.asarray(counts, dtype=np.int64).reshape(-1)
+        wanted = np.broadcast_to(np.asarray(keep, dtype=np.int64), tokens.shape)
+        if tokens.size and (tokens.min() < 0 or wanted.min() < 0) or first < 0 or last < 0:
+            raise ValueError("counts, keep, first and last must not be negative")
+        if int(tokens.sum()) != slots.numel():
+            raise ValueError(f"counts add up to {int(tokens.sum())} tokens, slots has {slots.numel()}")
+        wanted = np.minimum(wanted, tokens)
+        total = int(wanted.sum())
+        results = torch.empty((3, total), dtype=torch.int64, device=device)
+        positions, kept_slots, shifts = results.unbind(0)
+        nbytes = native.lib.va_select_workspace_bytes(tokens.size, tokens.ctypes.data)
+        if nbytes < 0:
+            raise ValueError("a block holds at most 2^31 - 1 tokens")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        slots = slots.contiguous()
+        native.call_on(device, native.lib.va_select_tokens, weights.data_ptr(), weights.shape[0], weights.shape[1], slots.data_ptr(),
+                       tokens.size, tokens.ctypes.data, wanted.ctypes.data, first, last, positions.data_ptr(),
+                       kept_slots.data_ptr(), shifts.data_ptr(), None if workspace is None else workspace.data_ptr(), nbytes,
+                       native.current_stream_ptr(device))
+        return KeptTokens(positions, kept_slots, shifts, wanted.tolist())
+
+    # ------------------------------------------------------------------
+    # moving
+    # ------------------------------------------------------------------
+    def move(self, source: torch.Tensor, target: torch.Tensor, shifts: Optional[torch.Tensor] = None,
+             weights: Optional[torch.Tensor] = None) -> None:
+        """Copy the tokens of slots ``source`` to slots ``target`` (int64 on the device, each target once, none of them a source of
+        another token) in every layer, keys rotated by ``shifts`` (int64; ``None``: as they are), and their ``weights``."""
+        op, device, n = self.op, self.device, source.numel()
+        for name, t in (("source", source), ("target", target), ("shifts", shifts)):
+            if t is None and name == "shifts":
+                continue
+            native.require_device(t, name)
+            if t.dim() != 1 or t.dtype != torch.int64 or t.device != device or t.numel() != n:
+                raise ValueError(f"{name} must be one row of {n} int64 numbers on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if weights is not None:
+            self._check_weights(weights)
+        pool, source, target = self.kv_cache, source.contiguous(), target.contiguous()
+        shifts = None if shifts is None else shifts.contiguous()
+        slots = (source.data_ptr(), target.data_ptr(), None if shifts is None else shifts.data_ptr(), n)
+        rope = None if shifts is None else op._rope_descriptor()
+        sums = None if weights is None else weights.data_ptr()
+        if self._coded:
+            if pool.num_layers:
+                native.call_on(device, native.lib.va_move_kv_q8, pool.layer(0), pool.code_layer_bytes, pool.scale_layer_bytes,
+                               pool.num_layers, *slots, sums, op._shape, rope, native.current_stream_ptr(device))
+            return
+        width, stream = op.num_kv_heads * op.head_dim, native.current_stream_ptr(device)
+        for first, count, stride in layer_runs(pool):
+            native.call_on(device, native.lib.va_move_kv, pool.k_cache(first).data_ptr(), pool.v_cache(first).data_ptr(), width,
+                           stride, count, self.num_slots, *slots, sums, op._shape, rope, stream)
+            sums = None  # (moved with the first run)

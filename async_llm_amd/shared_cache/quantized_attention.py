@@ -148,6 +148,8 @@ class QuantizedCacheAttention(SharedCacheAttention):
         else:
             launch = LaunchPlan(wide.header, wide.blob, wide.kv_indices, wide.counts, wide.workspace)
         launch.readback = back
+        arrays = [np.ascontiguousarray(a, dtype=np.int32) for a in (qo, kvp, kv, seq_lens, flags, chain)]
+        launch.host_tables = (arrays, np.ascontiguousarray(sub_worker_host, dtype=np.int64), n_rows)
         return launch, dev_tables
 
     def _reads_back(self, pairs: int, pages: int) -> bool:

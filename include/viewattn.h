@@ -473,6 +473,123 @@ VA_API int va_attention_read_back_q8(const void* q_dev, int64_t q_row_stride, co
                               void* workspace_dev, int64_t workspace_bytes, void* scratch_dev,
                               int64_t scratch_bytes, const VaShape* shape, const VaRope* rope, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Positions: queries and keys rotated as a step makes them, for layers that call an
+ * attention without a view (reference layers/rotary.py:24-51), and the cos|sin
+ * table that VaRope takes.  The angle of pair i at position p is
+ * p * quarters[i] * pi / 2, the product taken in 64 bits, so that far positions
+ * lose nothing; cosines and sines are 32-bit numbers, times `factor`.
+ * ------------------------------------------------------------------------- */
+typedef struct VaTurns {
+  int32_t rotary_dim;         /* leading head dims that rotate, even                           */
+  int32_t neighbours;         /* pairs are (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2)   */
+  float factor;               /* on cosines and sines                                          */
+  const double* quarters_dev; /* [rotary_dim / 2]: frequencies in quarter turns a position     */
+} VaTurns;
+
+/*
+ * va_rotate_qk: out_q[i, h] = R(positions[i]) q[i, h], and the same of k, for
+ * i < n_rows; dims past rotary_dim pass through.  positions are int64 or int32
+ * (negative ones turn backwards).  Rows lie *_row_stride ELEMENTS apart, heads
+ * head_dim apart; out may be the input itself, row by row.  Either of q and k may
+ * have no heads.  Any alignment (16-byte aligned rows and rotary_dim a multiple
+ * of 16, 8 for VA_F32, are fast).
+ */
+VA_API int va_rotate_qk(const void* q_dev, int64_t q_row_stride, int32_t num_q_heads, void* out_q_dev,
+                 int64_t out_q_row_stride, const void* k_dev, int64_t k_row_stride, int32_t num_k_heads,
+                 void* out_k_dev, int64_t out_k_row_stride, const void* positions_dev,
+                 int32_t positions_are_i64, int64_t n_rows, int32_t head_dim, int32_t dtype,
+                 const VaTurns* turns, void* stream);
+
+/* va_rotary_table: rows [first_position, first_position + n_rows) of the table, fp32 [n_rows, rotary_dim] cos | sin. */
+VA_API int va_rotary_table(const VaTurns* turns, int64_t first_position, int64_t n_rows, float* table_dev,
+                    void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Eviction: what attention looked at stays, the rest of a block goes.  It has no
+ * counterpart in the reference.  Weights are fp32 [num_kv_heads, num_slots], one
+ * sum for every token slot and kv head of a pool.
+ * ------------------------------------------------------------------------- */
+
+/*
+ * va_select_tokens: of each block b, whose token slots are counts_host[b]
+ * consecutive entries of slots_dev (blocks one after the other), keep_host[b]
+ * tokens stay: the first `first` and last `last` of the block (the lower positions,
+ * where those are more than stay), then those with the largest fp32(sum over heads of
+ * weights[h][slot], taken in 64 bits), ties to the lower position.  A NaN counts as
+ * more than anything, a slot outside [0, num_slots) as 0.  Results, keep_host[b]
+ * entries a block: positions within the block in rising order, their slots, and
+ * shifts = new position - position, the new one counting what stays.
+ * workspace_dev, on a 16-byte boundary, must hold va_select_workspace_bytes (0 where no block
+ * is long; -1: a count is out of range).
+ */
+VA_API int64_t va_select_workspace_bytes(int32_t n_blocks, const int64_t* counts_host);
+VA_API int va_select_tokens(const float* weights_dev, int32_t num_heads, int64_t num_slots, const int64_t* slots_dev,
+                     int32_t n_blocks, const int64_t* counts_host, const int64_t* keep_host, int64_t first,
+                     int64_t last, int64_t* positions_dev, int64_t* out_slots_dev, int64_t* shifts_dev,
+                     void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/*
+ * va_move_kv: va_copy_shift_kv with a shift for every token.  For every layer and
+ * token i
+ *   k[dst[i]] = round(R(shifts[i]) float(k[src[i]])),  v[dst[i]] = v[src[i]],
+ * bit for bit where shifts[i] is 0 (shifts_dev NULL: everywhere), and
+ * weights[h][dst[i]] = weights[h][src[i]] where weights_dev is not NULL.  Tokens with
+ * a slot outside [0, num_slots) are skipped.  Destination slots must be distinct, and
+ * disjoint from the source slots or equal to them row by row.
+ * va_move_kv_q8: the same over a quantised pool; turned keys are quantised anew.
+ */
+VA_API int va_move_kv(void* k_pool_dev, void* v_pool_dev, int64_t pool_row_stride, int64_t layer_stride,
+               int32_t num_layers, int64_t num_slots, const int64_t* src_slots_dev, const int64_t* dst_slots_dev,
+               const int64_t* shifts_dev, int64_t n_tokens, float* weights_dev, const VaShape* shape,
+               const VaRope* rope, void* stream);
+VA_API int va_move_kv_q8(const VaQuantPool* pool, int64_t code_layer_stride, int64_t scale_layer_stride,
+                  int32_t num_layers, const int64_t* src_slots_dev, const int64_t* dst_slots_dev,
+                  const int64_t* shifts_dev, int64_t n_tokens, float* weights_dev, const VaShape* shape,
+                  const VaRope* rope, void* stream);
+
+/*
+ * va_weigh_plan / va_weigh: what every cached token was given by the attention of a step.
+ * For every token t in sight and kv head hk
+ *   weights_out[hk][slot(t)] = weights_in[hk][slot(t)] +
+ *       sum over the sub-rows i that see t and the q heads h of hk of
+ *       exp(R(sub_loc[i]) q[sub_worker[i], h] . k_t / sqrt(head_dim) - lse[sub_worker[i], h])
+ * with the tables, queries and log-sums of va_attention over the same step (a row
+ * whose log-sum is -inf counts nothing).  Rotations are taken in 32 bits and not rounded, under
+ * VA_ROPE_MROPE too; sums are 32-bit and do not depend on the order of execution.
+ * Slots that nobody sees are left as they are; weights_out may be weights_in.
+ *
+ * The plan is made on the host from the sub-request tables (kv_indices must be there; chain and
+ * sub_worker are not used); window > 0 counts only the last `window` rows of each sub-request.
+ * Entries outside num_pages pages are refused.  As with va_plan_build a buffer that is too
+ * small gives VA_ERR_CAPACITY and the size in counts.  plan_header_host is the start of the host plan (24
+ * words); workspace_dev, on a 16-byte boundary, must hold counts.workspace_bytes.  Pools and
+ * queries of any alignment; 16-byte aligned rows and a head_dim of 64, 128 or 256 run on the matrix
+ * cores, with queries as sums of two (VA_F16 pools) or three 16-bit numbers (errors of 2^-22, 2^-24), others
+ * (VA_F32, head_dim up to 256) on the vector ALU.
+ */
+typedef struct VaWeighCounts {
+  int32_t n_items;   /* work items (a workgroup per kv head) incl. padding to a multiple of 8 */
+  int32_t n_rows;    /* query rows, once for every span that they see                        */
+  int32_t n_joins;   /* chunks of tokens whose rows are split among items                    */
+  int32_t n_spans;   /* runs of pages with the same readers                                  */
+  int32_t plan_words;
+  int64_t workspace_bytes;
+} VaWeighCounts;
+
+VA_API int va_weigh_plan(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, int32_t window,
+                  int32_t* plan_host, int64_t plan_capacity_words, VaWeighCounts* counts);
+VA_API int va_weigh(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, int64_t pool_row_stride,
+             const int32_t* plan_dev, const int32_t* plan_header_host, const int64_t* sub_worker_dev,
+             const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride, const float* lse_dev, int32_t lse_base2,
+             const float* weights_in_dev, float* weights_out_dev, void* workspace_dev, int64_t workspace_bytes,
+             const VaShape* shape, const VaRope* rope, void* stream);
+VA_API int va_weigh_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
+                const int32_t* plan_header_host, const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
+                int64_t sub_loc_axis_stride, const float* lse_dev, int32_t lse_base2,
+                const float* weights_in_dev, float* weights_out_dev, void* workspace_dev,
+                int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
