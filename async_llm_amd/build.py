@@ -41,7 +41,8 @@ HOST_FLAGS = ["--offload-arch=gfx950", "--cuda-host-only"]
 SOURCE_DEVICE_FLAGS = {"va_mfma_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                        "va_mfma_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                        "va_quant_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-                       "va_quant_scattered.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+                       "va_quant_scattered.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                       "va_weigh.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _run(cmd, verbose):

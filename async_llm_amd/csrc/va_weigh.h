@@ -11,7 +11,14 @@
 #define VA_WEIGH_HEADER_WORDS 24
 #define VA_WEIGH_ITEM_WORDS 8
 #define VA_WEIGH_JOIN_WORDS 8
-#define VA_WEIGH_CHUNK 128  // tokens of an item
+#define VA_WEIGH_MOST_TOKENS 2048  // of an item
+
+// How a launch's work is laid out.
+enum {
+  VA_WEIGH_WALK = 0,   // few rows a token: bound by the keys; items are walks of many tokens (weigh_walk_kernel)
+  VA_WEIGH_TILES = 1,  // many rows a token: bound by the products; items are VA_WEIGH_TILE_TOKENS tokens and many rows (weigh_tile_kernel)
+};
+#define VA_WEIGH_TILE_TOKENS 256
 
 // header word indices
 enum {
@@ -32,6 +39,7 @@ enum {
   VA_WH_DTYPE,
   VA_WH_POOL_PAGES,
   VA_WH_N_SUBROWS,
+  VA_WH_LAYOUT,
 };
 
 // item word indices (n_tok = 0: padding)

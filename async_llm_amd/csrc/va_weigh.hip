@@ -1,31 +1,35 @@
 // Attention weights by cached token: for every token and kv head the sum, over all rows and q heads that see the token, of
 // exp(score - lse), added to the sums of former steps.
 //
-//   S^T[16 tokens, 16 rows] = K . Q^T    v_mfma_f32_16x16x32, keys as the A operand (a lane's element of the result: four tokens of
-//                                        one row)
-//   sum[token] += exp2(S - lse2[row])    no running maximum: the log-sum is known, so rows may come in any order and split
+//   S^T[16 tokens, 16 rows] = K . Q^T    matrix cores, keys as the A operand (a lane's elements of the result: four tokens of one row)
+//   sum[token] += exp2(S - lse2[row])    no running maximum: the log-sum is known, so rows may come in any order and be split
 //
-// The keys of a workgroup's tokens are loaded once and stay in registers while the rows' queries pass by; a lane's sums stay in
-// registers too, and its rows are added up across lanes at the end.  Sums are 32-bit numbers that users compare and add up over many
-// steps, so queries are not rounded to 16 bits: they come as sums of 16-bit numbers (bf16: three, which hold all 24 bits; float16:
-// two of a row brought into its range by a power of two, 22 bits) and each product is taken that often.  A first pass over the
-// packed rows (weigh_rows_kernel) turns them, scales them by log2(e) / sqrt(D) and writes those parts as the matrix cores read
-// them.  Codes of a quantised pool become bf16, scale and all, exactly.
+// Sums are 32-bit numbers that users compare and add up over many steps, so queries are not rounded to 16 bits: they come as sums
+// of 16-bit numbers (bf16: three, which hold all 24 bits; float16: two of a row brought into its range by a power of two, 22
+// bits) and each product is taken that often.  A first pass over the packed rows (weigh_rows_kernel) turns them, scales them by
+// log2(e) / sqrt(D) and writes those parts as the matrix cores read them.
 //
+// Two layouts of the work (va_weigh.h):
+//   * walks (weigh_walk_kernel): a token has few rows, as in decode steps.  Bound by the keys: they travel to LDS in whole lines,
+//     each wave's tiles in a ring of its own, while its tile before is at the products.
+//   * tiles (weigh_tile_kernel): a token has many rows, as for many new tokens.  Bound by the products: 64 tokens' keys stay in a
+//     wave's registers while the rows' queries pass by through LDS, for all four waves at once.
 // Where a chunk's rows are split among workgroups each writes partial sums, and weigh_join_kernel adds them in their order.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "va_device.h"
 #include "va_internal.h"
 #include "va_launch.h"
 #include "va_mfma_common.h"
 #include "va_quant.h"
+#include "va_quant_mfma.h"
 #include "va_weigh.h"
 
 namespace va {
 
 constexpr int kWeighThreads = 256, kWeighWaves = kWeighThreads / kWave;
-constexpr int kWeighGroups = VA_WEIGH_CHUNK / (16 * kWeighWaves);  // groups of 16 tokens of a wave
 constexpr int kWeighMaxDim = 256;
 
 // What a (row, q head) brings besides its query: p = exp2(dot * scale + minus_lse), tokens [lo, hi) of the span.
@@ -60,6 +64,7 @@ struct WeighArgs {
   float* partials;  // [kv head][n_partials]
   long long n_partials;
   int num_q_heads, num_kv_heads, head_dim, dtype;
+  int pieces;  // queries start on 16-byte boundaries
   PageMap page_map;
   RopeDev rope;
   float scale_log2;
@@ -81,107 +86,219 @@ __device__ __forceinline__ uint32_t weigh_slot(const WeighArgs& a, int page_begi
 // ---------------------------------------------------------------------------
 // queries
 // ---------------------------------------------------------------------------
-enum { kRows32 = 0, kRowsF16 = 2, kRowsBF16 = 3 };  // 32-bit rows, or how many 16-bit parts
+// What a row's query becomes.  Parts lie as [tile][part][step][lane] of 16 bytes, lane 16 * group + j for row j, so that a wave reads
+// its operands of a step in one run; pieces of 8 (32-bit: 4) dims go to steps and contraction groups in the order in which lanes
+// hold the keys: piece 4 step + group, or over codes, of which a lane reads 16 at once, 8 (step / 2) + 2 group + step % 2.
+enum RowKind { kPlain32, kParts32, kPartsF16, kPartsBF16, kCodesF16, kCodesBF16 };
+__host__ __device__ constexpr int parts_of(int kind) { return kind == kPartsF16 || kind == kCodesF16 ? 2 : kind == kPartsBF16 || kind == kCodesBF16 ? 3 : 1; }
+__host__ __device__ constexpr int tile_bytes_of(int kind, int dim) { return 16 * dim * (kind <= kParts32 ? 4 : 2 * parts_of(kind)); }
 
-// 16-bit parts: element d of row j belongs to step 2 (d / 64) + (d / 8) % 2, contraction group (d / 16) % 4, so that a lane's
-// pieces of two steps are neighbours in the row: [tile][part][step][lane] of 16 bytes, lane 16 * group + j.
-template <int kParts>
+// Eight neighbouring elements of a row, piece `piece` of row j (32-bit: pieces 2 piece and 2 piece + 1); y is used up.
+template <int kKind>
+__device__ __forceinline__ void write_row_piece(char* tile_at, int dim, int j, int piece, float* y) {
+  if constexpr (kKind == kPlain32) {
+    float* to = (float*)tile_at + j * dim + 8 * piece;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) to[e] = y[e];
+  } else if constexpr (kKind == kParts32) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = 2 * piece + i;
+      *(va_f32x4*)(tile_at + (p / 4) * 1024 + (16 * (p % 4) + j) * 16) = va_f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
+    }
+  } else {
+    constexpr bool kHalf = kKind == kPartsF16 || kKind == kCodesF16;
+    const bool codes = kKind == kCodesF16 || kKind == kCodesBF16;
+    const int step = codes ? 2 * (piece / 8) + piece % 2 : piece / 4, group = codes ? piece % 8 / 2 : piece % 4;
+#pragma unroll
+    for (int part = 0; part < parts_of(kKind); ++part) {
+      va_u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (kHalf) {
+          w[e] = Mma<F16>::pack(y[2 * e], y[2 * e + 1]);
+          y[2 * e] -= F16::load(__builtin_bit_cast(__half, (uint16_t)w[e])), y[2 * e + 1] -= F16::load(__builtin_bit_cast(__half, (uint16_t)(w[e] >> 16)));
+        } else {
+          w[e] = Mma<BF16>::pack(y[2 * e], y[2 * e + 1]);
+          y[2 * e] -= __uint_as_float(w[e] << 16), y[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+        }
+      }
+      *(va_u32x4*)(tile_at + (part * (dim / 32) + step) * 1024 + (16 * group + j) * 16) = w;
+    }
+  }
+}
+
+// The power of two that brings a row whose largest element is `most` to 2^10 .. 2^11, as its exponent.
+__device__ __forceinline__ int row_exponent(float most) {
+  return most > 0.f && most < INFINITY ? min(max(10 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100) : 0;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// The row's other half: a row that is padding, or whose log-sum is -inf, adds exp2(-inf) = 0 to every token.
+__device__ __forceinline__ WeighRow row_beside(const WeighArgs& a, int row, bool counts, float lse, float scale) {
+  if (!counts) return WeighRow{-INFINITY, 0.f, 0, 0x7fffffff};
+  return WeighRow{a.lse_base2 ? -lse : -lse * kLog2e, scale, a.lo[row], a.hi[row]};
+}
+
+__device__ __forceinline__ void weigh_activations8(const void* x, long long at, int dtype, int pieces, float* y) {
+  if (pieces && dtype == VA_F32) {
+    const float4 u = *(const float4*)((const float*)x + at), v = *(const float4*)((const float*)x + at + 4);
+    y[0] = u.x, y[1] = u.y, y[2] = u.z, y[3] = u.w, y[4] = v.x, y[5] = v.y, y[6] = v.z, y[7] = v.w;
+  } else if (pieces) {
+    const va_u32x4 w = *(const va_u32x4*)((const uint16_t*)x + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t u = (uint16_t)w[i], v = (uint16_t)(w[i] >> 16);
+      y[2 * i] = dtype == VA_BF16 ? BF16::load(u) : __half2float(__builtin_bit_cast(__half, u));
+      y[2 * i + 1] = dtype == VA_BF16 ? BF16::load(v) : __half2float(__builtin_bit_cast(__half, v));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = weigh_activation(x, at + e, dtype);
+  }
+}
+
+// A thread per 16 elements of a row: both halves of eight pairs, or two pieces past the rotary part.  head_dim 64, 128 or 256 and
+// rotary_dim a multiple of 16.
+template <int kKind>
 __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighArgs a) {
+  const int D = a.head_dim, units = D / 16, G = a.num_q_heads / a.num_kv_heads, hk = blockIdx.y;
+  const int task = blockIdx.x * kWeighThreads + threadIdx.x, pair = task / units, x = task - pair * units;
+  if (pair >= a.n_tiles * 16) return;  // (whole rows leave)
+  const int row = pair / G, hq = hk * G + pair - row * G, sub = a.sub_rows[row];
+  float y[2][8], scale = 1.f, lse = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[0][e] = y[1][e] = 0.f;
+  const int pairs = a.rope.half / 8, d0 = x < pairs ? 8 * x : 16 * x, d1 = x < pairs ? 8 * x + a.rope.half : 16 * x + 8;
+  if (sub >= 0) {
+    const long long worker = a.sub_worker[sub], at = worker * a.q_row_stride + (long long)hq * D;
+    lse = a.lse[worker * a.num_q_heads + hq];
+    weigh_activations8(a.q, at + d0, a.dtype, a.pieces, y[0]);
+    weigh_activations8(a.q, at + d1, a.dtype, a.pieces, y[1]);
+    if (x < pairs) {
+      float c[8], s[8];
+      turns8(a.rope, load_pos(a.sub_loc, a.sub_loc_axis_stride, sub), d0, c, s);
+      turn8(c, s, y[0], y[1]);
+    }
+  }
+  const bool counts = sub >= 0 && lse != -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[0][e] = counts ? y[0][e] * a.scale_log2 : 0.f, y[1][e] = counts ? y[1][e] * a.scale_log2 : 0.f;
+  if constexpr (kKind == kPartsF16 || kKind == kCodesF16) {
+    float most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fmaxf(fabsf(y[0][e]), fabsf(y[1][e])));
+    for (int off = 1; off < units; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, kWave));
+    const int e = row_exponent(most);
+    scale = power_of_two(-e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[0][i] *= power_of_two(e), y[1][i] *= power_of_two(e);
+  }
+  char* at = a.queries + ((long long)hk * a.n_tiles + pair / 16) * tile_bytes_of(kKind, D);
+  write_row_piece<kKind>(at, D, pair % 16, d0 / 8, y[0]);
+  write_row_piece<kKind>(at, D, pair % 16, d1 / 8, y[1]);
+  if (x == 0) a.rows[(long long)hk * a.n_tiles * 16 + pair] = row_beside(a, row, counts, lse, scale);
+}
+
+// Any head_dim up to kWeighMaxDim and any rotary_dim: a tile a workgroup, through LDS.
+template <int kKind>
+__global__ __launch_bounds__(kWeighThreads) void weigh_rows_any_kernel(WeighArgs a) {
   __shared__ float x[16][kWeighMaxDim + 1];
   const int tile = blockIdx.x, hk = blockIdx.y, D = a.head_dim, G = a.num_q_heads / a.num_kv_heads;
   const int j = threadIdx.x / 16, c = threadIdx.x % 16;
   const int pair = tile * 16 + j, row = pair / G, hq = hk * G + pair - row * G;
   const int sub = a.sub_rows[row];
   const long long worker = sub < 0 ? 0 : a.sub_worker[sub];
-  if (sub >= 0) {
+  const float lse = sub < 0 ? -INFINITY : a.lse[worker * a.num_q_heads + hq];
+  const bool counts = lse != -INFINITY;
+  float most = 0.f;
+  auto put = [&](int d, float v) __attribute__((always_inline)) {
+    x[j][d] = v;
+    most = fmaxf(most, fabsf(v));
+  };
+  if (counts) {
     const Pos3 pos = load_pos(a.sub_loc, a.sub_loc_axis_stride, sub);
     const long long at = worker * a.q_row_stride + (long long)hq * D;
     for (int i = c; i < a.rope.half; i += 16) {
       float cs, sn;
       rope_cos_sin(a.rope, pos, i, cs, sn);
       const float x1 = weigh_activation(a.q, at + i, a.dtype), x2 = weigh_activation(a.q, at + i + a.rope.half, a.dtype);
-      x[j][i] = (mul_rounded(cs, x1) - mul_rounded(sn, x2)) * a.scale_log2;
-      x[j][i + a.rope.half] = (mul_rounded(cs, x2) + mul_rounded(sn, x1)) * a.scale_log2;
+      put(i, (mul_rounded(cs, x1) - mul_rounded(sn, x2)) * a.scale_log2);
+      put(i + a.rope.half, (mul_rounded(cs, x2) + mul_rounded(sn, x1)) * a.scale_log2);
     }
-    for (int d = 2 * a.rope.half + c; d < D; d += 16) x[j][d] = weigh_activation(a.q, at + d, a.dtype) * a.scale_log2;
+    for (int d = 2 * a.rope.half + c; d < D; d += 16) put(d, weigh_activation(a.q, at + d, a.dtype) * a.scale_log2);
   } else {
     for (int d = c; d < D; d += 16) x[j][d] = 0.f;
   }
   __syncthreads();
   float scale = 1.f, up = 1.f;
-  if constexpr (kParts == kRowsF16) {  // the largest element to 2^10 .. 2^11
-    float most = 0.f;
-    for (int d = c; d < D; d += 16) most = fmaxf(most, fabsf(x[j][d]));
+  if constexpr (kKind == kPartsF16 || kKind == kCodesF16) {
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, kWave));
-    const int e = most > 0.f && most < INFINITY ? min(max(10 - ((int)(__float_as_uint(most) >> 23) - 127), -100), 100) : 0;
-    up = __uint_as_float((uint32_t)(127 + e) << 23), scale = __uint_as_float((uint32_t)(127 - e) << 23);
+    const int e = row_exponent(most);
+    up = power_of_two(e), scale = power_of_two(-e);
   }
-  if constexpr (kParts == kRows32) {
-    float* to = (float*)a.queries + ((long long)hk * a.n_tiles * 16 + pair) * D;
-    for (int d = c; d < D; d += 16) to[d] = x[j][d];
+  char* at = a.queries + ((long long)hk * a.n_tiles + tile) * tile_bytes_of(kKind, D);
+  if constexpr (kKind == kPlain32) {
+    for (int d = c; d < D; d += 16) ((float*)at)[j * D + d] = x[j][d];
   } else {
     for (int piece = c; piece < D / 8; piece += 16) {
-      const int step = 2 * (piece / 8) + piece % 2, group = piece % 8 / 2;
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = x[j][8 * piece + e] * up;
-#pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        va_u32x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (kParts == kRowsF16) {
-            w[e] = Mma<F16>::pack(y[2 * e], y[2 * e + 1]);
-            y[2 * e] -= F16::load(__builtin_bit_cast(__half, (uint16_t)w[e])), y[2 * e + 1] -= F16::load(__builtin_bit_cast(__half, (uint16_t)(w[e] >> 16)));
-          } else {
-            w[e] = Mma<BF16>::pack(y[2 * e], y[2 * e + 1]);
-            y[2 * e] -= __uint_as_float(w[e] << 16), y[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
-          }
-        }
-        *(va_u32x4*)(a.queries + ((((long long)hk * a.n_tiles + tile) * kParts + part) * (D / 32) + step) * 1024 + (16 * group + j) * 16) = w;
-      }
+      write_row_piece<kKind>(at, D, j, piece, y);
     }
   }
-  if (c == 0) {
-    WeighRow r{0.f, scale, 0, 0};
-    if (sub >= 0) {
-      const float lse = a.lse[worker * a.num_q_heads + hq];
-      r.minus_lse = a.lse_base2 ? -lse : -lse * kLog2e;
-      if (lse != -INFINITY) r.lo = a.lo[row], r.hi = a.hi[row];
-    }
-    a.rows[(long long)hk * a.n_tiles * 16 + pair] = r;
-  }
+  if (c == 0) a.rows[(long long)hk * a.n_tiles * 16 + pair] = row_beside(a, row, counts, lse, scale);
 }
 
 // ---------------------------------------------------------------------------
 // matrix cores
 // ---------------------------------------------------------------------------
-// Pool element types: what their keys are in the products.
+// Sum over the 16 lanes of a row.
+__device__ __forceinline__ float row_sum(float x) {
+#define VA_DPP_ADD(ctrl) x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), ctrl, 0xf, 0xf, false))
+  VA_DPP_ADD(0xb1);   // quad_perm 1 0 3 2
+  VA_DPP_ADD(0x4e);   // quad_perm 2 3 0 1
+  VA_DPP_ADD(0x141);  // row_half_mirror
+  VA_DPP_ADD(0x140);  // row_mirror
+#undef VA_DPP_ADD
+  return x;
+}
+
+// What the keys of a pool are in the products of the walks: 16-byte pieces of the parts' type.
 template <typename E>
-struct WeighKeys {
-  using M = E;
+struct WalkKeys {  // bf16
+  static constexpr int kBytes = 2, kRows = kPartsBF16;
   static constexpr bool kCodes = false;
-  static constexpr int kParts = kRowsBF16;
+  static __device__ __forceinline__ va_f32x4 run(va_u32x4 k, va_u32x4 q, va_f32x4 c) { return Mma<BF16>::run(k, q, c); }
 };
 template <>
-struct WeighKeys<F16> {
-  using M = F16;
+struct WalkKeys<F16> {
+  static constexpr int kBytes = 2, kRows = kPartsF16;
   static constexpr bool kCodes = false;
-  static constexpr int kParts = kRowsF16;
+  static __device__ __forceinline__ va_f32x4 run(va_u32x4 k, va_u32x4 q, va_f32x4 c) { return Mma<F16>::run(k, q, c); }
 };
 template <>
-struct WeighKeys<E4M3> {
-  using M = BF16;
+struct WalkKeys<F32> {
+  static constexpr int kBytes = 4, kRows = kParts32;
+  static constexpr bool kCodes = false;
+  static __device__ __forceinline__ va_f32x4 run(va_u32x4 k, va_u32x4 q, va_f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]), __uint_as_float(q[e]), c, 0, 0, 0);
+    return c;
+  }
+};
+template <>
+struct WalkKeys<E4M3> : WalkKeys<BF16> {
+  static constexpr int kBytes = 1, kRows = kCodesBF16;
   static constexpr bool kCodes = true;
-  static constexpr int kParts = kRowsBF16;
   static __device__ __forceinline__ va_u32x4 keys(va_u32x2 codes, float scale) { return E4M3::bf16x8(codes, scale); }
 };
 template <>
-struct WeighKeys<INT8> {
-  using M = BF16;
+struct WalkKeys<INT8> : WalkKeys<BF16> {
+  static constexpr int kBytes = 1, kRows = kCodesBF16;
   static constexpr bool kCodes = true;
-  static constexpr int kParts = kRowsBF16;
   static __device__ __forceinline__ va_u32x4 keys(va_u32x2 codes, float scale) {  // (bf16 has the eight bits of a code)
     float x[8];
     INT8::unpack4(codes[0], x), INT8::unpack4(codes[1], x + 4);
@@ -192,90 +309,434 @@ struct WeighKeys<INT8> {
 };
 
 template <int kD, typename C>
-__global__ __launch_bounds__(kWeighThreads) void weigh_mfma_kernel(WeighArgs a) {
-  using K = WeighKeys<C>;
-  using M = Mma<typename K::M>;
-  constexpr int kParts = K::kParts, kSteps = kD / 32;
+struct WalkShape {
+  using K = WalkKeys<C>;
+  static constexpr int kRowBytes = kD * K::kBytes;
+  static constexpr int kPieces = kRowBytes / 16;           // of a token's row
+  static constexpr int kRaw = kPieces / 4;                 // pieces of a row that a lane takes
+  static constexpr int kSteps = K::kCodes ? 2 * kRaw : kRaw;  // operand pieces of a lane, per part
+  static constexpr int kParts = parts_of(K::kRows);
+  // groups of 16 tokens of a wave's tile: 16 KB of 16- and 32-bit rows (up to 64 tokens), as many tokens of codes
+  static constexpr int kGroups = 1024 / (K::kCodes ? 2 * kD : kRowBytes) < 1 ? 1 : 1024 / (K::kCodes ? 2 * kD : kRowBytes) > 4 ? 4 : 1024 / (K::kCodes ? 2 * kD : kRowBytes);
+  static constexpr int kTokens = 16 * kGroups;
+  static constexpr int kGroupBytes = 16 * kRowBytes;
+  static constexpr int kLoads = kGroupBytes / 1024;        // wave-level loads of a group
+  static constexpr int kTileBytes = kGroups * kGroupBytes + (K::kCodes ? 256 : 0);  // with a word for every scale
+  static constexpr int kBuffers = kTileBytes > 8 * 1024 + 256 ? 1 : 2;
+  static constexpr int kTileLoads = kGroups * kLoads + (K::kCodes ? 1 : 0);  // what the counter of outstanding loads sees of a tile
+  static constexpr int kSumsOffset = kWeighWaves * kBuffers * kTileBytes;
+  static constexpr int kLdsBytes = kSumsOffset + VA_WEIGH_MOST_TOKENS * 4;
+  static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups share the LDS of a CU");
+  static_assert((kBuffers - 1) * kTileLoads < kAnyInFlight, "the counter of outstanding loads");
+};
+// Piece c of row r of a group lies at position c ^ walk_swz(r): the fragments of sixteen rows then lie in different banks.
+template <int kPieces>
+__device__ __forceinline__ int walk_swz(int r) {
+  if constexpr (kPieces >= 16) return ((r & 7) << 1) | ((r >> 3) & 1);
+  if constexpr (kPieces == 8) return (r & 6) | ((r >> 3) & 1);
+  return (r >> 2) & 3;
+}
+
+// A workgroup's sums to where they go.
+__device__ __forceinline__ void finish_sums(const WeighArgs& a, int page_begin, int first, int n_tok, int partial, int hk, const float* sums) {
+  for (int t = threadIdx.x; t < n_tok; t += kWeighThreads) {
+    if (partial >= 0) {
+      a.partials[hk * a.n_partials + partial + t] = sums[t];
+    } else {
+      const long long to = hk * a.num_slots + weigh_slot(a, page_begin, first + t);
+      a.weights_out[to] = a.weights_in[to] + sums[t];
+    }
+  }
+}
+
+template <int kD, typename C>
+__global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs a) {
+  using Sh = WalkShape<kD, C>;
+  using K = WalkKeys<C>;
+  using Words = const __attribute__((address_space(4))) int32_t*;
+  constexpr int kGroups = Sh::kGroups, kLoads = Sh::kLoads, kPieces = Sh::kPieces, kSteps = Sh::kSteps, kRaw = Sh::kRaw, kParts = Sh::kParts;
+  constexpr int kTokens = Sh::kTokens, kBuffers = Sh::kBuffers;
+  extern __shared__ va_u32x4 smem[];
+  char* lds = (char*)smem;
   const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
-  const int32_t* item = a.items + (long long)where.item * VA_WEIGH_ITEM_WORDS;
+  const Words item = (Words)a.items + (long long)where.item * VA_WEIGH_ITEM_WORDS;
   const int n_tok = item[VA_WI_N_TOK], hk = where.head;
   if (n_tok == 0) return;
-  const int page_begin = item[VA_WI_PAGES], first = item[VA_WI_FIRST], tile_end = item[VA_WI_TILE_END], partial = item[VA_WI_PARTIAL];
+  const int page_begin = item[VA_WI_PAGES], first = item[VA_WI_FIRST], partial = item[VA_WI_PARTIAL];
+  const int tile_begin = item[VA_WI_TILE_BEGIN], tile_end = item[VA_WI_TILE_END];
   const int lane = threadIdx.x % kWave, j = lane % 16, kg = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int w0 = 16 * kWeighGroups * wave;  // first token of the wave, in the chunk
-  if (w0 >= n_tok) return;
+  const int last = n_tok - 1, n_tiles = (n_tok + kTokens - 1) / kTokens;
+  const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_address(lds)) + (uint32_t)(wave * kBuffers * Sh::kTileBytes);
+  float* sums = (float*)(lds + Sh::kSumsOffset);
+  // (16 tokens of a group lie in one page; their rows within 32-bit offsets)
+  const bool whole = a.page_map.shift >= 4 && first % 16 == 0;
+  const long long row_bytes = K::kCodes ? kD : a.pool_row_stride * K::kBytes;
 
-  va_u32x4 keys[kWeighGroups][kSteps];
+  // This lane's part of load u of a group: row and piece, which belongs at its LDS position.  Loads in groups of up to four share one
+  // setting of M0, whose immediate offsets move the pool address as well (grouped_lane_offset; the base gives the bias back).
+  constexpr int kBias = 1024 * (kLoads - 1);
+  auto ld_row = [&](int u) __attribute__((always_inline)) { return u * (kWave / kPieces) + lane / kPieces; };
+  auto ld_piece = [&](int u) __attribute__((always_inline)) { return (lane % kPieces) ^ walk_swz<kPieces>(ld_row(u)); };
+  uint32_t ld_off[kLoads];
 #pragma unroll
-  for (int g = 0; g < kWeighGroups; ++g) {
-    const uint32_t slot = weigh_slot(a, page_begin, first + min(w0 + 16 * g + j, n_tok - 1));
-    if constexpr (K::kCodes) {
-      const long long row = quant_row(a.page_map, slot, hk, a.num_kv_heads);
-      const float scale = scale_value(a.k_scales[row]);
-      va_u32x4 raw[kSteps / 2];
+  for (int u = 0; u < kLoads; ++u) ld_off[u] = grouped_lane_offset((uint32_t)(ld_row(u) * row_bytes + 16 * ld_piece(u) + kBias), u);
+  auto row_at = [&](uint32_t slot) __attribute__((always_inline)) {  // byte of a slot's row of this head
+    if constexpr (K::kCodes) return quant_row(a.page_map, slot, hk, a.num_kv_heads) * kD;
+    return (long long)slot * row_bytes + hk * (long long)Sh::kRowBytes;
+  };
+  auto request = [&](int n) __attribute__((always_inline)) {  // this wave's tile n
+    const uint32_t dst = ring + (uint32_t)(n % kBuffers) * Sh::kTileBytes;
+    const int t0 = (n * kWeighWaves + wave) * kTokens;
+    if (whole) {
+      long long of_lane = 0;  // of the token whose scale this lane brings
 #pragma unroll
-      for (int s = 0; s < kSteps / 2; ++s) raw[s] = *(const va_u32x4*)((const uint8_t*)a.k_pool + row * kD + 64 * s + 16 * kg);
+      for (int g = 0; g < kGroups; ++g) {
+        const int t = min(t0 + 16 * g, last / 16 * 16);  // (a group past the end: the last one)
+        const uint32_t at = (uint32_t)(first + t);
+        const uint32_t slot = ((uint32_t)((Words)a.pages)[page_begin + (int)(at >> a.page_map.shift)] << a.page_map.shift) + (at & (a.page_map.size - 1));
+        const long long base = row_at(slot);
+        const char* from = (const char*)a.k_pool + (base - kBias);
+        const int most = last - t;  // rows behind the last one repeat it
+        if (most >= 15) {
+          if constexpr (kLoads >= 4) {
 #pragma unroll
-      for (int s = 0; s < kSteps / 2; ++s) {
-        keys[g][2 * s] = K::keys(va_u32x2{raw[s][0], raw[s][1]}, scale);
-        keys[g][2 * s + 1] = K::keys(va_u32x2{raw[s][2], raw[s][3]}, scale);
+            for (int u = 0; u < kLoads; u += 4) load_group_to_lds<4, true>(from, ld_off + u, dst + g * Sh::kGroupBytes + 1024 * u);
+          } else if constexpr (kLoads == 2) {
+            load_group_to_lds<2, true>(from, ld_off, dst + g * Sh::kGroupBytes);
+          } else {
+            load_to_lds(from, ld_off[0], dst + g * Sh::kGroupBytes);
+          }
+        } else {
+          uint32_t off[kLoads];
+#pragma unroll
+          for (int u = 0; u < kLoads; ++u) off[u] = ld_off[u] - (uint32_t)(max(0, ld_row(u) - most) * row_bytes);
+          if constexpr (kLoads >= 4) {
+#pragma unroll
+            for (int u = 0; u < kLoads; u += 4) load_group_to_lds<4, true>(from, off + u, dst + g * Sh::kGroupBytes + 1024 * u);
+          } else if constexpr (kLoads == 2) {
+            load_group_to_lds<2, true>(from, off, dst + g * Sh::kGroupBytes);
+          } else {
+            load_to_lds(from, off[0], dst + g * Sh::kGroupBytes);
+          }
+        }
+        if constexpr (K::kCodes) of_lane = kg == g ? base / kD + min(j, most) : of_lane;
       }
-    } else {
-      const uint16_t* row = (const uint16_t*)a.k_pool + (long long)slot * a.pool_row_stride + (long long)hk * kD;
+      if constexpr (K::kCodes) load_bytes_to_lds((unsigned long long)a.k_scales + of_lane, dst + kGroups * Sh::kGroupBytes);
+    } else {  // tokens looked up one by one: each lane one, handed to those that load it
+      const uint32_t mine = weigh_slot(a, page_begin, first + min(t0 + lane % kTokens, last));
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) keys[g][s] = *(const va_u32x4*)(row + 64 * (s / 2) + 16 * kg + 8 * (s % 2));
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+          const uint32_t slot = (uint32_t)__shfl((int)mine, 16 * g + ld_row(u), kWave);
+          load_to_lds((const char*)a.k_pool + row_at(slot) + 16 * ld_piece(u), dst + g * Sh::kGroupBytes + 1024 * u);
+        }
+      if constexpr (K::kCodes) load_bytes_to_lds((unsigned long long)a.k_scales + row_at(mine) / kD, dst + kGroups * Sh::kGroupBytes);
     }
-  }
+  };
 
-  const int t_wave = first + w0, t_end = min(t_wave + 16 * kWeighGroups, first + n_tok);
-  float sum[kWeighGroups][4];
+  va_u32x4 q[kParts][kSteps];
+  WeighRow row;
+  const char* queries = a.queries + (long long)hk * a.n_tiles * tile_bytes_of(K::kRows, kD) + 16 * lane;
+  auto load_queries = [&](int tile) __attribute__((always_inline)) {
+    row = a.rows[((long long)hk * a.n_tiles + tile) * 16 + j];
+    const char* at = queries + (long long)tile * tile_bytes_of(K::kRows, kD);
 #pragma unroll
-  for (int g = 0; g < kWeighGroups; ++g)
+    for (int p = 0; p < kParts; ++p)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) q[p][s] = *(const va_u32x4*)(at + (p * kSteps + s) * 1024);
+  };
+  const int mine = n_tiles > wave ? (n_tiles - wave + kWeighWaves - 1) / kWeighWaves : 0;  // this wave's tiles
+
+  // kSingle: one tile of rows, whose queries stay in registers; the next tile of keys is on its way before the products of the last.
+  // Otherwise queries are loaded tile by tile, and a wait for those would be one for the keys as well, which are asked for later.
+  auto walk = [&](auto single) __attribute__((always_inline)) {
+    constexpr bool kSingle = decltype(single)::value;
+#pragma unroll
+    for (int b = 0; b < kBuffers; ++b)
+      if (b < mine) request(b);
+    if constexpr (kSingle) {
+      load_queries(tile_begin);
+#pragma unroll
+      for (int p = 0; p < kParts; ++p)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q[p][s]));  // (waited for here, not in the loop)
+      asm volatile("" : "+v"(row.minus_lse), "+v"(row.scale), "+v"(row.lo), "+v"(row.hi));
+    }
+    for (int n = 0; n < mine; ++n) {
+      if (n + kBuffers - 1 < mine) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBuffers - 1) * Sh::kTileLoads) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      const char* tile = lds + (wave * kBuffers + n % kBuffers) * Sh::kTileBytes;
+      va_u32x4 keys[kGroups][kRaw];
+      float scale[kGroups];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+        for (int s = 0; s < kRaw; ++s)
+          keys[g][s] = *(const va_u32x4*)(tile + g * Sh::kGroupBytes + j * Sh::kRowBytes + 16 * ((4 * s + kg) ^ walk_swz<kPieces>(j)));
+        if constexpr (K::kCodes) scale[g] = scale_value(*(const uint32_t*)(tile + kGroups * Sh::kGroupBytes + 4 * (16 * g + j)));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (kSingle && n + kBuffers < mine) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        request(n + kBuffers);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+
+      const int t_tile = first + (n * kWeighWaves + wave) * kTokens, t_end = min(t_tile + kTokens, first + n_tok);
+      float sum[kGroups][4];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[g][r] = 0.f;
+      for (int of = tile_begin; of < (kSingle ? tile_begin + 1 : tile_end); ++of) {
+        if constexpr (!kSingle) load_queries(of);
+        va_f32x4 dots[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) dots[g] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            va_u32x4 k;
+            if constexpr (K::kCodes) {
+              const va_u32x4 raw = keys[g][s / 2];
+              k = K::keys(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]}, scale[g]);
+            } else {
+              k = keys[g][s];
+            }
+#pragma unroll
+            for (int p = kParts - 1; p >= 0; --p) dots[g] = K::run(k, q[p][s], dots[g]);
+          }
+        if (__any(row.lo > t_tile || row.hi < t_end)) {  // some row does not see some token
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int t = t_tile + 16 * g + 4 * kg + r;
+              const float p = __builtin_amdgcn_exp2f(fmaf(dots[g][r], row.scale, row.minus_lse));
+              sum[g][r] += t >= row.lo && t < row.hi ? p : 0.f;
+            }
+        } else {
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[g][r] += __builtin_amdgcn_exp2f(fmaf(dots[g][r], row.scale, row.minus_lse));
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[g][r] = row_sum(sum[g][r]);
+        // lane j < 4 has token 4 kg + j
+        const float of_token = j == 0 ? sum[g][0] : j == 1 ? sum[g][1] : j == 2 ? sum[g][2] : sum[g][3];
+        if (j < 4) sums[(n * kWeighWaves + wave) * kTokens + 16 * g + 4 * kg + j] = of_token;
+      }
+      if (!kSingle && n + kBuffers < mine) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        request(n + kBuffers);
+      }
+    }
+  };
+  if (tile_end - tile_begin == 1) walk(std::true_type{}); else walk(std::false_type{});
+  __syncthreads();
+  finish_sums(a, page_begin, first, n_tok, partial, hk, sums);
+}
+
+// What the keys of a pool are in the products of the tiles: float16, and a factor of each token on its scores.  16-bit keys come
+// within float16's range by a power of two of their own, which leaves every element that is over 2^-32 of the row's largest
+// exact; codes are float16 numbers as they are.  Two parts of a query instead of bf16's three: a third of the products less.
+template <int kD, typename C>
+struct TileKeys;
+template <int kD>
+struct TileKeys<kD, F16> {
+  static constexpr int kRows = kPartsF16;
+  static constexpr bool kFactor = false;
+  static __device__ __forceinline__ float load(const WeighArgs& a, uint32_t slot, int hk, int kg, va_u32x4 (&keys)[kD / 32]) {
+    const uint16_t* row = (const uint16_t*)a.k_pool + (long long)slot * a.pool_row_stride + (long long)hk * kD;
+#pragma unroll
+    for (int s = 0; s < kD / 32; ++s) keys[s] = *(const va_u32x4*)(row + 32 * s + 8 * kg);
+    return 1.f;
+  }
+};
+template <int kD>
+struct TileKeys<kD, BF16> {
+  static constexpr int kRows = kPartsF16;
+  static constexpr bool kFactor = true;
+  static __device__ __forceinline__ float load(const WeighArgs& a, uint32_t slot, int hk, int kg, va_u32x4 (&keys)[kD / 32]) {
+    TileKeys<kD, F16>::load(a, slot, hk, kg, keys);
+    uint32_t most = 0;  // magnitudes as whole numbers, which order them
+#pragma unroll
+    for (int s = 0; s < kD / 32; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = max(most, max(keys[s][e] & 0x7fffu, keys[s][e] >> 16 & 0x7fffu));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+    const int e = most == 0 || most >= 0x7f80u ? 0 : min(14 + 127 - (int)(most >> 7), 126);  // the largest to 2^14 .. 2^15
+    const float up = power_of_two(e);
+#pragma unroll
+    for (int s = 0; s < kD / 32; ++s)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        keys[s][w] = Mma<F16>::pack(__uint_as_float(keys[s][w] << 16) * up, __uint_as_float(keys[s][w] & 0xffff0000u) * up);
+    return power_of_two(-e);
+  }
+};
+template <int kD>
+struct TileKeys<kD, E4M3> {
+  static constexpr int kRows = kCodesF16;
+  static constexpr bool kFactor = true;
+  static __device__ __forceinline__ float load(const WeighArgs& a, uint32_t slot, int hk, int kg, va_u32x4 (&keys)[kD / 32]) {
+    const long long row = quant_row(a.page_map, slot, hk, a.num_kv_heads);
+#pragma unroll
+    for (int s = 0; s < kD / 64; ++s) {
+      const va_u32x4 raw = *(const va_u32x4*)((const uint8_t*)a.k_pool + row * kD + 64 * s + 16 * kg);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        keys[2 * s + w / 2][2 * (w % 2)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[w], 1.f, false));
+        keys[2 * s + w / 2][2 * (w % 2) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[w], 1.f, true));
+      }
+    }
+    return scale_value(a.k_scales[row]);
+  }
+};
+template <int kD>
+struct TileKeys<kD, INT8> {
+  static constexpr int kRows = kCodesF16;
+  static constexpr bool kFactor = true;
+  static __device__ __forceinline__ float load(const WeighArgs& a, uint32_t slot, int hk, int kg, va_u32x4 (&keys)[kD / 32]) {
+    const long long row = quant_row(a.page_map, slot, hk, a.num_kv_heads);
+#pragma unroll
+    for (int s = 0; s < kD / 64; ++s) {
+      const va_u32x4 raw = *(const va_u32x4*)((const uint8_t*)a.k_pool + row * kD + 64 * s + 16 * kg);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float x[4];
+        INT8::unpack4(raw[w], x);
+        keys[2 * s + w / 2][2 * (w % 2)] = Mma<F16>::pack(x[0], x[1]);
+        keys[2 * s + w / 2][2 * (w % 2) + 1] = Mma<F16>::pack(x[2], x[3]);
+      }
+    }
+    return scale_value(a.k_scales[row]);
+  }
+};
+
+template <int kD>
+struct TileShape {
+  static constexpr int kSteps = kD / 32, kParts = 2;
+  static constexpr int kGroups = VA_WEIGH_TILE_TOKENS / (16 * kWeighWaves);  // of 16 tokens, a wave
+  static constexpr int kQueryBytes = 16 * kD * 2 * kParts;
+  static constexpr int kBufferBytes = kQueryBytes + kWeighWaves * 256;  // with the rows' other halves, a copy a wave
+  static constexpr int kBuffers = 3;
+  static constexpr int kLoads = kQueryBytes / 1024 / kWeighWaves + 1;  // a wave's of a tile of rows
+  static constexpr int kLdsBytes = kBuffers * kBufferBytes;
+  static_assert(kQueryBytes % (1024 * kWeighWaves) == 0, "whole loads");
+  static_assert(kLdsBytes >= VA_WEIGH_TILE_TOKENS * 4, "room for the sums");
+};
+
+template <int kD, typename C>
+__global__ __launch_bounds__(kWeighThreads, 2) void weigh_tile_kernel(WeighArgs a) {
+  using Sh = TileShape<kD>;
+  using K = TileKeys<kD, C>;
+  using Words = const __attribute__((address_space(4))) int32_t*;
+  constexpr int kGroups = Sh::kGroups, kSteps = Sh::kSteps, kParts = Sh::kParts, kLoads = Sh::kLoads;
+  extern __shared__ va_u32x4 smem[];
+  char* lds = (char*)smem;
+  const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
+  const Words item = (Words)a.items + (long long)where.item * VA_WEIGH_ITEM_WORDS;
+  const int n_tok = item[VA_WI_N_TOK], hk = where.head;
+  if (n_tok == 0) return;
+  const int page_begin = item[VA_WI_PAGES], first = item[VA_WI_FIRST], partial = item[VA_WI_PARTIAL];
+  const int tile_begin = item[VA_WI_TILE_BEGIN], n_tiles = item[VA_WI_TILE_END] - tile_begin;
+  const int lane = threadIdx.x % kWave, j = lane % 16, kg = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
+  const char* queries = a.queries + ((long long)hk * a.n_tiles + tile_begin) * Sh::kQueryBytes + wave * (kLoads - 1) * 1024 + 16 * lane;
+  const WeighRow* rows = a.rows + ((long long)hk * a.n_tiles + tile_begin) * 16 + lane % 16;
+  auto request = [&](int i) __attribute__((always_inline)) {
+    const uint32_t dst = lds_base + (uint32_t)(i % Sh::kBuffers) * Sh::kBufferBytes;
+#pragma unroll
+    for (int u = 0; u < kLoads - 1; ++u)
+      load_to_lds(queries + (long long)i * Sh::kQueryBytes + 1024 * u, dst + (uint32_t)(wave * (kLoads - 1) + u) * 1024);
+    if (lane < 16) load_to_lds(rows + (long long)i * 16, dst + Sh::kQueryBytes + 256 * wave);
+  };
+
+  va_u32x4 keys[kGroups][kSteps];
+  float factor[kGroups][4];
+  const int w0 = 16 * kGroups * wave;  // first token of the wave, in the chunk
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const float mine = K::load(a, weigh_slot(a, page_begin, first + min(w0 + 16 * g + j, n_tok - 1)), hk, kg, keys[g]);
+    if constexpr (K::kFactor)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) factor[g][r] = __shfl(mine, 4 * kg + r, kWave);
+  }
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(keys[g][s]));  // (waited for here, not in the loop)
+  const int t_wave = first + w0, t_end = min(t_wave + 16 * kGroups, first + n_tok);
+  float sum[kGroups][4];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g)
 #pragma unroll
     for (int r = 0; r < 4; ++r) sum[g][r] = 0.f;
-  for (int tile = item[VA_WI_TILE_BEGIN]; tile < tile_end; ++tile) {
-    const long long at = (long long)hk * a.n_tiles + tile;
-    const WeighRow row = a.rows[at * 16 + j];
-    if (!__any(row.lo < t_end && row.hi > t_wave)) continue;
-    const va_u32x4* queries = (const va_u32x4*)(a.queries + at * (kParts * kSteps * 1024)) + lane;
-    va_f32x4 dots[kWeighGroups];
+  request(0);
+  if (n_tiles > 1) request(1);
+  for (int i = 0; i < n_tiles; ++i) {
+    // everyone's part of tile i has landed, and everyone is done with the buffer that tile i + 2 goes to
+    if (i + 1 < n_tiles) ring_barrier<kLoads>(); else ring_barrier<0>();
+    if (i + 2 < n_tiles) request(i + 2);
+    const char* buffer = lds + (i % Sh::kBuffers) * Sh::kBufferBytes;
+    const WeighRow row = *(const WeighRow*)(buffer + Sh::kQueryBytes + 256 * wave + 16 * j);
+    if (!__any(row.lo < t_end && row.hi > t_wave && row.scale != 0.f)) continue;
+    va_f32x4 dots[kGroups];
 #pragma unroll
-    for (int g = 0; g < kWeighGroups; ++g) dots[g] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < kGroups; ++g) dots[g] = va_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int part = kParts - 1; part >= 0; --part)  // (small ones first)
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const va_u32x4 q = queries[(part * kSteps + s) * kWave];
+      for (int p = kParts - 1; p >= 0; --p) {
+        const va_u32x4 q = *(const va_u32x4*)(buffer + (p * kSteps + s) * 1024 + 16 * lane);
 #pragma unroll
-        for (int g = 0; g < kWeighGroups; ++g) dots[g] = M::run(keys[g][s], q, dots[g]);
+        for (int g = 0; g < kGroups; ++g) dots[g] = Mma<F16>::run(keys[g][s], q, dots[g]);
       }
-    const bool all = !__any(row.lo > t_wave || row.hi < t_end);
+    auto weight = [&](int g, int r) __attribute__((always_inline)) {
+      float x = dots[g][r];
+      if constexpr (K::kFactor) x *= factor[g][r];
+      return __builtin_amdgcn_exp2f(fmaf(x, row.scale, row.minus_lse));
+    };
+    if (__any(row.lo > t_wave || row.hi < t_end)) {  // some row does not see some token
 #pragma unroll
-    for (int g = 0; g < kWeighGroups; ++g)
+      for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(dots[g][r], row.scale, row.minus_lse));
-        const int t = t_wave + 16 * g + 4 * kg + r;
-        sum[g][r] += all || (t >= row.lo && t < row.hi) ? p : 0.f;
-      }
-  }
+        for (int r = 0; r < 4; ++r) {
+          const int t = t_wave + 16 * g + 4 * kg + r;
+          const float p = weight(g, r);
+          sum[g][r] += t >= row.lo && t < row.hi ? p : 0.f;
+        }
+    } else {
 #pragma unroll
-  for (int g = 0; g < kWeighGroups; ++g) {
+      for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sum[g][r] = group_sum<16>(sum[g][r]);
-    // lane j < 4 has token 4 kg + j
-    const float mine = j == 0 ? sum[g][0] : j == 1 ? sum[g][1] : j == 2 ? sum[g][2] : sum[g][3];
-    const int t = w0 + 16 * g + 4 * kg + j;
-    if (j < 4 && t < n_tok) {
-      if (partial >= 0) {
-        a.partials[hk * a.n_partials + partial + t] = mine;
-      } else {
-        const long long to = hk * a.num_slots + weigh_slot(a, page_begin, first + t);
-        a.weights_out[to] = a.weights_in[to] + mine;
-      }
+        for (int r = 0; r < 4; ++r) sum[g][r] += weight(g, r);
     }
   }
+  __syncthreads();
+  float* sums = (float*)lds;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum[g][r] = row_sum(sum[g][r]);
+    const float of_token = j == 0 ? sum[g][0] : j == 1 ? sum[g][1] : j == 2 ? sum[g][2] : sum[g][3];
+    if (j < 4) sums[w0 + 16 * g + 4 * kg + j] = of_token;
+  }
+  __syncthreads();
+  finish_sums(a, page_begin, first, n_tok, partial, hk, sums);
 }
 
 // ---------------------------------------------------------------------------
@@ -345,15 +806,16 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_generic_kernel(WeighArgs 
   }
 }
 
-__global__ __launch_bounds__(VA_WEIGH_CHUNK) void weigh_join_kernel(WeighArgs a) {
+__global__ __launch_bounds__(kWeighThreads) void weigh_join_kernel(WeighArgs a) {
   const int32_t* join = a.joins + (long long)blockIdx.x * VA_WEIGH_JOIN_WORDS;
-  const int n_tok = join[VA_WJ_N_TOK], n_parts = join[VA_WJ_N_PARTS], hk = blockIdx.y, t = threadIdx.x;
-  if (t >= n_tok) return;
-  const float* from = a.partials + hk * a.n_partials + join[VA_WJ_PARTIAL] + t;
-  float sum = 0.f;
-  for (int p = 0; p < n_parts; ++p) sum += from[(long long)p * n_tok];
-  const long long to = hk * a.num_slots + weigh_slot(a, join[VA_WJ_PAGES], join[VA_WJ_FIRST] + t);
-  a.weights_out[to] = a.weights_in[to] + sum;
+  const int n_tok = join[VA_WJ_N_TOK], n_parts = join[VA_WJ_N_PARTS], hk = blockIdx.y;
+  for (int t = threadIdx.x; t < n_tok; t += kWeighThreads) {
+    const float* from = a.partials + hk * a.n_partials + join[VA_WJ_PARTIAL] + t;
+    float sum = 0.f;
+    for (int p = 0; p < n_parts; ++p) sum += from[(long long)p * n_tok];
+    const long long to = hk * a.num_slots + weigh_slot(a, join[VA_WJ_PAGES], join[VA_WJ_FIRST] + t);
+    a.weights_out[to] = a.weights_in[to] + sum;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -364,30 +826,54 @@ static int weigh_launched(const char* what) {
   return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }
 
-template <typename C>
-static int launch_weigh(const WeighArgs& a, int n_items, bool matrix, hipStream_t stream) {
-  const dim3 rows_grid((unsigned)a.n_tiles, (unsigned)a.num_kv_heads), grid((unsigned)n_items * (unsigned)a.num_kv_heads), block(kWeighThreads);
+template <int kKind>
+static void launch_rows(const WeighArgs& a, bool fast, hipStream_t stream) {
+  const unsigned hkv = (unsigned)a.num_kv_heads;
+  if (fast) {
+    const long long tasks = (long long)a.n_tiles * 16 * (a.head_dim / 16);
+    hipLaunchKernelGGL(weigh_rows_kernel<kKind>, dim3((unsigned)((tasks + kWeighThreads - 1) / kWeighThreads), hkv), dim3(kWeighThreads), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL(weigh_rows_any_kernel<kKind>, dim3((unsigned)a.n_tiles, hkv), dim3(kWeighThreads), 0, stream, a);
+  }
+}
+
+template <int kD, typename C>
+static int launch_matrix(const WeighArgs& a, int layout, int n_items, bool fast, hipStream_t stream) {
+  const dim3 grid((unsigned)n_items * (unsigned)a.num_kv_heads), block(kWeighThreads);
   if constexpr (!std::is_same_v<C, F32>) {
-    if (matrix) {
-      hipLaunchKernelGGL(weigh_rows_kernel<WeighKeys<C>::kParts>, rows_grid, block, 0, stream, a);
-      switch (a.head_dim) {
-        case 64:
-          hipLaunchKernelGGL((weigh_mfma_kernel<64, C>), grid, block, 0, stream, a);
-          break;
-        case 128:
-          hipLaunchKernelGGL((weigh_mfma_kernel<128, C>), grid, block, 0, stream, a);
-          break;
-        default:
-          hipLaunchKernelGGL((weigh_mfma_kernel<256, C>), grid, block, 0, stream, a);
-      }
+    if (layout == VA_WEIGH_TILES) {
+      launch_rows<TileKeys<kD, C>::kRows>(a, fast, stream);
+      hipLaunchKernelGGL((weigh_tile_kernel<kD, C>), grid, block, TileShape<kD>::kLdsBytes, stream, a);
       return weigh_launched("attention weights");
     }
   }
+  using Sh = WalkShape<kD, C>;
+  static std::atomic<unsigned long long> devices{0};
+  const hipError_t e = allow_lds(reinterpret_cast<const void*>(&weigh_walk_kernel<kD, C>), Sh::kLdsBytes, devices);
+  if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
+  launch_rows<WalkKeys<C>::kRows>(a, fast, stream);
+  hipLaunchKernelGGL((weigh_walk_kernel<kD, C>), grid, block, Sh::kLdsBytes, stream, a);
+  return weigh_launched("attention weights");
+}
+
+template <typename C>
+static int launch_weigh(const WeighArgs& a, int layout, int n_items, bool matrix, bool fast, hipStream_t stream) {
+  if (matrix) {
+    switch (a.head_dim) {
+      case 64:
+        return launch_matrix<64, C>(a, layout, n_items, fast, stream);
+      case 128:
+        return launch_matrix<128, C>(a, layout, n_items, fast, stream);
+      default:
+        return launch_matrix<256, C>(a, layout, n_items, fast, stream);
+    }
+  }
+  const dim3 grid((unsigned)n_items * (unsigned)a.num_kv_heads), block(kWeighThreads);
   const int bytes = (64 * (a.head_dim + 1) + 64 * kWeighWaves) * 4;
   static std::atomic<unsigned long long> devices{0};
   const hipError_t e = allow_lds(reinterpret_cast<const void*>(&weigh_generic_kernel<C>), (64 * (kWeighMaxDim + 1) + 64 * kWeighWaves) * 4, devices);
   if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
-  hipLaunchKernelGGL(weigh_rows_kernel<kRows32>, rows_grid, block, 0, stream, a);
+  launch_rows<kPlain32>(a, false, stream);
   hipLaunchKernelGGL(weigh_generic_kernel<C>, grid, block, (unsigned)bytes, stream, a);
   return weigh_launched("attention weights");
 }
@@ -427,29 +913,34 @@ static int weigh(WeighArgs& a, int code_type, int num_pages, const int32_t* plan
   a.page_map = page_map(shape->page_size);
   a.scale_log2 = kLog2e / sqrtf((float)shape->head_dim);
   const bool dims = shape->head_dim == 64 || shape->head_dim == 128 || shape->head_dim == 256;
-  const bool rows16 = code_type >= 0 || (a.pool_row_stride % 8 == 0 && (uintptr_t)a.k_pool % 16 == 0);
-  const bool matrix = dims && rows16;
+  const int size = shape->dtype == VA_F32 ? 4 : 2;
+  // (a walk addresses 16 rows of a page with 32-bit offsets)
+  const bool matrix = dims && (code_type >= 0 || (a.pool_row_stride * size % 16 == 0 && (uintptr_t)a.k_pool % 16 == 0 && a.pool_row_stride < 1 << 24));
+  const bool fast = a.rope.rotary_dim % 16 == 0 && (a.rope.mode != VA_ROPE_TABLE || (uintptr_t)a.rope.cos_sin % 16 == 0);
+  a.pieces = a.q_row_stride * size % 16 == 0 && (uintptr_t)a.q % 16 == 0;
+  const int layout = h[VA_WH_LAYOUT];
+  if (layout == VA_WEIGH_TILES && shape->dtype == VA_F32) return va_fail(VA_ERR_ARG, "plan header: no tiles over 32-bit rows");
   if (code_type == VA_CODE_E4M3) {
-    rc = launch_weigh<E4M3>(a, n_items, matrix, stream);
+    rc = launch_weigh<E4M3>(a, layout, n_items, matrix, fast, stream);
   } else if (code_type == VA_CODE_INT8) {
-    rc = launch_weigh<INT8>(a, n_items, matrix, stream);
+    rc = launch_weigh<INT8>(a, layout, n_items, matrix, fast, stream);
   } else {
     switch (shape->dtype) {
       case VA_F32:
-        rc = launch_weigh<F32>(a, n_items, false, stream);
+        rc = launch_weigh<F32>(a, layout, n_items, matrix, fast, stream);
         break;
       case VA_F16:
-        rc = launch_weigh<F16>(a, n_items, matrix, stream);
+        rc = launch_weigh<F16>(a, layout, n_items, matrix, fast, stream);
         break;
       case VA_BF16:
-        rc = launch_weigh<BF16>(a, n_items, matrix, stream);
+        rc = launch_weigh<BF16>(a, layout, n_items, matrix, fast, stream);
         break;
       default:
         rc = va_fail(VA_ERR_ARG, "unknown dtype %d", (int)shape->dtype);
     }
   }
   if (rc || h[VA_WH_N_JOINS] == 0) return rc;
-  hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)h[VA_WH_N_JOINS], (unsigned)hkv), dim3(VA_WEIGH_CHUNK), 0, stream, a);
+  hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)h[VA_WH_N_JOINS], (unsigned)hkv), dim3(kWeighThreads), 0, stream, a);
   return weigh_launched("joining attention weights");
 }
 

@@ -22,6 +22,7 @@ struct Planner {
   const VaSubRequests& in;
   const VaShape& shape;
   int num_pages, window;
+  Planner(const VaSubRequests& s, const VaShape& sh, int pages_, int w) : in(s), shape(sh), num_pages(pages_), window(w) {}
   std::vector<int64_t> first_visitor;  // by page, [num_pages + 1]
   std::vector<Visitor> visitors;
   std::vector<int32_t> pages, items, joins, sub_row, lo, hi;
@@ -113,7 +114,8 @@ struct Planner {
     }
     if ((int64_t)sub_row.size() == row_begin) return VA_OK;
     while (sub_row.size() % unit) sub_row.push_back(-1), lo.push_back(0), hi.push_back(0);
-    if ((int64_t)sub_row.size() * G > INT32_MAX) return va_fail(VA_ERR_ARG, "too many query rows for one plan");
+    if ((int64_t)sub_row.size() * G > INT32_MAX / 16)  // (a thread for each 16 elements of a row)
+       return va_fail(VA_ERR_ARG, "too many query rows for one plan");
     spans.push_back(Span{(int64_t)pages.size(), (int32_t)first, (int32_t)end, row_begin, (int64_t)sub_row.size()});
     pages.insert(pages.end(), run.begin(), run.end());
     return VA_OK;
@@ -141,30 +143,49 @@ struct Planner {
     return close(run);
   }
 
-  // Rows of a chunk are split where the launch has too few workgroups otherwise.
+  int layout = VA_WEIGH_WALK;
+
+  // Walks where a token has few rows (tiles of 16 of them, on average over the tokens), else tiles.
+  bool many_rows(int64_t tokens, int64_t products) const {
+    const bool halves = shape.dtype != VA_F32 && (shape.head_dim == 64 || shape.head_dim == 128 || shape.head_dim == 256);
+    return halves && products >= 8 * tokens;
+  }
+
   int make_items() {
-    const int G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G), T = VA_WEIGH_CHUNK;
-    constexpr int64_t kWanted = 1024;
-    int64_t chunks = 0;
-    for (const Span& s : spans) chunks += ((int64_t)s.end - s.first + T - 1) / T;
-    const int64_t groups = chunks * shape.num_kv_heads, cuts = std::max<int64_t>(1, (kWanted + groups - 1) / std::max<int64_t>(1, groups));
+    const int G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G);
+    int64_t tokens = 0, products = 0;  // products: (token, tile of rows)
+    for (const Span& s : spans) tokens += s.end - s.first, products += (int64_t)(s.end - s.first) * ((s.row_end - s.row_begin) * G / 16);
+    layout = many_rows(tokens, products) ? VA_WEIGH_TILES : VA_WEIGH_WALK;
+    // tokens of an item, and how many (token, tile)s it should have at most
+    int64_t T = VA_WEIGH_TILE_TOKENS, most;
+    if (layout == VA_WEIGH_TILES) {
+      most = std::max<int64_t>(8 * T, products * shape.num_kv_heads / 2048);
+    } else {
+      // a workgroup's four waves take a tile each: of 16 tokens or more, 16 KB
+      const int row = shape.head_dim * (shape.dtype == VA_F32 ? 4 : 2);
+      const int64_t least = 4 * 16 * std::clamp(1024 / std::max(row, 1), 1, 4);
+      T = least * std::clamp<int64_t>(tokens * shape.num_kv_heads / (least * 1536), 1, VA_WEIGH_MOST_TOKENS / least);
+      most = std::max<int64_t>(4 * T, products * shape.num_kv_heads / 1024);
+    }
     for (const Span& s : spans) {
-      for (int64_t t = s.first; t < s.end; t += T) {
-        const int n_tok = (int)std::min<int64_t>(T, s.end - t);
+      // (chunks start on multiples of 16 tokens of the span: pages of as many are read in runs)
+      for (int64_t t = s.first / 16 * 16; t < s.end; t += T) {
+        const int64_t begin = std::max<int64_t>(t, s.first);
+        const int n_tok = (int)(std::min<int64_t>(t + T, s.end) - begin);
         // the rows that see any of it lie between these (a request's rows see ever more)
         int64_t a = s.row_begin, b = s.row_end;
-        while (a < b && (hi[(size_t)a] <= t || lo[(size_t)a] >= t + n_tok)) ++a;
-        while (b > a && (hi[(size_t)b - 1] <= t || lo[(size_t)b - 1] >= t + n_tok)) --b;
+        while (a < b && (hi[(size_t)a] <= begin || lo[(size_t)a] >= begin + n_tok)) ++a;
+        while (b > a && (hi[(size_t)b - 1] <= begin || lo[(size_t)b - 1] >= begin + n_tok)) --b;
         if (a == b) continue;
         const int64_t tile_a = a / unit * unit * G / 16, tile_b = ((b + unit - 1) / unit * unit) * G / 16;
-        const int64_t parts = std::min(cuts, tile_b - tile_a);
+        const int64_t parts = std::min((n_tok * (tile_b - tile_a) + most - 1) / most, tile_b - tile_a);
         if (parts > 1) {
           if (n_partials + parts * n_tok > INT32_MAX) return va_fail(VA_ERR_ARG, "too many partial sums for one plan");
-          const int32_t join[VA_WEIGH_JOIN_WORDS] = {(int32_t)s.page_begin, (int32_t)t, n_tok, (int32_t)n_partials, (int32_t)parts, 0, 0, 0};
+          const int32_t join[VA_WEIGH_JOIN_WORDS] = {(int32_t)s.page_begin, (int32_t)begin, n_tok, (int32_t)n_partials, (int32_t)parts, 0, 0, 0};
           joins.insert(joins.end(), join, join + VA_WEIGH_JOIN_WORDS);
         }
         for (int64_t p = 0; p < parts; ++p) {
-          const int32_t item[VA_WEIGH_ITEM_WORDS] = {(int32_t)s.page_begin, (int32_t)t, n_tok, (int32_t)(tile_a + (tile_b - tile_a) * p / parts),
+          const int32_t item[VA_WEIGH_ITEM_WORDS] = {(int32_t)s.page_begin, (int32_t)begin, n_tok, (int32_t)(tile_a + (tile_b - tile_a) * p / parts),
                                                      (int32_t)(tile_a + (tile_b - tile_a) * (p + 1) / parts),
                                                      parts > 1 ? (int32_t)(n_partials + p * n_tok) : -1, 0, 0};
           items.insert(items.end(), item, item + VA_WEIGH_ITEM_WORDS);
@@ -184,7 +205,7 @@ int build(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, in
     return va_fail(VA_ERR_ARG, "bad shape");
   if (num_pages < 0 || (int64_t)num_pages * shape->page_size > INT32_MAX || window < 0)
     return va_fail(VA_ERR_ARG, "%d pages of %d tokens, window %d", (int)num_pages, (int)shape->page_size, (int)window);
-  Planner p{*subs, *shape, num_pages, window, {}, {}, {}, {}, {}, {}, {}, {}, 0, {}};
+  Planner p{*subs, *shape, num_pages, window};
   int rc = p.check();
   if (rc) return rc;
   p.find_visitors();
@@ -224,6 +245,7 @@ int build(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, in
   put(p.hi);
   h[VA_WH_HQ] = shape->num_q_heads, h[VA_WH_HKV] = shape->num_kv_heads, h[VA_WH_D] = shape->head_dim;
   h[VA_WH_PAGE] = shape->page_size, h[VA_WH_DTYPE] = shape->dtype, h[VA_WH_POOL_PAGES] = num_pages, h[VA_WH_N_SUBROWS] = subs->n_subrows;
+  h[VA_WH_LAYOUT] = p.layout;
   return VA_OK;
 }
 
