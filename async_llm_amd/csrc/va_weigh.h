@@ -11,11 +11,10 @@
 #define VA_WEIGH_HEADER_WORDS 24
 #define VA_WEIGH_ITEM_WORDS 8
 #define VA_WEIGH_JOIN_WORDS 8
-#define VA_WEIGH_MOST_TOKENS 2048  // of an item
 
 // How a launch's work is laid out.
 enum {
-  VA_WEIGH_WALK = 0,   // few rows a token: bound by the keys; items are walks of many tokens (weigh_walk_kernel)
+  VA_WEIGH_WALK = 0,   // few rows a token: bound by the keys; a workgroup walks a strip of items (weigh_walk_kernel)
   VA_WEIGH_TILES = 1,  // many rows a token: bound by the products; items are VA_WEIGH_TILE_TOKENS tokens and many rows (weigh_tile_kernel)
 };
 #define VA_WEIGH_TILE_TOKENS 256
@@ -23,7 +22,7 @@ enum {
 // header word indices
 enum {
   VA_WH_MAGIC = 0,
-  VA_WH_N_ITEMS,   // a multiple of 8, padding included
+  VA_WH_N_ITEMS,   // tiles: a multiple of 8, padding included
   VA_WH_N_ROWS,    // packed rows: a multiple of what makes whole tiles of 16 (row, q head) pairs
   VA_WH_N_JOINS,
   VA_WH_N_PARTIALS,  // partial sums, in tokens (per kv head)
@@ -40,6 +39,8 @@ enum {
   VA_WH_POOL_PAGES,
   VA_WH_N_SUBROWS,
   VA_WH_LAYOUT,
+  VA_WH_N_STRIPS,  // walks: a multiple of 8
+  VA_WH_OFF_STRIPS,  // [n_strips + 1]: strip s is the items [strips[s], strips[s + 1])
 };
 
 // item word indices (n_tok = 0: padding)

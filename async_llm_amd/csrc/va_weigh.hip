@@ -45,6 +45,7 @@ struct WeighArgs {
   const uint8_t* k_scales;
   long long pool_row_stride;  // elements between token slots (16- and 32-bit pools)
   const int32_t* items;
+  const int32_t* strips;
   const int32_t* joins;
   const int32_t* pages;
   const int32_t* sub_rows;
@@ -321,11 +322,13 @@ struct WalkShape {
   static constexpr int kTokens = 16 * kGroups;
   static constexpr int kGroupBytes = 16 * kRowBytes;
   static constexpr int kLoads = kGroupBytes / 1024;        // wave-level loads of a group
-  static constexpr int kTileBytes = kGroups * kGroupBytes + (K::kCodes ? 256 : 0);  // with a word for every scale
-  static constexpr int kBuffers = kTileBytes > 8 * 1024 + 256 ? 1 : 2;
-  static constexpr int kTileLoads = kGroups * kLoads + (K::kCodes ? 1 : 0);  // what the counter of outstanding loads sees of a tile
-  static constexpr int kSumsOffset = kWeighWaves * kBuffers * kTileBytes;
-  static constexpr int kLdsBytes = kSumsOffset + VA_WEIGH_MOST_TOKENS * 4;
+  // behind a tile's rows: the tokens' sums so far, a word for every scale, the tokens' slots
+  static constexpr int kSumsAt = kGroups * kGroupBytes, kScalesAt = kSumsAt + 256, kSlotsAt = kScalesAt + (K::kCodes ? 256 : 0);
+  static constexpr int kTileBytes = kSlotsAt + 256;
+  static constexpr int kBuffers = kTileBytes > 10 * 1024 ? 1 : 2;
+  static constexpr int kTileLoads = kGroups * kLoads + (K::kCodes ? 2 : 1);  // what the counter of outstanding loads sees of a tile
+  static constexpr int kTurnOffset = kWeighWaves * kBuffers * kTileBytes;  // where a wave turns a tile's sums from lanes to tokens
+  static constexpr int kLdsBytes = kTurnOffset + kWeighWaves * 256;
   static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups share the LDS of a CU");
   static_assert((kBuffers - 1) * kTileLoads < kAnyInFlight, "the counter of outstanding loads");
 };
@@ -337,18 +340,10 @@ __device__ __forceinline__ int walk_swz(int r) {
   return (r >> 2) & 3;
 }
 
-// A workgroup's sums to where they go.
-__device__ __forceinline__ void finish_sums(const WeighArgs& a, int page_begin, int first, int n_tok, int partial, int hk, const float* sums) {
-  for (int t = threadIdx.x; t < n_tok; t += kWeighThreads) {
-    if (partial >= 0) {
-      a.partials[hk * a.n_partials + partial + t] = sums[t];
-    } else {
-      const long long to = hk * a.num_slots + weigh_slot(a, page_begin, first + t);
-      a.weights_out[to] = a.weights_in[to] + sums[t];
-    }
-  }
-}
-
+// A workgroup walks a strip of items, its four waves on their own: each takes every fourth tile of an item's tokens, brings it
+// global -> LDS into a ring of its own (keys, the sums so far and, over codes, scales) and asks for the next one, of the next item
+// where this one ends, as soon as the keys are in registers.  There is no barrier, and nothing but the first tile of a strip
+// is waited for idly.
 template <int kD, typename C>
 __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs a) {
   using Sh = WalkShape<kD, C>;
@@ -359,20 +354,28 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
   extern __shared__ va_u32x4 smem[];
   char* lds = (char*)smem;
   const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
-  const Words item = (Words)a.items + (long long)where.item * VA_WEIGH_ITEM_WORDS;
-  const int n_tok = item[VA_WI_N_TOK], hk = where.head;
-  if (n_tok == 0) return;
-  const int page_begin = item[VA_WI_PAGES], first = item[VA_WI_FIRST], partial = item[VA_WI_PARTIAL];
-  const int tile_begin = item[VA_WI_TILE_BEGIN], tile_end = item[VA_WI_TILE_END];
+  const int hk = where.head, strip_begin = ((Words)a.strips)[where.item], strip_end = ((Words)a.strips)[where.item + 1];
+  if (strip_begin == strip_end) return;
   const int lane = threadIdx.x % kWave, j = lane % 16, kg = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int last = n_tok - 1, n_tiles = (n_tok + kTokens - 1) / kTokens;
-  const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_address(lds)) + (uint32_t)(wave * kBuffers * Sh::kTileBytes);
-  float* sums = (float*)(lds + Sh::kSumsOffset);
-  // (16 tokens of a group lie in one page; their rows within 32-bit offsets)
-  const bool whole = a.page_map.shift >= 4 && first % 16 == 0;
+  char* own = lds + wave * kBuffers * Sh::kTileBytes;
+  const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_address(own));
+  float* turn = (float*)(lds + Sh::kTurnOffset) + 64 * wave;
+  const bool pages16 = a.page_map.shift >= 4;
   const long long row_bytes = K::kCodes ? kD : a.pool_row_stride * K::kBytes;
+  const float* sums_in = a.weights_in + hk * a.num_slots;
 
+  struct Piece {
+    int pages, first, n_tok, tile_begin, tile_end, partial, tiles;  // tiles: this wave's, of tokens
+  };
+  auto piece_at = [&](int index) __attribute__((always_inline)) {
+    const Words w = (Words)a.items + (long long)index * VA_WEIGH_ITEM_WORDS;
+    Piece p{w[VA_WI_PAGES], w[VA_WI_FIRST], w[VA_WI_N_TOK], w[VA_WI_TILE_BEGIN], w[VA_WI_TILE_END], w[VA_WI_PARTIAL], 0};
+    p.tiles = ((p.n_tok + kTokens - 1) / kTokens - wave + kWeighWaves - 1) / kWeighWaves;
+    return p;
+  };
+
+  // ---- keys ----
   // This lane's part of load u of a group: row and piece, which belongs at its LDS position.  Loads in groups of up to four share one
   // setting of M0, whose immediate offsets move the pool address as well (grouped_lane_offset; the base gives the bias back).
   constexpr int kBias = 1024 * (kLoads - 1);
@@ -385,57 +388,64 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
     if constexpr (K::kCodes) return quant_row(a.page_map, slot, hk, a.num_kv_heads) * kD;
     return (long long)slot * row_bytes + hk * (long long)Sh::kRowBytes;
   };
-  auto request = [&](int n) __attribute__((always_inline)) {  // this wave's tile n
-    const uint32_t dst = ring + (uint32_t)(n % kBuffers) * Sh::kTileBytes;
-    const int t0 = (n * kWeighWaves + wave) * kTokens;
-    if (whole) {
-      long long of_lane = 0;  // of the token whose scale this lane brings
+  auto request_group = [&](const char* from, const uint32_t* off, uint32_t dst) __attribute__((always_inline)) {
+    if constexpr (kLoads >= 4) {
+#pragma unroll
+      for (int u = 0; u < kLoads; u += 4) load_group_to_lds<4, true>(from, off + u, dst + 1024 * u);
+    } else if constexpr (kLoads == 2) {
+      load_group_to_lds<2, true>(from, off, dst);
+    } else {
+      load_to_lds(from, off[0], dst);
+    }
+  };
+  auto request = [&](const Piece& p, int n, int buffer) __attribute__((always_inline)) {  // this wave's tile n of an item
+    const uint32_t dst = ring + (uint32_t)buffer * Sh::kTileBytes;
+    const int t0 = (n * kWeighWaves + wave) * kTokens, last = p.n_tok - 1;
+    uint32_t of_lane = 0;  // slot of the token whose words this lane brings: token `lane` of the tile
+    if (pages16 && p.first % 16 == 0) {  // 16 tokens of a group lie in one page
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         const int t = min(t0 + 16 * g, last / 16 * 16);  // (a group past the end: the last one)
-        const uint32_t at = (uint32_t)(first + t);
-        const uint32_t slot = ((uint32_t)((Words)a.pages)[page_begin + (int)(at >> a.page_map.shift)] << a.page_map.shift) + (at & (a.page_map.size - 1));
-        const long long base = row_at(slot);
-        const char* from = (const char*)a.k_pool + (base - kBias);
+        const uint32_t at = (uint32_t)(p.first + t);
+        const uint32_t slot = ((uint32_t)((Words)a.pages)[p.pages + (int)(at >> a.page_map.shift)] << a.page_map.shift) + (at & (a.page_map.size - 1));
+        const char* from = (const char*)a.k_pool + (row_at(slot) - kBias);
         const int most = last - t;  // rows behind the last one repeat it
         if (most >= 15) {
-          if constexpr (kLoads >= 4) {
-#pragma unroll
-            for (int u = 0; u < kLoads; u += 4) load_group_to_lds<4, true>(from, ld_off + u, dst + g * Sh::kGroupBytes + 1024 * u);
-          } else if constexpr (kLoads == 2) {
-            load_group_to_lds<2, true>(from, ld_off, dst + g * Sh::kGroupBytes);
-          } else {
-            load_to_lds(from, ld_off[0], dst + g * Sh::kGroupBytes);
-          }
+          request_group(from, ld_off, dst + g * Sh::kGroupBytes);
         } else {
           uint32_t off[kLoads];
 #pragma unroll
           for (int u = 0; u < kLoads; ++u) off[u] = ld_off[u] - (uint32_t)(max(0, ld_row(u) - most) * row_bytes);
-          if constexpr (kLoads >= 4) {
-#pragma unroll
-            for (int u = 0; u < kLoads; u += 4) load_group_to_lds<4, true>(from, off + u, dst + g * Sh::kGroupBytes + 1024 * u);
-          } else if constexpr (kLoads == 2) {
-            load_group_to_lds<2, true>(from, off, dst + g * Sh::kGroupBytes);
-          } else {
-            load_to_lds(from, off[0], dst + g * Sh::kGroupBytes);
-          }
+          request_group(from, off, dst + g * Sh::kGroupBytes);
         }
-        if constexpr (K::kCodes) of_lane = kg == g ? base / kD + min(j, most) : of_lane;
+        of_lane = kg == g || g == 0 ? slot + min(j, most) : of_lane;
       }
-      if constexpr (K::kCodes) load_bytes_to_lds((unsigned long long)a.k_scales + of_lane, dst + kGroups * Sh::kGroupBytes);
     } else {  // tokens looked up one by one: each lane one, handed to those that load it
-      const uint32_t mine = weigh_slot(a, page_begin, first + min(t0 + lane % kTokens, last));
+      of_lane = weigh_slot(a, p.pages, p.first + min(t0 + lane % kTokens, last));
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
-          const uint32_t slot = (uint32_t)__shfl((int)mine, 16 * g + ld_row(u), kWave);
+          const uint32_t slot = (uint32_t)__shfl((int)of_lane, 16 * g + ld_row(u), kWave);
           load_to_lds((const char*)a.k_pool + row_at(slot) + 16 * ld_piece(u), dst + g * Sh::kGroupBytes + 1024 * u);
         }
-      if constexpr (K::kCodes) load_bytes_to_lds((unsigned long long)a.k_scales + row_at(mine) / kD, dst + kGroups * Sh::kGroupBytes);
     }
+    load_word_to_lds(sums_in + of_lane, dst + Sh::kSumsAt);
+    if constexpr (K::kCodes) load_bytes_to_lds((unsigned long long)a.k_scales + row_at(of_lane) / kD, dst + Sh::kScalesAt);
+    *(uint32_t*)(own + buffer * Sh::kTileBytes + Sh::kSlotsAt + 4 * lane) = of_lane;
+  };
+  int asked = 0, ask_index = strip_begin, ask_n = 0;  // tiles asked for so far; the next one
+  Piece ask = piece_at(strip_begin);
+  auto request_next = [&]() __attribute__((always_inline)) {
+    while (ask_n == ask.tiles) {
+      if (ask_index + 1 >= strip_end) return;
+      ask = piece_at(++ask_index);
+      ask_n = 0;
+    }
+    request(ask, ask_n++, asked++ % kBuffers);
   };
 
+  // ---- queries ----
   va_u32x4 q[kParts][kSteps];
   WeighRow row;
   const char* queries = a.queries + (long long)hk * a.n_tiles * tile_bytes_of(K::kRows, kD) + 16 * lane;
@@ -447,104 +457,147 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) q[p][s] = *(const va_u32x4*)(at + (p * kSteps + s) * 1024);
   };
-  const int mine = n_tiles > wave ? (n_tiles - wave + kWeighWaves - 1) / kWeighWaves : 0;  // this wave's tiles
-
-  // kSingle: one tile of rows, whose queries stay in registers; the next tile of keys is on its way before the products of the last.
-  // Otherwise queries are loaded tile by tile, and a wait for those would be one for the keys as well, which are asked for later.
-  auto walk = [&](auto single) __attribute__((always_inline)) {
-    constexpr bool kSingle = decltype(single)::value;
+  auto queries_here = [&]() __attribute__((always_inline)) {  // (waited for here, not in the loop)
 #pragma unroll
-    for (int b = 0; b < kBuffers; ++b)
-      if (b < mine) request(b);
-    if constexpr (kSingle) {
-      load_queries(tile_begin);
+    for (int p = 0; p < kParts; ++p)
 #pragma unroll
-      for (int p = 0; p < kParts; ++p)
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q[p][s]));  // (waited for here, not in the loop)
-      asm volatile("" : "+v"(row.minus_lse), "+v"(row.scale), "+v"(row.lo), "+v"(row.hi));
-    }
-    for (int n = 0; n < mine; ++n) {
-      if (n + kBuffers - 1 < mine) {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBuffers - 1) * Sh::kTileLoads) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      const char* tile = lds + (wave * kBuffers + n % kBuffers) * Sh::kTileBytes;
-      va_u32x4 keys[kGroups][kRaw];
-      float scale[kGroups];
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-#pragma unroll
-        for (int s = 0; s < kRaw; ++s)
-          keys[g][s] = *(const va_u32x4*)(tile + g * Sh::kGroupBytes + j * Sh::kRowBytes + 16 * ((4 * s + kg) ^ walk_swz<kPieces>(j)));
-        if constexpr (K::kCodes) scale[g] = scale_value(*(const uint32_t*)(tile + kGroups * Sh::kGroupBytes + 4 * (16 * g + j)));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (kSingle && n + kBuffers < mine) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        request(n + kBuffers);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-
-      const int t_tile = first + (n * kWeighWaves + wave) * kTokens, t_end = min(t_tile + kTokens, first + n_tok);
-      float sum[kGroups][4];
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum[g][r] = 0.f;
-      for (int of = tile_begin; of < (kSingle ? tile_begin + 1 : tile_end); ++of) {
-        if constexpr (!kSingle) load_queries(of);
-        va_f32x4 dots[kGroups];
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) dots[g] = va_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
-            va_u32x4 k;
-            if constexpr (K::kCodes) {
-              const va_u32x4 raw = keys[g][s / 2];
-              k = K::keys(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]}, scale[g]);
-            } else {
-              k = keys[g][s];
-            }
-#pragma unroll
-            for (int p = kParts - 1; p >= 0; --p) dots[g] = K::run(k, q[p][s], dots[g]);
-          }
-        if (__any(row.lo > t_tile || row.hi < t_end)) {  // some row does not see some token
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int t = t_tile + 16 * g + 4 * kg + r;
-              const float p = __builtin_amdgcn_exp2f(fmaf(dots[g][r], row.scale, row.minus_lse));
-              sum[g][r] += t >= row.lo && t < row.hi ? p : 0.f;
-            }
-        } else {
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sum[g][r] += __builtin_amdgcn_exp2f(fmaf(dots[g][r], row.scale, row.minus_lse));
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum[g][r] = row_sum(sum[g][r]);
-        // lane j < 4 has token 4 kg + j
-        const float of_token = j == 0 ? sum[g][0] : j == 1 ? sum[g][1] : j == 2 ? sum[g][2] : sum[g][3];
-        if (j < 4) sums[(n * kWeighWaves + wave) * kTokens + 16 * g + 4 * kg + j] = of_token;
-      }
-      if (!kSingle && n + kBuffers < mine) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        request(n + kBuffers);
-      }
-    }
+      for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q[p][s]));
+    asm volatile("" : "+v"(row.minus_lse), "+v"(row.scale), "+v"(row.lo), "+v"(row.hi));
   };
-  if (tile_end - tile_begin == 1) walk(std::true_type{}); else walk(std::false_type{});
-  __syncthreads();
-  finish_sums(a, page_begin, first, n_tok, partial, hk, sums);
+
+  // ---- the walk ----
+#pragma unroll
+  for (int b = 0; b < kBuffers; ++b) request_next();
+  int done = 0, index = strip_begin, n = 0, q_tile = -1;
+  Piece at = piece_at(strip_begin);
+  float* to = nullptr;  // the sums of the tile before, written behind the wait of this one
+  float value = 0.f;
+  while (true) {
+    while (n == at.tiles) {
+      if (index + 1 >= strip_end) break;
+      at = piece_at(++index);
+      n = 0;
+    }
+    if (n == at.tiles) break;
+    const bool single = at.tile_end - at.tile_begin == 1;
+    if (single && at.tile_begin != q_tile) {
+      load_queries(at.tile_begin);
+      queries_here();
+      q_tile = at.tile_begin;
+    }
+    // The tile has landed once at most the loads of the kBuffers - 1 tiles asked for after it are outstanding.
+    if (asked - done >= kBuffers && kBuffers > 1) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBuffers - 1) * Sh::kTileLoads) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const char* tile = own + (done % kBuffers) * Sh::kTileBytes;
+    va_u32x4 keys[kGroups][kRaw];
+    float scale[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+      for (int s = 0; s < kRaw; ++s)
+        keys[g][s] = *(const va_u32x4*)(tile + g * Sh::kGroupBytes + j * Sh::kRowBytes + 16 * ((4 * s + kg) ^ walk_swz<kPieces>(j)));
+      if constexpr (K::kCodes) scale[g] = scale_value(*(const uint32_t*)(tile + Sh::kScalesAt + 4 * (16 * g + j)));
+    }
+    const float before = *(const float*)(tile + Sh::kSumsAt + 4 * lane);
+    const uint32_t slot = *(const uint32_t*)(tile + Sh::kSlotsAt + 4 * lane);
+    if (to) *to = value;
+    __builtin_amdgcn_sched_barrier(0);
+    if (single) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      request_next();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    const int t0 = (n * kWeighWaves + wave) * kTokens, t_tile = at.first + t0, t_end = min(t_tile + kTokens, at.first + at.n_tok);
+    float sum[kGroups][4];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[g][r] = 0.f;
+    auto add_rows = [&]() __attribute__((always_inline)) {
+      va_f32x4 dots[kGroups];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) dots[g] = va_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          va_u32x4 k;
+          if constexpr (K::kCodes) {
+            const va_u32x4 raw = keys[g][s / 2];
+            k = K::keys(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]}, scale[g]);
+          } else {
+            k = keys[g][s];
+          }
+#pragma unroll
+          for (int p = kParts - 1; p >= 0; --p) dots[g] = K::run(k, q[p][s], dots[g]);  // (small parts first)
+        }
+      if (__any(row.lo > t_tile || row.hi < t_end)) {  // some row does not see some token
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int t = t_tile + 16 * g + 4 * kg + r;
+            const float p = __builtin_amdgcn_exp2f(fmaf(dots[g][r], row.scale, row.minus_lse));
+            sum[g][r] += t >= row.lo && t < row.hi ? p : 0.f;
+          }
+      } else {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[g][r] += __builtin_amdgcn_exp2f(fmaf(dots[g][r], row.scale, row.minus_lse));
+      }
+    };
+    if (single) {
+      add_rows();
+    } else {
+      // Queries are loaded tile by tile; a wait for those would be one for the next keys as well, which are asked for behind them.
+      for (int of = at.tile_begin; of < at.tile_end; ++of) {
+        load_queries(of);
+        add_rows();
+      }
+      q_tile = -1;
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[g][r] = row_sum(sum[g][r]);
+      // lane j < 4 has token 4 kg + j
+      const float of_token = j == 0 ? sum[g][0] : j == 1 ? sum[g][1] : j == 2 ? sum[g][2] : sum[g][3];
+      if (j < 4) turn[16 * g + 4 * kg + j] = of_token;
+    }
+    value = turn[lane % kTokens];
+    to = nullptr;
+    if (lane < kTokens && t0 + lane < at.n_tok) {
+      if (at.partial < 0) {
+        value += before;
+        to = a.weights_out + hk * a.num_slots + slot;
+      } else {
+        to = a.partials + hk * a.n_partials + at.partial + t0 + lane;
+      }
+    }
+    if (!single) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      request_next();
+    }
+    ++n, ++done;
+  }
+  if (to) *to = value;
+}
+
+// A workgroup's sums to where they go.
+__device__ __forceinline__ void finish_sums(const WeighArgs& a, int page_begin, int first, int n_tok, int partial, int hk, const float* sums) {
+  for (int t = threadIdx.x; t < n_tok; t += kWeighThreads) {
+    if (partial >= 0) {
+      a.partials[hk * a.n_partials + partial + t] = sums[t];
+    } else {
+      const long long to = hk * a.num_slots + weigh_slot(a, page_begin, first + t);
+      a.weights_out[to] = a.weights_in[to] + sums[t];
+    }
+  }
 }
 
 // What the keys of a pool are in the products of the tiles: float16, and a factor of each token on its scores.  16-bit keys come
@@ -747,9 +800,9 @@ constexpr int kWeighBatch = 4;  // rows of a wave at a time
 template <typename C>
 __global__ __launch_bounds__(kWeighThreads) void weigh_generic_kernel(WeighArgs a) {
   extern __shared__ float lds[];  // [64 tokens][D + 1], then [waves][64]
-  const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
-  const int32_t* item = a.items + (long long)where.item * VA_WEIGH_ITEM_WORDS;
-  const int n_tok = item[VA_WI_N_TOK], hk = where.head, D = a.head_dim;
+  const int hk = (int)(blockIdx.x % (unsigned)a.num_kv_heads);
+  const int32_t* item = a.items + (long long)(blockIdx.x / (unsigned)a.num_kv_heads) * VA_WEIGH_ITEM_WORDS;
+  const int n_tok = item[VA_WI_N_TOK], D = a.head_dim;
   if (n_tok == 0) return;
   const int page_begin = item[VA_WI_PAGES], first = item[VA_WI_FIRST], partial = item[VA_WI_PARTIAL];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -838,7 +891,7 @@ static void launch_rows(const WeighArgs& a, bool fast, hipStream_t stream) {
 }
 
 template <int kD, typename C>
-static int launch_matrix(const WeighArgs& a, int layout, int n_items, bool fast, hipStream_t stream) {
+static int launch_matrix(const WeighArgs& a, int layout, int n_items, int n_strips, bool fast, hipStream_t stream) {
   const dim3 grid((unsigned)n_items * (unsigned)a.num_kv_heads), block(kWeighThreads);
   if constexpr (!std::is_same_v<C, F32>) {
     if (layout == VA_WEIGH_TILES) {
@@ -852,20 +905,20 @@ static int launch_matrix(const WeighArgs& a, int layout, int n_items, bool fast,
   const hipError_t e = allow_lds(reinterpret_cast<const void*>(&weigh_walk_kernel<kD, C>), Sh::kLdsBytes, devices);
   if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
   launch_rows<WalkKeys<C>::kRows>(a, fast, stream);
-  hipLaunchKernelGGL((weigh_walk_kernel<kD, C>), grid, block, Sh::kLdsBytes, stream, a);
+  hipLaunchKernelGGL((weigh_walk_kernel<kD, C>), dim3((unsigned)n_strips * (unsigned)a.num_kv_heads), block, Sh::kLdsBytes, stream, a);
   return weigh_launched("attention weights");
 }
 
 template <typename C>
-static int launch_weigh(const WeighArgs& a, int layout, int n_items, bool matrix, bool fast, hipStream_t stream) {
+static int launch_weigh(const WeighArgs& a, int layout, int n_items, int n_strips, bool matrix, bool fast, hipStream_t stream) {
   if (matrix) {
     switch (a.head_dim) {
       case 64:
-        return launch_matrix<64, C>(a, layout, n_items, fast, stream);
+        return launch_matrix<64, C>(a, layout, n_items, n_strips, fast, stream);
       case 128:
-        return launch_matrix<128, C>(a, layout, n_items, fast, stream);
+        return launch_matrix<128, C>(a, layout, n_items, n_strips, fast, stream);
       default:
-        return launch_matrix<256, C>(a, layout, n_items, fast, stream);
+        return launch_matrix<256, C>(a, layout, n_items, n_strips, fast, stream);
     }
   }
   const dim3 grid((unsigned)n_items * (unsigned)a.num_kv_heads), block(kWeighThreads);
@@ -897,6 +950,7 @@ static int weigh(WeighArgs& a, int code_type, int num_pages, const int32_t* plan
   if (!workspace || (uintptr_t)workspace % 16) return va_fail(VA_ERR_ARG, "the workspace must lie on a 16-byte boundary");
   if (hkv > 65535 || h[VA_WH_N_JOINS] < 0) return va_fail(VA_ERR_ARG, "too many heads for one launch");
   a.items = plan_dev + h[VA_WH_OFF_ITEMS];
+  a.strips = plan_dev + h[VA_WH_OFF_STRIPS];
   a.joins = plan_dev + h[VA_WH_OFF_JOINS];
   a.pages = plan_dev + h[VA_WH_OFF_PAGES];
   a.sub_rows = plan_dev + h[VA_WH_OFF_ROWS];
@@ -921,19 +975,19 @@ static int weigh(WeighArgs& a, int code_type, int num_pages, const int32_t* plan
   const int layout = h[VA_WH_LAYOUT];
   if (layout == VA_WEIGH_TILES && shape->dtype == VA_F32) return va_fail(VA_ERR_ARG, "plan header: no tiles over 32-bit rows");
   if (code_type == VA_CODE_E4M3) {
-    rc = launch_weigh<E4M3>(a, layout, n_items, matrix, fast, stream);
+    rc = launch_weigh<E4M3>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
   } else if (code_type == VA_CODE_INT8) {
-    rc = launch_weigh<INT8>(a, layout, n_items, matrix, fast, stream);
+    rc = launch_weigh<INT8>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
   } else {
     switch (shape->dtype) {
       case VA_F32:
-        rc = launch_weigh<F32>(a, layout, n_items, matrix, fast, stream);
+        rc = launch_weigh<F32>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       case VA_F16:
-        rc = launch_weigh<F16>(a, layout, n_items, matrix, fast, stream);
+        rc = launch_weigh<F16>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       case VA_BF16:
-        rc = launch_weigh<BF16>(a, layout, n_items, matrix, fast, stream);
+        rc = launch_weigh<BF16>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       default:
         rc = va_fail(VA_ERR_ARG, "unknown dtype %d", (int)shape->dtype);

@@ -151,50 +151,106 @@ struct Planner {
     return halves && products >= 8 * tokens;
   }
 
+  std::vector<int32_t> strips;
+
   int make_items() {
-    const int G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G);
+    const int G = shape.num_q_heads / shape.num_kv_heads;
     int64_t tokens = 0, products = 0;  // products: (token, tile of rows)
     for (const Span& s : spans) tokens += s.end - s.first, products += (int64_t)(s.end - s.first) * ((s.row_end - s.row_begin) * G / 16);
     layout = many_rows(tokens, products) ? VA_WEIGH_TILES : VA_WEIGH_WALK;
-    // tokens of an item, and how many (token, tile)s it should have at most
-    int64_t T = VA_WEIGH_TILE_TOKENS, most;
-    if (layout == VA_WEIGH_TILES) {
-      most = std::max<int64_t>(8 * T, products * shape.num_kv_heads / 2048);
-    } else {
-      // a workgroup's four waves take a tile each: of 16 tokens or more, 16 KB
-      const int row = shape.head_dim * (shape.dtype == VA_F32 ? 4 : 2);
-      const int64_t least = 4 * 16 * std::clamp(1024 / std::max(row, 1), 1, 4);
-      T = least * std::clamp<int64_t>(tokens * shape.num_kv_heads / (least * 1536), 1, VA_WEIGH_MOST_TOKENS / least);
-      most = std::max<int64_t>(4 * T, products * shape.num_kv_heads / 1024);
+    if (const int rc = layout == VA_WEIGH_TILES ? make_tiles(products) : make_strips()) return rc;
+    if ((items.size() / VA_WEIGH_ITEM_WORDS + strips.size()) * (size_t)shape.num_kv_heads > INT32_MAX)
+      return va_fail(VA_ERR_ARG, "too many work items for one launch");
+    return VA_OK;
+  }
+
+  // The tiles of a span's rows that see any of its tokens [begin, end): they lie between these (a request's rows see ever more).
+  void tiles_of(const Span& s, int64_t begin, int64_t end, int64_t& tile_a, int64_t& tile_b) const {
+    const int G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G);
+    int64_t a = s.row_begin, b = s.row_end;
+    while (a < b && (hi[(size_t)a] <= begin || lo[(size_t)a] >= end)) ++a;
+    while (b > a && (hi[(size_t)b - 1] <= begin || lo[(size_t)b - 1] >= end)) --b;
+    tile_a = a / unit * unit * G / 16, tile_b = ((b + unit - 1) / unit * unit) * G / 16;
+    if (a == b) tile_b = tile_a;
+  }
+  // Tokens [begin, begin + n_tok) under tiles [tile_a, tile_b), in `parts` items: `each(part, item words)`.
+  template <typename F>
+  int put_items(const Span& s, int64_t begin, int n_tok, int64_t tile_a, int64_t tile_b, int64_t parts, F&& each) {
+    if (parts > 1) {
+      if (n_partials + parts * n_tok > INT32_MAX) return va_fail(VA_ERR_ARG, "too many partial sums for one plan");
+      const int32_t join[VA_WEIGH_JOIN_WORDS] = {(int32_t)s.page_begin, (int32_t)begin, n_tok, (int32_t)n_partials, (int32_t)parts, 0, 0, 0};
+      joins.insert(joins.end(), join, join + VA_WEIGH_JOIN_WORDS);
     }
+    for (int64_t p = 0; p < parts; ++p) {
+      each(p);
+      const int32_t item[VA_WEIGH_ITEM_WORDS] = {(int32_t)s.page_begin, (int32_t)begin, n_tok, (int32_t)(tile_a + (tile_b - tile_a) * p / parts),
+                                                 (int32_t)(tile_a + (tile_b - tile_a) * (p + 1) / parts),
+                                                 parts > 1 ? (int32_t)(n_partials + p * n_tok) : -1, 0, 0};
+      items.insert(items.end(), item, item + VA_WEIGH_ITEM_WORDS);
+    }
+    if (parts > 1) n_partials += parts * n_tok;
+    return VA_OK;
+  }
+
+  int make_tiles(int64_t products) {
+    const int64_t T = VA_WEIGH_TILE_TOKENS, most = std::max<int64_t>(8 * T, products * shape.num_kv_heads / 2048);
+    for (const Span& s : spans)
+      for (int64_t t = s.first; t < s.end; t += T) {
+        const int n_tok = (int)std::min<int64_t>(T, s.end - t);
+        int64_t tile_a, tile_b;
+        tiles_of(s, t, t + n_tok, tile_a, tile_b);
+        if (tile_a == tile_b) continue;
+        if (const int rc = put_items(s, t, n_tok, tile_a, tile_b, std::min((n_tok * (tile_b - tile_a) + most - 1) / most, tile_b - tile_a), [](int64_t) {})) return rc;
+      }
+    while (items.size() % (8 * VA_WEIGH_ITEM_WORDS)) items.push_back(0);
+    return VA_OK;
+  }
+
+  // Strips of equal cost, two workgroups a CU where there is that much: a token costs its key, and a quarter of that more for every
+  // further tile of rows.  Tokens are cut at multiples of what the waves of a workgroup take at a time.
+  int make_strips() {
+    constexpr int64_t kWorkgroups = 512, kKey = 4;
+    const int G = shape.num_q_heads / shape.num_kv_heads, row = shape.head_dim * (shape.dtype == VA_F32 ? 4 : 2);
+    const int64_t least = 4 * 16 * std::clamp(1024 / std::max(row, 1), 1, 4);
+    auto cost_of = [&](int64_t tiles) { return kKey + tiles - 1; };
+    int64_t total = 0, pieces = 0;
     for (const Span& s : spans) {
-      // (chunks start on multiples of 16 tokens of the span: pages of as many are read in runs)
-      for (int64_t t = s.first / 16 * 16; t < s.end; t += T) {
-        const int64_t begin = std::max<int64_t>(t, s.first);
-        const int n_tok = (int)(std::min<int64_t>(t + T, s.end) - begin);
-        // the rows that see any of it lie between these (a request's rows see ever more)
-        int64_t a = s.row_begin, b = s.row_end;
-        while (a < b && (hi[(size_t)a] <= begin || lo[(size_t)a] >= begin + n_tok)) ++a;
-        while (b > a && (hi[(size_t)b - 1] <= begin || lo[(size_t)b - 1] >= begin + n_tok)) --b;
-        if (a == b) continue;
-        const int64_t tile_a = a / unit * unit * G / 16, tile_b = ((b + unit - 1) / unit * unit) * G / 16;
-        const int64_t parts = std::min((n_tok * (tile_b - tile_a) + most - 1) / most, tile_b - tile_a);
-        if (parts > 1) {
-          if (n_partials + parts * n_tok > INT32_MAX) return va_fail(VA_ERR_ARG, "too many partial sums for one plan");
-          const int32_t join[VA_WEIGH_JOIN_WORDS] = {(int32_t)s.page_begin, (int32_t)begin, n_tok, (int32_t)n_partials, (int32_t)parts, 0, 0, 0};
-          joins.insert(joins.end(), join, join + VA_WEIGH_JOIN_WORDS);
+      const int64_t tiles = (s.row_end - s.row_begin) * G / 16;
+      total += (s.end - s.first) * cost_of(tiles);
+      pieces += ((int64_t)s.end - s.first + least - 1) / least * tiles;
+    }
+    const int64_t n = std::max<int64_t>(1, std::min(pieces, std::max<int64_t>(1, kWorkgroups / shape.num_kv_heads)));
+    const int64_t room = std::max<int64_t>(1, (total + n - 1) / n);  // cost of a strip
+    int64_t used = 0;
+    strips.push_back(0);
+    auto next_item = [&](int64_t cost) {  // opens another strip where this one has what it should
+      if (used > 0 && used + cost / 2 > room) strips.push_back((int32_t)(items.size() / VA_WEIGH_ITEM_WORDS)), used = 0;
+      used += cost;
+    };
+    for (const Span& s : spans) {
+      int64_t t = s.first;
+      while (t < s.end) {
+        int64_t tile_a, tile_b;
+        tiles_of(s, t, s.end, tile_a, tile_b);
+        if (tile_a == tile_b) break;
+        const int64_t cost = cost_of(tile_b - tile_a);
+        // as many tokens as the strip has room for, to the nearest cut; rows are split where the least number costs more than a strip
+        int64_t parts = std::min(tile_b - tile_a, std::max<int64_t>(1, std::min<int64_t>(least, s.end - t) * cost / room));
+        int64_t n_tok = least;
+        if (parts == 1) {
+          if (used > 0 && used + least * cost / 2 > room) strips.push_back((int32_t)(items.size() / VA_WEIGH_ITEM_WORDS)), used = 0;
+          n_tok = std::max<int64_t>(1, ((room - used) / cost + least / 2) / least) * least;
         }
-        for (int64_t p = 0; p < parts; ++p) {
-          const int32_t item[VA_WEIGH_ITEM_WORDS] = {(int32_t)s.page_begin, (int32_t)begin, n_tok, (int32_t)(tile_a + (tile_b - tile_a) * p / parts),
-                                                     (int32_t)(tile_a + (tile_b - tile_a) * (p + 1) / parts),
-                                                     parts > 1 ? (int32_t)(n_partials + p * n_tok) : -1, 0, 0};
-          items.insert(items.end(), item, item + VA_WEIGH_ITEM_WORDS);
-        }
-        if (parts > 1) n_partials += parts * n_tok;
+        // (chunks start on multiples of 16 tokens of the span: pages of as many are read in runs)
+        const int64_t end = std::min<int64_t>(s.end, (t + n_tok) / 16 * 16);
+        const int rc = put_items(s, t, (int)(end - t), tile_a, tile_b, parts,
+                                 [&](int64_t) { parts == 1 ? (void)(used += (end - t) * cost) : next_item((end - t) * (cost / parts)); });
+        if (rc) return rc;
+        t = end;
       }
     }
-    while (items.size() % (8 * VA_WEIGH_ITEM_WORDS)) items.push_back(0);
-    if (items.size() / VA_WEIGH_ITEM_WORDS * (size_t)shape.num_kv_heads > INT32_MAX) return va_fail(VA_ERR_ARG, "too many work items for one launch");
+    strips.push_back((int32_t)(items.size() / VA_WEIGH_ITEM_WORDS));
+    while ((strips.size() - 1) % 8) strips.push_back(strips.back());
     return VA_OK;
   }
 };
@@ -211,7 +267,7 @@ int build(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, in
   p.find_visitors();
   if ((rc = p.find_spans()) || (rc = p.make_items())) return rc;
   const int64_t n_rows = (int64_t)p.sub_row.size();
-  const int64_t words = VA_WEIGH_HEADER_WORDS + (int64_t)p.items.size() + (int64_t)p.joins.size() + (int64_t)p.pages.size() + 3 * n_rows;
+  const int64_t words = VA_WEIGH_HEADER_WORDS + (int64_t)p.items.size() + (int64_t)p.joins.size() + (int64_t)p.strips.size() + (int64_t)p.pages.size() + 3 * n_rows;
   if (words > INT32_MAX) return va_fail(VA_ERR_ARG, "too large a plan");
   const int64_t pairs = n_rows * (shape->num_q_heads / shape->num_kv_heads);
   counts->n_items = (int32_t)(p.items.size() / VA_WEIGH_ITEM_WORDS);
@@ -239,6 +295,8 @@ int build(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, in
   h[VA_WH_N_PAGES] = (int32_t)p.pages.size();
   h[VA_WH_OFF_ITEMS] = put(p.items);
   h[VA_WH_OFF_JOINS] = put(p.joins);
+  h[VA_WH_N_STRIPS] = std::max((int32_t)p.strips.size() - 1, 0);
+  h[VA_WH_OFF_STRIPS] = put(p.strips);
   h[VA_WH_OFF_PAGES] = put(p.pages);
   h[VA_WH_OFF_ROWS] = put(p.sub_row);
   put(p.lo);

@@ -569,7 +569,7 @@ VA_API int va_move_kv_q8(const VaQuantPool* pool, int64_t code_layer_stride, int
  * (VA_F32, head_dim up to 256) on the vector ALU.
  */
 typedef struct VaWeighCounts {
-  int32_t n_items;   /* work items (a workgroup per kv head) incl. padding to a multiple of 8 */
+  int32_t n_items;   /* work items, padding included                                         */
   int32_t n_rows;    /* query rows, once for every span that they see                        */
   int32_t n_joins;   /* chunks of tokens whose rows are split among items                    */
   int32_t n_spans;   /* runs of pages with the same readers                                  */

@@ -11,8 +11,6 @@ from async_llm_amd import native
 from async_llm_amd.shared_cache import CacheEviction, SharedCacheAttention
 from async_llm_amd.kvcache import MHAKVCache
 
-CHUNK = 2048
-
 
 def plan_of(subs, heads=(8, 2, 64), page=4, pages=64, window=0, capacity=None, dtype=native.VA_BF16):
     """``subs``: (rows, entries, seq_len, flags)."""
@@ -35,12 +33,15 @@ def counted(words, heads, page):
     pages = words[off[2]:]
     sub, lo, hi = (words[off[3] + i * n_rows: off[3] + (i + 1) * n_rows] for i in range(3))
     g = heads[0] // heads[1]
-    assert n_items % 8 == 0 and n_rows * g % 16 == 0
+    layout, n_strips, strips = h[17], h[18], words[h[19]: h[19] + h[18] + 1]
+    assert n_rows * g % 16 == 0 and (layout == 0 or n_items % 8 == 0)
+    if layout == 0 and n_items:  # walks: strips hold every item once
+        assert n_strips % 8 == 0 and strips[0] == 0 and strips[-1] == n_items and (np.diff(strips) >= 0).all()
     pairs, owners, parts = {}, {}, {}
     for first_page, first, n, begin, end, partial in items[:, :6]:
         if n == 0:
             continue
-        assert 0 < n <= CHUNK and 0 <= begin < end <= n_rows * g // 16
+        assert 0 < n <= (256 if layout else 1 << 20) and 0 <= begin < end <= n_rows * g // 16
         slots = [int(pages[first_page + t // page]) * page + t % page for t in range(first, first + n)]
         if partial >= 0:
             parts[int(partial)] = (int(first_page), int(first), int(n))
@@ -126,7 +127,28 @@ def test_readers_of_a_block_share_its_tokens():
     rc, words, counts = plan_of(subs, (8, 8, 64), 16, 300)
     assert rc == 0 and counts.n_spans == 5
     assert counts.n_rows == 16 * 5  # a row an q head: whole tiles of 16
-    assert counts.n_items == 16 and counts.n_joins == 0  # seven chunks of the prompt and four blocks, padded
+    assert counts.n_joins == 0
+    strips = np.diff(words[words[19]: words[19] + words[18] + 1])
+    tokens = words[words[6]: words[6] + 8 * counts.n_items].reshape(-1, 8)[:, 2]
+    assert tokens.sum() == 1600 + 4 * 150 and (strips <= 2).all()  # few items: workgroups for all
+
+
+def test_strips_cost_the_same():
+    """Long and short blocks, some with many readers, over as many workgroups as the GPU holds."""
+    r = random.Random(1)
+    free = list(range(20000))
+    prompt = [free.pop() for _ in range(512)]
+    subs = []
+    for _ in range(64):
+        subs.append((1, prompt, 8192, 0))
+        n = r.randint(20, 400)
+        subs.append((1, [free.pop() for _ in range(n)], n * 16 - r.randint(0, 15), 0))
+    rc, words, counts = plan_of(subs, (16, 4, 256), 16, 20000)
+    counted_strips = words[words[19]: words[19] + words[18] + 1]
+    items = words[words[6]: words[6] + 8 * counts.n_items].reshape(-1, 8)
+    cost = [sum(n * (3 + b - a) for _, _, n, a, b, *_ in items[s: e]) for s, e in zip(counted_strips, counted_strips[1:])]
+    cost = [c for c in cost if c]
+    assert rc == 0 and 120 <= len(cost) <= 130 and max(cost) < 1.15 * sum(cost) / len(cost)
 
 
 def test_rows_are_split_where_tokens_are_few():
