@@ -12,17 +12,14 @@
 #define VA_WEIGH_ITEM_WORDS 8
 #define VA_WEIGH_JOIN_WORDS 8
 
-// How a launch's work is laid out.
-enum {
-  VA_WEIGH_WALK = 0,   // few rows a token: bound by the keys; a workgroup walks a strip of items (weigh_walk_kernel)
-  VA_WEIGH_TILES = 1,  // many rows a token: bound by the products; items are VA_WEIGH_TILE_TOKENS tokens and many rows (weigh_tile_kernel)
-};
+// Spans whose tokens have more than one tile of 16 (row, q head) pairs are cut into tile items of this many tokens (16-bit rows and
+// codes, head dims of the matrix cores), the others into items of strips: see va_weigh.hip.
 #define VA_WEIGH_TILE_TOKENS 256
 
 // header word indices
 enum {
   VA_WH_MAGIC = 0,
-  VA_WH_N_ITEMS,   // tiles: a multiple of 8, padding included
+  VA_WH_N_ITEMS,   // tile items first, then those of strips
   VA_WH_N_ROWS,    // packed rows: a multiple of what makes whole tiles of 16 (row, q head) pairs
   VA_WH_N_JOINS,
   VA_WH_N_PARTIALS,  // partial sums, in tokens (per kv head)
@@ -36,10 +33,12 @@ enum {
   VA_WH_D,
   VA_WH_PAGE,
   VA_WH_DTYPE,
+  VA_WH_CODES,
   VA_WH_POOL_PAGES,
   VA_WH_N_SUBROWS,
-  VA_WH_LAYOUT,
-  VA_WH_N_STRIPS,  // walks: a multiple of 8
+  VA_WH_N_TILE_ITEMS,  // a multiple of 8, padding included
+  VA_WH_N_TILE_ROWS,   // packed rows of spans in tile items: the first ones
+  VA_WH_N_STRIPS,      // a multiple of 8
   VA_WH_OFF_STRIPS,  // [n_strips + 1]: strip s is the items [strips[s], strips[s + 1])
 };
 

@@ -9,11 +9,11 @@
 // bits) and each product is taken that often.  A first pass over the packed rows (weigh_rows_kernel) turns them, scales them by
 // log2(e) / sqrt(D) and writes those parts as the matrix cores read them.
 //
-// Two layouts of the work (va_weigh.h):
-//   * walks (weigh_walk_kernel): a token has few rows, as in decode steps.  Bound by the keys: they travel to LDS in whole lines,
-//     each wave's tiles in a ring of its own, while its tile before is at the products.
-//   * tiles (weigh_tile_kernel): a token has many rows, as for many new tokens.  Bound by the products: 64 tokens' keys stay in a
-//     wave's registers while the rows' queries pass by through LDS, for all four waves at once.
+// Two ways, by span (va_weigh.h), in one launch where a step has both:
+//   * strips (weigh_strip): the rows that see a token make one tile of 16, as in decode steps.  Bound by the keys: they travel to LDS
+//     in whole lines, each wave's tiles in a ring of its own, while its tile before is at the products.
+//   * tile items (weigh_tiles): many rows see a token, as those of many new tokens.  Bound by the products: 64 tokens' keys stay
+//     in a wave's registers while the rows' queries pass by through LDS, for all four waves at once.
 // Where a chunk's rows are split among workgroups each writes partial sums, and weigh_join_kernel adds them in their order.
 #include <hip/hip_runtime.h>
 
@@ -52,6 +52,7 @@ struct WeighArgs {
   const int32_t* lo;
   const int32_t* hi;
   int n_rows, n_tiles;
+  int n_first_tiles;  // tiles of rows of tile items, the first ones
   const int64_t* sub_worker;
   const int64_t* sub_loc;
   long long sub_loc_axis_stride;
@@ -92,7 +93,7 @@ __device__ __forceinline__ uint32_t weigh_slot(const WeighArgs& a, int page_begi
 // hold the keys: piece 4 step + group, or over codes, of which a lane reads 16 at once, 8 (step / 2) + 2 group + step % 2.
 enum RowKind { kPlain32, kParts32, kPartsF16, kPartsBF16, kCodesF16, kCodesBF16 };
 __host__ __device__ constexpr int parts_of(int kind) { return kind == kPartsF16 || kind == kCodesF16 ? 2 : kind == kPartsBF16 || kind == kCodesBF16 ? 3 : 1; }
-__host__ __device__ constexpr int tile_bytes_of(int kind, int dim) { return 16 * dim * (kind <= kParts32 ? 4 : 2 * parts_of(kind)); }
+__host__ __device__ constexpr int tile_bytes(int dim) { return 16 * dim * 6; }  // (room for any of them)
 
 // Eight neighbouring elements of a row, piece `piece` of row j (32-bit: pieces 2 piece and 2 piece + 1); y is used up.
 template <int kKind>
@@ -162,7 +163,7 @@ __device__ __forceinline__ void weigh_activations8(const void* x, long long at, 
 // A thread per 16 elements of a row: both halves of eight pairs, or two pieces past the rotary part.  head_dim 64, 128 or 256 and
 // rotary_dim a multiple of 16.
 template <int kKind>
-__global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighArgs a) {
+__device__ __forceinline__ void weigh_row_units(const WeighArgs& a) {
   const int D = a.head_dim, units = D / 16, G = a.num_q_heads / a.num_kv_heads, hk = blockIdx.y;
   const int task = blockIdx.x * kWeighThreads + threadIdx.x, pair = task / units, x = task - pair * units;
   if (pair >= a.n_tiles * 16) return;  // (whole rows leave)
@@ -195,16 +196,25 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighArgs a) 
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[0][i] *= power_of_two(e), y[1][i] *= power_of_two(e);
   }
-  char* at = a.queries + ((long long)hk * a.n_tiles + pair / 16) * tile_bytes_of(kKind, D);
+  char* at = a.queries + ((long long)hk * a.n_tiles + pair / 16) * tile_bytes(D);
   write_row_piece<kKind>(at, D, pair % 16, d0 / 8, y[0]);
   write_row_piece<kKind>(at, D, pair % 16, d1 / 8, y[1]);
   if (x == 0) a.rows[(long long)hk * a.n_tiles * 16 + pair] = row_beside(a, row, counts, lse, scale);
 }
+// kFirst: what the rows of tile items become, the others kKind.  (A wave's rows are of one kind: 16 of them are a wave or more.)
+template <int kFirst, int kKind>
+__global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighArgs a) {
+  if constexpr (kFirst == kKind) {
+    weigh_row_units<kKind>(a);
+  } else {
+    const int wave = blockIdx.x * kWeighWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if ((long long)wave * kWave / (a.head_dim / 16) < (long long)a.n_first_tiles * 16) weigh_row_units<kFirst>(a); else weigh_row_units<kKind>(a);
+  }
+}
 
 // Any head_dim up to kWeighMaxDim and any rotary_dim: a tile a workgroup, through LDS.
 template <int kKind>
-__global__ __launch_bounds__(kWeighThreads) void weigh_rows_any_kernel(WeighArgs a) {
-  __shared__ float x[16][kWeighMaxDim + 1];
+__device__ __forceinline__ void weigh_row_tile(const WeighArgs& a, float (&x)[16][kWeighMaxDim + 1]) {
   const int tile = blockIdx.x, hk = blockIdx.y, D = a.head_dim, G = a.num_q_heads / a.num_kv_heads;
   const int j = threadIdx.x / 16, c = threadIdx.x % 16;
   const int pair = tile * 16 + j, row = pair / G, hq = hk * G + pair - row * G;
@@ -239,7 +249,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_any_kernel(WeighArgs
     const int e = row_exponent(most);
     up = power_of_two(e), scale = power_of_two(-e);
   }
-  char* at = a.queries + ((long long)hk * a.n_tiles + tile) * tile_bytes_of(kKind, D);
+  char* at = a.queries + ((long long)hk * a.n_tiles + tile) * tile_bytes(D);
   if constexpr (kKind == kPlain32) {
     for (int d = c; d < D; d += 16) ((float*)at)[j * D + d] = x[j][d];
   } else {
@@ -251,6 +261,11 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_any_kernel(WeighArgs
     }
   }
   if (c == 0) a.rows[(long long)hk * a.n_tiles * 16 + pair] = row_beside(a, row, counts, lse, scale);
+}
+template <int kFirst, int kKind>
+__global__ __launch_bounds__(kWeighThreads) void weigh_rows_any_kernel(WeighArgs a) {
+  __shared__ float x[16][kWeighMaxDim + 1];
+  if (kFirst != kKind && (int)blockIdx.x < a.n_first_tiles) weigh_row_tile<kFirst>(a, x); else weigh_row_tile<kKind>(a, x);
 }
 
 // ---------------------------------------------------------------------------
@@ -327,8 +342,10 @@ struct WalkShape {
   static constexpr int kTileBytes = kSlotsAt + 256;
   static constexpr int kBuffers = kTileBytes > 10 * 1024 ? 1 : 2;
   static constexpr int kTileLoads = kGroups * kLoads + (K::kCodes ? 2 : 1);  // what the counter of outstanding loads sees of a tile
-  static constexpr int kTurnOffset = kWeighWaves * kBuffers * kTileBytes;  // where a wave turns a tile's sums from lanes to tokens
-  static constexpr int kLdsBytes = kTurnOffset + kWeighWaves * 256;
+  // behind the rings: where a wave turns a tile's sums from lanes to tokens, and holds those of several tiles with their places
+  static constexpr int kTurnOffset = kWeighWaves * kBuffers * kTileBytes, kHold = 256;
+  static constexpr int kWaveBytes = 256 + kHold * 8;
+  static constexpr int kLdsBytes = kTurnOffset + kWeighWaves * kWaveBytes;
   static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups share the LDS of a CU");
   static_assert((kBuffers - 1) * kTileLoads < kAnyInFlight, "the counter of outstanding loads");
 };
@@ -343,24 +360,28 @@ __device__ __forceinline__ int walk_swz(int r) {
 // A workgroup walks a strip of items, its four waves on their own: each takes every fourth tile of an item's tokens, brings it
 // global -> LDS into a ring of its own (keys, the sums so far and, over codes, scales) and asks for the next one, of the next item
 // where this one ends, as soon as the keys are in registers.  There is no barrier, and nothing but the first tile of a strip
-// is waited for idly.
+// is waited for idly.  Sums are written some tiles at a time: a store is waited for with the keys asked for behind it, and one a
+// tile cost an eighth of the time.
 template <int kD, typename C>
-__global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs a) {
+__device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) {
   using Sh = WalkShape<kD, C>;
   using K = WalkKeys<C>;
   using Words = const __attribute__((address_space(4))) int32_t*;
   constexpr int kGroups = Sh::kGroups, kLoads = Sh::kLoads, kPieces = Sh::kPieces, kSteps = Sh::kSteps, kRaw = Sh::kRaw, kParts = Sh::kParts;
   constexpr int kTokens = Sh::kTokens, kBuffers = Sh::kBuffers;
+  constexpr bool kSeveral = std::is_same_v<C, F32>;  // tokens may have several tiles of rows
   extern __shared__ va_u32x4 smem[];
   char* lds = (char*)smem;
-  const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
+  const ItemHead where = item_and_head(block, a.num_kv_heads);
   const int hk = where.head, strip_begin = ((Words)a.strips)[where.item], strip_end = ((Words)a.strips)[where.item + 1];
   if (strip_begin == strip_end) return;
   const int lane = threadIdx.x % kWave, j = lane % 16, kg = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   char* own = lds + wave * kBuffers * Sh::kTileBytes;
   const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_address(own));
-  float* turn = (float*)(lds + Sh::kTurnOffset) + 64 * wave;
+  float* turn = (float*)(lds + Sh::kTurnOffset + wave * Sh::kWaveBytes);
+  float* held_sums = turn + 64;
+  uint32_t* held_places = (uint32_t*)(held_sums + Sh::kHold);
   const bool pages16 = a.page_map.shift >= 4;
   const long long row_bytes = K::kCodes ? kD : a.pool_row_stride * K::kBytes;
   const float* sums_in = a.weights_in + hk * a.num_slots;
@@ -448,10 +469,10 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
   // ---- queries ----
   va_u32x4 q[kParts][kSteps];
   WeighRow row;
-  const char* queries = a.queries + (long long)hk * a.n_tiles * tile_bytes_of(K::kRows, kD) + 16 * lane;
+  const char* queries = a.queries + (long long)hk * a.n_tiles * tile_bytes(kD) + 16 * lane;
   auto load_queries = [&](int tile) __attribute__((always_inline)) {
     row = a.rows[((long long)hk * a.n_tiles + tile) * 16 + j];
-    const char* at = queries + (long long)tile * tile_bytes_of(K::kRows, kD);
+    const char* at = queries + (long long)tile * tile_bytes(kD);
 #pragma unroll
     for (int p = 0; p < kParts; ++p)
 #pragma unroll
@@ -470,8 +491,16 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
   for (int b = 0; b < kBuffers; ++b) request_next();
   int done = 0, index = strip_begin, n = 0, q_tile = -1;
   Piece at = piece_at(strip_begin);
-  float* to = nullptr;  // the sums of the tile before, written behind the wait of this one
-  float value = 0.f;
+  int held = 0;  // sums not yet written, all of one kind
+  bool held_partial = false;
+  auto write_held = [&]() __attribute__((always_inline)) {
+    float* to = held_partial ? a.partials + hk * a.n_partials : a.weights_out + hk * a.num_slots;
+    for (int i = lane; i < held; i += kWave) {
+      const uint32_t place = held_places[i];
+      if (place != ~0u) to[place] = held_sums[i];
+    }
+    held = 0;
+  };
   while (true) {
     while (n == at.tiles) {
       if (index + 1 >= strip_end) break;
@@ -479,7 +508,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
       n = 0;
     }
     if (n == at.tiles) break;
-    const bool single = at.tile_end - at.tile_begin == 1;
+    const bool single = !kSeveral || at.tile_end - at.tile_begin == 1;
     if (single && at.tile_begin != q_tile) {
       load_queries(at.tile_begin);
       queries_here();
@@ -503,7 +532,8 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
     }
     const float before = *(const float*)(tile + Sh::kSumsAt + 4 * lane);
     const uint32_t slot = *(const uint32_t*)(tile + Sh::kSlotsAt + 4 * lane);
-    if (to) *to = value;
+    if (held + kTokens > Sh::kHold || held_partial != (at.partial >= 0)) write_held();
+    held_partial = at.partial >= 0;
     __builtin_amdgcn_sched_barrier(0);
     if (single) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -553,7 +583,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
     };
     if (single) {
       add_rows();
-    } else {
+    } else if constexpr (kSeveral) {
       // Queries are loaded tile by tile; a wait for those would be one for the next keys as well, which are asked for behind them.
       for (int of = at.tile_begin; of < at.tile_end; ++of) {
         load_queries(of);
@@ -569,23 +599,19 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_walk_kernel(WeighArgs 
       const float of_token = j == 0 ? sum[g][0] : j == 1 ? sum[g][1] : j == 2 ? sum[g][2] : sum[g][3];
       if (j < 4) turn[16 * g + 4 * kg + j] = of_token;
     }
-    value = turn[lane % kTokens];
-    to = nullptr;
-    if (lane < kTokens && t0 + lane < at.n_tok) {
-      if (at.partial < 0) {
-        value += before;
-        to = a.weights_out + hk * a.num_slots + slot;
-      } else {
-        to = a.partials + hk * a.n_partials + at.partial + t0 + lane;
-      }
+    if (lane < kTokens) {
+      const bool within = t0 + lane < at.n_tok;
+      held_sums[held + lane] = held_partial ? turn[lane] : before + turn[lane];
+      held_places[held + lane] = !within ? ~0u : held_partial ? (uint32_t)(at.partial + t0 + lane) : slot;
     }
+    held += kTokens;
     if (!single) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       request_next();
     }
     ++n, ++done;
   }
-  if (to) *to = value;
+  write_held();
 }
 
 // A workgroup's sums to where they go.
@@ -692,14 +718,14 @@ struct TileShape {
 };
 
 template <int kD, typename C>
-__global__ __launch_bounds__(kWeighThreads, 2) void weigh_tile_kernel(WeighArgs a) {
+__device__ __forceinline__ void weigh_tiles(const WeighArgs& a, unsigned block) {
   using Sh = TileShape<kD>;
   using K = TileKeys<kD, C>;
   using Words = const __attribute__((address_space(4))) int32_t*;
   constexpr int kGroups = Sh::kGroups, kSteps = Sh::kSteps, kParts = Sh::kParts, kLoads = Sh::kLoads;
   extern __shared__ va_u32x4 smem[];
   char* lds = (char*)smem;
-  const ItemHead where = item_and_head(blockIdx.x, a.num_kv_heads);
+  const ItemHead where = item_and_head(block, a.num_kv_heads);
   const Words item = (Words)a.items + (long long)where.item * VA_WEIGH_ITEM_WORDS;
   const int n_tok = item[VA_WI_N_TOK], hk = where.head;
   if (n_tok == 0) return;
@@ -708,13 +734,13 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_tile_kernel(WeighArgs 
   const int lane = threadIdx.x % kWave, j = lane % 16, kg = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_address(lds));
-  const char* queries = a.queries + ((long long)hk * a.n_tiles + tile_begin) * Sh::kQueryBytes + wave * (kLoads - 1) * 1024 + 16 * lane;
+  const char* queries = a.queries + ((long long)hk * a.n_tiles + tile_begin) * tile_bytes(kD) + wave * (kLoads - 1) * 1024 + 16 * lane;
   const WeighRow* rows = a.rows + ((long long)hk * a.n_tiles + tile_begin) * 16 + lane % 16;
   auto request = [&](int i) __attribute__((always_inline)) {
     const uint32_t dst = lds_base + (uint32_t)(i % Sh::kBuffers) * Sh::kBufferBytes;
 #pragma unroll
     for (int u = 0; u < kLoads - 1; ++u)
-      load_to_lds(queries + (long long)i * Sh::kQueryBytes + 1024 * u, dst + (uint32_t)(wave * (kLoads - 1) + u) * 1024);
+      load_to_lds(queries + (long long)i * tile_bytes(kD) + 1024 * u, dst + (uint32_t)(wave * (kLoads - 1) + u) * 1024);
     if (lane < 16) load_to_lds(rows + (long long)i * 16, dst + Sh::kQueryBytes + 256 * wave);
   };
 
@@ -792,6 +818,20 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_tile_kernel(WeighArgs 
   finish_sums(a, page_begin, first, n_tok, partial, hk, sums);
 }
 
+template <int kD, typename C>
+__global__ __launch_bounds__(kWeighThreads, 2) void weigh_strip_kernel(WeighArgs a) {
+  weigh_strip<kD, C>(a, blockIdx.x);
+}
+template <int kD, typename C>
+__global__ __launch_bounds__(kWeighThreads, 2) void weigh_tile_kernel(WeighArgs a) {
+  weigh_tiles<kD, C>(a, blockIdx.x);
+}
+// Both, tile items first.
+template <int kD, typename C>
+__global__ __launch_bounds__(kWeighThreads, 2) void weigh_both_kernel(WeighArgs a, unsigned tile_blocks) {
+  if (blockIdx.x < tile_blocks) weigh_tiles<kD, C>(a, blockIdx.x); else weigh_strip<kD, C>(a, blockIdx.x - tile_blocks);
+}
+
 // ---------------------------------------------------------------------------
 // vector ALU: any type, alignment and head_dim up to kWeighMaxDim
 // ---------------------------------------------------------------------------
@@ -827,7 +867,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_generic_kernel(WeighArgs 
     const int t_span = first + t0 + lane;
     float sum = 0.f;
     for (int pair = item[VA_WI_TILE_BEGIN] * 16 + wave * kWeighBatch; pair < item[VA_WI_TILE_END] * 16; pair += kWeighWaves * kWeighBatch) {
-      const float* q = (const float*)a.queries + ((long long)hk * a.n_tiles * 16 + pair) * D;
+      const float* q = (const float*)(a.queries + ((long long)hk * a.n_tiles + pair / 16) * tile_bytes(D)) + pair % 16 * D;
       float dots[kWeighBatch];
 #pragma unroll
       for (int u = 0; u < kWeighBatch; ++u) dots[u] = 0.f;
@@ -879,46 +919,56 @@ static int weigh_launched(const char* what) {
   return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }
 
-template <int kKind>
+template <int kFirst, int kKind>
 static void launch_rows(const WeighArgs& a, bool fast, hipStream_t stream) {
   const unsigned hkv = (unsigned)a.num_kv_heads;
   if (fast) {
     const long long tasks = (long long)a.n_tiles * 16 * (a.head_dim / 16);
-    hipLaunchKernelGGL(weigh_rows_kernel<kKind>, dim3((unsigned)((tasks + kWeighThreads - 1) / kWeighThreads), hkv), dim3(kWeighThreads), 0, stream, a);
+    hipLaunchKernelGGL((weigh_rows_kernel<kFirst, kKind>), dim3((unsigned)((tasks + kWeighThreads - 1) / kWeighThreads), hkv), dim3(kWeighThreads), 0, stream, a);
   } else {
-    hipLaunchKernelGGL(weigh_rows_any_kernel<kKind>, dim3((unsigned)a.n_tiles, hkv), dim3(kWeighThreads), 0, stream, a);
+    hipLaunchKernelGGL((weigh_rows_any_kernel<kFirst, kKind>), dim3((unsigned)a.n_tiles, hkv), dim3(kWeighThreads), 0, stream, a);
   }
 }
 
 template <int kD, typename C>
-static int launch_matrix(const WeighArgs& a, int layout, int n_items, int n_strips, bool fast, hipStream_t stream) {
-  const dim3 grid((unsigned)n_items * (unsigned)a.num_kv_heads), block(kWeighThreads);
-  if constexpr (!std::is_same_v<C, F32>) {
-    if (layout == VA_WEIGH_TILES) {
-      launch_rows<TileKeys<kD, C>::kRows>(a, fast, stream);
-      hipLaunchKernelGGL((weigh_tile_kernel<kD, C>), grid, block, TileShape<kD>::kLdsBytes, stream, a);
+static int launch_matrix(const WeighArgs& a, int n_tile_items, int n_strips, bool fast, hipStream_t stream) {
+  const unsigned tiles = (unsigned)n_tile_items * (unsigned)a.num_kv_heads, strips = (unsigned)n_strips * (unsigned)a.num_kv_heads;
+  const dim3 block(kWeighThreads);
+  using Sh = WalkShape<kD, C>;
+  if constexpr (std::is_same_v<C, F32>) {
+    launch_rows<kParts32, kParts32>(a, fast, stream);
+  } else {
+    launch_rows<TileKeys<kD, C>::kRows, WalkKeys<C>::kRows>(a, fast, stream);
+    if (strips == 0) {
+      hipLaunchKernelGGL((weigh_tile_kernel<kD, C>), dim3(tiles), block, TileShape<kD>::kLdsBytes, stream, a);
+      return weigh_launched("attention weights");
+    }
+    if (tiles > 0) {
+      constexpr int bytes = Sh::kLdsBytes > TileShape<kD>::kLdsBytes ? Sh::kLdsBytes : TileShape<kD>::kLdsBytes;
+      static std::atomic<unsigned long long> devices{0};
+      const hipError_t e = allow_lds(reinterpret_cast<const void*>(&weigh_both_kernel<kD, C>), bytes, devices);
+      if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
+      hipLaunchKernelGGL((weigh_both_kernel<kD, C>), dim3(tiles + strips), block, bytes, stream, a, tiles);
       return weigh_launched("attention weights");
     }
   }
-  using Sh = WalkShape<kD, C>;
   static std::atomic<unsigned long long> devices{0};
-  const hipError_t e = allow_lds(reinterpret_cast<const void*>(&weigh_walk_kernel<kD, C>), Sh::kLdsBytes, devices);
+  const hipError_t e = allow_lds(reinterpret_cast<const void*>(&weigh_strip_kernel<kD, C>), Sh::kLdsBytes, devices);
   if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
-  launch_rows<WalkKeys<C>::kRows>(a, fast, stream);
-  hipLaunchKernelGGL((weigh_walk_kernel<kD, C>), dim3((unsigned)n_strips * (unsigned)a.num_kv_heads), block, Sh::kLdsBytes, stream, a);
+  hipLaunchKernelGGL((weigh_strip_kernel<kD, C>), dim3(strips), block, Sh::kLdsBytes, stream, a);
   return weigh_launched("attention weights");
 }
 
 template <typename C>
-static int launch_weigh(const WeighArgs& a, int layout, int n_items, int n_strips, bool matrix, bool fast, hipStream_t stream) {
+static int launch_weigh(const WeighArgs& a, int n_items, int n_tile_items, int n_strips, bool matrix, bool fast, hipStream_t stream) {
   if (matrix) {
     switch (a.head_dim) {
       case 64:
-        return launch_matrix<64, C>(a, layout, n_items, n_strips, fast, stream);
+        return launch_matrix<64, C>(a, n_tile_items, n_strips, fast, stream);
       case 128:
-        return launch_matrix<128, C>(a, layout, n_items, n_strips, fast, stream);
+        return launch_matrix<128, C>(a, n_tile_items, n_strips, fast, stream);
       default:
-        return launch_matrix<256, C>(a, layout, n_items, n_strips, fast, stream);
+        return launch_matrix<256, C>(a, n_tile_items, n_strips, fast, stream);
     }
   }
   const dim3 grid((unsigned)n_items * (unsigned)a.num_kv_heads), block(kWeighThreads);
@@ -926,7 +976,7 @@ static int launch_weigh(const WeighArgs& a, int layout, int n_items, int n_strip
   static std::atomic<unsigned long long> devices{0};
   const hipError_t e = allow_lds(reinterpret_cast<const void*>(&weigh_generic_kernel<C>), (64 * (kWeighMaxDim + 1) + 64 * kWeighWaves) * 4, devices);
   if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
-  launch_rows<kPlain32>(a, false, stream);
+  launch_rows<kPlain32, kPlain32>(a, false, stream);
   hipLaunchKernelGGL(weigh_generic_kernel<C>, grid, block, (unsigned)bytes, stream, a);
   return weigh_launched("attention weights");
 }
@@ -935,7 +985,7 @@ static int weigh(WeighArgs& a, int code_type, int num_pages, const int32_t* plan
                  const VaShape* shape, const VaRope* rope, hipStream_t stream) {
   if (!h || h[VA_WH_MAGIC] != VA_WEIGH_MAGIC) return va_fail(VA_ERR_ARG, "not a plan of attention weights");
   if (h[VA_WH_HQ] != shape->num_q_heads || h[VA_WH_HKV] != shape->num_kv_heads || h[VA_WH_D] != shape->head_dim ||
-      h[VA_WH_PAGE] != shape->page_size || h[VA_WH_DTYPE] != shape->dtype || (num_pages >= 0 && h[VA_WH_POOL_PAGES] != num_pages))
+      h[VA_WH_PAGE] != shape->page_size || h[VA_WH_DTYPE] != shape->dtype || h[VA_WH_CODES] != (code_type >= 0) || (num_pages >= 0 && h[VA_WH_POOL_PAGES] != num_pages))
     return va_fail(VA_ERR_ARG, "the plan was made for another shape or pool");
   const int n_items = h[VA_WH_N_ITEMS];
   if (n_items == 0) return VA_OK;
@@ -972,22 +1022,22 @@ static int weigh(WeighArgs& a, int code_type, int num_pages, const int32_t* plan
   const bool matrix = dims && (code_type >= 0 || (a.pool_row_stride * size % 16 == 0 && (uintptr_t)a.k_pool % 16 == 0 && a.pool_row_stride < 1 << 24));
   const bool fast = a.rope.rotary_dim % 16 == 0 && (a.rope.mode != VA_ROPE_TABLE || (uintptr_t)a.rope.cos_sin % 16 == 0);
   a.pieces = a.q_row_stride * size % 16 == 0 && (uintptr_t)a.q % 16 == 0;
-  const int layout = h[VA_WH_LAYOUT];
-  if (layout == VA_WEIGH_TILES && shape->dtype == VA_F32) return va_fail(VA_ERR_ARG, "plan header: no tiles over 32-bit rows");
+  const int n_tile_items = h[VA_WH_N_TILE_ITEMS];
+  a.n_first_tiles = (int)((int64_t)h[VA_WH_N_TILE_ROWS] * G / 16);
   if (code_type == VA_CODE_E4M3) {
-    rc = launch_weigh<E4M3>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+    rc = launch_weigh<E4M3>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
   } else if (code_type == VA_CODE_INT8) {
-    rc = launch_weigh<INT8>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+    rc = launch_weigh<INT8>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
   } else {
     switch (shape->dtype) {
       case VA_F32:
-        rc = launch_weigh<F32>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+        rc = launch_weigh<F32>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       case VA_F16:
-        rc = launch_weigh<F16>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+        rc = launch_weigh<F16>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       case VA_BF16:
-        rc = launch_weigh<BF16>(a, layout, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+        rc = launch_weigh<BF16>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       default:
         rc = va_fail(VA_ERR_ARG, "unknown dtype %d", (int)shape->dtype);

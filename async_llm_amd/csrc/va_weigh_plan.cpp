@@ -21,8 +21,9 @@ struct Visitor {
 struct Planner {
   const VaSubRequests& in;
   const VaShape& shape;
+  bool rows32;  // 32-bit keys
   int num_pages, window;
-  Planner(const VaSubRequests& s, const VaShape& sh, int pages_, int w) : in(s), shape(sh), num_pages(pages_), window(w) {}
+  Planner(const VaSubRequests& s, const VaShape& sh, bool wide, int pages_, int w) : in(s), shape(sh), rows32(wide), num_pages(pages_), window(w) {}
   std::vector<int64_t> first_visitor;  // by page, [num_pages + 1]
   std::vector<Visitor> visitors;
   std::vector<int32_t> pages, items, joins, sub_row, lo, hi;
@@ -94,36 +95,12 @@ struct Planner {
     int64_t row_begin, row_end;  // packed
   };
   std::vector<Span> spans;
+  std::vector<int32_t> run_pages;  // pages by span, before it is known which spans come first
+  std::vector<int64_t> run_begin;
 
-  int close(const std::vector<int32_t>& run) {
-    const int P = shape.page_size, G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G);
-    const int64_t room = (int64_t)run.size() * P;
-    const int64_t row_begin = (int64_t)sub_row.size();
-    int64_t first = INT64_MAX, end = 0;
-    for (int64_t k = first_visitor[run[0]]; k < first_visitor[run[0] + 1]; ++k) {
-      const Visitor& v = visitors[(size_t)k];
-      for (int i = skipped(v.sub); i < rows_of(v.sub); ++i) {
-        int64_t from = 0, to = std::min(room, seen(v.sub, i) - (int64_t)v.entry * P);
-        if (v.place >= 0) from = v.place, to = seen(v.sub, i) > v.entry ? v.place + 1 : 0;
-        if (to <= from) continue;
-        sub_row.push_back(in.qo_indptr[v.sub] + i);
-        lo.push_back((int32_t)from);
-        hi.push_back((int32_t)to);
-        first = std::min(first, from), end = std::max(end, to);
-      }
-    }
-    if ((int64_t)sub_row.size() == row_begin) return VA_OK;
-    while (sub_row.size() % unit) sub_row.push_back(-1), lo.push_back(0), hi.push_back(0);
-    if ((int64_t)sub_row.size() * G > INT32_MAX / 16)  // (a thread for each 16 elements of a row)
-       return va_fail(VA_ERR_ARG, "too many query rows for one plan");
-    spans.push_back(Span{(int64_t)pages.size(), (int32_t)first, (int32_t)end, row_begin, (int64_t)sub_row.size()});
-    pages.insert(pages.end(), run.begin(), run.end());
-    return VA_OK;
-  }
-
-  int find_spans() {
+  void find_runs() {
     std::vector<char> done((size_t)num_pages, 0);
-    std::vector<int32_t> run;
+    int32_t before = -1;
     for (int s = 0; s < in.n_sub; ++s) {
       if (rows_of(s) == 0) continue;
       const int32_t* list = in.kv_indices + in.kv_indptr[s];
@@ -131,34 +108,71 @@ struct Planner {
         const int32_t page = slots(s) ? list[e] / shape.page_size : list[e];
         if (done[page]) continue;
         done[page] = 1;
-        // (tokens of a span are counted in 32 bits)
-        if (!run.empty() && !(follows(run.back(), page) && ((int64_t)run.size() + 1) * shape.page_size <= INT32_MAX)) {
-          if (const int rc = close(run)) return rc;
-          run.clear();
-        }
-        run.push_back(page);
+        if (before < 0 || !follows(before, page)) run_begin.push_back((int64_t)run_pages.size());
+        run_pages.push_back(before = page);
       }
     }
-    if (run.empty()) return VA_OK;
-    return close(run);
+    run_begin.push_back((int64_t)run_pages.size());
   }
 
-  int layout = VA_WEIGH_WALK;
-
-  // Walks where a token has few rows (tiles of 16 of them, on average over the tokens), else tiles.
-  bool many_rows(int64_t tokens, int64_t products) const {
-    const bool halves = shape.dtype != VA_F32 && (shape.head_dim == 64 || shape.head_dim == 128 || shape.head_dim == 256);
-    return halves && products >= 8 * tokens;
+  // Rows of a run's visitors that see any of it: `each(sub-row, first token, end)`.
+  template <typename F>
+  void rows_of_run(int64_t begin, int64_t end, F&& each) const {
+    const int P = shape.page_size;
+    const int64_t room = (end - begin) * P;  // (within the pool, whose slots 32 bits count)
+    const int32_t page = run_pages[(size_t)begin];
+    for (int64_t k = first_visitor[page]; k < first_visitor[page + 1]; ++k) {
+      const Visitor& v = visitors[(size_t)k];
+      for (int i = skipped(v.sub); i < rows_of(v.sub); ++i) {
+        int64_t from = 0, to = std::min(room, seen(v.sub, i) - (int64_t)v.entry * P);
+        if (v.place >= 0) from = v.place, to = seen(v.sub, i) > v.entry ? v.place + 1 : 0;
+        if (to > from) each(in.qo_indptr[v.sub] + i, (int32_t)from, (int32_t)to);
+      }
+    }
   }
 
+  size_t n_tile_spans = 0;
+  int64_t n_tile_rows = 0;
+
+  int find_spans() {
+    find_runs();
+    const int G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G);
+    const bool halves = !rows32 && (shape.head_dim == 64 || shape.head_dim == 128 || shape.head_dim == 256);
+    const size_t n = run_begin.size() - 1;
+    std::vector<char> many(n, 0);
+    for (size_t i = 0; i < n && halves; ++i) {
+      int64_t rows = 0;
+      rows_of_run(run_begin[i], run_begin[i + 1], [&](int32_t, int32_t, int32_t) { ++rows; });
+      many[i] = rows * G > 16;
+    }
+    for (int which = 1; which >= 0; --which) {  // those of tile items first
+      for (size_t i = 0; i < n; ++i) {
+        if (many[i] != which) continue;
+        const int64_t row_begin = (int64_t)sub_row.size();
+        int32_t first = INT32_MAX, end = 0;
+        rows_of_run(run_begin[i], run_begin[i + 1], [&](int32_t row, int32_t from, int32_t to) {
+          sub_row.push_back(row), lo.push_back(from), hi.push_back(to);
+          first = std::min(first, from), end = std::max(end, to);
+        });
+        if ((int64_t)sub_row.size() == row_begin) continue;
+        while (sub_row.size() % unit) sub_row.push_back(-1), lo.push_back(0), hi.push_back(0);
+        if ((int64_t)sub_row.size() * G > INT32_MAX / 16)  // (a thread for each 16 elements of a row)
+          return va_fail(VA_ERR_ARG, "too many query rows for one plan");
+        spans.push_back(Span{(int64_t)pages.size(), first, end, row_begin, (int64_t)sub_row.size()});
+        pages.insert(pages.end(), run_pages.begin() + run_begin[i], run_pages.begin() + run_begin[i + 1]);
+      }
+      if (which) n_tile_spans = spans.size(), n_tile_rows = (int64_t)sub_row.size();
+    }
+    return VA_OK;
+  }
+
+  static constexpr int64_t kWorkgroups = 512;  // that run at a time
   std::vector<int32_t> strips;
+  int64_t n_tile_items = 0;
 
   int make_items() {
-    const int G = shape.num_q_heads / shape.num_kv_heads;
-    int64_t tokens = 0, products = 0;  // products: (token, tile of rows)
-    for (const Span& s : spans) tokens += s.end - s.first, products += (int64_t)(s.end - s.first) * ((s.row_end - s.row_begin) * G / 16);
-    layout = many_rows(tokens, products) ? VA_WEIGH_TILES : VA_WEIGH_WALK;
-    if (const int rc = layout == VA_WEIGH_TILES ? make_tiles(products) : make_strips()) return rc;
+    if (const int rc = make_tiles()) return rc;
+    if (const int rc = make_strips()) return rc;
     if ((items.size() / VA_WEIGH_ITEM_WORDS + strips.size()) * (size_t)shape.num_kv_heads > INT32_MAX)
       return va_fail(VA_ERR_ARG, "too many work items for one launch");
     return VA_OK;
@@ -166,12 +180,11 @@ struct Planner {
 
   // The tiles of a span's rows that see any of its tokens [begin, end): they lie between these (a request's rows see ever more).
   void tiles_of(const Span& s, int64_t begin, int64_t end, int64_t& tile_a, int64_t& tile_b) const {
-    const int G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G);
+    const int G = shape.num_q_heads / shape.num_kv_heads;
     int64_t a = s.row_begin, b = s.row_end;
     while (a < b && (hi[(size_t)a] <= begin || lo[(size_t)a] >= end)) ++a;
     while (b > a && (hi[(size_t)b - 1] <= begin || lo[(size_t)b - 1] >= end)) --b;
-    tile_a = a / unit * unit * G / 16, tile_b = ((b + unit - 1) / unit * unit) * G / 16;
-    if (a == b) tile_b = tile_a;
+    tile_a = a * G / 16, tile_b = a == b ? tile_a : (b * G + 15) / 16;
   }
   // Tokens [begin, begin + n_tok) under tiles [tile_a, tile_b), in `parts` items: `each(part, item words)`.
   template <typename F>
@@ -192,42 +205,61 @@ struct Planner {
     return VA_OK;
   }
 
-  int make_tiles(int64_t products) {
-    const int64_t T = VA_WEIGH_TILE_TOKENS, most = std::max<int64_t>(8 * T, products * shape.num_kv_heads / 2048);
-    for (const Span& s : spans)
+  // Tile items of 256 tokens, with as many rows as make about 2048 workgroups of equal products, but not fewer than eight tiles, nor
+  // less than takes as long as a strip beside them (whose token takes about sixteen times as long as a token's one tile of rows).
+  int make_tiles() {
+    int64_t products = 0, walked = 0, tile_a, tile_b;  // (token, tile of rows); tokens of strips
+    for (size_t i = 0; i < spans.size(); ++i) {
+      const int64_t n = spans[i].end - spans[i].first;
+      if (i >= n_tile_spans) {
+        walked += n;
+      } else {
+        tiles_of(spans[i], spans[i].first, spans[i].end, tile_a, tile_b);
+        products += n * (tile_b - tile_a);
+      }
+    }
+    const int64_t T = VA_WEIGH_TILE_TOKENS, hkv = shape.num_kv_heads;
+    const int64_t most = std::max({8 * T, products * hkv / 2048, 16 * walked * hkv / kWorkgroups});
+    for (size_t i = 0; i < n_tile_spans; ++i) {
+      const Span& s = spans[i];
       for (int64_t t = s.first; t < s.end; t += T) {
         const int n_tok = (int)std::min<int64_t>(T, s.end - t);
-        int64_t tile_a, tile_b;
         tiles_of(s, t, t + n_tok, tile_a, tile_b);
         if (tile_a == tile_b) continue;
         if (const int rc = put_items(s, t, n_tok, tile_a, tile_b, std::min((n_tok * (tile_b - tile_a) + most - 1) / most, tile_b - tile_a), [](int64_t) {})) return rc;
       }
+    }
     while (items.size() % (8 * VA_WEIGH_ITEM_WORDS)) items.push_back(0);
+    n_tile_items = (int64_t)items.size() / VA_WEIGH_ITEM_WORDS;
     return VA_OK;
   }
 
   // Strips of equal cost, two workgroups a CU where there is that much: a token costs its key, and a quarter of that more for every
-  // further tile of rows.  Tokens are cut at multiples of what the waves of a workgroup take at a time.
+  // further tile of rows (of 32-bit rows, which have no tile items).  Tokens are cut at multiples of what the waves of a workgroup take at a time.
   int make_strips() {
-    constexpr int64_t kWorkgroups = 512, kKey = 4;
-    const int G = shape.num_q_heads / shape.num_kv_heads, row = shape.head_dim * (shape.dtype == VA_F32 ? 4 : 2);
+    constexpr int64_t kKey = 4;
+    const int row = shape.head_dim * (rows32 ? 4 : 2);
     const int64_t least = 4 * 16 * std::clamp(1024 / std::max(row, 1), 1, 4);
     auto cost_of = [&](int64_t tiles) { return kKey + tiles - 1; };
     int64_t total = 0, pieces = 0;
-    for (const Span& s : spans) {
-      const int64_t tiles = (s.row_end - s.row_begin) * G / 16;
-      total += (s.end - s.first) * cost_of(tiles);
-      pieces += ((int64_t)s.end - s.first + least - 1) / least * tiles;
+    if (n_tile_spans == spans.size()) return VA_OK;
+    for (size_t i = n_tile_spans; i < spans.size(); ++i) {
+      const Span& s = spans[i];
+      int64_t tile_a, tile_b;
+      tiles_of(s, s.first, s.end, tile_a, tile_b);
+      total += (s.end - s.first) * cost_of(tile_b - tile_a);
+      pieces += ((int64_t)s.end - s.first + least - 1) / least * (tile_b - tile_a);
     }
     const int64_t n = std::max<int64_t>(1, std::min(pieces, std::max<int64_t>(1, kWorkgroups / shape.num_kv_heads)));
     const int64_t room = std::max<int64_t>(1, (total + n - 1) / n);  // cost of a strip
     int64_t used = 0;
-    strips.push_back(0);
+    strips.push_back((int32_t)n_tile_items);
     auto next_item = [&](int64_t cost) {  // opens another strip where this one has what it should
       if (used > 0 && used + cost / 2 > room) strips.push_back((int32_t)(items.size() / VA_WEIGH_ITEM_WORDS)), used = 0;
       used += cost;
     };
-    for (const Span& s : spans) {
+    for (size_t i = n_tile_spans; i < spans.size(); ++i) {
+      const Span& s = spans[i];
       int64_t t = s.first;
       while (t < s.end) {
         int64_t tile_a, tile_b;
@@ -255,13 +287,13 @@ struct Planner {
   }
 };
 
-int build(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, int32_t window, int32_t* plan, int64_t capacity, VaWeighCounts* counts) {
+int build(const VaSubRequests* subs, const VaShape* shape, int32_t over_codes, int32_t num_pages, int32_t window, int32_t* plan, int64_t capacity, VaWeighCounts* counts) {
   if (!subs || !shape || !counts) return va_fail(VA_ERR_ARG, "null pointer");
   if (shape->num_kv_heads <= 0 || shape->num_q_heads <= 0 || shape->num_q_heads % shape->num_kv_heads || shape->head_dim <= 0 || shape->page_size <= 0)
     return va_fail(VA_ERR_ARG, "bad shape");
   if (num_pages < 0 || (int64_t)num_pages * shape->page_size > INT32_MAX || window < 0)
     return va_fail(VA_ERR_ARG, "%d pages of %d tokens, window %d", (int)num_pages, (int)shape->page_size, (int)window);
-  Planner p{*subs, *shape, num_pages, window};
+  Planner p{*subs, *shape, shape->dtype == VA_F32 && !over_codes, num_pages, window};
   int rc = p.check();
   if (rc) return rc;
   p.find_visitors();
@@ -302,17 +334,18 @@ int build(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, in
   put(p.lo);
   put(p.hi);
   h[VA_WH_HQ] = shape->num_q_heads, h[VA_WH_HKV] = shape->num_kv_heads, h[VA_WH_D] = shape->head_dim;
+  h[VA_WH_CODES] = over_codes != 0;
   h[VA_WH_PAGE] = shape->page_size, h[VA_WH_DTYPE] = shape->dtype, h[VA_WH_POOL_PAGES] = num_pages, h[VA_WH_N_SUBROWS] = subs->n_subrows;
-  h[VA_WH_LAYOUT] = p.layout;
+  h[VA_WH_N_TILE_ITEMS] = (int32_t)p.n_tile_items, h[VA_WH_N_TILE_ROWS] = (int32_t)p.n_tile_rows;
   return VA_OK;
 }
 
 }  // namespace
 
-extern "C" int va_weigh_plan(const VaSubRequests* subs, const VaShape* shape, int32_t num_pages, int32_t window, int32_t* plan_host,
+extern "C" int va_weigh_plan(const VaSubRequests* subs, const VaShape* shape, int32_t over_codes, int32_t num_pages, int32_t window, int32_t* plan_host,
                              int64_t plan_capacity_words, VaWeighCounts* counts) {
   try {
-    return build(subs, shape, num_pages, window, plan_host, plan_capacity_words, counts);
+    return build(subs, shape, over_codes, num_pages, window, plan_host, plan_capacity_words, counts);
   } catch (const std::exception& e) {  // (no memory: nothing may leave a C entry)
     return va_fail(VA_ERR_CAPACITY, "planning weights: %s", e.what());
   }

@@ -114,7 +114,7 @@ class CacheEviction:
         counts = native.VaWeighCounts()
         words = np.empty(1 << 14, dtype=np.int32)
         for _ in range(2):
-            rc = native.lib.va_weigh_plan(subs, self.op._shape, self.num_pages, window, words.ctypes.data, words.size, counts)
+            rc = native.lib.va_weigh_plan(subs, self.op._shape, int(self._coded), self.num_pages, window, words.ctypes.data, words.size, counts)
             if rc != native.VA_ERR_CAPACITY or counts.plan_words <= words.size:
                 break
             words = np.empty(counts.plan_words, dtype=np.int32)

@@ -92,7 +92,7 @@ def test_pages_and_writers_outside_their_views(dev, page, codes):
     check(op, decode_step(op, r, 6, [1, 3, 64, 129], shared=200, aside=True), gen)
 
 
-@pytest.mark.parametrize("dtype, codes", [(BF16, None), (F16, None), (F32, None), (BF16, INT8)])
+@pytest.mark.parametrize("dtype, codes", [(BF16, None), (F16, None), (F32, None), (BF16, INT8), (F32, E4M3)])
 @pytest.mark.parametrize("heads", [(8, 2, 128), (4, 4, 64), (6, 2, 256), (3, 1, 16)])
 @pytest.mark.parametrize("window", [0, 7])
 def test_chunks(dev, dtype, codes, heads, window):
@@ -251,6 +251,9 @@ def test_refusals(dev):
             e.accumulate(q, lse, 0, plan, bad)
         with pytest.raises(ValueError, match="out"):
             e.accumulate(q, lse, 0, plan, weights, out=bad)
+    coded = CacheEviction(make_op(dev, 8, 2, 128, 16, BF16, 100, E4M3))
+    with pytest.raises(native.ViewAttnError, match="another shape"):
+        coded.accumulate(q, lse, 0, plan, coded.new_weights())
     other = make_op(dev, 8, 4, 128, 16, BF16, 100)
     f = CacheEviction(other)
     with pytest.raises(native.ViewAttnError, match="another shape"):

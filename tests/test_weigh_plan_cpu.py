@@ -12,7 +12,7 @@ from async_llm_amd.shared_cache import CacheEviction, SharedCacheAttention
 from async_llm_amd.kvcache import MHAKVCache
 
 
-def plan_of(subs, heads=(8, 2, 64), page=4, pages=64, window=0, capacity=None, dtype=native.VA_BF16):
+def plan_of(subs, heads=(8, 2, 64), page=4, pages=64, window=0, capacity=None, dtype=native.VA_BF16, codes=False):
     """``subs``: (rows, entries, seq_len, flags)."""
     arrays = [np.concatenate([[0], np.cumsum([r for r, *_ in subs])]), np.concatenate([[0], np.cumsum([len(e) for _, e, *_ in subs])]),
               np.concatenate([np.asarray(e) for _, e, *_ in subs] or [[]]), [n for _, _, n, _ in subs], [f for *_, f in subs]]
@@ -21,10 +21,10 @@ def plan_of(subs, heads=(8, 2, 64), page=4, pages=64, window=0, capacity=None, d
                              a[2].ctypes.data if a[2].size else None, a[3].ctypes.data, a[4].ctypes.data, None, None)
     shape, counts = native.VaShape(*heads, page, dtype), native.VaWeighCounts()
     words = np.zeros(1 << 20 if capacity is None else capacity, dtype=np.int32)
-    return native.lib.va_weigh_plan(s, shape, pages, window, words.ctypes.data, words.size, counts), words, counts
+    return native.lib.va_weigh_plan(s, shape, int(codes), pages, window, words.ctypes.data, words.size, counts), words, counts
 
 
-def counted(words, heads, page):
+def counted(words, heads, page, dtype=native.VA_BF16):
     """{(sub-row, slot): times} of what the plan's items count, and {slot: owners}."""
     h = words[:24]
     n_items, n_rows, n_joins, n_partials, off = h[1], h[2], h[3], h[4], h[6:10]
@@ -33,15 +33,21 @@ def counted(words, heads, page):
     pages = words[off[2]:]
     sub, lo, hi = (words[off[3] + i * n_rows: off[3] + (i + 1) * n_rows] for i in range(3))
     g = heads[0] // heads[1]
-    layout, n_strips, strips = h[17], h[18], words[h[19]: h[19] + h[18] + 1]
-    assert n_rows * g % 16 == 0 and (layout == 0 or n_items % 8 == 0)
-    if layout == 0 and n_items:  # walks: strips hold every item once
-        assert n_strips % 8 == 0 and strips[0] == 0 and strips[-1] == n_items and (np.diff(strips) >= 0).all()
+    n_tile_items, n_tile_rows, n_strips = h[18], h[19], h[20]
+    strips = words[h[21]: h[21] + n_strips + 1]
+    assert n_rows * g % 16 == 0 and n_tile_items % 8 == 0 and n_tile_rows * g % 16 == 0
+    if n_items > n_tile_items:  # strips hold every other item once
+        assert n_strips % 8 == 0 and strips[0] == n_tile_items and strips[-1] == n_items and (np.diff(strips) >= 0).all()
     pairs, owners, parts = {}, {}, {}
-    for first_page, first, n, begin, end, partial in items[:, :6]:
+    for k, (first_page, first, n, begin, end, partial) in enumerate(items[:, :6]):
         if n == 0:
+            assert k < n_tile_items
             continue
-        assert 0 < n <= (256 if layout else 1 << 20) and 0 <= begin < end <= n_rows * g // 16
+        first_rows = n_tile_rows * g // 16
+        assert end <= first_rows and n <= 256 if k < n_tile_items else begin >= first_rows
+        if k >= n_tile_items and dtype != native.VA_F32 and heads[2] == 64:
+            assert end == begin + 1
+        assert 0 < n and 0 <= begin < end <= n_rows * g // 16
         slots = [int(pages[first_page + t // page]) * page + t % page for t in range(first, first + n)]
         if partial >= 0:
             parts[int(partial)] = (int(first_page), int(first), int(n))
@@ -128,7 +134,7 @@ def test_readers_of_a_block_share_its_tokens():
     assert rc == 0 and counts.n_spans == 5
     assert counts.n_rows == 16 * 5  # a row an q head: whole tiles of 16
     assert counts.n_joins == 0
-    strips = np.diff(words[words[19]: words[19] + words[18] + 1])
+    strips = np.diff(words[words[21]: words[21] + words[20] + 1])
     tokens = words[words[6]: words[6] + 8 * counts.n_items].reshape(-1, 8)[:, 2]
     assert tokens.sum() == 1600 + 4 * 150 and (strips <= 2).all()  # few items: workgroups for all
 
@@ -144,18 +150,19 @@ def test_strips_cost_the_same():
         n = r.randint(20, 400)
         subs.append((1, [free.pop() for _ in range(n)], n * 16 - r.randint(0, 15), 0))
     rc, words, counts = plan_of(subs, (16, 4, 256), 16, 20000)
-    counted_strips = words[words[19]: words[19] + words[18] + 1]
+    counted_strips = words[words[21]: words[21] + words[20] + 1]
     items = words[words[6]: words[6] + 8 * counts.n_items].reshape(-1, 8)
     cost = [sum(n * (3 + b - a) for _, _, n, a, b, *_ in items[s: e]) for s, e in zip(counted_strips, counted_strips[1:])]
     cost = [c for c in cost if c]
+    assert words[18] == 32  # the prompt: tiles
     assert rc == 0 and 120 <= len(cost) <= 130 and max(cost) < 1.15 * sum(cost) / len(cost)
 
 
 def test_rows_are_split_where_tokens_are_few():
-    for dtype in (native.VA_BF16, native.VA_F32):
+    for dtype in (native.VA_BF16, native.VA_F32):  # tile items; strips, of parts of the rows
         rc, words, counts = plan_of([(500, list(range(40)), 640, native.VA_SUB_CAUSAL)], (8, 2, 64), 16, 64, dtype=dtype)
         assert rc == 0 and counts.n_joins >= 2 and counts.n_items >= 16
-        counted(words, (8, 2, 64), 16)
+        counted(words, (8, 2, 64), 16, dtype)
 
 
 @pytest.mark.parametrize("subs, message", [
