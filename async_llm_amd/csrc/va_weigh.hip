@@ -324,6 +324,11 @@ struct WalkKeys<INT8> : WalkKeys<BF16> {
   }
 };
 
+// kv heads of a strip's workgroup.
+__host__ __device__ inline int strip_heads(int num_kv_heads) { return num_kv_heads % 4 == 0 ? 4 : num_kv_heads % 2 == 0 ? 2 : 1; }
+
+constexpr int groups_of(int row_bytes) { return row_bytes > 256 ? 1 : row_bytes > 128 ? 2 : 4; }
+
 template <int kD, typename C>
 struct WalkShape {
   using K = WalkKeys<C>;
@@ -332,19 +337,20 @@ struct WalkShape {
   static constexpr int kRaw = kPieces / 4;                 // pieces of a row that a lane takes
   static constexpr int kSteps = K::kCodes ? 2 * kRaw : kRaw;  // operand pieces of a lane, per part
   static constexpr int kParts = parts_of(K::kRows);
-  // groups of 16 tokens of a wave's tile: 16 KB of 16- and 32-bit rows (up to 64 tokens), as many tokens of codes
-  static constexpr int kGroups = 1024 / (K::kCodes ? 2 * kD : kRowBytes) < 1 ? 1 : 1024 / (K::kCodes ? 2 * kD : kRowBytes) > 4 ? 4 : 1024 / (K::kCodes ? 2 * kD : kRowBytes);
+  // groups of 16 tokens of a wave's tile: 8 KB of 16- and 32-bit rows (up to 64 tokens, 16 at least), as many tokens of codes
+  static constexpr int kGroups = groups_of(K::kCodes ? 2 * kD : kRowBytes);
   static constexpr int kTokens = 16 * kGroups;
   static constexpr int kGroupBytes = 16 * kRowBytes;
   static constexpr int kLoads = kGroupBytes / 1024;        // wave-level loads of a group
   // behind a tile's rows: the tokens' sums so far, a word for every scale, the tokens' slots
   static constexpr int kSumsAt = kGroups * kGroupBytes, kScalesAt = kSumsAt + 256, kSlotsAt = kScalesAt + (K::kCodes ? 256 : 0);
   static constexpr int kTileBytes = kSlotsAt + 256;
-  static constexpr int kBuffers = kTileBytes > 10 * 1024 ? 1 : 2;
+  static constexpr int kBuffers = K::kCodes ? 2 : 1;  // (8 KB a wave on their way are enough)
   static constexpr int kTileLoads = kGroups * kLoads + (K::kCodes ? 2 : 1);  // what the counter of outstanding loads sees of a tile
   // behind the rings: where a wave turns a tile's sums from lanes to tokens, and holds those of several tiles with their places
-  static constexpr int kTurnOffset = kWeighWaves * kBuffers * kTileBytes, kHold = 256;
-  static constexpr int kWaveBytes = 256 + kHold * 8;
+  static constexpr int kTurnOffset = kWeighWaves * kBuffers * kTileBytes;
+  static constexpr int kHold = kBuffers * kTileBytes > 10 * 1024 ? 512 : 2048;
+  static constexpr int kWaveBytes = 256 + kHold * 4 + kHold / 16 * 8;
   static constexpr int kLdsBytes = kTurnOffset + kWeighWaves * kWaveBytes;
   static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups share the LDS of a CU");
   static_assert((kBuffers - 1) * kTileLoads < kAnyInFlight, "the counter of outstanding loads");
@@ -357,11 +363,12 @@ __device__ __forceinline__ int walk_swz(int r) {
   return (r >> 2) & 3;
 }
 
-// A workgroup walks a strip of items, its four waves on their own: each takes every fourth tile of an item's tokens, brings it
+// A workgroup walks a strip of items for up to four kv heads, whose rows of a token lie side by side, its waves on their own: each takes
+// its head's tiles of an item's tokens (every second or fourth where there are fewer heads), brings them
 // global -> LDS into a ring of its own (keys, the sums so far and, over codes, scales) and asks for the next one, of the next item
 // where this one ends, as soon as the keys are in registers.  There is no barrier, and nothing but the first tile of a strip
-// is waited for idly.  Sums are written some tiles at a time: a store is waited for with the keys asked for behind it, and one a
-// tile cost an eighth of the time.
+// is waited for idly.  Sums are held in LDS and written many at a time: each store between the loads costs the memory about as
+// much as 1 KB of keys (8 requests of 131072 tokens: 427 us with one a tile, 408 with one every eighth, FINAL with HOLD sums held).
 template <int kD, typename C>
 __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) {
   using Sh = WalkShape<kD, C>;
@@ -372,16 +379,17 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
   constexpr bool kSeveral = std::is_same_v<C, F32>;  // tokens may have several tiles of rows
   extern __shared__ va_u32x4 smem[];
   char* lds = (char*)smem;
-  const ItemHead where = item_and_head(block, a.num_kv_heads);
-  const int hk = where.head, strip_begin = ((Words)a.strips)[where.item], strip_end = ((Words)a.strips)[where.item + 1];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int heads = strip_heads(a.num_kv_heads), turns = kWeighWaves / heads, place = wave / heads;  // tiles of a wave: place, + turns, ...
+  const ItemHead where = item_and_head(block, a.num_kv_heads / heads);
+  const int hk = where.head * heads + wave % heads, strip_begin = ((Words)a.strips)[where.item], strip_end = ((Words)a.strips)[where.item + 1];
   if (strip_begin == strip_end) return;
   const int lane = threadIdx.x % kWave, j = lane % 16, kg = lane / 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   char* own = lds + wave * kBuffers * Sh::kTileBytes;
   const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_address(own));
   float* turn = (float*)(lds + Sh::kTurnOffset + wave * Sh::kWaveBytes);
   float* held_sums = turn + 64;
-  uint32_t* held_places = (uint32_t*)(held_sums + Sh::kHold);
+  uint2* held_groups = (uint2*)(held_sums + Sh::kHold);  // of 16 sums: where the first goes, how many there are
   const bool pages16 = a.page_map.shift >= 4;
   const long long row_bytes = K::kCodes ? kD : a.pool_row_stride * K::kBytes;
   const float* sums_in = a.weights_in + hk * a.num_slots;
@@ -392,7 +400,7 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
   auto piece_at = [&](int index) __attribute__((always_inline)) {
     const Words w = (Words)a.items + (long long)index * VA_WEIGH_ITEM_WORDS;
     Piece p{w[VA_WI_PAGES], w[VA_WI_FIRST], w[VA_WI_N_TOK], w[VA_WI_TILE_BEGIN], w[VA_WI_TILE_END], w[VA_WI_PARTIAL], 0};
-    p.tiles = ((p.n_tok + kTokens - 1) / kTokens - wave + kWeighWaves - 1) / kWeighWaves;
+    p.tiles = ((p.n_tok + kTokens - 1) / kTokens - place + turns - 1) / turns;
     return p;
   };
 
@@ -419,18 +427,42 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
       load_to_lds(from, off[0], dst);
     }
   };
-  auto request = [&](const Piece& p, int n, int buffer) __attribute__((always_inline)) {  // this wave's tile n of an item
+  // The tile to ask for next: its pages are looked up (in scalar loads) when the one before it has been asked for, so that nothing
+  // is waited for between a tile's landing and the next request.
+  struct Next {
+    int pages, first, last, t0, page[kGroups];
+  };
+  Next next{};
+  int asked = 0, found = 0;  // tiles asked for, and found, so far
+  int find_index = strip_begin, find_n = 0;
+  Piece find = piece_at(strip_begin);
+  auto find_next = [&]() __attribute__((always_inline)) {
+    while (find_n == find.tiles) {
+      if (find_index + 1 >= strip_end) return;
+      find = piece_at(++find_index);
+      find_n = 0;
+    }
+    next.pages = find.pages, next.first = find.first, next.last = find.n_tok - 1;
+    next.t0 = (find_n++ * turns + place) * kTokens;
+    if (pages16 && next.first % 16 == 0) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)  // (a group past the end: the last one)
+        next.page[g] = ((Words)a.pages)[next.pages + ((next.first + min(next.t0 + 16 * g, next.last / 16 * 16)) >> a.page_map.shift)];
+    }
+    ++found;
+  };
+  auto request_next = [&]() __attribute__((always_inline)) {
+    if (asked == found) return;
+    const int buffer = asked++ % kBuffers;
     const uint32_t dst = ring + (uint32_t)buffer * Sh::kTileBytes;
-    const int t0 = (n * kWeighWaves + wave) * kTokens, last = p.n_tok - 1;
     uint32_t of_lane = 0;  // slot of the token whose words this lane brings: token `lane` of the tile
-    if (pages16 && p.first % 16 == 0) {  // 16 tokens of a group lie in one page
+    if (pages16 && next.first % 16 == 0) {  // 16 tokens of a group lie in one page
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const int t = min(t0 + 16 * g, last / 16 * 16);  // (a group past the end: the last one)
-        const uint32_t at = (uint32_t)(p.first + t);
-        const uint32_t slot = ((uint32_t)((Words)a.pages)[p.pages + (int)(at >> a.page_map.shift)] << a.page_map.shift) + (at & (a.page_map.size - 1));
+        const int t = min(next.t0 + 16 * g, next.last / 16 * 16);
+        const uint32_t slot = ((uint32_t)next.page[g] << a.page_map.shift) + ((uint32_t)(next.first + t) & (a.page_map.size - 1));
         const char* from = (const char*)a.k_pool + (row_at(slot) - kBias);
-        const int most = last - t;  // rows behind the last one repeat it
+        const int most = next.last - t;  // rows behind the last one repeat it
         if (most >= 15) {
           request_group(from, ld_off, dst + g * Sh::kGroupBytes);
         } else {
@@ -442,7 +474,7 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
         of_lane = kg == g || g == 0 ? slot + min(j, most) : of_lane;
       }
     } else {  // tokens looked up one by one: each lane one, handed to those that load it
-      of_lane = weigh_slot(a, p.pages, p.first + min(t0 + lane % kTokens, last));
+      of_lane = weigh_slot(a, next.pages, next.first + min(next.t0 + lane % kTokens, next.last));
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
 #pragma unroll
@@ -454,17 +486,9 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
     load_word_to_lds(sums_in + of_lane, dst + Sh::kSumsAt);
     if constexpr (K::kCodes) load_bytes_to_lds((unsigned long long)a.k_scales + row_at(of_lane) / kD, dst + Sh::kScalesAt);
     *(uint32_t*)(own + buffer * Sh::kTileBytes + Sh::kSlotsAt + 4 * lane) = of_lane;
+    find_next();
   };
-  int asked = 0, ask_index = strip_begin, ask_n = 0;  // tiles asked for so far; the next one
-  Piece ask = piece_at(strip_begin);
-  auto request_next = [&]() __attribute__((always_inline)) {
-    while (ask_n == ask.tiles) {
-      if (ask_index + 1 >= strip_end) return;
-      ask = piece_at(++ask_index);
-      ask_n = 0;
-    }
-    request(ask, ask_n++, asked++ % kBuffers);
-  };
+  find_next();
 
   // ---- queries ----
   va_u32x4 q[kParts][kSteps];
@@ -491,13 +515,22 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
   for (int b = 0; b < kBuffers; ++b) request_next();
   int done = 0, index = strip_begin, n = 0, q_tile = -1;
   Piece at = piece_at(strip_begin);
-  int held = 0;  // sums not yet written, all of one kind
-  bool held_partial = false;
+  // Sums not yet written, all of one kind: of this workgroup's part of a span's rows or not, in groups of 16 that lie side by side
+  // or, of scattered tokens, with a place for each in the upper half.
+  int held = 0;
+  bool held_partial = false, held_scattered = false;
   auto write_held = [&]() __attribute__((always_inline)) {
     float* to = held_partial ? a.partials + hk * a.n_partials : a.weights_out + hk * a.num_slots;
-    for (int i = lane; i < held; i += kWave) {
-      const uint32_t place = held_places[i];
-      if (place != ~0u) to[place] = held_sums[i];
+    if (held_scattered) {
+      for (int i = lane; i < held; i += kWave) {
+        const uint32_t at = ((const uint32_t*)held_sums)[Sh::kHold / 2 + i];
+        if (at != ~0u) to[at] = held_sums[i];
+      }
+    } else {
+      for (int i = lane; i < held; i += kWave) {
+        const uint2 group = held_groups[i / 16];
+        if (i % 16 < (int)group.y) to[group.x + i % 16] = held_sums[i];
+      }
     }
     held = 0;
   };
@@ -532,8 +565,9 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
     }
     const float before = *(const float*)(tile + Sh::kSumsAt + 4 * lane);
     const uint32_t slot = *(const uint32_t*)(tile + Sh::kSlotsAt + 4 * lane);
-    if (held + kTokens > Sh::kHold || held_partial != (at.partial >= 0)) write_held();
-    held_partial = at.partial >= 0;
+    const bool partial = at.partial >= 0, scattered = !partial && !(pages16 && at.first % 16 == 0);
+    if (held + kTokens > (scattered ? Sh::kHold / 2 : Sh::kHold) || held_partial != partial || held_scattered != scattered) write_held();
+    held_partial = partial, held_scattered = scattered;
     __builtin_amdgcn_sched_barrier(0);
     if (single) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -541,7 +575,7 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
     }
     __builtin_amdgcn_sched_barrier(0);
 
-    const int t0 = (n * kWeighWaves + wave) * kTokens, t_tile = at.first + t0, t_end = min(t_tile + kTokens, at.first + at.n_tok);
+    const int t0 = (n * turns + place) * kTokens, t_tile = at.first + t0, t_end = min(t_tile + kTokens, at.first + at.n_tok);
     float sum[kGroups][4];
 #pragma unroll
     for (int g = 0; g < kGroups; ++g)
@@ -600,9 +634,12 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
       if (j < 4) turn[16 * g + 4 * kg + j] = of_token;
     }
     if (lane < kTokens) {
-      const bool within = t0 + lane < at.n_tok;
-      held_sums[held + lane] = held_partial ? turn[lane] : before + turn[lane];
-      held_places[held + lane] = !within ? ~0u : held_partial ? (uint32_t)(at.partial + t0 + lane) : slot;
+      held_sums[held + lane] = partial ? turn[lane] : before + turn[lane];
+      if (scattered) {
+        ((uint32_t*)held_sums)[Sh::kHold / 2 + held + lane] = t0 + lane < at.n_tok ? slot : ~0u;
+      } else if (j == 0) {
+        held_groups[(held + lane) / 16] = make_uint2(partial ? (uint32_t)(at.partial + t0 + lane) : slot, (uint32_t)min(16, max(0, at.n_tok - t0 - lane)));
+      }
     }
     held += kTokens;
     if (!single) {
@@ -932,7 +969,7 @@ static void launch_rows(const WeighArgs& a, bool fast, hipStream_t stream) {
 
 template <int kD, typename C>
 static int launch_matrix(const WeighArgs& a, int n_tile_items, int n_strips, bool fast, hipStream_t stream) {
-  const unsigned tiles = (unsigned)n_tile_items * (unsigned)a.num_kv_heads, strips = (unsigned)n_strips * (unsigned)a.num_kv_heads;
+  const unsigned tiles = (unsigned)n_tile_items * (unsigned)a.num_kv_heads, strips = (unsigned)n_strips * (unsigned)(a.num_kv_heads / strip_heads(a.num_kv_heads));
   const dim3 block(kWeighThreads);
   using Sh = WalkShape<kD, C>;
   if constexpr (std::is_same_v<C, F32>) {

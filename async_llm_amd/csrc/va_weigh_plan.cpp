@@ -239,7 +239,8 @@ struct Planner {
   int make_strips() {
     constexpr int64_t kKey = 4;
     const int row = shape.head_dim * (rows32 ? 4 : 2);
-    const int64_t least = 4 * 16 * std::clamp(1024 / std::max(row, 1), 1, 4);
+    const int hkv = shape.num_kv_heads, heads = hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;  // of a workgroup, whose four waves share them
+    const int64_t least = 4 / heads * 16 * (row > 256 ? 1 : row > 128 ? 2 : 4);
     auto cost_of = [&](int64_t tiles) { return kKey + tiles - 1; };
     int64_t total = 0, pieces = 0;
     if (n_tile_spans == spans.size()) return VA_OK;
@@ -250,13 +251,14 @@ struct Planner {
       total += (s.end - s.first) * cost_of(tile_b - tile_a);
       pieces += ((int64_t)s.end - s.first + least - 1) / least * (tile_b - tile_a);
     }
-    const int64_t n = std::max<int64_t>(1, std::min(pieces, std::max<int64_t>(1, kWorkgroups / shape.num_kv_heads)));
-    const int64_t room = std::max<int64_t>(1, (total + n - 1) / n);  // cost of a strip
-    int64_t used = 0;
+    const int64_t n = std::max<int64_t>(1, std::min(pieces, std::max<int64_t>(1, kWorkgroups * heads / hkv)));
+    // Strip k ends where the cost so far is nearest to (k + 1) / n of all: never more than n of them, which run at a time.
+    int64_t used = 0, k = 0, target = total / n;
     strips.push_back((int32_t)n_tile_items);
-    auto next_item = [&](int64_t cost) {  // opens another strip where this one has what it should
-      if (used > 0 && used + cost / 2 > room) strips.push_back((int32_t)(items.size() / VA_WEIGH_ITEM_WORDS)), used = 0;
-      used += cost;
+    auto close_at = [&](int64_t margin) {  // begins another strip where this one is within `margin` of its end
+      if (k + 1 >= n || used + margin < target || (size_t)strips.back() * VA_WEIGH_ITEM_WORDS == items.size()) return;
+      strips.push_back((int32_t)(items.size() / VA_WEIGH_ITEM_WORDS));
+      while (k + 1 < n && used + margin >= target) target = total * (++k + 1) / n;
     };
     for (size_t i = n_tile_spans; i < spans.size(); ++i) {
       const Span& s = spans[i];
@@ -267,16 +269,16 @@ struct Planner {
         if (tile_a == tile_b) break;
         const int64_t cost = cost_of(tile_b - tile_a);
         // as many tokens as the strip has room for, to the nearest cut; rows are split where the least number costs more than a strip
-        int64_t parts = std::min(tile_b - tile_a, std::max<int64_t>(1, std::min<int64_t>(least, s.end - t) * cost / room));
+        const int64_t parts = std::min(tile_b - tile_a, std::max<int64_t>(1, std::min<int64_t>(least, s.end - t) * cost * n / std::max<int64_t>(1, total)));
         int64_t n_tok = least;
-        if (parts == 1) {
-          if (used > 0 && used + least * cost / 2 > room) strips.push_back((int32_t)(items.size() / VA_WEIGH_ITEM_WORDS)), used = 0;
-          n_tok = std::max<int64_t>(1, ((room - used) / cost + least / 2) / least) * least;
-        }
+        close_at(parts == 1 ? least * cost / 2 : 0);
+        if (parts == 1) n_tok = k + 1 < n ? std::max<int64_t>(1, ((target - used) / cost + least / 2) / least) * least : s.end - t + least;
         // (chunks start on multiples of 16 tokens of the span: pages of as many are read in runs)
-        const int64_t end = std::min<int64_t>(s.end, (t + n_tok) / 16 * 16);
-        const int rc = put_items(s, t, (int)(end - t), tile_a, tile_b, parts,
-                                 [&](int64_t) { parts == 1 ? (void)(used += (end - t) * cost) : next_item((end - t) * (cost / parts)); });
+        const int64_t end = std::min<int64_t>(s.end, (t + n_tok) / 16 * 16), each = (end - t) * cost / parts;
+        const int rc = put_items(s, t, (int)(end - t), tile_a, tile_b, parts, [&](int64_t p) {
+          if (p > 0) close_at(each / 2);
+          used += each;
+        });
         if (rc) return rc;
         t = end;
       }

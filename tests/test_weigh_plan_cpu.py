@@ -136,7 +136,7 @@ def test_readers_of_a_block_share_its_tokens():
     assert counts.n_joins == 0
     strips = np.diff(words[words[21]: words[21] + words[20] + 1])
     tokens = words[words[6]: words[6] + 8 * counts.n_items].reshape(-1, 8)[:, 2]
-    assert tokens.sum() == 1600 + 4 * 150 and (strips <= 2).all()  # few items: workgroups for all
+    assert tokens.sum() == 1600 + 4 * 150 and (strips <= 3).all()  # few items: workgroups for all
 
 
 def test_strips_cost_the_same():
@@ -155,7 +155,7 @@ def test_strips_cost_the_same():
     cost = [sum(n * (3 + b - a) for _, _, n, a, b, *_ in items[s: e]) for s, e in zip(counted_strips, counted_strips[1:])]
     cost = [c for c in cost if c]
     assert words[18] == 32  # the prompt: tiles
-    assert rc == 0 and 120 <= len(cost) <= 130 and max(cost) < 1.15 * sum(cost) / len(cost)
+    assert rc == 0 and 480 <= len(cost) <= 512 and max(cost) < 1.05 * sum(cost) / len(cost)
 
 
 def test_rows_are_split_where_tokens_are_few():
