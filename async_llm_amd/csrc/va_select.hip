@@ -7,9 +7,10 @@
 // is found digit by digit from histograms, most significant first, and then every token above it stays, and of those equal to
 // it the first that are wanted.  No sort, and no order of execution that the result depends on.
 //
-// Blocks of up to kSelectInLds tokens: a workgroup each, keys in LDS, one launch (1500 tokens of 8 heads: 16.1 us).  Longer ones:
-// the keys are made by many workgroups, then one per block finds the key at which its list ends and where each run of tokens
-// writes, then many write (8 blocks of 60000 .. 131072 tokens: 133 us).
+// Blocks of up to kSelectInLds tokens: a workgroup each, keys in LDS, one launch.  Longer ones: four launches of a workgroup for
+// each run of tokens.  The first makes keys and counts those of a run by their upper digit; each further one adds the counts of all
+// runs up, every workgroup for itself, finds the cut's digit, and counts the run's keys that have it by their next one, and the last
+// writes.  What lies above the cut in the runs in front falls out of the same sums.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,14 +24,16 @@ namespace va {
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
 constexpr int kSelectInLds = 16384;  // tokens of a block whose keys stay in LDS
 constexpr int kSelectBlocks = 64;    // blocks of a launch
-constexpr int kSelectRun = 4096;     // tokens of a workgroup that makes keys or writes
+constexpr int kSelectRun = 4096;     // tokens of a run, at least
 constexpr int kSelectBins = 256;
+// digits of a long block's keys: eleven bits, eleven, ten
+constexpr int kSelectTop = 2048, kSelectCounts = 5120;
 
 struct SelectBlock {
   long long begin, out;  // first entry of its slots, of its results
   long long count, keep;
   long long keys;  // long blocks: first key in the workspace
-  int runs, first_run;  // long blocks: runs of kSelectRun tokens; number of the first one in the workspace
+  int runs, first_run, run_tokens;  // long blocks: runs, number of the first one in the workspace, tokens of a run
 };
 struct SelectArgs {
   const float* weights;
@@ -41,26 +44,62 @@ struct SelectArgs {
   int64_t* positions;
   int64_t* out_slots;
   int64_t* shifts;
-  uint32_t* keys;    // long blocks
-  uint32_t* cut;     // [block][2]: the last key that stays, how many of those equal to it do
-  uint32_t* starts;  // [run][2]: kept tokens, tokens equal to the last key in front of a run
+  // long blocks
+  uint32_t* keys;
+  uint32_t* found;   // [block][2 stages][2]: the cut's digits so far, how many of the keys with them are wanted
+  uint32_t* before;  // [run][2 stages]: tokens of the runs in front of it that are above the cut in this stage's digit
+  uint32_t* counts;  // [run][kSelectCounts]: tokens by the upper digit of their keys, of those with the cut's by the middle one, then by the lower one
   SelectBlock blocks[kSelectBlocks];
 };
 
-__device__ __forceinline__ uint32_t select_key(const SelectArgs& a, const SelectBlock& b, long long t) {
-  if (t < a.first || t >= b.count - a.last) return 0xffffffffu;
-  const long long slot = a.slots[b.begin + t];
-  double sum = 0.0;
-  if (slot >= 0 && slot < a.num_slots) {
-    const float* w = a.weights + slot;
-#pragma unroll 8
-    for (int h = 0; h < a.num_heads; ++h) sum += (double)w[h * a.num_slots];
-  }
-  const float score = (float)sum;
+__device__ __forceinline__ uint32_t key_of(float score) {
   if (score != score) return 0xfffffffeu;
   const uint32_t bits = __float_as_uint(score + 0.f);  // (-0 counts as 0)
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
+
+// Keys of tokens [begin, end) of a block, this thread's every kSelectThreads-th: `put(t, key)`.  A slot and its weights are two trips to
+// memory; those of kBatch tokens are made together.
+template <typename Put>
+__device__ __forceinline__ void make_keys(const SelectArgs& a, const SelectBlock& b, long long begin, long long end, Put&& put) {
+  constexpr int kBatch = 4, kHeads = 4;
+  for (long long t0 = begin + threadIdx.x; t0 < end; t0 += kBatch * kSelectThreads) {
+    long long slot[kBatch];
+    bool protect[kBatch];
+    double sum[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const long long t = min(t0 + u * kSelectThreads, end - 1);
+      protect[u] = t < a.first || t >= b.count - a.last;
+      slot[u] = a.slots[b.begin + t];
+      sum[u] = 0.0;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (slot[u] < 0 || slot[u] >= a.num_slots) slot[u] = -1;
+    for (int h0 = 0; h0 < a.num_heads; h0 += kHeads) {
+      float w[kBatch][kHeads];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) w[u][i] = a.weights[min(h0 + i, a.num_heads - 1) * a.num_slots + max(slot[u], 0ll)];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+          if (h0 + i < a.num_heads && slot[u] >= 0) sum[u] += (double)w[u][i];
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const long long t = t0 + u * kSelectThreads;
+      if (t < end) put(t, protect[u] ? 0xffffffffu : key_of((float)sum[u]));
+    }
+  }
+}
+
+// Scores of tokens that nobody looked at are equal, and most others share a few upper digits: lanes count in sixteen copies, or adds
+// to one bin would take a clock each.
+constexpr int kSelectCopies = 16;
 
 // The keep-th largest of `count` keys and how many of the keys equal to it are among the first `keep`; 1 <= keep <= count.
 // All threads of the workgroup call it and get the same.
@@ -68,22 +107,33 @@ struct Cut {
   uint32_t key, equal;
 };
 template <typename Keys>
-__device__ __forceinline__ Cut find_cut(Keys key_at, long long count, long long keep, uint32_t (&bins)[kSelectBins], uint32_t (&found)[2]) {
+__device__ __forceinline__ Cut find_cut(Keys key_at, long long count, long long keep, uint32_t (&bins)[kSelectBins * kSelectCopies],
+                                        uint32_t (&found)[3]) {
   uint32_t prefix = 0, wanted = (uint32_t)keep;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+    for (int i = threadIdx.x; i < kSelectBins * kSelectCopies; i += kSelectThreads) bins[i] = 0;
     __syncthreads();
     for (long long t = threadIdx.x; t < count; t += kSelectThreads) {
       const uint32_t key = key_at(t);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&bins[(key >> shift) & 255u], 1u);
+      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
+        atomicAdd(&bins[((key >> shift) & 255u) * kSelectCopies + threadIdx.x % kSelectCopies], 1u);
     }
     __syncthreads();
-    if (threadIdx.x < kWave) {  // lane l: bins 4 l .. + 3; the digit is where the count from above reaches `wanted`
+    // thread 4 d + i: four copies of digit d
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine += bins[threadIdx.x * 4 + i];
+    mine += __shfl_xor(mine, 1, kWave);
+    mine += __shfl_xor(mine, 2, kWave);
+    __syncthreads();
+    if (threadIdx.x % 4 == 0) bins[threadIdx.x / 4] = mine;
+    __syncthreads();
+    if (threadIdx.x < kWave) {  // lane l: digits 4 l .. + 3; the digit is where the count from above reaches `wanted`
       const int lane = threadIdx.x;
       uint32_t n[4], sum = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum += n[i] = bins[4 * lane + i];
-      uint32_t above = sum;  // of this lane's bins and all higher ones
+      uint32_t above = sum;  // of this lane's digits and all higher ones
 #pragma unroll
       for (int off = 1; off < kWave; off <<= 1) {
         const uint32_t other = __shfl_down(above, off, kWave);
@@ -105,37 +155,48 @@ __device__ __forceinline__ Cut find_cut(Keys key_at, long long count, long long 
 
 __device__ __forceinline__ uint32_t bits_below(unsigned long long mask, int lane) { return (uint32_t)__popcll(mask & ((1ull << lane) - 1)); }
 
-// A wave's walk over tokens [begin, end) of a block: `write` (or only count) those that stay.  `taken`: kept tokens in front of it,
-// `equal`: tokens equal to the cut's key in front of it.
-template <bool kWrite, typename Keys>
-__device__ __forceinline__ void walk_kept(const SelectArgs& a, const SelectBlock& b, Keys key_at, Cut cut, long long begin, long long end,
-                                          uint32_t& taken, uint32_t& equal) {
+// Write those of tokens [begin, end) of a block that stay; a wave's part, four times 64 tokens at a time, whose slots are on their way
+// together.  `taken`: kept tokens in front of it, `equal`: tokens equal to the cut's key in front of it.
+template <typename Keys>
+__device__ __forceinline__ void write_kept(const SelectArgs& a, const SelectBlock& b, Keys key_at, Cut cut, long long begin, long long end,
+                                           uint32_t taken, uint32_t equal) {
+  constexpr int kBatch = 4;
   const int lane = threadIdx.x % kWave;
-  for (long long t0 = begin; t0 < end; t0 += kWave) {
-    const long long t = t0 + lane;
-    const uint32_t key = t < end ? key_at(t) : 0u;
-    const bool same = t < end && key == cut.key;
-    const unsigned long long sames = __ballot(same);
-    const bool stays = t < end && (key > cut.key || (same && equal + bits_below(sames, lane) < cut.equal));
-    const unsigned long long kept = __ballot(stays);
-    if (kWrite && stays) {
-      const long long rank = (long long)taken + bits_below(kept, lane), at = b.out + rank;
-      a.positions[at] = t;
-      a.out_slots[at] = a.slots[b.begin + t];
-      a.shifts[at] = rank - t;
+  for (long long t0 = begin; t0 < end; t0 += kBatch * kWave) {
+    uint32_t key[kBatch];
+    int64_t slot[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const long long t = min(t0 + u * kWave + lane, end - 1);
+      key[u] = key_at(t);
+      slot[u] = a.slots[b.begin + t];
     }
-    equal += (uint32_t)__popcll(sames);
-    taken += (uint32_t)__popcll(kept);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const long long t = t0 + u * kWave + lane;
+      const bool same = t < end && key[u] == cut.key;
+      const unsigned long long sames = __ballot(same);
+      const bool stays = t < end && (key[u] > cut.key || (same && equal + bits_below(sames, lane) < cut.equal));
+      const unsigned long long kept = __ballot(stays);
+      if (stays) {
+        const long long rank = (long long)taken + bits_below(kept, lane), at = b.out + rank;
+        a.positions[at] = t;
+        a.out_slots[at] = slot[u];
+        a.shifts[at] = rank - t;
+      }
+      equal += (uint32_t)__popcll(sames);
+      taken += (uint32_t)__popcll(kept);
+    }
   }
 }
 
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
   extern __shared__ uint32_t keys[];
-  __shared__ uint32_t bins[kSelectBins], found[2], of_wave[kSelectWaves][2];
+  __shared__ uint32_t bins[kSelectBins * kSelectCopies], found[3], of_wave[kSelectWaves][2];
   const SelectBlock& b = a.blocks[blockIdx.x];
   if (b.keep == 0) return;
   const int count = (int)b.count;
-  for (int t = threadIdx.x; t < count; t += kSelectThreads) keys[t] = select_key(a, b, t);
+  make_keys(a, b, 0, count, [&](long long t, uint32_t key) __attribute__((always_inline)) { keys[t] = key; });
   __syncthreads();
   auto key_at = [&](long long t) __attribute__((always_inline)) { return keys[t]; };
   const Cut cut = find_cut(key_at, count, b.keep, bins, found);
@@ -153,64 +214,145 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
   __syncthreads();
   above = same = 0;
   for (int w = 0; w < wave; ++w) above += of_wave[w][0], same += of_wave[w][1];
-  uint32_t taken = above + min(same, cut.equal);
-  walk_kept<true>(a, b, key_at, cut, begin, end, taken, same);
+  write_kept(a, b, key_at, cut, begin, end, above + min(same, cut.equal), same);
 }
 
 // ---- long blocks ----
-__global__ __launch_bounds__(kSelectThreads) void select_keys_kernel(SelectArgs a) {
-  const SelectBlock& b = a.blocks[blockIdx.y];
-  if ((int)blockIdx.x >= b.runs) return;
-  const long long begin = (long long)blockIdx.x * kSelectRun, end = min(begin + kSelectRun, b.count);
-  for (long long t = begin + threadIdx.x; t < end; t += kSelectThreads) a.keys[b.keys + t] = select_key(a, b, t);
+// The digit of the workgroup's counts n at which the number from above reaches `wanted`, and what is then still wanted: found[0],
+// found[1].  Every thread has kEach digits side by side, from above: thread 0 the highest.
+template <int kEach>
+__device__ __forceinline__ void find_digit(const uint32_t (&n)[kEach], uint32_t wanted, uint32_t (&of_wave)[kSelectWaves], uint32_t (&found)[2]) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  uint32_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum += n[i];
+  uint32_t upto = sum;  // of this thread's and all higher digits of the wave
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const uint32_t other = __shfl_up(upto, off, kWave);
+    if (lane >= off) upto += other;
+  }
+  if (lane == kWave - 1) of_wave[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += of_wave[w];
+  uint32_t higher = upto - sum;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (higher < wanted && higher + n[i] >= wanted) found[0] = (uint32_t)(threadIdx.x * kEach + i), found[1] = wanted - higher;
+    higher += n[i];
+  }
+  __syncthreads();
 }
 
-__global__ __launch_bounds__(kSelectThreads) void select_cut_kernel(SelectArgs a) {
-  __shared__ uint32_t bins[kSelectBins], found[2];
-  const SelectBlock& b = a.blocks[blockIdx.x];
-  if (b.keep == 0) return;
-  const uint32_t* keys = a.keys + b.keys;
-  auto key_at = [&](long long t) __attribute__((always_inline)) { return keys[t]; };
-  const Cut cut = find_cut(key_at, b.count, b.keep, bins, found);
-  if (threadIdx.x == 0) a.cut[2 * blockIdx.x] = cut.key, a.cut[2 * blockIdx.x + 1] = cut.equal;
-  // counts of the runs, a wave each
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  for (int run = wave; run < b.runs; run += kSelectWaves) {
-    const long long begin = (long long)run * kSelectRun, end = min(begin + kSelectRun, b.count);
-    uint32_t above = 0, same = 0;
-    for (long long t = begin + lane; t < end; t += kWave) above += keys[t] > cut.key, same += keys[t] == cut.key;
+// Stage 0: keys, counted by their upper digit.  Stage 1 (2): the cut's upper (middle) digit, the run's keys that have it counted by
+// the next one.  Stage 3: the lower digit, and the run writes what stays.
+template <int kStage>
+__global__ __launch_bounds__(kSelectThreads) void select_run_kernel(SelectArgs a) {
+  constexpr int kDigits = kStage == 3 ? 1024 : kSelectTop, kEach = kDigits / kSelectThreads;  // of the digit that is found
+  constexpr int kNext = kStage == 2 ? 1024 : kSelectTop, kCopies = 4;                         // of the one that is counted
+  constexpr int kFrom = kStage == 1 ? 0 : kStage == 2 ? 2048 : 4096, kTo = kStage == 0 ? 0 : kStage == 1 ? 2048 : 4096;
+  __shared__ uint32_t bins[kStage == 3 ? 1 : kCopies][kStage == 3 ? 1 : kNext + 8];
+  __shared__ uint32_t of_wave[kSelectWaves], found[2], total[2], per_wave[kSelectWaves][2];
+  const SelectBlock& b = a.blocks[blockIdx.y];
+  const int run = (int)blockIdx.x;
+  if (run >= b.runs) return;
+  const long long begin = (long long)run * b.run_tokens, end = min(begin + b.run_tokens, b.count);
+  uint32_t* keys = a.keys + b.keys;
+  if constexpr (kStage < 3) {
+    for (int i = threadIdx.x; i < kCopies * (kNext + 8); i += kSelectThreads) bins[0][i] = 0;
+    __syncthreads();
+  }
+  uint32_t prefix = 0, equal = 0, above = 0;
+  if constexpr (kStage > 0) {
+    // counts of all runs, and of those in front of this one
+    uint32_t n[kEach], front[kEach];
 #pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) above += __shfl_xor(above, off, kWave), same += __shfl_xor(same, off, kWave);
-    if (lane == 0) a.starts[2 * (b.first_run + run)] = above, a.starts[2 * (b.first_run + run) + 1] = same;
+    for (int e = 0; e < kEach; ++e) n[e] = front[e] = 0;
+    const uint32_t* from = a.counts + (long long)b.first_run * kSelectCounts + kFrom + kDigits - kEach - threadIdx.x * kEach;
+#pragma unroll 16
+    for (int r = 0; r < b.runs; ++r) {
+      uint32_t x[kEach];
+      if constexpr (kEach == 2) {
+        const uint2 two = *(const uint2*)(from + (long long)r * kSelectCounts);
+        x[0] = two.y, x[1] = two.x;  // (from above)
+      } else {
+        x[0] = from[(long long)r * kSelectCounts];
+      }
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) n[e] += x[e], front[e] += r < run ? x[e] : 0u;
+    }
+    const uint32_t* last = a.found + 4 * blockIdx.y + 2 * (kStage - 2);
+    find_digit<kEach>(n, kStage == 1 ? (uint32_t)b.keep : last[1], of_wave, found);
+    const uint32_t place = found[0];  // from above
+    prefix = (kStage == 1 ? 0u : last[0]) | (uint32_t)(kDigits - 1 - place) << (kStage == 1 ? 21 : kStage == 2 ? 10 : 0);
+    equal = found[1];
+    // what is above the digit in the runs in front, and (last stage) equal to the cut
+    uint32_t mine = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) mine += (uint32_t)threadIdx.x * kEach + e < place ? front[e] : 0u;
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) mine += __shfl_xor(mine, off, kWave);
+    if (threadIdx.x % kWave == 0) per_wave[threadIdx.x / kWave][0] = mine;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if ((uint32_t)threadIdx.x * kEach + e == place) total[1] = front[e];
+    __syncthreads();
+    for (int w = 0; w < kSelectWaves; ++w) above += per_wave[w][0];
+    if constexpr (kStage < 3) {
+      if (threadIdx.x == 0) {
+        a.before[2 * (b.first_run + run) + kStage - 1] = above;
+        if (run == 0) a.found[4 * blockIdx.y + 2 * (kStage - 1)] = prefix, a.found[4 * blockIdx.y + 2 * (kStage - 1) + 1] = equal;
+      }
+    } else {
+      above += a.before[2 * (b.first_run + run)] + a.before[2 * (b.first_run + run) + 1];
+    }
+  }
+  if constexpr (kStage < 3) {
+    auto count = [&](uint32_t digit) __attribute__((always_inline)) { atomicAdd(&bins[threadIdx.x % kCopies][digit], 1u); };
+    if constexpr (kStage == 0) {
+      make_keys(a, b, begin, end, [&](long long t, uint32_t key) __attribute__((always_inline)) {
+        keys[t] = key;
+        count(key >> 21);
+      });
+    } else {
+#pragma unroll 4
+      for (long long t = begin + threadIdx.x; t < end; t += kSelectThreads) {
+        const uint32_t key = keys[t];
+        constexpr int kShift = kStage == 1 ? 21 : 10;
+        if (key >> kShift == prefix >> kShift) count(kStage == 1 ? key >> 10 & 2047u : key & 1023u);
+      }
+    }
+    __syncthreads();
+    uint32_t* to = a.counts + (long long)(b.first_run + run) * kSelectCounts + kTo;
+    for (int i = threadIdx.x; i < kNext; i += kSelectThreads) {
+      uint32_t sum = 0;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) sum += bins[c][i];
+      to[i] = sum;
+    }
+  } else {
+    const Cut cut{prefix, equal};
+    uint32_t same = total[1];
+    // this wave's part of the run, and what stays in front of it
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const long long each = b.run_tokens / kSelectWaves;
+    const long long from = min(begin + wave * each, end), to = min(from + each, end);
+    uint32_t own_above = 0, own_same = 0;
+#pragma unroll 4
+    for (long long t = from + lane; t < to; t += kWave) own_above += keys[t] > cut.key, own_same += keys[t] == cut.key;
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) own_above += __shfl_xor(own_above, off, kWave), own_same += __shfl_xor(own_same, off, kWave);
+    __syncthreads();
+    if (lane == 0) per_wave[wave][0] = own_above, per_wave[wave][1] = own_same;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) above += per_wave[w][0], same += per_wave[w][1];
+    write_kept(a, b, [&](long long t) __attribute__((always_inline)) { return keys[t]; }, cut, from, to, above + min(same, cut.equal), same);
   }
 }
 
-__global__ __launch_bounds__(kSelectThreads) void select_write_kernel(SelectArgs a) {
-  __shared__ uint32_t of_wave[kSelectWaves][2];
-  const SelectBlock& b = a.blocks[blockIdx.y];
-  if ((int)blockIdx.x >= b.runs || b.keep == 0) return;
-  const uint32_t* keys = a.keys + b.keys;
-  const Cut cut{a.cut[2 * blockIdx.y], a.cut[2 * blockIdx.y + 1]};
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  // what stays in front of this run, and of this wave's part of it
-  uint32_t above = 0, same = 0;
-  for (int run = lane; run < (int)blockIdx.x; run += kWave) above += a.starts[2 * (b.first_run + run)], same += a.starts[2 * (b.first_run + run) + 1];
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) above += __shfl_xor(above, off, kWave), same += __shfl_xor(same, off, kWave);
-  constexpr int kEach = kSelectRun / kSelectWaves;
-  const long long begin = min((long long)blockIdx.x * kSelectRun + wave * kEach, b.count), end = min(begin + kEach, b.count);
-  uint32_t own_above = 0, own_same = 0;
-  for (long long t = begin + lane; t < end; t += kWave) own_above += keys[t] > cut.key, own_same += keys[t] == cut.key;
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) own_above += __shfl_xor(own_above, off, kWave), own_same += __shfl_xor(own_same, off, kWave);
-  if (lane == 0) of_wave[wave][0] = own_above, of_wave[wave][1] = own_same;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) above += of_wave[w][0], same += of_wave[w][1];
-  uint32_t taken = above + min(same, cut.equal);
-  walk_kept<true>(a, b, [&](long long t) __attribute__((always_inline)) { return keys[t]; }, cut, begin, end, taken, same);
-}
-
-static long long runs_of(long long count) { return (count + kSelectRun - 1) / kSelectRun; }
+// Runs of kSelectRun tokens, or of a multiple of those that makes about 64.
+static int run_tokens_of(long long count) { return kSelectRun * (int)std::max<long long>(1, count / (64ll * kSelectRun)); }
+static long long runs_of(long long count) { return (count + run_tokens_of(count) - 1) / run_tokens_of(count); }
 
 static int launch_select_batch(SelectArgs& a, int n, bool in_lds, hipStream_t stream) {
   if (n == 0) return VA_OK;
@@ -223,20 +365,22 @@ static int launch_select_batch(SelectArgs& a, int n, bool in_lds, hipStream_t st
     if (e != hipSuccess) return va_fail(VA_ERR_HIP, "raising the LDS limit: %s", hipGetErrorString(e));
     hipLaunchKernelGGL(select_kernel, dim3((unsigned)n), block, (unsigned)(most * 4), stream, a);
   } else {
-    hipLaunchKernelGGL(select_keys_kernel, dim3((unsigned)runs, (unsigned)n), block, 0, stream, a);
-    hipLaunchKernelGGL(select_cut_kernel, dim3((unsigned)n), block, 0, stream, a);
-    hipLaunchKernelGGL(select_write_kernel, dim3((unsigned)runs, (unsigned)n), block, 0, stream, a);
+    const dim3 grid((unsigned)runs, (unsigned)n);
+    hipLaunchKernelGGL(select_run_kernel<0>, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(select_run_kernel<1>, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(select_run_kernel<2>, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(select_run_kernel<3>, grid, block, 0, stream, a);
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "selection launch: %s", hipGetErrorString(e));
 }
 
-// Words of the workspace: keys, cuts, starts of the runs of all long blocks (batches start on 16-byte boundaries); -1 for counts that no selection takes.
+// Words of the workspace: keys, digits found and counts of all long blocks (batches start on 16-byte boundaries); -1 for counts that no selection takes.
 static int64_t select_words(int32_t n_blocks, const int64_t* counts) {
   int64_t words = 0;
   for (int32_t i = 0; i < n_blocks; ++i) {
     if (counts[i] < 0 || counts[i] > 0x7fffffffLL) return -1;
-    if (counts[i] > kSelectInLds) words += (counts[i] + 3) / 4 * 4 + 4 + 2 * runs_of(counts[i]);
+    if (counts[i] > kSelectInLds) words += (counts[i] + 3) / 4 * 4 + 8 + (2 + kSelectCounts) * runs_of(counts[i]);
   }
   return words;
 }
@@ -280,17 +424,17 @@ extern "C" int va_select_tokens(const float* weights_dev, int32_t num_heads, int
     for (int32_t i = 0; i <= n_blocks; ++i) {
       const bool whole = i == n_blocks || n == va::kSelectBlocks;
       if (whole) {
-        a.keys = at, a.cut = at + keys, a.starts = a.cut + 2 * n;
+        a.keys = at, a.found = at + keys, a.before = a.found + 4 * n, a.counts = a.before + 2 * runs + (-2 * runs & 3);
         const int rc = va::launch_select_batch(a, n, !large, (hipStream_t)stream);
         if (rc) return rc;
-        if (large) at = a.starts + 2 * runs + (-(2 * n + 2 * runs) & 3);
+        if (large) at = a.counts + (long long)runs * va::kSelectCounts;
         n = runs = 0, keys = 0;
       }
       if (i == n_blocks) break;
       const long long count = counts_host[i];
       if ((count > va::kSelectInLds) == (large != 0) && keep_host[i] > 0) {
         const int r = large ? (int)va::runs_of(count) : 0;
-        a.blocks[n++] = va::SelectBlock{begin, out, count, keep_host[i], keys, r, runs};
+        a.blocks[n++] = va::SelectBlock{begin, out, count, keep_host[i], keys, r, runs, large ? va::run_tokens_of(count) : 0};
         runs += r;
         if (large) keys += (count + 3) / 4 * 4;
       }

@@ -22,6 +22,8 @@ positions as before.
 
 from __future__ import annotations
 
+import ctypes
+import numbers
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Union
 
@@ -176,26 +178,28 @@ class CacheEviction:
             raise ValueError(f"weights must be a contiguous float32 tensor [heads, slots], got {weights.dtype} {tuple(weights.shape)}")
         if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != device:
             raise ValueError(f"slots must be one row of int64 on {device}, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
-        tokens = np.asarray(counts, dtype=np.int64).reshape(-1)
-        wanted = np.broadcast_to(np.asarray(keep, dtype=np.int64), tokens.shape)
-        if tokens.size and (tokens.min() < 0 or wanted.min() < 0) or first < 0 or last < 0:
+        tokens = [int(n) for n in counts]
+        wanted = [int(keep)] * len(tokens) if isinstance(keep, numbers.Integral) else [int(n) for n in keep]
+        if len(wanted) != len(tokens):
+            raise ValueError(f"{len(wanted)} numbers of tokens to keep of {len(tokens)} blocks")
+        if tokens and (min(tokens) < 0 or min(wanted) < 0) or first < 0 or last < 0:
             raise ValueError("counts, keep, first and last must not be negative")
-        if int(tokens.sum()) != slots.numel():
-            raise ValueError(f"counts add up to {int(tokens.sum())} tokens, slots has {slots.numel()}")
-        wanted = np.minimum(wanted, tokens)
-        total = int(wanted.sum())
-        results = torch.empty((3, total), dtype=torch.int64, device=device)
+        if sum(tokens) != slots.numel():
+            raise ValueError(f"counts add up to {sum(tokens)} tokens, slots has {slots.numel()}")
+        wanted = [min(a, b) for a, b in zip(wanted, tokens)]
+        results = torch.empty((3, sum(wanted)), dtype=torch.int64, device=device)
         positions, kept_slots, shifts = results.unbind(0)
-        nbytes = native.lib.va_select_workspace_bytes(tokens.size, tokens.ctypes.data)
+        many = ctypes.c_int64 * len(tokens)
+        tokens, stay = many(*tokens), many(*wanted)
+        nbytes = native.lib.va_select_workspace_bytes(len(wanted), tokens)
         if nbytes < 0:
             raise ValueError("a block holds at most 2^31 - 1 tokens")
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         slots = slots.contiguous()
         native.call_on(device, native.lib.va_select_tokens, weights.data_ptr(), weights.shape[0], weights.shape[1], slots.data_ptr(),
-                       tokens.size, tokens.ctypes.data, wanted.ctypes.data, first, last, positions.data_ptr(),
-                       kept_slots.data_ptr(), shifts.data_ptr(), None if workspace is None else workspace.data_ptr(), nbytes,
-                       native.current_stream_ptr(device))
-        return KeptTokens(positions, kept_slots, shifts, wanted.tolist())
+                       len(wanted), tokens, stay, first, last, positions.data_ptr(), kept_slots.data_ptr(), shifts.data_ptr(),
+                       None if workspace is None else workspace.data_ptr(), nbytes, native.current_stream_ptr(device))
+        return KeptTokens(positions, kept_slots, shifts, wanted)
 
     # ------------------------------------------------------------------
     # moving
