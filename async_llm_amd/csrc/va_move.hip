@@ -19,8 +19,7 @@
 
 namespace va {
 
-constexpr int kMoveTokens = 16;  // tokens per workgroup
-constexpr int kMoveBatch = 4;    // tokens whose loads are in flight together
+constexpr int kMoveTokens = 4;  // tokens per workgroup, whose loads are in flight together
 constexpr int kMoveTurnBytes = 48 * 1024;
 
 struct MoveArgs {
@@ -43,21 +42,18 @@ __global__ __launch_bounds__(1024) void move_kernel(MoveArgs a) {
   using S = typename E::storage;
   using P = Piece<S, kVec>;
   extern __shared__ float2 turns[];  // [token][pair]
-  __shared__ long long from[kMoveTokens], to[kMoveTokens];  // pool rows; a skipped token's are -1
+  __shared__ long long from[kMoveTokens], to[kMoveTokens];  // pool rows; a token that is skipped goes to -1
   __shared__ int still[kMoveTokens];
   const long long layer = blockIdx.y;
   const long long t0 = (long long)blockIdx.x * a.tokens;
   const int n_tok = (int)min((long long)a.tokens, a.n_tokens - t0);
-  S* kp = (S*)a.k_pool + layer * a.layer_stride;
-  S* vp = (S*)a.v_pool + layer * a.layer_stride;
   const int D = a.head_dim, half = a.shifts ? a.rope.half : 0;
 
   if ((int)threadIdx.x < n_tok) {
     const long long s = a.src[t0 + threadIdx.x], d = a.dst[t0 + threadIdx.x];
     const bool ok = s >= 0 && s < a.num_slots && d >= 0 && d < a.num_slots;
-    from[threadIdx.x] = ok ? s : -1, to[threadIdx.x] = ok ? d : -1;
+    from[threadIdx.x] = ok ? s : 0, to[threadIdx.x] = ok ? d : -1;
     still[threadIdx.x] = !a.shifts || a.shifts[t0 + threadIdx.x] == 0;
-    if (ok && layer == 0) move_weights(a.weights, a.num_kv_heads, s, d, 0, 1);
   }
   for (int i = threadIdx.x; i < n_tok * half; i += blockDim.x) {
     const int t = i / half;
@@ -67,39 +63,43 @@ __global__ __launch_bounds__(1024) void move_kernel(MoveArgs a) {
     turns[i] = make_float2(c, s);
   }
   __syncthreads();
+  if (layer == 0 && a.weights.sums)
+    for (int i = threadIdx.x; i < n_tok * a.num_kv_heads; i += blockDim.x) {
+      const int h = i / n_tok, t = i - h * n_tok;
+      if (to[t] >= 0) move_weights(a.weights, h + 1, from[t], to[t], h, 1);
+    }
 
   const int pair_pieces = half / kVec, pass_pieces = (D - 2 * half) / kVec;  // per head
   const int n_pair = a.num_kv_heads * pair_pieces, n_pass = a.num_kv_heads * pass_pieces, n_v = a.num_kv_heads * D / kVec;
+  S* kp = (S*)a.k_pool + layer * a.layer_stride;
+  S* vp = (S*)a.v_pool + layer * a.layer_stride;
   for (int task = threadIdx.x; task < n_pair + n_pass + n_v; task += blockDim.x) {
     if (task < n_pair) {
       const int h = task / pair_pieces, j = task - h * pair_pieces;
       const long long off = (long long)h * D + (long long)j * kVec;
-      for (int b = 0; b < n_tok; b += kMoveBatch) {
-        P x1[kMoveBatch], x2[kMoveBatch];
+      P x1[kMoveTokens], x2[kMoveTokens];
 #pragma unroll
-        for (int u = 0; u < kMoveBatch; ++u)
-          if (b + u < n_tok && from[b + u] >= 0) {
-            const S* row = kp + from[b + u] * a.pool_row_stride + off;
-            x1[u] = load_piece<S, kVec>(row);
-            x2[u] = load_piece<S, kVec>(row + half);
-          }
-#pragma unroll
-        for (int u = 0; u < kMoveBatch; ++u)
-          if (b + u < n_tok && from[b + u] >= 0) {
-            if (!still[b + u])
-#pragma unroll
-              for (int e = 0; e < kVec; ++e) {
-                const float2 cs = turns[(b + u) * half + j * kVec + e];
-                float r1, r2;
-                rope_pair<F32>(a.rope, cs.x, cs.y, E::load(x1[u].v[e]), E::load(x2[u].v[e]), r1, r2);
-                x1[u].v[e] = E::store(r1);
-                x2[u].v[e] = E::store(r2);
-              }
-            S* row = kp + to[b + u] * a.pool_row_stride + off;
-            store_piece<S, kVec>(row, x1[u]);
-            store_piece<S, kVec>(row + half, x2[u]);
-          }
+      for (int u = 0; u < kMoveTokens; ++u) {
+        const S* row = kp + from[min(u, n_tok - 1)] * a.pool_row_stride + off;
+        x1[u] = load_piece<S, kVec>(row);
+        x2[u] = load_piece<S, kVec>(row + half);
       }
+#pragma unroll
+      for (int u = 0; u < kMoveTokens; ++u)
+        if (u < n_tok && to[u] >= 0) {
+          if (!still[u])
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+              const float2 cs = turns[u * half + j * kVec + e];
+              float r1, r2;
+              rope_pair<F32>(a.rope, cs.x, cs.y, E::load(x1[u].v[e]), E::load(x2[u].v[e]), r1, r2);
+              x1[u].v[e] = E::store(r1);
+              x2[u].v[e] = E::store(r2);
+            }
+          S* row = kp + to[u] * a.pool_row_stride + off;
+          store_piece<S, kVec>(row, x1[u]);
+          store_piece<S, kVec>(row + half, x2[u]);
+        }
     } else {
       // plain pieces: the rest of K, then V
       S* pool = kp;
@@ -112,15 +112,12 @@ __global__ __launch_bounds__(1024) void move_kernel(MoveArgs a) {
         pool = vp;
         off = (long long)(t - n_pass) * kVec;
       }
-      for (int b = 0; b < n_tok; b += kMoveBatch) {
-        P x[kMoveBatch];
+      P x[kMoveTokens];
 #pragma unroll
-        for (int u = 0; u < kMoveBatch; ++u)
-          if (b + u < n_tok && from[b + u] >= 0) x[u] = load_piece<S, kVec>(pool + from[b + u] * a.pool_row_stride + off);
+      for (int u = 0; u < kMoveTokens; ++u) x[u] = load_piece<S, kVec>(pool + from[min(u, n_tok - 1)] * a.pool_row_stride + off);
 #pragma unroll
-        for (int u = 0; u < kMoveBatch; ++u)
-          if (b + u < n_tok && from[b + u] >= 0) store_piece<S, kVec>(pool + to[b + u] * a.pool_row_stride + off, x[u]);
-      }
+      for (int u = 0; u < kMoveTokens; ++u)
+        if (u < n_tok && to[u] >= 0) store_piece<S, kVec>(pool + to[u] * a.pool_row_stride + off, x[u]);
     }
   }
 }
@@ -158,7 +155,7 @@ extern "C" int va_move_kv(void* k_pool_dev, void* v_pool_dev, int64_t pool_row_s
                           int64_t n_tokens, float* weights_dev, const VaShape* shape, const VaRope* rope, void* stream) {
   if (!shape) return va_fail(VA_ERR_ARG, "null shape");
   if (n_tokens < 0 || num_layers < 0 || num_slots < 0) return va_fail(VA_ERR_ARG, "negative count");
-  if (n_tokens == 0 || num_layers == 0) return VA_OK;
+  if (n_tokens == 0 || num_layers == 0 || num_slots == 0) return VA_OK;
   if (!k_pool_dev || !v_pool_dev || !src_slots_dev || !dst_slots_dev) return va_fail(VA_ERR_ARG, "null pointer");
   if (shape->num_kv_heads <= 0 || shape->head_dim <= 0) return va_fail(VA_ERR_ARG, "bad shape");
   if (pool_row_stride < (int64_t)shape->num_kv_heads * shape->head_dim)

@@ -104,61 +104,80 @@ class RotaryEmbedding:
         self._turns = native.VaTurns(rotary_dim, int(self.interleaved), self.attention_factor, self._quarters.data_ptr())
 
     def _rows(self, x: torch.Tensor, n: int, name: str):
-        """``x`` as ``n`` rows of whole heads, and how many heads that is."""
-        if x.dim() == 3 and x.shape[2] == self.head_dim:
-            heads = x.shape[1]
-            if x.stride(2) != 1 or (heads > 1 and x.stride(1) != self.head_dim):
-                x = x.contiguous()
-        elif x.dim() == 2 and x.shape[1] % self.head_dim == 0:
-            heads = x.shape[1] // self.head_dim
-            if x.stride(1) != 1:
-                x = x.contiguous()
+        """``x`` as ``n`` rows of whole heads, how far apart they are, and how many heads that is."""
+        shape, dim = x.shape, self.head_dim
+        if len(shape) == 2 and shape[1] % dim == 0:
+            heads = shape[1] // dim
+            row, element = x.stride()
+            if element != 1:
+                x, row = x.contiguous(), heads * dim
+        elif len(shape) == 3 and shape[2] == dim:
+            heads = shape[1]
+            row, head, element = x.stride()
+            if element != 1 or (heads > 1 and head != dim):
+                x, row = x.contiguous(), heads * dim
         else:
-            raise ValueError(f"{name} must be rows of heads of {self.head_dim} elements, got {tuple(x.shape)}")
-        if x.shape[0] != n or x.device != self.device:
-            raise ValueError(f"{name} must be {n} rows on {self.device}, got {tuple(x.shape)} on {x.device}")
-        return x, heads
+            raise ValueError(f"{name} must be rows of heads of {dim} elements, got {tuple(shape)}")
+        if shape[0] != n or x.device != self.device:
+            native.require_device(x, name)
+            raise ValueError(f"{name} must be {n} rows on {self.device}, got {tuple(shape)} on {x.device}")
+        return x, row, heads
 
     def __call__(self, positions: torch.Tensor, q: torch.Tensor, k: Optional[torch.Tensor] = None,
                  out: Optional[tuple] = None):
         """``q`` and ``k`` (``[n, heads * head_dim]`` or ``[n, heads, head_dim]``, rows may lie apart) rotated by
         ``positions [n]`` (int64 or int32): new contiguous tensors, or ``out``, a pair that may be ``(q, k)`` themselves.
         ``k`` may be ``None``."""
-        native.require_device(q, "q")
-        device, n = self.device, q.shape[0]
-        if positions.dim() != 1 or positions.dtype not in (torch.int64, torch.int32) or positions.device != device \
+        device, n, wide = self.device, q.shape[0], positions.dtype is torch.int64
+        if not q.is_cuda:
+            native.require_device(q, "q")
+        if positions.dim() != 1 or not (wide or positions.dtype is torch.int32) or positions.device != device \
                 or positions.shape[0] != n:
             raise ValueError(f"positions must be {n} int64 or int32 numbers on {device}, got {positions.dtype} "
                              f"{tuple(positions.shape)} on {positions.device}")
-        if k is not None and k.dtype != q.dtype:
-            raise ValueError(f"q and k must be of one type, got {q.dtype} and {k.dtype}")
-        dtype = native.dtype_id(q.dtype)
-        q2, q_heads = self._rows(q, n, "q")
-        k2, k_heads = (None, 0) if k is None else self._rows(k, n, "k")
+        dtype = q.dtype
+        if k is not None and k.dtype is not dtype:
+            raise ValueError(f"q and k must be of one type, got {dtype} and {k.dtype}")
+        dtype_id = native.dtype_id(dtype)
+        q2, q_row, q_heads = self._rows(q, n, "q")
+        dim = self.head_dim
         if out is None:
-            out_q = torch.empty(q.shape, dtype=q.dtype, device=device)
-            out_k = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
-            q_out, k_out = out_q, out_k
+            out_q, out_k = torch.empty(q.shape, dtype=dtype, device=device), None
+            keys = (None, 0, 0, None, 0)
+            if k is not None:
+                k2, k_row, k_heads = self._rows(k, n, "k")
+                out_k = torch.empty(k.shape, dtype=dtype, device=device)
+                keys = (k2.data_ptr(), k_row, k_heads, out_k.data_ptr(), k_heads * dim)
+            queries = (q2.data_ptr(), q_row, q_heads, out_q.data_ptr(), q_heads * dim)
         else:
             out_q, out_k = out
-            q_out = self._out(out_q, q, n, "out[0]")
-            k_out = None if k is None else self._out(out_k, k, n, "out[1]")
+            queries = (q2.data_ptr(), q_row, q_heads, *self._out(out_q, q, q2, n, "out[0]"))
+            keys = (None, 0, 0, None, 0)
+            if k is not None:
+                k2, k_row, k_heads = self._rows(k, n, "k")
+                keys = (k2.data_ptr(), k_row, k_heads, *self._out(out_k, k, k2, n, "out[1]"))
         positions = positions.contiguous()
-        none = (None, 0, 0, None, 0)
-        native.call_on(
-            device, native.lib.va_rotate_qk, q2.data_ptr(), q2.stride(0), q_heads, q_out.data_ptr(), q_out.stride(0),
-            *(none if k is None else (k2.data_ptr(), k2.stride(0), k_heads, k_out.data_ptr(), k_out.stride(0))),
-            positions.data_ptr(), int(positions.dtype is torch.int64), n, self.head_dim, dtype, self._turns,
-            native.current_stream_ptr(device))
+        native.call_on(device, native.lib.va_rotate_qk, *queries, *keys, positions.data_ptr(), int(wide), n, dim, dtype_id,
+                       self._turns, native.current_stream_ptr(device))
         return out_q, out_k
 
-    def _out(self, y, x, n: int, name: str) -> torch.Tensor:
+    def _out(self, y, x, rows, n: int, name: str):
+        """Where the results of ``x`` go, ``y``, and how far apart its rows are; ``rows``: what is read of ``x``."""
         if not isinstance(y, torch.Tensor) or y.shape != x.shape or y.dtype != x.dtype or y.device != self.device:
             raise ValueError(f"{name} must be a {x.dtype} tensor {tuple(x.shape)} on {self.device}")
-        inner = y.stride()[1:]
-        if inner != ((1,) if y.dim() == 2 else (self.head_dim, 1)) or (n > 1 and y.stride(0) < x[0].numel()):
+        width, stride = x[:1].numel(), y.stride()
+        inner = stride[1:] == (1,) if len(stride) == 2 else stride[2] == 1 and (y.shape[1] <= 1 or stride[1] == self.head_dim)
+        if not inner or (n > 1 and stride[0] < width):
             raise ValueError(f"{name} must have contiguous rows that do not overlap")
-        return y
+        # results over the input row by row, or apart from it
+        if n and y.untyped_storage().data_ptr() == rows.untyped_storage().data_ptr():
+            a, b, step = rows.data_ptr(), y.data_ptr(), y.element_size()
+            same = a == b and (n == 1 or stride[0] == rows.stride(0))
+            ends = [(p, p + ((n - 1) * s + width) * step) for p, s in ((a, rows.stride(0)), (b, stride[0]))]
+            beside = n > 1 and stride[0] == rows.stride(0) and width * step <= abs(b - a) % (stride[0] * step) <= (stride[0] - width) * step
+            if not same and not beside and ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]:
+                raise ValueError(f"{name} must be the input itself or lie apart from it")
+        return y.data_ptr(), stride[0] if n > 1 else width
 
     def cos_sin_cache(self, max_position: int) -> torch.Tensor:
         """The fp32 ``[max_position, rotary_dim]`` table of cosines and sines that ``SharedCacheAttention`` takes.  Its keys and

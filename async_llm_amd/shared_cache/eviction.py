@@ -25,13 +25,13 @@ from __future__ import annotations
 import ctypes
 import numbers
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Union
+from typing import Dict, List, Optional, Sequence, Union
 
 import numpy as np
 import torch
 
 from .. import native
-from ..kvcache.mha_pool import layer_runs
+from ..kvcache.mha_pool import MHAKVCache, layer_runs
 from ..kvcache.quantized_pool import QuantizedKVCache
 from .attention import SharedCacheAttention, SharedCacheAttnMetadata
 
@@ -40,13 +40,10 @@ from .attention import SharedCacheAttention, SharedCacheAttnMetadata
 class WeightPlan:
     """Who sees which token in a step, by token; serves all layers of the step."""
 
-    header: np.ndarray  # int32, host
-    blob: torch.Tensor  # int32, device
-    counts: native.VaWeighCounts
-    sub_worker: torch.Tensor
-    sub_loc: torch.Tensor
     rows: int  # query rows of the step
-    refs: tuple = ()
+    counts: native.VaWeighCounts
+    tables: tuple  # what the library takes of it: addresses of the plan and its header, of the step's rows and positions
+    refs: tuple  # the tensors and arrays behind those
 
 
 @dataclass
@@ -80,6 +77,9 @@ class CacheEviction:
         self.num_slots = self.num_pages * op.page_size
         if self.num_slots > 2**31 - 1:
             raise ValueError(f"{self.num_pages} pages of {op.page_size} tokens are more slots than 32 bits address")
+        self._weights_shape = (op.num_kv_heads, self.num_slots)
+        self._key_addresses: Dict[int, int] = {}
+        self._moved: Optional[list] = None
 
     # ------------------------------------------------------------------
     # weights
@@ -89,11 +89,11 @@ class CacheEviction:
         return torch.zeros((self.op.num_kv_heads, self.num_slots), dtype=torch.float32, device=self.device)
 
     def _check_weights(self, weights: torch.Tensor, name: str = "weights") -> None:
-        want = (self.op.num_kv_heads, self.num_slots)
-        if weights.shape != want or weights.dtype != torch.float32 or weights.device != self.device or not weights.is_contiguous():
+        if weights.shape != self._weights_shape or weights.dtype is not torch.float32 or weights.device != self.device \
+                or not weights.is_contiguous():
             native.require_device(weights, name)
-            raise ValueError(f"{name} must be a contiguous float32 tensor {list(want)} on {self.device}, got {weights.dtype} "
-                             f"{list(weights.shape)} on {weights.device}")
+            raise ValueError(f"{name} must be a contiguous float32 tensor {list(self._weights_shape)} on {self.device}, got "
+                             f"{weights.dtype} {list(weights.shape)} on {weights.device}")
 
     def clear(self, weights: torch.Tensor, slots: torch.Tensor) -> None:
         """Forget what the tokens of ``slots`` (int64) were given."""
@@ -124,8 +124,10 @@ class CacheEviction:
         host = torch.empty(counts.plan_words, dtype=torch.int32, pin_memory=self.device.type == "cuda")
         host.numpy()[:] = words[: counts.plan_words]
         blob = host.to(self.device, non_blocking=True)
-        return WeightPlan(words[: native.WEIGH_HEADER_WORDS].copy(), blob, counts, meta.sub_worker, meta.sub_loc, meta.num_workers,
-                          (host,))
+        header, sub_loc = words[: native.WEIGH_HEADER_WORDS].copy(), meta.sub_loc
+        tables = (blob.data_ptr(), header.ctypes.data, meta.sub_worker.data_ptr(), sub_loc.data_ptr(),
+                  sub_loc.stride(0) if sub_loc.dim() == 2 else 0)
+        return WeightPlan(meta.num_workers, counts, tables, (host, blob, header, meta.sub_worker, sub_loc))
 
     def accumulate(self, q: torch.Tensor, lse: torch.Tensor, layer_id: int, plan: WeightPlan, weights: torch.Tensor,
                    out: Optional[torch.Tensor] = None, lse_base2: bool = False) -> torch.Tensor:
@@ -133,35 +135,47 @@ class CacheEviction:
         to ``weights``, and return it.  ``lse [rows, q_heads]``: the log-sums that ``forward_with_lse`` returned for the same
         queries.  With ``out`` the sums of the tokens in sight go there instead, and ``weights`` and the other slots of
         ``out`` stay as they are."""
-        op, device = self.op, self.device
-        native.require_device(q, "q")
+        if not q.is_cuda:
+            native.require_device(q, "q")
+        op, device, rows = self.op, self.device, plan.rows
         q2, q_stride = op._rows(q, op.num_qo_heads)
-        if q2.dtype != op.dtype or q2.device != device or q2.shape[0] < plan.rows:
-            raise ValueError(f"q must be {plan.rows} rows of {op.dtype} on {device}, got {q2.dtype} {tuple(q2.shape)} on {q2.device}")
-        if lse.dim() != 2 or lse.shape[0] < plan.rows or lse.shape[1] != op.num_qo_heads or lse.dtype != torch.float32 \
+        if q2.dtype is not op.dtype or q2.device != device or q2.shape[0] < rows:
+            raise ValueError(f"q must be {rows} rows of {op.dtype} on {device}, got {q2.dtype} {tuple(q2.shape)} on {q2.device}")
+        shape = lse.shape
+        if len(shape) != 2 or shape[0] < rows or shape[1] != op.num_qo_heads or lse.dtype is not torch.float32 \
                 or lse.device != device or not lse.is_contiguous():
-            raise ValueError(f"lse must be a contiguous float32 tensor [{plan.rows}, {op.num_qo_heads}] on {device}, got {lse.dtype} "
-                             f"{tuple(lse.shape)} on {lse.device}")
+            raise ValueError(f"lse must be a contiguous float32 tensor [{rows}, {op.num_qo_heads}] on {device}, got {lse.dtype} "
+                             f"{tuple(shape)} on {lse.device}")
         self._check_weights(weights)
         if out is None:
             out = weights
         else:
             self._check_weights(out, "out")
         # (from the allocator, call by call: streams and graphs that share a plan have scratch of their own)
-        workspace = torch.empty(plan.counts.workspace_bytes, dtype=torch.uint8, device=device)
-        sub_loc = plan.sub_loc
-        tables = (plan.blob.data_ptr(), plan.header.ctypes.data, plan.sub_worker.data_ptr(), sub_loc.data_ptr(),
-                  sub_loc.stride(0) if sub_loc.dim() == 2 else 0, lse.data_ptr(), int(lse_base2), weights.data_ptr(),
-                  out.data_ptr(), workspace.data_ptr(), plan.counts.workspace_bytes, op._shape, op._rope_descriptor(),
-                  native.current_stream_ptr(device))
+        nbytes = plan.counts.workspace_bytes
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        tables = (*plan.tables, lse.data_ptr(), int(lse_base2), weights.data_ptr(), out.data_ptr(), workspace.data_ptr(), nbytes,
+                  op._shape, op._rope_descriptor(), native.current_stream_ptr(device))
         if self._coded:
             native.call_on(device, native.lib.va_weigh_q8, q2.data_ptr(), q_stride, self.kv_cache.layer(layer_id), *tables)
-            return out
-        pool = self.kv_cache.k_cache(layer_id)
-        if pool.shape[0] != self.num_pages or pool.dtype != op.dtype or not pool.is_contiguous():
-            raise ValueError(f"kv_cache.k_cache({layer_id}) must be a contiguous {op.dtype} tensor of {self.num_pages} pages")
-        native.call_on(device, native.lib.va_weigh, q2.data_ptr(), q_stride, pool.data_ptr(), op.num_kv_heads * op.head_dim, *tables)
+        else:
+            native.call_on(device, native.lib.va_weigh, q2.data_ptr(), q_stride, self._keys_at(layer_id),
+                           op.num_kv_heads * op.head_dim, *tables)
         return out
+
+    def _keys_at(self, layer_id: int) -> int:
+        """Address of a layer's keys, asked for once where the pool is this package's own, whose arrays stay."""
+        at = self._key_addresses.get(layer_id)
+        if at is None:
+            pool, op = self.kv_cache.k_cache(layer_id), self.op
+            if tuple(pool.shape) != (self.num_pages, op.page_size, op.num_kv_heads, op.head_dim) or pool.dtype != op.dtype \
+                    or pool.device != self.device or not pool.is_contiguous():
+                raise ValueError(f"kv_cache.k_cache({layer_id}) must be a contiguous {op.dtype} tensor of {self.num_pages} pages on "
+                                 f"{self.device}")
+            at = pool.data_ptr()
+            if type(self.kv_cache) is MHAKVCache:
+                self._key_addresses[layer_id] = at
+        return at
 
     # ------------------------------------------------------------------
     # choosing
@@ -212,23 +226,39 @@ class CacheEviction:
         for name, t in (("source", source), ("target", target), ("shifts", shifts)):
             if t is None and name == "shifts":
                 continue
-            native.require_device(t, name)
-            if t.dim() != 1 or t.dtype != torch.int64 or t.device != device or t.numel() != n:
+            if t.dim() != 1 or t.dtype is not torch.int64 or t.device != device or t.numel() != n:
+                native.require_device(t, name)
                 raise ValueError(f"{name} must be one row of {n} int64 numbers on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        native.require_device(source, "source")
         if weights is not None:
             self._check_weights(weights)
-        pool, source, target = self.kv_cache, source.contiguous(), target.contiguous()
+        source, target = source.contiguous(), target.contiguous()
         shifts = None if shifts is None else shifts.contiguous()
-        slots = (source.data_ptr(), target.data_ptr(), None if shifts is None else shifts.data_ptr(), n)
-        rope = None if shifts is None else op._rope_descriptor()
+        rest = (source.data_ptr(), target.data_ptr(), None if shifts is None else shifts.data_ptr(), n)
+        shape, rope, stream = op._shape, None if shifts is None else op._rope_descriptor(), native.current_stream_ptr(device)
         sums = None if weights is None else weights.data_ptr()
         if self._coded:
+            pool = self.kv_cache
             if pool.num_layers:
                 native.call_on(device, native.lib.va_move_kv_q8, pool.layer(0), pool.code_layer_bytes, pool.scale_layer_bytes,
-                               pool.num_layers, *slots, sums, op._shape, rope, native.current_stream_ptr(device))
+                               pool.num_layers, *rest, sums, shape, rope, stream)
             return
-        width, stream = op.num_kv_heads * op.head_dim, native.current_stream_ptr(device)
-        for first, count, stride in layer_runs(pool):
-            native.call_on(device, native.lib.va_move_kv, pool.k_cache(first).data_ptr(), pool.v_cache(first).data_ptr(), width,
-                           stride, count, self.num_slots, *slots, sums, op._shape, rope, stream)
+        for run in self._layers_at():
+            native.call_on(device, native.lib.va_move_kv, *run, *rest, sums, shape, rope, stream)
             sums = None  # (moved with the first run)
+
+    def _layers_at(self) -> list:
+        """Where the pool's layers lie, as the library takes them; found once where the pool is this package's own."""
+        runs = self._moved
+        if runs is None:
+            pool, op = self.kv_cache, self.op
+            for layer in range(pool.num_layers):
+                op._check_pool_layout(layer)
+                if pool.k_cache(layer).shape[0] != self.num_pages or pool.v_cache(layer).shape[0] != self.num_pages:
+                    raise ValueError(f"layer {layer} of kv_cache must hold {self.num_pages} pages")
+            width = op.num_kv_heads * op.head_dim
+            runs = [(pool.k_cache(first).data_ptr(), pool.v_cache(first).data_ptr(), width, stride, count, self.num_slots)
+                    for first, count, stride in layer_runs(pool)]
+            if type(pool) is MHAKVCache:
+                self._moved = runs
+        return runs

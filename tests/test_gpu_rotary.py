@@ -137,5 +137,12 @@ def test_refusals(dev):
             r(at, q, out=out)
     with pytest.raises(ValueError, match="overlap"):
         r(at, q, out=(torch.zeros(200, device=dev).as_strided((4, 128), (10, 1)), None))
+    both = torch.randn(5, 300, device=dev)
+    for bad in (both[1:, :128], both[:4, 8:136]):  # results over rows that are still to be read
+        with pytest.raises(ValueError, match="apart"):
+            r(at, both[:4, :128], out=(bad, None))
+    want = r(at, both[:4, :128].clone())[0]
+    r(at, both[:4, :128], out=(both[:4, 140: 268], None))  # beside them
+    assert torch.equal(both[:4, 140: 268], want)
     with pytest.raises(ValueError, match="max_position"):
         r.cos_sin_cache(0)
