@@ -15,12 +15,13 @@
 // Spans whose tokens have more than one tile of 16 (row, q head) pairs are cut into tile items of this many tokens (16-bit rows and
 // codes, head dims of the matrix cores), the others into items of strips: see va_weigh.hip.
 #define VA_WEIGH_TILE_TOKENS 256
+#define VA_WEIGH_TILE_ROWS 32  // (row, q head) pairs of a tile of tile items; 16 in strips
 
 // header word indices
 enum {
   VA_WH_MAGIC = 0,
   VA_WH_N_ITEMS,   // tile items first, then those of strips
-  VA_WH_N_ROWS,    // packed rows: a multiple of what makes whole tiles of 16 (row, q head) pairs
+  VA_WH_N_ROWS,    // packed rows, padded to whole tiles of (row, q head) pairs
   VA_WH_N_JOINS,
   VA_WH_N_PARTIALS,  // partial sums, in tokens (per kv head)
   VA_WH_N_PAGES,
@@ -47,7 +48,7 @@ enum {
   VA_WI_PAGES = 0,   // first entry of the span's pages
   VA_WI_FIRST,       // first token of the chunk, within the span
   VA_WI_N_TOK,
-  VA_WI_TILE_BEGIN,  // tiles of 16 (row, q head) pairs
+  VA_WI_TILE_BEGIN,  // tiles of (row, q head) pairs
   VA_WI_TILE_END,
   VA_WI_PARTIAL,     // where its sums go, in tokens; -1: it adds them to the weights itself
 };

@@ -93,6 +93,7 @@ struct Planner {
     int64_t page_begin;
     int32_t first, end;  // tokens that anybody sees
     int64_t row_begin, row_end;  // packed
+    int pairs;  // of a tile
   };
   std::vector<Span> spans;
   std::vector<int32_t> run_pages;  // pages by span, before it is known which spans come first
@@ -136,7 +137,7 @@ struct Planner {
 
   int find_spans() {
     find_runs();
-    const int G = shape.num_q_heads / shape.num_kv_heads, unit = 16 / std::gcd(16, G);
+    const int G = shape.num_q_heads / shape.num_kv_heads;
     const bool halves = !rows32 && (shape.head_dim == 64 || shape.head_dim == 128 || shape.head_dim == 256);
     const size_t n = run_begin.size() - 1;
     std::vector<char> many(n, 0);
@@ -146,6 +147,7 @@ struct Planner {
       many[i] = rows * G > 16;
     }
     for (int which = 1; which >= 0; --which) {  // those of tile items first
+      const int pairs = which ? VA_WEIGH_TILE_ROWS : 16, unit = pairs / std::gcd(pairs, G);
       for (size_t i = 0; i < n; ++i) {
         if (many[i] != which) continue;
         const int64_t row_begin = (int64_t)sub_row.size();
@@ -158,7 +160,7 @@ struct Planner {
         while (sub_row.size() % unit) sub_row.push_back(-1), lo.push_back(0), hi.push_back(0);
         if ((int64_t)sub_row.size() * G > INT32_MAX / 16)  // (a thread for each 16 elements of a row)
           return va_fail(VA_ERR_ARG, "too many query rows for one plan");
-        spans.push_back(Span{(int64_t)pages.size(), first, end, row_begin, (int64_t)sub_row.size()});
+        spans.push_back(Span{(int64_t)pages.size(), first, end, row_begin, (int64_t)sub_row.size(), pairs});
         pages.insert(pages.end(), run_pages.begin() + run_begin[i], run_pages.begin() + run_begin[i + 1]);
       }
       if (which) n_tile_spans = spans.size(), n_tile_rows = (int64_t)sub_row.size();
@@ -184,7 +186,7 @@ struct Planner {
     int64_t a = s.row_begin, b = s.row_end;
     while (a < b && (hi[(size_t)a] <= begin || lo[(size_t)a] >= end)) ++a;
     while (b > a && (hi[(size_t)b - 1] <= begin || lo[(size_t)b - 1] >= end)) --b;
-    tile_a = a * G / 16, tile_b = a == b ? tile_a : (b * G + 15) / 16;
+    tile_a = a * G / s.pairs, tile_b = a == b ? tile_a : (b * G + s.pairs - 1) / s.pairs;
   }
   // Tokens [begin, begin + n_tok) under tiles [tile_a, tile_b), in `parts` items: `each(part, item words)`.
   template <typename F>
@@ -205,8 +207,8 @@ struct Planner {
     return VA_OK;
   }
 
-  // Tile items of 256 tokens, with as many rows as make about 2048 workgroups of equal products, but not fewer than eight tiles, nor
-  // less than takes as long as a strip beside them (whose token takes about sixteen times as long as a token's one tile of rows).
+  // Tile items of 256 tokens, with as many rows as make about 2048 workgroups of equal products, but not fewer than four tiles, nor
+  // less than takes as long as a strip beside them (whose token takes about eight times as long as a token's one tile of rows).
   int make_tiles() {
     int64_t products = 0, walked = 0, tile_a, tile_b;  // (token, tile of rows); tokens of strips
     for (size_t i = 0; i < spans.size(); ++i) {
@@ -219,7 +221,7 @@ struct Planner {
       }
     }
     const int64_t T = VA_WEIGH_TILE_TOKENS, hkv = shape.num_kv_heads;
-    const int64_t most = std::max({8 * T, products * hkv / 2048, 16 * walked * hkv / kWorkgroups});
+    const int64_t most = std::max({4 * T, products * hkv / 2048, 8 * walked * hkv / kWorkgroups});
     for (size_t i = 0; i < n_tile_spans; ++i) {
       const Span& s = spans[i];
       for (int64_t t = s.first; t < s.end; t += T) {

@@ -35,7 +35,7 @@ def counted(words, heads, page, dtype=native.VA_BF16):
     g = heads[0] // heads[1]
     n_tile_items, n_tile_rows, n_strips = h[18], h[19], h[20]
     strips = words[h[21]: h[21] + n_strips + 1]
-    assert n_rows * g % 16 == 0 and n_tile_items % 8 == 0 and n_tile_rows * g % 16 == 0
+    assert n_rows * g % 16 == 0 and n_tile_items % 8 == 0 and n_tile_rows * g % 32 == 0
     if n_items > n_tile_items:  # strips hold every other item once
         assert n_strips % 8 == 0 and strips[0] == n_tile_items and strips[-1] == n_items and (np.diff(strips) >= 0).all()
     pairs, owners, parts = {}, {}, {}
@@ -43,11 +43,11 @@ def counted(words, heads, page, dtype=native.VA_BF16):
         if n == 0:
             assert k < n_tile_items
             continue
-        first_rows = n_tile_rows * g // 16
-        assert end <= first_rows and n <= 256 if k < n_tile_items else begin >= first_rows
+        of_tile = 32 if k < n_tile_items else 16  # (row, q head) pairs
+        assert end * 32 <= n_tile_rows * g and n <= 256 if k < n_tile_items else begin * 16 >= n_tile_rows * g
         if k >= n_tile_items and dtype != native.VA_F32 and heads[2] == 64:
             assert end == begin + 1
-        assert 0 < n and 0 <= begin < end <= n_rows * g // 16
+        assert 0 < n and 0 <= begin < end <= n_rows * g // of_tile
         slots = [int(pages[first_page + t // page]) * page + t % page for t in range(first, first + n)]
         if partial >= 0:
             parts[int(partial)] = (int(first_page), int(first), int(n))
@@ -56,7 +56,7 @@ def counted(words, heads, page, dtype=native.VA_BF16):
             for s in slots:
                 owners[s] = owners.get(s, 0) + 1
         # (q heads of a row may lie in two tiles of an item that splits: count them)
-        for p in range(begin * 16, end * 16):
+        for p in range(begin * of_tile, end * of_tile):
             r = p // g
             if sub[r] >= 0:
                 for t, s in zip(range(first, first + n), slots):
