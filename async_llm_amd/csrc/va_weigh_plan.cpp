@@ -1,8 +1,11 @@
 // Host side of attention weights: the sub-request tables of a step, turned round (va_weigh.h).
 #include <algorithm>
 #include <climits>
+#include <cstring>
 #include <numeric>
 #include <stdexcept>
+#include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include "../../include/viewattn.h"
@@ -12,10 +15,10 @@
 namespace {
 
 struct Visitor {
-  int32_t sub;
+  int32_t list;  // one of `lists`
   int32_t entry;  // of its list
   int32_t place;  // -1: the whole page; a token of it, for lists of slots
-  bool operator==(const Visitor& o) const { return sub == o.sub && entry == o.entry && place == o.place; }
+  bool operator==(const Visitor& o) const { return list == o.list && entry == o.entry && place == o.place; }
 };
 
 struct Planner {
@@ -24,7 +27,17 @@ struct Planner {
   bool rows32;  // 32-bit keys
   int num_pages, window;
   Planner(const VaSubRequests& s, const VaShape& sh, bool wide, int pages_, int w) : in(s), shape(sh), rows32(wide), num_pages(pages_), window(w) {}
-  std::vector<int64_t> first_visitor;  // by page, [num_pages + 1]
+  // Lists of entries that differ: readers of a shared block bring the same one, which is then looked through once.
+  struct List {
+    const int32_t* at;
+    int32_t entries;
+    bool by_slot;
+    int32_t first_reader, last_reader;  // sub-requests, linked by next_reader
+    bool alone;                         // none of its pages is another entry's too
+  };
+  std::vector<List> lists;
+  std::vector<int32_t> next_reader;  // by sub-request; -1 behind the last
+  std::vector<int32_t> first_visitor;  // by page, [num_pages + 1]
   std::vector<Visitor> visitors;
   std::vector<int32_t> pages, items, joins, sub_row, lo, hi;
   int64_t n_partials = 0;
@@ -39,53 +52,90 @@ struct Planner {
   bool slots(int s) const { return in.flags[s] & VA_SUB_SLOTS; }
   int64_t entries(int s) const { return slots(s) ? in.seq_lens[s] : ((int64_t)in.seq_lens[s] + shape.page_size - 1) / shape.page_size; }
 
-  int check() const {
+  int find_lists() {
     if (in.n_sub < 0 || in.n_subrows < 0) return va_fail(VA_ERR_ARG, "negative count");
     if (in.n_sub == 0) return VA_OK;
     if (!in.qo_indptr || !in.kv_indptr || !in.seq_lens || !in.flags) return va_fail(VA_ERR_ARG, "null table");
     if (in.qo_indptr[0] != 0 || in.qo_indptr[in.n_sub] != in.n_subrows || in.kv_indptr[0] != 0)
       return va_fail(VA_ERR_ARG, "tables do not start at 0 or end at n_subrows");
     const int64_t pool = (int64_t)num_pages * shape.page_size;
+    next_reader.assign((size_t)in.n_sub, -1);
+    std::unordered_multimap<int32_t, int32_t> by_first;  // first entry -> list
     for (int s = 0; s < in.n_sub; ++s) {
       if (in.qo_indptr[s + 1] < in.qo_indptr[s] || in.kv_indptr[s + 1] < in.kv_indptr[s] || in.seq_lens[s] < 0)
         return va_fail(VA_ERR_ARG, "sub-request %d: tables must not fall", s);
       const int64_t n = entries(s);
       if (n > in.kv_indptr[s + 1] - in.kv_indptr[s]) return va_fail(VA_ERR_ARG, "sub-request %d: %d tokens in %d entries", s, in.seq_lens[s], in.kv_indptr[s + 1] - in.kv_indptr[s]);
-      if (n && !in.kv_indices) return va_fail(VA_ERR_ARG, "null table");
-      for (int64_t e = 0; e < n; ++e) {
-        const int32_t x = in.kv_indices[in.kv_indptr[s] + e];
-        if (x < 0 || x >= (slots(s) ? pool : num_pages))
-          return va_fail(VA_ERR_ARG, "%s %d lies outside the pool of %d pages of %d tokens", slots(s) ? "slot" : "page", x, num_pages, shape.page_size);
+      if (n == 0) continue;
+      if (!in.kv_indices) return va_fail(VA_ERR_ARG, "null table");
+      const List list{in.kv_indices + in.kv_indptr[s], (int32_t)n, slots(s), s, s, false};
+      int32_t known = -1;
+      for (auto [i, end] = by_first.equal_range(list.at[0]); i != end && known < 0; ++i) {
+        const List& o = lists[(size_t)i->second];
+        if (o.entries == list.entries && o.by_slot == list.by_slot && !std::memcmp(o.at, list.at, (size_t)n * 4)) known = i->second;
+      }
+      const int32_t limit = list.by_slot ? (int32_t)pool : num_pages;
+      if (const int32_t* bad = known < 0 ? outside(list, limit) : nullptr)
+        return va_fail(VA_ERR_ARG, "%s %d lies outside the pool of %d pages of %d tokens", list.by_slot ? "slot" : "page", *bad, num_pages, shape.page_size);
+      if (rows_of(s) == 0) continue;
+      if (known < 0) {
+        by_first.emplace(list.at[0], (int32_t)lists.size());
+        lists.push_back(list);
+      } else {
+        List& o = lists[(size_t)known];
+        o.last_reader = next_reader[(size_t)o.last_reader] = s;
       }
     }
     return VA_OK;
   }
 
+  static const int32_t* outside(const List& list, int32_t limit) {
+    int32_t any = 0;
+    for (int32_t e = 0; e < list.entries; ++e) any |= (list.at[e] < 0) | (list.at[e] >= limit);
+    return any ? std::find_if(list.at, list.at + list.entries, [&](int32_t x) { return x < 0 || x >= limit; }) : nullptr;
+  }
+
+  // Who visits the pages of the lists that are not alone.
   void find_visitors() {
-    first_visitor.assign((size_t)num_pages + 1, 0);
     const int P = shape.page_size;
-    auto each = [&](auto&& f) {
-      for (int s = 0; s < in.n_sub; ++s) {
-        if (rows_of(s) == 0) continue;
-        const int32_t* list = in.kv_indices + in.kv_indptr[s];
-        const bool by_slot = slots(s);
-        for (int64_t e = 0, n = entries(s); e < n; ++e) by_slot ? f(list[e] / P, Visitor{s, (int32_t)e, list[e] % P}) : f(list[e], Visitor{s, (int32_t)e, -1});
-      }
+    first_visitor.assign((size_t)num_pages + 1, 0);
+    auto count = [&](const List& list) {
+      for (int32_t e = 0; e < list.entries; ++e) ++first_visitor[(size_t)(list.by_slot ? list.at[e] / P : list.at[e])];
     };
-    each([&](int32_t page, const Visitor&) { ++first_visitor[page + 1]; });
-    for (int p = 0; p < num_pages; ++p) first_visitor[p + 1] += first_visitor[p];
-    visitors.resize((size_t)first_visitor[num_pages]);
-    std::vector<int64_t> at(first_visitor.begin(), first_visitor.end() - 1);
-    each([&](int32_t page, const Visitor& v) { visitors[(size_t)at[page]++] = v; });
+    for (const List& list : lists) count(list);
+    bool others = false;
+    for (List& list : lists) {
+      int32_t more = 0;
+      for (int32_t e = 0; e < list.entries && !list.by_slot; ++e) more |= first_visitor[(size_t)list.at[e]] - 1;
+      list.alone = !list.by_slot && more == 0;
+      others = others || !list.alone;
+    }
+    if (!others) return;
+    first_visitor.assign((size_t)num_pages + 1, 0);
+    for (const List& list : lists)
+      if (!list.alone) count(list);
+    int32_t sum = 0;  // (of entries, which 32 bits count)
+    for (int32_t& n : first_visitor) sum += n, n = sum;
+    visitors.resize((size_t)sum);
+    // (from the last to the first: what was a page's end becomes its beginning)
+    for (size_t l = lists.size(); l-- > 0;) {
+      const List& list = lists[l];
+      if (list.alone) continue;
+      for (int32_t e = list.entries; e-- > 0;) {
+        const int32_t x = list.at[e];
+        const Visitor v = list.by_slot ? Visitor{(int32_t)l, e, x % P} : Visitor{(int32_t)l, e, -1};
+        visitors[(size_t)--first_visitor[(size_t)(list.by_slot ? x / P : x)]] = v;
+      }
+    }
   }
 
   // Whether the sub-requests that read page a read page b as their next one, and nobody else does.
   bool follows(int32_t a, int32_t b) const {
-    const int64_t n = first_visitor[a + 1] - first_visitor[a];
+    const int32_t n = first_visitor[a + 1] - first_visitor[a];
     if (n != first_visitor[b + 1] - first_visitor[b]) return false;
     const Visitor *x = &visitors[(size_t)first_visitor[a]], *y = &visitors[(size_t)first_visitor[b]];
-    for (int64_t i = 0; i < n; ++i)
-      if (x[i].place >= 0 || !(Visitor{x[i].sub, x[i].entry + 1, -1} == y[i])) return false;
+    for (int32_t i = 0; i < n; ++i)
+      if (x[i].place >= 0 || !(Visitor{x[i].list, x[i].entry + 1, -1} == y[i])) return false;
     return true;
   }
 
@@ -96,40 +146,53 @@ struct Planner {
     int pairs;  // of a tile
   };
   std::vector<Span> spans;
-  std::vector<int32_t> run_pages;  // pages by span, before it is known which spans come first
-  std::vector<int64_t> run_begin;
+  // Pages that follow one another for all who read them: a list that is alone, or some of run_pages.
+  struct Run {
+    int32_t list;  // -1: run_pages
+    int64_t begin, end;
+  };
+  std::vector<int32_t> run_pages;
+  std::vector<Run> runs;
 
   void find_runs() {
-    std::vector<char> done((size_t)num_pages, 0);
-    int32_t before = -1;
-    for (int s = 0; s < in.n_sub; ++s) {
-      if (rows_of(s) == 0) continue;
-      const int32_t* list = in.kv_indices + in.kv_indptr[s];
-      for (int64_t e = 0, n = entries(s); e < n; ++e) {
-        const int32_t page = slots(s) ? list[e] / shape.page_size : list[e];
+    std::vector<char> done;
+    for (size_t l = 0; l < lists.size(); ++l) {
+      const List& list = lists[l];
+      if (list.alone) {
+        runs.push_back(Run{(int32_t)l, 0, list.entries});
+        continue;
+      }
+      if (done.empty()) done.assign((size_t)num_pages, 0);
+      int32_t before = -1;
+      for (int32_t e = 0; e < list.entries; ++e) {
+        const int32_t page = list.by_slot ? list.at[e] / shape.page_size : list.at[e];
         if (done[page]) continue;
         done[page] = 1;
-        if (before < 0 || !follows(before, page)) run_begin.push_back((int64_t)run_pages.size());
+        if (before < 0 || !follows(before, page)) runs.push_back(Run{-1, (int64_t)run_pages.size(), 0});
         run_pages.push_back(before = page);
+        runs.back().end = (int64_t)run_pages.size();
       }
     }
-    run_begin.push_back((int64_t)run_pages.size());
   }
 
   // Rows of a run's visitors that see any of it: `each(sub-row, first token, end)`.
   template <typename F>
-  void rows_of_run(int64_t begin, int64_t end, F&& each) const {
+  void rows_of_run(const Run& run, F&& each) const {
     const int P = shape.page_size;
-    const int64_t room = (end - begin) * P;  // (within the pool, whose slots 32 bits count)
-    const int32_t page = run_pages[(size_t)begin];
-    for (int64_t k = first_visitor[page]; k < first_visitor[page + 1]; ++k) {
-      const Visitor& v = visitors[(size_t)k];
-      for (int i = skipped(v.sub); i < rows_of(v.sub); ++i) {
-        int64_t from = 0, to = std::min(room, seen(v.sub, i) - (int64_t)v.entry * P);
-        if (v.place >= 0) from = v.place, to = seen(v.sub, i) > v.entry ? v.place + 1 : 0;
-        if (to > from) each(in.qo_indptr[v.sub] + i, (int32_t)from, (int32_t)to);
-      }
+    const int64_t room = (run.end - run.begin) * P;  // (within the pool, whose slots 32 bits count)
+    const Visitor itself{run.list, 0, -1};
+    const Visitor *v = &itself, *last = v + 1;
+    if (run.list < 0) {
+      const int32_t page = run_pages[(size_t)run.begin];
+      v = visitors.data() + first_visitor[page], last = visitors.data() + first_visitor[page + 1];
     }
+    for (; v < last; ++v)
+      for (int32_t s = lists[(size_t)v->list].first_reader; s >= 0; s = next_reader[(size_t)s])
+        for (int i = skipped(s); i < rows_of(s); ++i) {
+          int64_t from = 0, to = std::min(room, seen(s, i) - (int64_t)v->entry * P);
+          if (v->place >= 0) from = v->place, to = seen(s, i) > v->entry ? v->place + 1 : 0;
+          if (to > from) each(in.qo_indptr[s] + i, (int32_t)from, (int32_t)to);
+        }
   }
 
   size_t n_tile_spans = 0;
@@ -139,11 +202,11 @@ struct Planner {
     find_runs();
     const int G = shape.num_q_heads / shape.num_kv_heads;
     const bool halves = !rows32 && (shape.head_dim == 64 || shape.head_dim == 128 || shape.head_dim == 256);
-    const size_t n = run_begin.size() - 1;
+    const size_t n = runs.size();
     std::vector<char> many(n, 0);
     for (size_t i = 0; i < n && halves; ++i) {
       int64_t rows = 0;
-      rows_of_run(run_begin[i], run_begin[i + 1], [&](int32_t, int32_t, int32_t) { ++rows; });
+      rows_of_run(runs[i], [&](int32_t, int32_t, int32_t) { ++rows; });
       many[i] = rows * G > 16;
     }
     for (int which = 1; which >= 0; --which) {  // those of tile items first
@@ -152,7 +215,7 @@ struct Planner {
         if (many[i] != which) continue;
         const int64_t row_begin = (int64_t)sub_row.size();
         int32_t first = INT32_MAX, end = 0;
-        rows_of_run(run_begin[i], run_begin[i + 1], [&](int32_t row, int32_t from, int32_t to) {
+        rows_of_run(runs[i], [&](int32_t row, int32_t from, int32_t to) {
           sub_row.push_back(row), lo.push_back(from), hi.push_back(to);
           first = std::min(first, from), end = std::max(end, to);
         });
@@ -161,7 +224,8 @@ struct Planner {
         if ((int64_t)sub_row.size() * G > INT32_MAX / 16)  // (a thread for each 16 elements of a row)
           return va_fail(VA_ERR_ARG, "too many query rows for one plan");
         spans.push_back(Span{(int64_t)pages.size(), first, end, row_begin, (int64_t)sub_row.size(), pairs});
-        pages.insert(pages.end(), run_pages.begin() + run_begin[i], run_pages.begin() + run_begin[i + 1]);
+        const int32_t* from = runs[i].list < 0 ? run_pages.data() : lists[(size_t)runs[i].list].at;
+        pages.insert(pages.end(), from + runs[i].begin, from + runs[i].end);
       }
       if (which) n_tile_spans = spans.size(), n_tile_rows = (int64_t)sub_row.size();
     }
@@ -298,7 +362,7 @@ int build(const VaSubRequests* subs, const VaShape* shape, int32_t over_codes, i
   if (num_pages < 0 || (int64_t)num_pages * shape->page_size > INT32_MAX || window < 0)
     return va_fail(VA_ERR_ARG, "%d pages of %d tokens, window %d", (int)num_pages, (int)shape->page_size, (int)window);
   Planner p{*subs, *shape, shape->dtype == VA_F32 && !over_codes, num_pages, window};
-  int rc = p.check();
+  int rc = p.find_lists();
   if (rc) return rc;
   p.find_visitors();
   if ((rc = p.find_spans()) || (rc = p.make_items())) return rc;

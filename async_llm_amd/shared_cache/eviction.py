@@ -114,16 +114,17 @@ class CacheEviction:
                                     arrays[2].ctypes.data if arrays[2].size else None, arrays[3].ctypes.data,
                                     arrays[4].ctypes.data, None, None)
         counts = native.VaWeighCounts()
-        words = np.empty(1 << 14, dtype=np.int32)
-        for _ in range(2):
-            rc = native.lib.va_weigh_plan(subs, self.op._shape, int(self._coded), self.num_pages, window, words.ctypes.data, words.size, counts)
-            if rc != native.VA_ERR_CAPACITY or counts.plan_words <= words.size:
+        pinned = self.device.type == "cuda"
+        capacity = (1 << 14) + 2 * arrays[2].size + 8 * len(sub_worker)  # (room for most plans)
+        while True:
+            host = torch.empty(capacity, dtype=torch.int32, pin_memory=pinned)
+            words = host.numpy()
+            rc = native.lib.va_weigh_plan(subs, self.op._shape, int(self._coded), self.num_pages, window, host.data_ptr(), capacity, counts)
+            if rc != native.VA_ERR_CAPACITY or counts.plan_words <= capacity:
                 break
-            words = np.empty(counts.plan_words, dtype=np.int32)
+            capacity = counts.plan_words
         native.check(rc)
-        host = torch.empty(counts.plan_words, dtype=torch.int32, pin_memory=self.device.type == "cuda")
-        host.numpy()[:] = words[: counts.plan_words]
-        blob = host.to(self.device, non_blocking=True)
+        blob = host[: counts.plan_words].to(self.device, non_blocking=True)
         header, sub_loc = words[: native.WEIGH_HEADER_WORDS].copy(), meta.sub_loc
         tables = (blob.data_ptr(), header.ctypes.data, meta.sub_worker.data_ptr(), sub_loc.data_ptr(),
                   sub_loc.stride(0) if sub_loc.dim() == 2 else 0)
