@@ -122,6 +122,14 @@ __global__ __launch_bounds__(1024) void move_kernel(MoveArgs a) {
   }
 }
 
+// A thread per slot and head: weights[h][slots[i]] = 0.
+__global__ __launch_bounds__(256) void clear_weights_kernel(TokenWeights weights, const int64_t* slots, long long n) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long long slot = slots[i];
+  if (slot >= 0 && slot < weights.slots) weights.sums[(long long)blockIdx.y * weights.slots + slot] = 0.f;
+}
+
 template <typename E>
 static int launch_move(MoveArgs& a, int num_layers, hipStream_t stream) {
   using S = typename E::storage;
@@ -178,4 +186,15 @@ extern "C" int va_move_kv(void* k_pool_dev, void* v_pool_dev, int64_t pool_row_s
     default:
       return va_fail(VA_ERR_ARG, "unknown dtype %d", (int)shape->dtype);
   }
+}
+
+extern "C" int va_clear_weights(float* weights_dev, int32_t num_heads, int64_t num_slots, const int64_t* slots_dev, int64_t n, void* stream) {
+  if (num_heads < 0 || num_slots < 0 || n < 0) return va_fail(VA_ERR_ARG, "negative count");
+  if (num_heads == 0 || num_slots == 0 || n == 0) return VA_OK;
+  if (!weights_dev || !slots_dev) return va_fail(VA_ERR_ARG, "null pointer");
+  if (num_heads > 65535 || n > 0x7fffffffLL * 256) return va_fail(VA_ERR_ARG, "too many slots or heads for one launch");
+  hipLaunchKernelGGL(va::clear_weights_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)num_heads), dim3(256), 0, (hipStream_t)stream,
+                     va::TokenWeights{weights_dev, (long long)num_slots}, slots_dev, n);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "clearing weights: %s", hipGetErrorString(e));
 }

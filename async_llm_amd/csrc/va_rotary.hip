@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "va_device.h"
 #include "va_internal.h"
@@ -163,6 +164,7 @@ extern "C" int va_rotate_qk(const void* q_dev, int64_t q_row_stride, int32_t num
   if (rotary < 0 || rotary > head_dim || rotary % 2)
     return va_fail(VA_ERR_ARG, "rotary_dim %d must be even and within head_dim %d", rotary, head_dim);
   if (rotary / 2 > va::kRotPairs) return va_fail(VA_ERR_ARG, "rotary_dim %d is over %d", rotary, 2 * va::kRotPairs);
+  if ((int64_t)num_q_heads + num_k_heads > INT32_MAX) return va_fail(VA_ERR_ARG, "too many heads");
   if (n_rows == 0 || num_q_heads + num_k_heads == 0) return VA_OK;
   if ((num_q_heads && (!q_dev || !out_q_dev)) || (num_k_heads && (!k_dev || !out_k_dev)) || (rotary && (!turns->quarters_dev || !positions_dev)))
     return va_fail(VA_ERR_ARG, "null pointer");
@@ -187,7 +189,7 @@ extern "C" int va_rotate_qk(const void* q_dev, int64_t q_row_stride, int32_t num
 
 extern "C" int va_rotary_table(const VaTurns* turns, int64_t first_position, int64_t n_rows, float* table_dev, void* stream) {
   if (!turns) return va_fail(VA_ERR_ARG, "null rotation description");
-  if (n_rows < 0 || turns->rotary_dim < 0 || turns->rotary_dim % 2) return va_fail(VA_ERR_ARG, "bad shape");
+  if (n_rows < 0 || turns->rotary_dim < 0 || turns->rotary_dim % 2 || turns->rotary_dim / 2 > va::kRotPairs) return va_fail(VA_ERR_ARG, "bad shape");
   const int half = turns->rotary_dim / 2;
   if (n_rows == 0 || half == 0) return VA_OK;
   if (!turns->quarters_dev || !table_dev) return va_fail(VA_ERR_ARG, "null pointer");

@@ -221,7 +221,7 @@ struct Planner {
         });
         if ((int64_t)sub_row.size() == row_begin) continue;
         while (sub_row.size() % unit) sub_row.push_back(-1), lo.push_back(0), hi.push_back(0);
-        if ((int64_t)sub_row.size() * G > INT32_MAX / 16)  // (a thread for each 16 elements of a row)
+        if ((int64_t)sub_row.size() * G > INT32_MAX / 32)  // (a thread for each 16 elements of a row)
           return va_fail(VA_ERR_ARG, "too many query rows for one plan");
         spans.push_back(Span{(int64_t)pages.size(), first, end, row_begin, (int64_t)sub_row.size(), pairs});
         const int32_t* from = runs[i].list < 0 ? run_pages.data() : lists[(size_t)runs[i].list].at;

@@ -59,6 +59,7 @@ EXPORTED_SYMBOLS = (
     "va_select_tokens",
     "va_move_kv",
     "va_move_kv_q8",
+    "va_clear_weights",
     "va_weigh_plan",
     "va_weigh",
     "va_weigh_q8",
@@ -248,6 +249,8 @@ def _load() -> C.CDLL:
     lib.va_select_tokens.argtypes = [vp, i32, i64, vp, i32, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp]
     lib.va_move_kv.restype = C.c_int
     lib.va_move_kv.argtypes = [vp, vp, i64, i64, i32, i64, vp, vp, vp, i64, vp, C.POINTER(VaShape), C.POINTER(VaRope), vp]
+    lib.va_clear_weights.restype = C.c_int
+    lib.va_clear_weights.argtypes = [vp, i32, i64, vp, i64, vp]
     lib.va_move_kv_q8.restype = C.c_int
     lib.va_move_kv_q8.argtypes = [pool, i64, i64, i32, vp, vp, vp, i64, vp, C.POINTER(VaShape), C.POINTER(VaRope), vp]
     lib.va_weigh_plan.restype = C.c_int

@@ -81,6 +81,19 @@ def _frequencies(rotary_dim: int, base: float, scaling: Optional[dict]) -> Tuple
     return out, attention
 
 
+def _apart(x: torch.Tensor, y: torch.Tensor, n: int) -> bool:
+    """Whether ``n`` rows of ``x`` and of ``y``, contiguous each, share no element: one behind the other, or side by side."""
+    if n == 0 or x.numel() == 0 or y.numel() == 0 or x.untyped_storage().data_ptr() != y.untyped_storage().data_ptr():
+        return True
+    step = x.element_size()
+    (a, wide_a, row_a), (b, wide_b, row_b) = sorted(
+        (t.data_ptr(), t[0].numel() * step, t.stride(0) * step) for t in (x, y))
+    if a + (n - 1) * max(row_a, 0) + wide_a <= b:
+        return True
+    at = (b - a) % row_a if n > 1 and row_a == row_b and row_a > 0 else 0
+    return wide_a <= at <= row_a - wide_b
+
+
 class RotaryEmbedding:
     """Rotates heads of ``head_dim`` elements, the first ``rotary_dim`` of them (all by default), as pairs ``(i, i +
     rotary_dim / 2)`` or, ``interleaved``, ``(2 i, 2 i + 1)``.  ``scaling``: a dictionary as model configurations have it
@@ -156,6 +169,8 @@ class RotaryEmbedding:
             if k is not None:
                 k2, k_row, k_heads = self._rows(k, n, "k")
                 keys = (k2.data_ptr(), k_row, k_heads, *self._out(out_k, k, k2, n, "out[1]"))
+                if not (_apart(out_q, k2, n) and _apart(out_k, q2, n) and _apart(out_q, out_k, n)):
+                    raise ValueError("what becomes of q must lie apart from k, and from what becomes of k, and the other way round")
         positions = positions.contiguous()
         native.call_on(device, native.lib.va_rotate_qk, *queries, *keys, positions.data_ptr(), int(wide), n, dim, dtype_id,
                        self._turns, native.current_stream_ptr(device))
@@ -170,13 +185,9 @@ class RotaryEmbedding:
         if not inner or (n > 1 and stride[0] < width):
             raise ValueError(f"{name} must have contiguous rows that do not overlap")
         # results over the input row by row, or apart from it
-        if n and y.untyped_storage().data_ptr() == rows.untyped_storage().data_ptr():
-            a, b, step = rows.data_ptr(), y.data_ptr(), y.element_size()
-            same = a == b and (n == 1 or stride[0] == rows.stride(0))
-            ends = [(p, p + ((n - 1) * s + width) * step) for p, s in ((a, rows.stride(0)), (b, stride[0]))]
-            beside = n > 1 and stride[0] == rows.stride(0) and width * step <= abs(b - a) % (stride[0] * step) <= (stride[0] - width) * step
-            if not same and not beside and ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]:
-                raise ValueError(f"{name} must be the input itself or lie apart from it")
+        same = y.data_ptr() == rows.data_ptr() and (n == 1 or stride[0] == rows.stride(0))
+        if not same and not _apart(y, rows, n):
+            raise ValueError(f"{name} must be the input itself or lie apart from it")
         return y.data_ptr(), stride[0] if n > 1 else width
 
     def cos_sin_cache(self, max_position: int) -> torch.Tensor:

@@ -96,9 +96,14 @@ class CacheEviction:
                              f"{weights.dtype} {list(weights.shape)} on {weights.device}")
 
     def clear(self, weights: torch.Tensor, slots: torch.Tensor) -> None:
-        """Forget what the tokens of ``slots`` (int64) were given."""
+        """Forget what the tokens of ``slots`` (whole numbers; those outside the pool are skipped) were given."""
         self._check_weights(weights)
-        weights.index_fill_(1, slots.to(device=self.device, dtype=torch.int64), 0.0)
+        if slots.dim() != 1 or slots.is_floating_point() or slots.is_complex() or slots.dtype is torch.bool:
+            raise ValueError(f"slots must be one row of whole numbers, got {slots.dtype} {tuple(slots.shape)}")
+        native.require_device(weights, "weights")
+        slots = slots.to(device=self.device, dtype=torch.int64).contiguous()
+        native.call_on(self.device, native.lib.va_clear_weights, weights.data_ptr(), *self._weights_shape, slots.data_ptr(),
+                       slots.numel(), native.current_stream_ptr(self.device))
 
     def plan(self, meta: SharedCacheAttnMetadata, window: int = 0) -> WeightPlan:
         """Turn a step's plan (of ``prepare``, ``prepare_prefill_batch`` or ``prepare_mixed``) round.  ``window > 0``: of many new

@@ -548,6 +548,10 @@ VA_API int va_move_kv_q8(const VaQuantPool* pool, int64_t code_layer_stride, int
                   const int64_t* shifts_dev, int64_t n_tokens, float* weights_dev, const VaShape* shape,
                   const VaRope* rope, void* stream);
 
+/* va_clear_weights: weights[h][slots[i]] = 0 for every head h and i < n; slots outside [0, num_slots) are skipped. */
+VA_API int va_clear_weights(float* weights_dev, int32_t num_heads, int64_t num_slots, const int64_t* slots_dev,
+                     int64_t n, void* stream);
+
 /*
  * va_weigh_plan / va_weigh: what every cached token was given by the attention of a step.
  * For every token t in sight and kv head hk
@@ -559,14 +563,18 @@ VA_API int va_move_kv_q8(const VaQuantPool* pool, int64_t code_layer_stride, int
  * VA_ROPE_MROPE too; sums are 32-bit and do not depend on the order of execution.
  * Slots that nobody sees are left as they are; weights_out may be weights_in.
  *
- * The plan is made on the host from the sub-request tables (kv_indices must be there; chain and
- * sub_worker are not used), for va_weigh_q8 where over_codes is not 0; window > 0 counts only the last `window` rows of each sub-request.
- * Entries outside num_pages pages are refused.  As with va_plan_build a buffer that is too
- * small gives VA_ERR_CAPACITY and the size in counts.  plan_header_host is the start of the host plan (24
- * words); workspace_dev, on a 16-byte boundary, must hold counts.workspace_bytes.  Pools and
- * queries of any alignment; 16-byte aligned rows and a head_dim of 64, 128 or 256 run on the matrix
- * cores, with queries as sums of two (VA_F16 pools) or three 16-bit numbers (errors of 2^-22, 2^-24), others
- * (VA_F32, head_dim up to 256) on the vector ALU.
+ * The plan is made on the host from the sub-request tables (kv_indices must be there;
+ * chain and sub_worker are not used), for va_weigh_q8 where over_codes is not 0; window > 0
+ * counts only the last `window` rows of each sub-request.  Entries outside num_pages pages
+ * are refused.  As with va_plan_build a buffer that is too small gives VA_ERR_CAPACITY and
+ * the size in counts.  plan_header_host is the start of the host plan (24 words);
+ * workspace_dev, on a 16-byte boundary, must hold counts.workspace_bytes.  Pools and queries
+ * of any alignment, head_dim up to 256.  Aligned rows (16 bytes) of a head_dim of 64, 128 or
+ * 256 run on the matrix cores, others on the vector ALU.  There 16-bit keys and codes meet
+ * queries as sums of three 16-bit numbers (an error of 2^-24 of the row's largest element), or of two
+ * (2^-22: VA_F16 pools, and tokens that more than 16 (row, q head) pairs read); 32-bit
+ * keys meet 32-bit queries.  A key that is not finite makes sums of its own token only
+ * infinite or NaN.
  */
 typedef struct VaWeighCounts {
   int32_t n_items;   /* work items, padding included                                         */

@@ -335,3 +335,21 @@ def test_evictions_that_leave_all_or_nothing(dev):
             ops.evict_tokens(block, weights, **bad)
     with pytest.raises(ValueError, match="weights"):
         ops.evict_tokens(block, weights[:, :-1], 5)
+
+
+def test_weights_are_forgotten(dev):
+    """Of the slots that are in the pool; a slot may be named twice, and in any whole type."""
+    e = CacheEviction(make_op(dev, 8, 4, 64, 16, torch.float16, 8))
+    for slots in ([], [5], [-1, 3, 127, 128, 3, 2**40], [0, 64]):
+        weights = torch.rand(4, 128, device=dev)
+        want = weights.clone()
+        for s in slots:
+            if 0 <= s < 128:
+                want[:, s] = 0.0
+        e.clear(weights, torch.tensor(slots, dtype=torch.int64, device=dev))
+        assert torch.equal(weights, want)
+    weights = torch.rand(4, 128, device=dev)
+    want = weights.clone()
+    want[:, 1:9:2] = 0.0
+    e.clear(weights, torch.arange(10, dtype=torch.int32)[1:9:2])
+    assert torch.equal(weights, want)

@@ -144,5 +144,17 @@ def test_refusals(dev):
     want = r(at, both[:4, :128].clone())[0]
     r(at, both[:4, :128], out=(both[:4, 140: 268], None))  # beside them
     assert torch.equal(both[:4, 140: 268], want)
+    # q and k of one array: what becomes of either lies apart from the other
+    qkv = torch.randn(5, 192 + 64, device=dev)
+    q, k = qkv[:4, :128], qkv[:4, 128: 192]
+    want = r(at, q.clone(), k.clone())
+    for bad in ((k, q), (q, qkv[1:, 128: 192]), (qkv[:4, 64: 192], k), (torch.empty(4, 128, device=dev), qkv[:4, 64: 128])):
+        with pytest.raises(ValueError):
+            r(at, q, k, out=bad)
+    one = torch.empty(4, 128, device=dev)
+    with pytest.raises(ValueError, match="apart"):
+        r(at, q, k, out=(one, one[:, :64]))
+    r(at, q, k, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
     with pytest.raises(ValueError, match="max_position"):
         r.cos_sin_cache(0)

@@ -104,6 +104,8 @@ def random_subs(r, page, pages):
         elif kind < 0.75:  # many new tokens
             n = r.randint(1, len(b) * page)
             subs.append((r.randint(1, n + 2), b, n, native.VA_SUB_CAUSAL))
+        elif kind < 0.8:  # pages that a list names twice
+            subs.append((1, b + b[:2], r.randint(0, (len(b) + len(b[:2])) * page), 0))
         elif kind < 0.9:  # single slots
             subs.append((1, [r.choice(b) * page + r.randrange(page)], 1, native.VA_SUB_SLOTS))
         else:  # a list that shares some pages only
@@ -137,6 +139,21 @@ def test_readers_of_a_block_share_its_tokens():
     strips = np.diff(words[words[21]: words[21] + words[20] + 1])
     tokens = words[words[6]: words[6] + 8 * counts.n_items].reshape(-1, 8)[:, 2]
     assert tokens.sum() == 1600 + 4 * 150 and (strips <= 3).all()  # few items: workgroups for all
+
+
+def test_lists_that_are_alike_and_lists_that_are_almost():
+    """Readers of one list make one run of it, whatever they see of it; a list that goes on shares what is the same."""
+    a, longer = list(range(10)), list(range(12))
+    subs = [(1, a, 160, 0), (1, a, 150, 0), (0, a, 160, 0), (2, a, 159, native.VA_SUB_CAUSAL), (1, [20, 21], 32, 0)]
+    rc, words, counts = plan_of(subs, (8, 8, 64), 16, 30)
+    assert rc == 0 and counts.n_spans == 2
+    rc, words, counts = plan_of([*subs, (1, longer, 192, 0)], (8, 8, 64), 16, 30)
+    assert rc == 0 and counts.n_spans == 3
+    pairs, _ = counted(words, (8, 8, 64), 16)
+    assert pairs == expected([*subs, (1, longer, 192, 0)], 1, 16, 0)
+    # a bad page is found in the first of two lists that are alike
+    rc, _, _ = plan_of([(1, [3, 30], 20, 0), (1, [3, 30], 20, 0)], (8, 8, 64), 16, 30)
+    assert rc == native.VA_ERR_ARG and b"page 30 lies outside" in native.lib.va_last_error()
 
 
 def test_strips_cost_the_same():
@@ -215,6 +232,11 @@ def test_calls_without_a_gpu_are_refused():
     with pytest.raises(native.ViewAttnError, match="GPU only"):
         e.move(one, one)
     with pytest.raises(native.ViewAttnError, match="GPU only"):
+        e.clear(weights, one)
+    for slots in (one.float(), one[None], one.bool()):
+        with pytest.raises(ValueError, match="slots must be"):
+            e.clear(weights, slots)
+    with pytest.raises(native.ViewAttnError, match="GPU only"):
         e.accumulate(torch.zeros(1, 256), None, 0, None, weights)
     with pytest.raises(ValueError, match="no multiple"):
         eviction_on_the_cpu(3, 2)
@@ -232,3 +254,6 @@ def test_selection_entry_refuses():
     need = native.lib.va_select_workspace_bytes(1, long.ctypes.data)
     assert need >= 4 * 50000 and native.lib.va_select_workspace_bytes(1, (-long).ctypes.data) == -1
     assert native.lib.va_select_workspace_bytes(1, n.ctypes.data) == 0
+    clear = native.lib.va_clear_weights
+    assert clear(None, -1, 4, None, 1, None) == native.VA_ERR_ARG and clear(None, 2, 4, None, 1, None) == native.VA_ERR_ARG
+    assert clear(None, 0, 4, None, 1, None) == 0 and clear(None, 2, 4, None, 0, None) == 0
