@@ -52,7 +52,8 @@ struct WeighArgs {
   const int32_t* lo;
   const int32_t* hi;
   int n_rows, n_tiles;
-  int n_first_tiles;  // tiles of rows of tile items, the first ones
+  int n_tile_items;   // the first items
+  int n_first_tiles;  // tiles of 16 of their rows, the first ones
   const int64_t* sub_worker;
   const int64_t* sub_loc;
   long long sub_loc_axis_stride;
@@ -934,6 +935,8 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_generic_kernel(WeighArgs 
   const int n_tok = item[VA_WI_N_TOK], D = a.head_dim;
   if (n_tok == 0) return;
   const int page_begin = item[VA_WI_PAGES], first = item[VA_WI_FIRST], partial = item[VA_WI_PARTIAL];
+  const int tile = blockIdx.x / (unsigned)a.num_kv_heads < (unsigned)a.n_tile_items ? VA_WEIGH_TILE_ROWS : 16;
+  const int pair_begin = item[VA_WI_TILE_BEGIN] * tile, pair_end = item[VA_WI_TILE_END] * tile;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   float* of_waves = lds + 64 * (D + 1);
   for (int t0 = 0; t0 < n_tok; t0 += 64) {
@@ -955,7 +958,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_generic_kernel(WeighArgs 
     __syncthreads();
     const int t_span = first + t0 + lane;
     float sum = 0.f;
-    for (int pair = item[VA_WI_TILE_BEGIN] * 16 + wave * kWeighBatch; pair < item[VA_WI_TILE_END] * 16; pair += kWeighWaves * kWeighBatch) {
+    for (int pair = pair_begin + wave * kWeighBatch; pair < pair_end; pair += kWeighWaves * kWeighBatch) {
       const float* q = (const float*)(a.queries + ((long long)hk * a.n_tiles + pair / 16) * tile_bytes(D)) + pair % 16 * D;
       float dots[kWeighBatch];
 #pragma unroll
@@ -1024,8 +1027,8 @@ static void launch_rows(const WeighArgs& a, bool fast, hipStream_t stream) {
 }
 
 template <int kD, typename C>
-static int launch_matrix(const WeighArgs& a, int n_tile_items, int n_strips, bool fast, hipStream_t stream) {
-  const unsigned tiles = (unsigned)n_tile_items * (unsigned)a.num_kv_heads, strips = (unsigned)n_strips * (unsigned)(a.num_kv_heads / strip_heads(a.num_kv_heads));
+static int launch_matrix(const WeighArgs& a, int n_strips, bool fast, hipStream_t stream) {
+  const unsigned tiles = (unsigned)a.n_tile_items * (unsigned)a.num_kv_heads, strips = (unsigned)n_strips * (unsigned)(a.num_kv_heads / strip_heads(a.num_kv_heads));
   const dim3 block(kWeighThreads);
   using Sh = WalkShape<kD, C>;
   if constexpr (std::is_same_v<C, F32>) {
@@ -1056,15 +1059,15 @@ static int launch_matrix(const WeighArgs& a, int n_tile_items, int n_strips, boo
 }
 
 template <typename C>
-static int launch_weigh(const WeighArgs& a, int n_items, int n_tile_items, int n_strips, bool matrix, bool fast, hipStream_t stream) {
+static int launch_weigh(const WeighArgs& a, int n_items, int n_strips, bool matrix, bool fast, hipStream_t stream) {
   if (matrix) {
     switch (a.head_dim) {
       case 64:
-        return launch_matrix<64, C>(a, n_tile_items, n_strips, fast, stream);
+        return launch_matrix<64, C>(a, n_strips, fast, stream);
       case 128:
-        return launch_matrix<128, C>(a, n_tile_items, n_strips, fast, stream);
+        return launch_matrix<128, C>(a, n_strips, fast, stream);
       default:
-        return launch_matrix<256, C>(a, n_tile_items, n_strips, fast, stream);
+        return launch_matrix<256, C>(a, n_strips, fast, stream);
     }
   }
   const dim3 grid((unsigned)n_items * (unsigned)a.num_kv_heads), block(kWeighThreads);
@@ -1118,22 +1121,22 @@ static int weigh(WeighArgs& a, int code_type, int num_pages, const int32_t* plan
   const bool matrix = dims && (code_type >= 0 || (a.pool_row_stride * size % 16 == 0 && (uintptr_t)a.k_pool % 16 == 0 && a.pool_row_stride < 1 << 24));
   const bool fast = a.rope.rotary_dim % 16 == 0 && (a.rope.mode != VA_ROPE_TABLE || (uintptr_t)a.rope.cos_sin % 16 == 0);
   a.pieces = a.q_row_stride * size % 16 == 0 && (uintptr_t)a.q % 16 == 0;
-  const int n_tile_items = h[VA_WH_N_TILE_ITEMS];
+  a.n_tile_items = h[VA_WH_N_TILE_ITEMS];
   a.n_first_tiles = (int)((int64_t)h[VA_WH_N_TILE_ROWS] * G / 16);
   if (code_type == VA_CODE_E4M3) {
-    rc = launch_weigh<E4M3>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+    rc = launch_weigh<E4M3>(a, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
   } else if (code_type == VA_CODE_INT8) {
-    rc = launch_weigh<INT8>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+    rc = launch_weigh<INT8>(a, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
   } else {
     switch (shape->dtype) {
       case VA_F32:
-        rc = launch_weigh<F32>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+        rc = launch_weigh<F32>(a, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       case VA_F16:
-        rc = launch_weigh<F16>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+        rc = launch_weigh<F16>(a, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       case VA_BF16:
-        rc = launch_weigh<BF16>(a, n_items, n_tile_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
+        rc = launch_weigh<BF16>(a, n_items, h[VA_WH_N_STRIPS], matrix, fast, stream);
         break;
       default:
         rc = va_fail(VA_ERR_ARG, "unknown dtype %d", (int)shape->dtype);

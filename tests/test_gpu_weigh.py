@@ -6,8 +6,10 @@ import pytest
 import torch
 
 from async_llm_amd import native
-from async_llm_amd.shared_cache import CacheEviction, PrefillSpec, WorkerGroup
+from async_llm_amd.kvcache.mha_pool import MHAKVCache
+from async_llm_amd.shared_cache import CacheEviction, PrefillSpec, SharedCacheAttention, WorkerGroup
 from tests.eviction_util import blocks_of, fill, make_op, weights64
+from tests.quant_util import quantised32, write
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -130,6 +132,32 @@ def test_mixed_steps(dev):
     check(op, meta, gen)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_pools_off_16_byte_boundaries(dev, dtype):
+    """Pools that the matrix cores do not read from, under plans with items of all kinds."""
+    class Apart(MHAKVCache):
+        def __init__(self, pages):
+            self._num_layers, self._device = 1, dev
+            self._arrays = [torch.zeros(pages * 16 * 2 * 64 + 1, dtype=dtype, device=dev)[1:].view(pages, 16, 2, 64) for _ in "kv"]
+            self._kv_buffer = self._arrays[0]
+
+        def k_cache(self, layer):
+            return self._arrays[0]
+
+        def v_cache(self, layer):
+            return self._arrays[1]
+
+    r, gen = random.Random(6), torch.Generator().manual_seed(6)
+    like = make_op(dev, 8, 2, 64, 16, dtype, 4)
+    op = SharedCacheAttention(Apart(120), like.cos_sin_cache, 8, 2, 64, 16, dtype, dev)
+    fill(op, gen)
+    assert op.kv_cache.k_cache(0).data_ptr() % 16
+    pages = list(range(120))
+    for meta in (op.prepare_prefill_batch(chunk_specs(op, r, [70, 3], 20, 300, pages)), decode_step(op, r, 6, [1, 17, 130], shared=200)):
+        q = torch.randn(meta.num_workers, 512, generator=gen).to(dev, dtype)
+        check(op, meta, gen, q=q, lse=5.0 + torch.rand(meta.num_workers, 8, generator=gen).to(dev))  # (attention takes no such pool)
+
+
 def test_a_view_that_lists_a_block_twice(dev):
     r, gen = random.Random(6), torch.Generator().manual_seed(6)
     op = make_op(dev, 4, 2, 64, 16, BF16, 40)
@@ -181,6 +209,24 @@ def test_large_and_small_queries_and_keys(dev):
     q = (torch.randn(3, 256, generator=gen) * size).to(dev, F16)
     _, lse = op.attend(q, 0, meta, return_lse=True)
     check(op, meta, gen, q=q, lse=lse)
+
+
+@pytest.mark.parametrize("dtype, codes", [(BF16, None), (BF16, E4M3), (F16, INT8)])
+@pytest.mark.parametrize("least", [-5, -7, -60])
+def test_keys_of_very_different_sizes_under_many_rows(dev, dtype, codes, least):
+    """Tiles of many rows scale the keys of a token, or of 32 tokens, by a power of two: rows of zeros and tiny rows beside others."""
+    r, gen = random.Random(least), torch.Generator().manual_seed(-least)
+    op = make_op(dev, 8, 2, 64, 16, dtype, 80, codes)
+    size = 2.0 ** torch.randint(least, 2, (80, 16, 2, 1), generator=gen)
+    size[torch.rand(80, 16, 2, 1, generator=gen) < 0.1] = 0.0
+    x = torch.randn(80, 16, 2, 64, generator=gen) * size
+    if codes is None:
+        op.kv_cache.k_cache(0).copy_(x)
+        op.kv_cache.v_cache(0).zero_()
+    else:
+        for which in (0, 1):
+            write(op.kv_cache, which, 0, torch.arange(1280), *quantised32(x.view(1280, 2, 64), op.kv_cache.code_dtype))
+    check(op, op.prepare_prefill_batch(chunk_specs(op, r, [90, 35], 20, 300, list(range(80)))), gen)
 
 
 def test_sums_are_one_for_each_row(dev):
