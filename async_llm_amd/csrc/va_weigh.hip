@@ -93,8 +93,8 @@ __device__ __forceinline__ uint32_t weigh_slot(const WeighArgs& a, int page_begi
 // a tile of 16 (32), so that a wave reads its operands of a step in one run; pieces of 8 (32-bit: 4) dims go to steps and
 // contraction groups in the order in which lanes hold the keys: piece groups * step + group, or over codes, of which a lane reads 16 at
 // once, 2 groups (step / 2) + 2 group + step % 2.  kTile*: for tile items, 32 rows a tile; the others are for strips.
-enum RowKind { kPlain32, kParts32, kPartsF16, kPartsBF16, kCodesBF16, kTileF16, kTileCodes };
-__host__ __device__ constexpr int parts_of(int kind) { return kind == kPartsF16 || kind >= kTileF16 ? 2 : kind == kPartsBF16 || kind == kCodesBF16 ? 3 : 1; }
+enum RowKind { kPlain32, kParts32, kPartsBF16, kPartsF16, kCodesF16, kTileF16, kTileCodes };
+__host__ __device__ constexpr int parts_of(int kind) { return kind >= kPartsF16 ? 2 : kind == kPartsBF16 ? 3 : 1; }
 __host__ __device__ constexpr int rows_of(int kind) { return kind >= kTileF16 ? VA_WEIGH_TILE_ROWS : 16; }
 __host__ __device__ constexpr int tile_bytes(int dim) { return 16 * dim * 6; }  // (room for any of them)
 
@@ -112,7 +112,7 @@ __device__ __forceinline__ void write_row_piece(char* tile_at, int dim, int j, i
       *(va_f32x4*)(tile_at + (p / 4) * 1024 + (16 * (p % 4) + j) * 16) = va_f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
     }
   } else {
-    constexpr bool kHalf = parts_of(kKind) == 2, kCodes = kKind == kTileCodes || kKind == kCodesBF16;
+    constexpr bool kHalf = parts_of(kKind) == 2, kCodes = kKind == kTileCodes || kKind == kCodesF16;
     constexpr int kRows = rows_of(kKind), kGroups = 64 / kRows, kSteps = 8 * kGroups;  // contraction groups, dims of a step
     const int step = kCodes ? 2 * (piece / (2 * kGroups)) + piece % 2 : piece / kGroups, group = kCodes ? piece % (2 * kGroups) / 2 : piece % kGroups;
 #pragma unroll
@@ -313,22 +313,37 @@ struct WalkKeys<F32> {
     return c;
   }
 };
+// (codes are float16 numbers as they are; their row's scale comes to the scores)
 template <>
-struct WalkKeys<E4M3> : WalkKeys<BF16> {
-  static constexpr int kBytes = 1, kRows = kCodesBF16;
+struct WalkKeys<E4M3> : WalkKeys<F16> {
+  static constexpr int kBytes = 1, kRows = kCodesF16;
   static constexpr bool kCodes = true;
-  static __device__ __forceinline__ va_u32x4 keys(va_u32x2 codes, float scale) { return E4M3::bf16x8(codes, scale); }
+  static __device__ __forceinline__ va_u32x4 keys(va_u32x2 codes) {
+    va_u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      w[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[e], 1.f, false));
+      w[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[e], 1.f, true));
+    }
+    return w;
+  }
 };
 template <>
-struct WalkKeys<INT8> : WalkKeys<BF16> {
-  static constexpr int kBytes = 1, kRows = kCodesBF16;
+struct WalkKeys<INT8> : WalkKeys<F16> {
+  static constexpr int kBytes = 1, kRows = kCodesF16;
   static constexpr bool kCodes = true;
-  static __device__ __forceinline__ va_u32x4 keys(va_u32x2 codes, float scale) {  // (bf16 has the eight bits of a code)
-    float x[8];
-    INT8::unpack4(codes[0], x), INT8::unpack4(codes[1], x + 4);
+  // A code plus 128 as the low byte of 1024's mantissa is 1152 plus the code.
+  static __device__ __forceinline__ va_u32x4 keys(va_u32x2 codes) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 base = {(_Float16)1152.f, (_Float16)1152.f};
+    va_u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= scale;
-    return va_u32x4{Mma<BF16>::pack(x[0], x[1]), Mma<BF16>::pack(x[2], x[3]), Mma<BF16>::pack(x[4], x[5]), Mma<BF16>::pack(x[6], x[7])};
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t up = codes[e] ^ 0x80808080u;
+      w[2 * e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, up, 0x04010400u)) - base);
+      w[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, up, 0x04030402u)) - base);
+    }
+    return w;
   }
 };
 
@@ -563,13 +578,13 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
     }
     const char* tile = own + (done % kBuffers) * Sh::kTileBytes;
     va_u32x4 keys[kGroups][kRaw];
-    float scale[kGroups];
+    va_u32x4 scale[K::kCodes ? kGroups : 1];  // of a lane's four tokens
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
       for (int s = 0; s < kRaw; ++s)
         keys[g][s] = *(const va_u32x4*)(tile + g * Sh::kGroupBytes + j * Sh::kRowBytes + 16 * ((4 * s + kg) ^ walk_swz<kPieces>(j)));
-      if constexpr (K::kCodes) scale[g] = scale_value(*(const uint32_t*)(tile + Sh::kScalesAt + 4 * (16 * g + j)));
+      if constexpr (K::kCodes) scale[g] = *(const va_u32x4*)(tile + Sh::kScalesAt + 4 * (16 * g + 4 * kg));
     }
     const float before = *(const float*)(tile + Sh::kSumsAt + 4 * lane);
     const uint32_t slot = *(const uint32_t*)(tile + Sh::kSlotsAt + 4 * lane);
@@ -600,13 +615,19 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
           va_u32x4 k;
           if constexpr (K::kCodes) {
             const va_u32x4 raw = keys[g][s / 2];
-            k = K::keys(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]}, scale[g]);
+            k = K::keys(s % 2 ? va_u32x2{raw[2], raw[3]} : va_u32x2{raw[0], raw[1]});
           } else {
             k = keys[g][s];
           }
 #pragma unroll
           for (int p = kParts - 1; p >= 0; --p) dots[g] = K::run(k, q[p][s], dots[g]);  // (small parts first)
         }
+      if constexpr (K::kCodes) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) dots[g][r] *= scale_value(scale[g][r]);
+      }
       if (__any(row.lo > t_tile || row.hi < t_end)) {  // some row does not see some token
 #pragma unroll
         for (int g = 0; g < kGroups; ++g)
