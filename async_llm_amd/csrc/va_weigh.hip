@@ -391,7 +391,7 @@ __device__ __forceinline__ int walk_swz(int r) {
 // global -> LDS into a ring of its own (keys, the sums so far and, over codes, scales) and asks for the next one, of the next item
 // where this one ends, as soon as the keys are in registers.  There is no barrier, and nothing but the first tile of a strip
 // is waited for idly.  Sums are held in LDS and written many at a time: each store between the loads costs the memory about as
-// much as 1 KB of keys (8 requests of 131072 tokens: 427 us with one a tile, 408 with one every eighth, 367 with 2048 held).
+// much as 1 KB of keys (8 requests of 131072 tokens: 371 us with 512 held, 338 with 2048).
 template <int kD, typename C>
 __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) {
   using Sh = WalkShape<kD, C>;
@@ -656,10 +656,12 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
     }
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
+      float of_token = 0.f;  // lane j < 4 has token 4 kg + j (a choice among the elements of an array would be one among addresses)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum[g][r] = row_sum(sum[g][r]);
-      // lane j < 4 has token 4 kg + j
-      const float of_token = j == 0 ? sum[g][0] : j == 1 ? sum[g][1] : j == 2 ? sum[g][2] : sum[g][3];
+      for (int r = 0; r < 4; ++r) {
+        const float x = row_sum(sum[g][r]);
+        of_token = j == r ? x : of_token;
+      }
       if (j < 4) turn[16 * g + 4 * kg + j] = of_token;
     }
     if (lane < kTokens) {
