@@ -11,7 +11,7 @@
 //
 // Two ways, by span (va_weigh.h), in one launch where a step has both:
 //   * strips (weigh_strip): the rows that see a token make one tile of 16, as in decode steps.  Bound by the keys: they travel to LDS
-//     in whole lines, each wave's tiles in a ring of its own, while its tile before is at the products.
+//     in whole lines, each wave's tile in a place of its own, while the tile before it is at the products.
 //   * tile items (weigh_tiles): many rows see a token, as those of many new tokens.  Bound by the products: 64 tokens' keys stay
 //     in a wave's registers while the rows' queries pass by through LDS, for all four waves at once.
 // Where a chunk's rows are split among workgroups each writes partial sums, and weigh_join_kernel adds them in their order.
@@ -360,23 +360,20 @@ struct WalkShape {
   static constexpr int kRaw = kPieces / 4;                 // pieces of a row that a lane takes
   static constexpr int kSteps = K::kCodes ? 2 * kRaw : kRaw;  // operand pieces of a lane, per part
   static constexpr int kParts = parts_of(K::kRows);
-  // groups of 16 tokens of a wave's tile: 8 KB of 16- and 32-bit rows (up to 64 tokens, 16 at least), as many tokens of codes
-  static constexpr int kGroups = groups_of(K::kCodes ? 2 * kD : kRowBytes);
+  // groups of 16 tokens of a wave's tile: 8 KB, up to 64 tokens, 16 at least
+  static constexpr int kGroups = groups_of(kRowBytes);
   static constexpr int kTokens = 16 * kGroups;
   static constexpr int kGroupBytes = 16 * kRowBytes;
   static constexpr int kLoads = kGroupBytes / 1024;        // wave-level loads of a group
   // behind a tile's rows: the tokens' sums so far, a word for every scale, the tokens' slots
   static constexpr int kSumsAt = kGroups * kGroupBytes, kScalesAt = kSumsAt + 256, kSlotsAt = kScalesAt + (K::kCodes ? 256 : 0);
   static constexpr int kTileBytes = kSlotsAt + 256;
-  static constexpr int kBuffers = K::kCodes ? 2 : 1;  // (8 KB a wave on their way are enough)
-  static constexpr int kTileLoads = kGroups * kLoads + (K::kCodes ? 2 : 1);  // what the counter of outstanding loads sees of a tile
-  // behind the rings: where a wave turns a tile's sums from lanes to tokens, and holds those of several tiles with their places
-  static constexpr int kTurnOffset = kWeighWaves * kBuffers * kTileBytes;
-  static constexpr int kHold = kBuffers * kTileBytes > 10 * 1024 ? 512 : 2048;
+  // behind the tiles: where a wave turns a tile's sums from lanes to tokens, and holds those of several tiles with their places
+  static constexpr int kTurnOffset = kWeighWaves * kTileBytes;
+  static constexpr int kHold = kGroupBytes > 8 * 1024 ? 512 : 2048;
   static constexpr int kWaveBytes = 256 + kHold * 4 + kHold / 16 * 8;
   static constexpr int kLdsBytes = kTurnOffset + kWeighWaves * kWaveBytes;
   static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups share the LDS of a CU");
-  static_assert((kBuffers - 1) * kTileLoads < kAnyInFlight, "the counter of outstanding loads");
 };
 // Piece c of row r of a group lies at position c ^ walk_swz(r): the fragments of sixteen rows then lie in different banks.
 template <int kPieces>
@@ -388,7 +385,7 @@ __device__ __forceinline__ int walk_swz(int r) {
 
 // A workgroup walks a strip of items for up to four kv heads, whose rows of a token lie side by side, its waves on their own: each takes
 // its head's tiles of an item's tokens (every second or fourth where there are fewer heads), brings them
-// global -> LDS into a ring of its own (keys, the sums so far and, over codes, scales) and asks for the next one, of the next item
+// global -> LDS into a place of its own (keys, the sums so far and, over codes, scales) and asks for the next one, of the next item
 // where this one ends, as soon as the keys are in registers.  There is no barrier, and nothing but the first tile of a strip
 // is waited for idly.  Sums are held in LDS and written many at a time: each store between the loads costs the memory about as
 // much as 1 KB of keys (8 requests of 131072 tokens: 371 us with 512 held, 338 with 2048).
@@ -398,7 +395,7 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
   using K = WalkKeys<C>;
   using Words = const __attribute__((address_space(4))) int32_t*;
   constexpr int kGroups = Sh::kGroups, kLoads = Sh::kLoads, kPieces = Sh::kPieces, kSteps = Sh::kSteps, kRaw = Sh::kRaw, kParts = Sh::kParts;
-  constexpr int kTokens = Sh::kTokens, kBuffers = Sh::kBuffers;
+  constexpr int kTokens = Sh::kTokens;
   constexpr bool kSeveral = std::is_same_v<C, F32>;  // tokens may have several tiles of rows
   extern __shared__ va_u32x4 smem[];
   char* lds = (char*)smem;
@@ -408,8 +405,8 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
   const int hk = where.head * heads + wave % heads, strip_begin = ((Words)a.strips)[where.item], strip_end = ((Words)a.strips)[where.item + 1];
   if (strip_begin == strip_end) return;
   const int lane = threadIdx.x % kWave, j = lane % 16, kg = lane / 16;
-  char* own = lds + wave * kBuffers * Sh::kTileBytes;
-  const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_address(own));
+  char* tile = lds + wave * Sh::kTileBytes;
+  const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_address(tile));
   float* turn = (float*)(lds + Sh::kTurnOffset + wave * Sh::kWaveBytes);
   float* held_sums = turn + 64;
   uint2* held_groups = (uint2*)(held_sums + Sh::kHold);  // of 16 sums: where the first goes, how many there are
@@ -456,10 +453,11 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
     int pages, first, last, t0, page[kGroups];
   };
   Next next{};
-  int asked = 0, found = 0;  // tiles asked for, and found, so far
+  bool more = false;  // there is one
   int find_index = strip_begin, find_n = 0;
   Piece find = piece_at(strip_begin);
   auto find_next = [&]() __attribute__((always_inline)) {
+    more = false;
     while (find_n == find.tiles) {
       if (find_index + 1 >= strip_end) return;
       find = piece_at(++find_index);
@@ -472,12 +470,10 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
       for (int g = 0; g < kGroups; ++g)  // (a group past the end: the last one)
         next.page[g] = ((Words)a.pages)[next.pages + ((next.first + min(next.t0 + 16 * g, next.last / 16 * 16)) >> a.page_map.shift)];
     }
-    ++found;
+    more = true;
   };
   auto request_next = [&]() __attribute__((always_inline)) {
-    if (asked == found) return;
-    const int buffer = asked++ % kBuffers;
-    const uint32_t dst = ring + (uint32_t)buffer * Sh::kTileBytes;
+    if (!more) return;
     uint32_t of_lane = 0;  // slot of the token whose words this lane brings: token `lane` of the tile
     if (pages16 && next.first % 16 == 0) {  // 16 tokens of a group lie in one page
 #pragma unroll
@@ -508,7 +504,7 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
     }
     load_word_to_lds(sums_in + of_lane, dst + Sh::kSumsAt);
     if constexpr (K::kCodes) load_bytes_to_lds((unsigned long long)a.k_scales + row_at(of_lane) / kD, dst + Sh::kScalesAt);
-    *(uint32_t*)(own + buffer * Sh::kTileBytes + Sh::kSlotsAt + 4 * lane) = of_lane;
+    *(uint32_t*)(tile + Sh::kSlotsAt + 4 * lane) = of_lane;
     find_next();
   };
   find_next();
@@ -534,9 +530,8 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
   };
 
   // ---- the walk ----
-#pragma unroll
-  for (int b = 0; b < kBuffers; ++b) request_next();
-  int done = 0, index = strip_begin, n = 0, q_tile = -1;
+  request_next();
+  int index = strip_begin, n = 0, q_tile = -1;
   Piece at = piece_at(strip_begin);
   // Sums not yet written, all of one kind: of this workgroup's part of a span's rows or not, in groups of 16 that lie side by side
   // or, of scattered tokens, with a place for each in the upper half.
@@ -570,13 +565,7 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
       queries_here();
       q_tile = at.tile_begin;
     }
-    // The tile has landed once at most the loads of the kBuffers - 1 tiles asked for after it are outstanding.
-    if (asked - done >= kBuffers && kBuffers > 1) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBuffers - 1) * Sh::kTileLoads) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    const char* tile = own + (done % kBuffers) * Sh::kTileBytes;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tile has landed
     va_u32x4 keys[kGroups][kRaw];
     va_u32x4 scale[K::kCodes ? kGroups : 1];  // of a lane's four tokens
 #pragma unroll
@@ -677,7 +666,7 @@ __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) 
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       request_next();
     }
-    ++n, ++done;
+    ++n;
   }
   write_held();
 }
