@@ -19,7 +19,9 @@
 
 namespace va {
 
-constexpr int kMoveTokens = 4;  // tokens per workgroup, whose loads are in flight together
+// Tokens of a workgroup, whose loads are in flight together: 12556 tokens of 4 layers of 4 heads of 256 87 us (4.7 TB/s), 95 with one,
+// 92 with eight.
+constexpr int kMoveTokens = 4;
 constexpr int kMoveTurnBytes = 48 * 1024;
 
 struct MoveArgs {

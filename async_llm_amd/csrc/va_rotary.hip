@@ -7,9 +7,10 @@
 // whole number of them comes off exactly, so an angle at position 2^22 is as good as one at 1.  32 bits would be off by
 // position * 2^-25 quarter turns there.  Cosines and sines, products and sums are 32-bit numbers, rounded once to the element type.
 //
-// A workgroup takes a few tokens (one where there are few): it works their angles out once, a thread a pair, for all heads
+// A workgroup takes a token, or a few where a token's heads are few: it works their angles out once, a thread a pair, for all heads
 // through LDS, then each thread takes units of 2 * kVec elements -- the two 16-byte pieces that hold both halves of kVec pairs, or
-// two neighbouring ones -- of any token and head.  Bound by HBM, 2 * (Hq + Hkv) * head_dim elements a token.
+// two neighbouring ones -- of any token and head.  Bound by HBM, 2 * (Hq + Hkv) * head_dim elements a token: 16384 rows of 64 + 16 heads
+// of 64 in 32 bits 120 us, 5.6 TB/s; 64 rows of 16 + 4 heads of 256 4 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -51,7 +52,7 @@ struct RotateArgs {
   float factor;
 };
 
-template <typename E, int kVec, bool kNeighbours>
+template <typename E, int kVec, bool kNeighbours, bool kPast>  // kPast: reads go past the caches
 __global__ __launch_bounds__(kRotThreads) void rotate_kernel(RotateArgs a) {
   using S = typename E::storage;
   __shared__ float2 turns[kRotPairs];
@@ -76,8 +77,12 @@ __global__ __launch_bounds__(kRotThreads) void rotate_kernel(RotateArgs a) {
     const int d1 = turned && !kNeighbours ? d0 + a.half : d0 + kVec;
     S lo[kVec], hi[kVec];
     if constexpr (kVec > 1) {
-      *(va_rot_u32x4*)lo = *(const va_rot_u32x4*)(from + d0);
-      *(va_rot_u32x4*)hi = *(const va_rot_u32x4*)(from + d1);
+      const va_rot_u32x4 *p = (const va_rot_u32x4*)(from + d0), *q = (const va_rot_u32x4*)(from + d1);
+      if constexpr (kPast) {
+        *(va_rot_u32x4*)lo = __builtin_nontemporal_load(p), *(va_rot_u32x4*)hi = __builtin_nontemporal_load(q);
+      } else {
+        *(va_rot_u32x4*)lo = *p, *(va_rot_u32x4*)hi = *q;
+      }
     } else {
       lo[0] = from[d0], hi[0] = from[d1];
     }
@@ -132,21 +137,24 @@ static int launch_rotate(RotateArgs& a, bool neighbours, hipStream_t stream) {
   // (the quotients by reciprocals are exact below 2^32 / divisor)
   const long long row_tasks = (long long)heads * a.units;
   if (row_tasks * std::max(a.units, heads) >= (1ll << 31)) return va_fail(VA_ERR_ARG, "%d heads of %d dims are more than a workgroup counts", heads, a.head_dim);
-  // few tokens: one a workgroup, so that all CUs have some
-  long long most = std::min<long long>(4, (1ll << 31) / (row_tasks * std::max(a.units, heads)));
+  // As many tokens as give every thread a unit (16384 rows of 8 + 2 heads of 128: 15.1 us with four, 18.3 with one; of 64 + 16
+  // heads of 64 in 32 bits 132 and 122), and one where there are few, so that all CUs have some.
+  long long most = std::min<long long>((kRotThreads + row_tasks - 1) / row_tasks, (1ll << 31) / (row_tasks * std::max(a.units, heads)));
   if (a.half) most = std::min<long long>(most, kRotPairs / a.half);
   a.tokens = (int)std::max<long long>(1, std::min(most, a.n_rows / 2048));
   const long long groups = (a.n_rows + a.tokens - 1) / a.tokens;
   if (groups > 0x7fffffffLL) return va_fail(VA_ERR_ARG, "too many rows for one launch");
+  // Rows and results that the 256 MB of the last cache do not hold (16384 rows of 32 + 8 heads of 128: 53 us past the caches, 61
+  // through them; 4099 such rows, which it holds, 20.6 and 15.7).
+  const bool past = wide && 2 * a.n_rows * heads * a.head_dim * (long long)sizeof(typename E::storage) > 256ll << 20;
   const dim3 grid((unsigned)groups), block(kRotThreads);
-  if (wide && neighbours) {
-    hipLaunchKernelGGL((rotate_kernel<E, kWide, true>), grid, block, 0, stream, a);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
+  if (past) {
+    neighbours ? launch(rotate_kernel<E, kWide, true, true>) : launch(rotate_kernel<E, kWide, false, true>);
   } else if (wide) {
-    hipLaunchKernelGGL((rotate_kernel<E, kWide, false>), grid, block, 0, stream, a);
-  } else if (neighbours) {
-    hipLaunchKernelGGL((rotate_kernel<E, 1, true>), grid, block, 0, stream, a);
+    neighbours ? launch(rotate_kernel<E, kWide, true, false>) : launch(rotate_kernel<E, kWide, false, false>);
   } else {
-    hipLaunchKernelGGL((rotate_kernel<E, 1, false>), grid, block, 0, stream, a);
+    neighbours ? launch(rotate_kernel<E, 1, true, false>) : launch(rotate_kernel<E, 1, false, false>);
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "rotation launch: %s", hipGetErrorString(e));

@@ -387,8 +387,9 @@ __device__ __forceinline__ int walk_swz(int r) {
 // its head's tiles of an item's tokens (every second or fourth where there are fewer heads), brings them
 // global -> LDS into a place of its own (keys, the sums so far and, over codes, scales) and asks for the next one, of the next item
 // where this one ends, as soon as the keys are in registers.  There is no barrier, and nothing but the first tile of a strip
-// is waited for idly.  Sums are held in LDS and written many at a time: each store between the loads costs the memory about as
-// much as 1 KB of keys (8 requests of 131072 tokens: 371 us with 512 held, 338 with 2048).
+// is waited for idly.  8 requests of 131072 tokens and 4 heads of 256: 331 us, 6.6 TB/s; 16 heads of 64 5.5 TB/s, int8 codes 5.2.
+// Sums are held in LDS and written many at a time: each store between the loads costs the memory about as much as 1 KB of
+// keys (371 us with 512 held, 338 with 2048, rows' pass included).
 template <int kD, typename C>
 __device__ __forceinline__ void weigh_strip(const WeighArgs& a, unsigned block) {
   using Sh = WalkShape<kD, C>;
@@ -757,11 +758,11 @@ struct TileShape {
 
 // S^T[32 tokens, 32 rows] by v_mfma_f32_32x32x16: lane l has row l % 32 and tokens 8 (r / 4) + 4 (l / 32) + r % 4.
 //
-// 4 requests of 300 .. 1500 new tokens of 32 heads of 128 after a prompt of 8192: 749 us, or 965 TFLOP/s of the two parts' products, where
-// a large product of bf16 matrices reaches 1264 on the same card.  The matrix cores are busy for 48 % of that time and the vector
-// ALU, of which exp2 is two thirds, for 42 %; the scores of a tile becoming sums while the next tile's products run took more
-// registers than there are.  Tiles of 16 rows by 16x16x32 took as long (720 .. 760 us); with 32 rows a tile, 8 readers of 65536 tokens take
-// 49 us instead of 62, having half the barriers.
+// 4 requests of 300 .. 1500 new tokens of 32 heads of 128 after a prompt of 8000: 730 us, or 985 TFLOP/s of the two parts' products, where
+// a large product of bf16 matrices reaches 1264 on the same card.  The matrix cores are busy for 50 % of that time and the vector
+// ALU, of which exp2 is two thirds, for 44 %; scores becoming sums while the next tile's products run took more registers
+// than there are.  Tiles of 16 rows by 16x16x32 took 720 .. 760 us; with 32 rows a tile and half the barriers 8 readers of 65536 tokens
+// take 49 us instead of 62.
 template <int kD, typename C>
 __device__ __forceinline__ void weigh_tiles(const WeighArgs& a, unsigned block) {
   using Sh = TileShape<kD>;

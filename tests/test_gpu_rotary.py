@@ -125,6 +125,20 @@ def test_recorded_and_on_another_stream(dev):
         assert torch.equal(out, r(positions, q)[0])
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rows_that_no_cache_holds(dev, interleaved):
+    """What is rotated in one call is what is rotated row by row, past 256 MB too, and of a few narrow rows a workgroup."""
+    r = RotaryEmbedding(256, interleaved=interleaved, device=dev)
+    q = torch.randn(13000, 5120, dtype=torch.bfloat16, device=dev)
+    at = torch.arange(13000, device=dev) * 7
+    got, _ = r(at, q)
+    for first in (0, 6000, 12900):
+        part = slice(first, first + 100)
+        assert torch.equal(got[part], r(at[part], q[part])[0])
+    narrow = q[:, 512:1024]
+    assert torch.equal(r(at, narrow)[0], got[:, 512:1024])
+
+
 def test_refusals(dev):
     r = RotaryEmbedding(64, device=dev)
     q, at = torch.zeros(4, 128, device=dev), torch.arange(4, device=dev)
