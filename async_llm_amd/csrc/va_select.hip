@@ -7,11 +7,12 @@
 // is found digit by digit from histograms, most significant first, and then every token above it stays, and of those equal to
 // it the first that are wanted.  No sort, and no order of execution that the result depends on.
 //
-// Blocks of up to kSelectInLds tokens: a workgroup each, keys in LDS, one launch (64 blocks of 16384 tokens 31 us, 40 by runs; one
-// such block 28 and 25).  Longer ones: four launches of a workgroup for
+// Blocks of up to kSelectInLds tokens: a workgroup each, keys in LDS, one launch (64 blocks of 16384 tokens 31 us, 35 by runs; one
+// such block 28 and 23).  Longer ones: four launches of a workgroup for
 // each run of tokens.  The first makes keys and counts those of a run by their upper digit; each further one adds the counts of all
 // runs up, every workgroup for itself, finds the cut's digit, and counts the run's keys that have it by their next one, and the last
-// writes.  What lies above the cut in the runs in front falls out of the same sums.
+// writes.  What lies above the cut in the runs in front falls out of the same sums.  They are taken of groups of 32 digits first,
+// then of the one group that has the cut: 29 us instead of 41 with all of them, for an eighth of 8 blocks of 60000 to 131072 tokens.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -27,8 +28,8 @@ constexpr int kSelectInLds = 16384;  // tokens of a block whose keys stay in LDS
 constexpr int kSelectBlocks = 64;    // blocks of a launch
 constexpr int kSelectRun = 4096;     // tokens of a run, at least
 constexpr int kSelectBins = 256;
-// digits of a long block's keys: eleven bits, eleven, ten
-constexpr int kSelectTop = 2048, kSelectCounts = 5120;
+// digits of a long block's keys: eleven bits, eleven, ten; counts of a run by each, and of groups of 32 neighbouring ones
+constexpr int kSelectTop = 2048, kSelectGroup = 32, kSelectGroupsAt = 5120, kSelectCounts = kSelectGroupsAt + 5120 / kSelectGroup;
 
 struct SelectBlock {
   long long begin, out;  // first entry of its slots, of its results
@@ -49,7 +50,8 @@ struct SelectArgs {
   uint32_t* keys;
   uint32_t* found;   // [block][2 stages][2]: the cut's digits so far, how many of the keys with them are wanted
   uint32_t* before;  // [run][2 stages]: tokens of the runs in front of it that are above the cut in this stage's digit
-  uint32_t* counts;  // [run][kSelectCounts]: tokens by the upper digit of their keys, of those with the cut's by the middle one, then by the lower one
+  uint32_t* counts;  // [run][kSelectCounts]: tokens by the upper digit of their keys, of those with the cut's by the middle one, then by the lower one;
+                     // then the same by groups of digits
   SelectBlock blocks[kSelectBlocks];
 };
 
@@ -219,41 +221,51 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
 }
 
 // ---- long blocks ----
-// The digit of the workgroup's counts n at which the number from above reaches `wanted`, and what is then still wanted: found[0],
-// found[1].  Every thread has kEach digits side by side, from above: thread 0 the highest.
-template <int kEach>
-__device__ __forceinline__ void find_digit(const uint32_t (&n)[kEach], uint32_t wanted, uint32_t (&of_wave)[kSelectWaves], uint32_t (&found)[2]) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  uint32_t sum = 0;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) sum += n[i];
-  uint32_t upto = sum;  // of this thread's and all higher digits of the wave
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const uint32_t other = __shfl_up(upto, off, kWave);
-    if (lane >= off) upto += other;
+// Sums over the runs of kDigits neighbouring counts from `from`, those of a run kSelectCounts apart, from above: the digit at which they
+// reach `wanted`, what is then still wanted, and the counts in front of this run above that digit and at it.  All threads call it and get the same.
+struct Digit {
+  uint32_t digit, wanted, above, at;
+};
+template <int kDigits>
+__device__ __forceinline__ Digit find_digit(const uint32_t* from, int runs, int run, uint32_t wanted, uint32_t (&sums)[2][kSelectWaves][kWave], uint32_t (&found)[4]) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, digit = kDigits - 1 - threadIdx.x % kDigits;
+  uint32_t n = 0, front = 0;
+#pragma unroll 4
+  for (int r = threadIdx.x / kDigits; r < runs; r += kSelectThreads / kDigits) {
+    const uint32_t x = from[(long long)r * kSelectCounts + digit];
+    n += x, front += r < run ? x : 0u;
   }
-  if (lane == kWave - 1) of_wave[wave] = upto;
+  if constexpr (kDigits == 32) n += __shfl_xor(n, 32, kWave), front += __shfl_xor(front, 32, kWave);
+  sums[0][wave][lane] = n, sums[1][wave][lane] = front;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) upto += of_wave[w];
-  uint32_t higher = upto - sum;
+  if (wave == 0) {
+    n = front = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (higher < wanted && higher + n[i] >= wanted) found[0] = (uint32_t)(threadIdx.x * kEach + i), found[1] = wanted - higher;
-    higher += n[i];
+    for (int w = 0; w < kSelectWaves; ++w) n += sums[0][w][lane], front += sums[1][w][lane];
+    if (lane >= kDigits) n = front = 0;
+    uint32_t upto = n, fronts = front;  // with all that is above
+#pragma unroll
+    for (int off = 1; off < kDigits; off <<= 1) {
+      const uint32_t other = __shfl_up(upto, off, kWave), others = __shfl_up(fronts, off, kWave);
+      if (lane >= off) upto += other, fronts += others;
+    }
+    if (lane < kDigits && upto - n < wanted && upto >= wanted) found[0] = (uint32_t)digit, found[1] = wanted - (upto - n), found[2] = fronts - front, found[3] = front;
   }
   __syncthreads();
+  const Digit d{found[0], found[1], found[2], found[3]};
+  __syncthreads();
+  return d;
 }
 
 // Stage 0: keys, counted by their upper digit.  Stage 1 (2): the cut's upper (middle) digit, the run's keys that have it counted by
 // the next one.  Stage 3: the lower digit, and the run writes what stays.
 template <int kStage>
 __global__ __launch_bounds__(kSelectThreads) void select_run_kernel(SelectArgs a) {
-  constexpr int kDigits = kStage == 3 ? 1024 : kSelectTop, kEach = kDigits / kSelectThreads;  // of the digit that is found
-  constexpr int kNext = kStage == 2 ? 1024 : kSelectTop, kCopies = 4;                         // of the one that is counted
+  constexpr int kDigits = kStage == 3 ? 1024 : kSelectTop;  // of the digit that is found
+  constexpr int kNext = kStage == 2 ? 1024 : kSelectTop, kCopies = 4;  // of the one that is counted
   constexpr int kFrom = kStage == 1 ? 0 : kStage == 2 ? 2048 : 4096, kTo = kStage == 0 ? 0 : kStage == 1 ? 2048 : 4096;
   __shared__ uint32_t bins[kStage == 3 ? 1 : kCopies][kStage == 3 ? 1 : kNext + 8];
-  __shared__ uint32_t of_wave[kSelectWaves], found[2], total[2], per_wave[kSelectWaves][2];
+  __shared__ uint32_t sums[2][kSelectWaves][kWave], found[4], per_wave[kSelectWaves][2];
   const SelectBlock& b = a.blocks[blockIdx.y];
   const int run = (int)blockIdx.x;
   if (run >= b.runs) return;
@@ -263,42 +275,31 @@ __global__ __launch_bounds__(kSelectThreads) void select_run_kernel(SelectArgs a
     for (int i = threadIdx.x; i < kCopies * (kNext + 8); i += kSelectThreads) bins[0][i] = 0;
     __syncthreads();
   }
-  uint32_t prefix = 0, equal = 0, above = 0;
+  // this thread's keys: every kStep-th from `from`; the first ones are asked for at once
+  constexpr int kAhead = 4, kStep = kStage == 3 ? kWave : kSelectThreads;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const long long each = b.run_tokens / kSelectWaves;
+  const long long from = kStage == 3 ? min(begin + wave * each, end) : begin, to = kStage == 3 ? min(from + each, end) : end;
+  const long long t0 = from + threadIdx.x % kStep;
+  uint32_t first[kAhead];
+  if constexpr (kStage > 0)
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) first[u] = t0 + u * kStep < to ? keys[t0 + u * kStep] : 0u;
+  auto each_key = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (t0 + u * kStep < to) f(first[u]);
+#pragma unroll 4
+    for (long long t = t0 + kAhead * kStep; t < to; t += kStep) f(keys[t]);
+  };
+  uint32_t prefix = 0, equal = 0, above = 0, same = 0;
   if constexpr (kStage > 0) {
-    // counts of all runs, and of those in front of this one
-    uint32_t n[kEach], front[kEach];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) n[e] = front[e] = 0;
-    const uint32_t* from = a.counts + (long long)b.first_run * kSelectCounts + kFrom + kDigits - kEach - threadIdx.x * kEach;
-#pragma unroll 16
-    for (int r = 0; r < b.runs; ++r) {
-      uint32_t x[kEach];
-      if constexpr (kEach == 2) {
-        const uint2 two = *(const uint2*)(from + (long long)r * kSelectCounts);
-        x[0] = two.y, x[1] = two.x;  // (from above)
-      } else {
-        x[0] = from[(long long)r * kSelectCounts];
-      }
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) n[e] += x[e], front[e] += r < run ? x[e] : 0u;
-    }
     const uint32_t* last = a.found + 4 * blockIdx.y + 2 * (kStage - 2);
-    find_digit<kEach>(n, kStage == 1 ? (uint32_t)b.keep : last[1], of_wave, found);
-    const uint32_t place = found[0];  // from above
-    prefix = (kStage == 1 ? 0u : last[0]) | (uint32_t)(kDigits - 1 - place) << (kStage == 1 ? 21 : kStage == 2 ? 10 : 0);
-    equal = found[1];
-    // what is above the digit in the runs in front, and (last stage) equal to the cut
-    uint32_t mine = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) mine += (uint32_t)threadIdx.x * kEach + e < place ? front[e] : 0u;
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) mine += __shfl_xor(mine, off, kWave);
-    if (threadIdx.x % kWave == 0) per_wave[threadIdx.x / kWave][0] = mine;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if ((uint32_t)threadIdx.x * kEach + e == place) total[1] = front[e];
-    __syncthreads();
-    for (int w = 0; w < kSelectWaves; ++w) above += per_wave[w][0];
+    const uint32_t* counts = a.counts + (long long)b.first_run * kSelectCounts;
+    const Digit group = find_digit<kDigits / kSelectGroup>(counts + kSelectGroupsAt + kFrom / kSelectGroup, b.runs, run, kStage == 1 ? (uint32_t)b.keep : last[1], sums, found);
+    const Digit d = find_digit<kSelectGroup>(counts + kFrom + group.digit * kSelectGroup, b.runs, run, group.wanted, sums, found);
+    prefix = (kStage == 1 ? 0u : last[0]) | (group.digit * kSelectGroup + d.digit) << (kStage == 1 ? 21 : kStage == 2 ? 10 : 0);
+    equal = d.wanted, above = group.above + d.above, same = d.at;
     if constexpr (kStage < 3) {
       if (threadIdx.x == 0) {
         a.before[2 * (b.first_run + run) + kStage - 1] = above;
@@ -316,31 +317,28 @@ __global__ __launch_bounds__(kSelectThreads) void select_run_kernel(SelectArgs a
         count(key >> 21);
       });
     } else {
-#pragma unroll 4
-      for (long long t = begin + threadIdx.x; t < end; t += kSelectThreads) {
-        const uint32_t key = keys[t];
+      each_key([&](uint32_t key) __attribute__((always_inline)) {
         constexpr int kShift = kStage == 1 ? 21 : 10;
         if (key >> kShift == prefix >> kShift) count(kStage == 1 ? key >> 10 & 2047u : key & 1023u);
-      }
+      });
     }
     __syncthreads();
-    uint32_t* to = a.counts + (long long)(b.first_run + run) * kSelectCounts + kTo;
+    uint32_t* counts = a.counts + (long long)(b.first_run + run) * kSelectCounts;
+    uint32_t *digits = counts + kTo, *groups = counts + kSelectGroupsAt + kTo / kSelectGroup;
     for (int i = threadIdx.x; i < kNext; i += kSelectThreads) {
       uint32_t sum = 0;
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) sum += bins[c][i];
-      to[i] = sum;
+      digits[i] = sum;
+#pragma unroll
+      for (int off = 1; off < kSelectGroup; off <<= 1) sum += __shfl_xor(sum, off, kWave);
+      if (i % kSelectGroup == 0) groups[i / kSelectGroup] = sum;
     }
   } else {
     const Cut cut{prefix, equal};
-    uint32_t same = total[1];
     // this wave's part of the run, and what stays in front of it
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const long long each = b.run_tokens / kSelectWaves;
-    const long long from = min(begin + wave * each, end), to = min(from + each, end);
     uint32_t own_above = 0, own_same = 0;
-#pragma unroll 4
-    for (long long t = from + lane; t < to; t += kWave) own_above += keys[t] > cut.key, own_same += keys[t] == cut.key;
+    each_key([&](uint32_t key) __attribute__((always_inline)) { own_above += key > cut.key, own_same += key == cut.key; });
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) own_above += __shfl_xor(own_above, off, kWave), own_same += __shfl_xor(own_same, off, kWave);
     __syncthreads();
