@@ -7,12 +7,13 @@
 // is found digit by digit from histograms, most significant first, and then every token above it stays, and of those equal to
 // it the first that are wanted.  No sort, and no order of execution that the result depends on.
 //
-// Blocks of up to kSelectInLds tokens: a workgroup each, keys in LDS, one launch (64 blocks of 16384 tokens 31 us, 35 by runs; one
-// such block 28 and 23).  Longer ones: four launches of a workgroup for
-// each run of tokens.  The first makes keys and counts those of a run by their upper digit; each further one adds the counts of all
-// runs up, every workgroup for itself, finds the cut's digit, and counts the run's keys that have it by their next one, and the last
-// writes.  What lies above the cut in the runs in front falls out of the same sums.  They are taken of groups of 32 digits first,
-// then of the one group that has the cut: 29 us instead of 41 with all of them, for an eighth of 8 blocks of 60000 to 131072 tokens.
+// Blocks of up to kSelectInLds tokens: a workgroup each, keys in LDS, one launch (of 4 heads: 8192 tokens 16.7 us, 20.3 by runs, 12000
+// 21.7 and 20.7; 64 blocks of 8192 18.4 and 23.5, of 12000 24.1 and 25.3; of 16 heads 21.4 and 22.6, 28.9 and 23.1).  Longer ones: four
+// launches of a workgroup for each run of tokens.  The first makes keys and counts those of a run by their upper digit; each
+// further one adds the counts of all runs up, every workgroup for itself, finds the cut's digit, and counts the run's keys that have it
+// by their next one, and the last writes.  What lies above the cut in the runs in front falls out of the same sums.  They are
+// taken of groups of 32 digits first, then of the one group that has the cut: 29 us instead of 41 with all of them, for an eighth of 8
+// blocks of 60000 to 131072 tokens.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -24,7 +25,7 @@
 namespace va {
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
-constexpr int kSelectInLds = 16384;  // tokens of a block whose keys stay in LDS
+constexpr int kSelectInLds = 10240;  // tokens of a block whose keys stay in LDS
 constexpr int kSelectBlocks = 64;    // blocks of a launch
 constexpr int kSelectRun = 4096;     // tokens of a run, at least
 constexpr int kSelectBins = 256;

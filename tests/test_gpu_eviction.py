@@ -54,7 +54,7 @@ def check_select(dev, weights, blocks, keep, first, last):
     assert kept.positions.numel() == at
 
 
-@pytest.mark.parametrize("count", [1, 2, 63, 64, 65, 1000, 1024, 1500, 16383, 16384, 16385, 20481, 70001, 300001])
+@pytest.mark.parametrize("count", [1, 2, 63, 64, 65, 1000, 1024, 1500, 10239, 10240, 10241, 16384, 20481, 70001, 300001, 600001])
 @pytest.mark.parametrize("heads", [1, 3, 8])
 def test_one_block(dev, count, heads):
     gen = torch.Generator().manual_seed(count + heads)

@@ -77,7 +77,7 @@ def check(op, meta, gen, window=0, q=None, lse=None):
 
 
 @pytest.mark.parametrize("dtype, codes", [(BF16, None), (F16, None), (F32, None), (BF16, E4M3), (F16, INT8), (F32, E4M3)])
-@pytest.mark.parametrize("heads", [(4, 1, 128), (4, 4, 64), (32, 2, 64), (6, 2, 256), (5, 1, 32)])
+@pytest.mark.parametrize("heads", [(4, 1, 128), (4, 4, 64), (32, 2, 64), (6, 2, 256), (5, 1, 32), (6, 3, 128), (12, 12, 64)])
 def test_decode_steps(dev, dtype, codes, heads):
     r, gen = random.Random(1), torch.Generator().manual_seed(1)
     op = make_op(dev, *heads, 16, dtype, 200, codes)
