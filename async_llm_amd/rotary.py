@@ -155,11 +155,11 @@ class RotaryEmbedding:
         q2, q_row, q_heads = self._rows(q, n, "q")
         dim = self.head_dim
         if out is None:
-            out_q, out_k = torch.empty(q.shape, dtype=dtype, device=device), None
+            out_q, out_k = torch.empty_like(q, memory_format=torch.contiguous_format), None
             keys = (None, 0, 0, None, 0)
             if k is not None:
                 k2, k_row, k_heads = self._rows(k, n, "k")
-                out_k = torch.empty(k.shape, dtype=dtype, device=device)
+                out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
                 keys = (k2.data_ptr(), k_row, k_heads, out_k.data_ptr(), k_heads * dim)
             queries = (q2.data_ptr(), q_row, q_heads, out_q.data_ptr(), q_heads * dim)
         else:
