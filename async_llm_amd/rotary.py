@@ -190,15 +190,18 @@ class RotaryEmbedding:
             raise ValueError(f"{name} must be the input itself or lie apart from it")
         return y.data_ptr(), stride[0] if n > 1 else width
 
-    def cos_sin_cache(self, max_position: int) -> torch.Tensor:
+    def cos_sin_cache(self, max_position: int, unit: bool = False) -> torch.Tensor:
         """The fp32 ``[max_position, rotary_dim]`` table of cosines and sines that ``SharedCacheAttention`` takes.  Its keys and
-        queries are pairs ``(i, i + rotary_dim / 2)``: an interleaved rotation has no such table."""
+        queries are pairs ``(i, i + rotary_dim / 2)``: an interleaved rotation has no such table.  ``unit``: without
+        ``attention_factor``, for caches whose keys are turned again when blocks are merged or tokens move, which would grow by it
+        each time; queries are then to be multiplied by its square."""
         if self.interleaved:
             raise ValueError("the table's pairs are halves of a head: an interleaved rotation is applied to q and k only")
         if max_position <= 0:
             raise ValueError(f"max_position must be positive, got {max_position}")
         table = torch.empty((max_position, self.rotary_dim), dtype=torch.float32, device=self.device)
         native.require_device(table, "the table")
-        native.call_on(self.device, native.lib.va_rotary_table, self._turns, 0, max_position, table.data_ptr(),
+        turns = native.VaTurns(self.rotary_dim, 0, 1.0, self._quarters.data_ptr()) if unit else self._turns
+        native.call_on(self.device, native.lib.va_rotary_table, turns, 0, max_position, table.data_ptr(),
                        native.current_stream_ptr(self.device))
         return table

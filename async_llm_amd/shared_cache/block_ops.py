@@ -142,6 +142,8 @@ class BlockKVOps:
             self._eviction = CacheEviction(self.sc_attn)
         eviction = self._eviction
         eviction._check_weights(weights)
+        if close_gaps:
+            eviction._check_turns()
         n = min(keep, block.num_tokens)
         result = self.create_block()
         if n:

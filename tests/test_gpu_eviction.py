@@ -6,8 +6,9 @@ import pytest
 import torch
 
 from async_llm_amd import native
-from async_llm_amd.kvcache import PageAllocator
-from async_llm_amd.shared_cache import BlockKVOps, CacheEviction, WorkerGroup
+from async_llm_amd.kvcache import MHAKVCache, PageAllocator
+from async_llm_amd.rotary import RotaryEmbedding
+from async_llm_amd.shared_cache import BlockKVOps, CacheEviction, SharedCacheAttention, WorkerGroup
 from async_llm_amd.shared_cache.block_ops import token_slots
 from tests.eviction_util import blocks_of, fill, keys64, make_op, turned64, turned64_abs, weights64
 from tests.quant_util import quantised32, rows64, scales_of
@@ -353,3 +354,40 @@ def test_weights_are_forgotten(dev):
     want[:, 1:9:2] = 0.0
     e.clear(weights, torch.arange(10, dtype=torch.int32)[1:9:2])
     assert torch.equal(weights, want)
+
+
+def test_rotated_keys_move_to_where_they_would_have_been_rotated(dev):
+    """Keys turned by a stretched rotation and moved with its unit table: those of the new positions. Over its table with the
+    attention factor, by which they would grow, a turn is refused before anything is taken; a plain move is not."""
+    gen = torch.Generator().manual_seed(11)
+    yarn = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096}
+    r = RotaryEmbedding(64, 32, 1e5, scaling=yarn, device=dev)
+    pool = MHAKVCache(2, 1, 64, 40, 8, F32, dev)
+    op, scaled = (SharedCacheAttention(pool, r.cos_sin_cache(5000, unit=unit), 4, 2, 64, 8, F32, dev, rotary_dim=32) for unit in (True, False))
+    k = torch.randn(100, 2, 64, generator=gen)
+    positions, shifts = torch.randint(2000, 4000, (100,), generator=gen), torch.randint(-2000, 1000, (100,), generator=gen)
+    plain = RotaryEmbedding(64, 32, 1e5, scaling=dict(yarn, attention_factor=1.0), device=dev)
+    pool.k_cache(0).view(-1, 2, 64)[:100] = plain(positions.to(dev), k.to(dev))[0]
+    pool.v_cache(0).zero_()
+    source, target = torch.arange(100, device=dev), torch.arange(150, 250, device=dev)
+    CacheEviction(op).move(source, target, shifts.to(dev))
+    got = pool.k_cache(0).view(-1, 2, 64)[150:250].cpu().double()
+    angle = (positions + shifts).double()[:, None] * r.inv_freq.cpu()
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+    a, b = k.double()[..., :16], k.double()[..., 16:32]
+    want = torch.cat([a * c - b * s, b * c + a * s, k.double()[..., 32:]], dim=-1)
+    # a rotation is off by its cosine (four units), two products and a sum, of both elements of a pair; twice
+    size = torch.cat([a.abs() + b.abs()] * 2 + [torch.zeros(100, 2, 32)], dim=-1)
+    assert bool(((got - want).abs() <= 2 * 7 * 2.0**-24 * size).all())
+    e, allocator = CacheEviction(scaled), PageAllocator(40, 8, dev)
+    with pytest.raises(ValueError, match="unit"):
+        e.move(source, target, shifts.to(dev))
+    e.move(source, target)
+    ops = BlockKVOps(pool, scaled, allocator)
+    block = ops.create_block()
+    block.page_starts, block.num_tokens = allocator.alloc_pages(3).tolist(), 20
+    free = allocator.free_page_starts.numel()
+    with pytest.raises(ValueError, match="unit"):
+        ops.evict_tokens(block, e.new_weights(), 10, close_gaps=True)
+    assert allocator.free_page_starts.numel() == free
+    assert ops.evict_tokens(block, e.new_weights(), 10).num_tokens == 10

@@ -96,6 +96,8 @@ def test_table(dev, scaling):
     exact = torch.cat([angle.cos(), angle.sin()], dim=1) * r.attention_factor
     # a cosine is off by the angle's rounding (under a unit of pi / 4) and a unit and a half of its own, then the factor's
     assert float((table.cpu().double() - exact).abs().max()) <= 4 * 2.0**-24 * r.attention_factor
+    unit = r.cos_sin_cache(70001, unit=True)
+    assert float((unit.cpu().double() - exact / r.attention_factor).abs().max()) <= 4 * 2.0**-24
     # what takes the table turns as the rotation does
     k = torch.randn(50, 2, 64, generator=torch.Generator().manual_seed(1)).to(dev)
     small = RotaryEmbedding(64, 64, 1e6, scaling=scaling, device=dev)
