@@ -105,8 +105,8 @@ __device__ __forceinline__ void make_keys(const SelectArgs& a, const SelectBlock
 // to one bin would take a clock each.
 constexpr int kSelectCopies = 16;
 
-// The keep-th largest of `count` keys and how many of the keys equal to it are among the first `keep`; 1 <= keep <= count.
-// All threads of the workgroup call it and get the same.
+// The keep-th largest of `count` keys, or a number below it that is above all that do not stay, and how many of the keys equal to
+// it are among the first `keep`; 1 <= keep <= count.  All threads of the workgroup call it and get the same.
 struct Cut {
   uint32_t key, equal;
 };
@@ -146,13 +146,14 @@ __device__ __forceinline__ Cut find_cut(Keys key_at, long long count, long long 
       uint32_t higher = above - sum;
 #pragma unroll
       for (int i = 3; i >= 0; --i) {
-        if (higher < wanted && higher + n[i] >= wanted) found[0] = 4 * lane + i, found[1] = wanted - higher;
+        if (higher < wanted && higher + n[i] >= wanted) found[0] = 4 * lane + i, found[1] = wanted - higher, found[2] = n[i];
         higher += n[i];
       }
     }
     __syncthreads();
     prefix |= found[0] << shift;
     wanted = found[1];
+    if (found[2] == wanted) return Cut{prefix, ~0u};  // all keys with these digits stay (1500 tokens of 8 heads: 9.4 -> 8.4 us)
   }
   return Cut{prefix, wanted};
 }
