@@ -1099,7 +1099,7 @@ static int weigh(WeighArgs& a, int code_type, int num_pages, const int32_t* plan
                  const VaShape* shape, const VaRope* rope, hipStream_t stream) {
   if (!h || h[VA_WH_MAGIC] != VA_WEIGH_MAGIC) return va_fail(VA_ERR_ARG, "not a plan of attention weights");
   if (h[VA_WH_HQ] != shape->num_q_heads || h[VA_WH_HKV] != shape->num_kv_heads || h[VA_WH_D] != shape->head_dim ||
-      h[VA_WH_PAGE] != shape->page_size || h[VA_WH_DTYPE] != shape->dtype || h[VA_WH_CODES] != (code_type >= 0) || (num_pages >= 0 && h[VA_WH_POOL_PAGES] != num_pages))
+      h[VA_WH_PAGE] != shape->page_size || h[VA_WH_DTYPE] != shape->dtype || h[VA_WH_CODES] != (code_type >= 0) || h[VA_WH_POOL_PAGES] != num_pages)
     return va_fail(VA_ERR_ARG, "the plan was made for another shape or pool");
   const int n_items = h[VA_WH_N_ITEMS];
   if (n_items == 0) return VA_OK;
@@ -1164,10 +1164,10 @@ static int weigh(WeighArgs& a, int code_type, int num_pages, const int32_t* plan
 
 }  // namespace va
 
-extern "C" int va_weigh(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, int64_t pool_row_stride, const int32_t* plan_dev,
-                        const int32_t* plan_header_host, const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
-                        const float* lse_dev, int32_t lse_base2, const float* weights_in_dev, float* weights_out_dev, void* workspace_dev,
-                        int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream) {
+extern "C" int va_weigh(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, int64_t pool_row_stride, int32_t num_pages,
+                        const int32_t* plan_dev, const int32_t* plan_header_host, const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
+                        int64_t sub_loc_axis_stride, const float* lse_dev, int32_t lse_base2, const float* weights_in_dev, float* weights_out_dev,
+                        void* workspace_dev, int64_t workspace_bytes, const VaShape* shape, const VaRope* rope, void* stream) {
   if (!shape || shape->num_kv_heads <= 0 || shape->num_q_heads <= 0 || shape->num_q_heads % shape->num_kv_heads || shape->head_dim <= 0 || shape->page_size <= 0)
     return va_fail(VA_ERR_ARG, "bad shape");
   if (pool_row_stride < (int64_t)shape->num_kv_heads * shape->head_dim) return va_fail(VA_ERR_ARG, "pool rows overlap");
@@ -1175,7 +1175,7 @@ extern "C" int va_weigh(const void* q_dev, int64_t q_row_stride, const void* k_p
   a.q = q_dev, a.q_row_stride = q_row_stride, a.k_pool = k_pool_dev, a.pool_row_stride = pool_row_stride, a.sub_worker = sub_worker_dev;
   a.sub_loc = sub_loc_dev, a.sub_loc_axis_stride = sub_loc_axis_stride, a.lse = lse_dev, a.lse_base2 = lse_base2;
   a.weights_in = weights_in_dev, a.weights_out = weights_out_dev;
-  return va::weigh(a, -1, -1, plan_dev, plan_header_host, workspace_dev, workspace_bytes, shape, rope, (hipStream_t)stream);
+  return va::weigh(a, -1, num_pages, plan_dev, plan_header_host, workspace_dev, workspace_bytes, shape, rope, (hipStream_t)stream);
 }
 
 extern "C" int va_weigh_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev, const int32_t* plan_header_host,

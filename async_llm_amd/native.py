@@ -257,7 +257,7 @@ def _load() -> C.CDLL:
     lib.va_weigh_plan.argtypes = [C.POINTER(VaSubRequests), C.POINTER(VaShape), i32, i32, i32, vp, i64, C.POINTER(VaWeighCounts)]
     tables = [vp, vp, vp, vp, i64, vp, i32, vp, vp, vp, i64, C.POINTER(VaShape), C.POINTER(VaRope), vp]
     lib.va_weigh.restype = C.c_int
-    lib.va_weigh.argtypes = [vp, i64, vp, i64, *tables]
+    lib.va_weigh.argtypes = [vp, i64, vp, i64, i32, *tables]
     lib.va_weigh_q8.restype = C.c_int
     lib.va_weigh_q8.argtypes = [vp, i64, pool, *tables]
     return lib

@@ -169,7 +169,7 @@ class CacheEviction:
             native.call_on(device, native.lib.va_weigh_q8, q2.data_ptr(), q_stride, self.kv_cache.layer(layer_id), *tables)
         else:
             native.call_on(device, native.lib.va_weigh, q2.data_ptr(), q_stride, self._keys_at(layer_id),
-                           op.num_kv_heads * op.head_dim, *tables)
+                           op.num_kv_heads * op.head_dim, self.num_pages, *tables)
         return out
 
     def _keys_at(self, layer_id: int) -> int:

@@ -566,7 +566,8 @@ VA_API int va_clear_weights(float* weights_dev, int32_t num_heads, int64_t num_s
  * The plan is made on the host from the sub-request tables (kv_indices must be there;
  * chain and sub_worker are not used), for va_weigh_q8 where over_codes is not 0; window > 0
  * counts only the last `window` rows of each sub-request.  Entries outside num_pages pages
- * are refused.  As with va_plan_build a buffer that is too small gives VA_ERR_CAPACITY and
+ * are refused, and so are plans over a pool of another size (num_pages; weights have
+ * num_pages * page_size slots).  As with va_plan_build a buffer that is too small gives VA_ERR_CAPACITY and
  * the size in counts.  plan_header_host is the start of the host plan (24 words);
  * workspace_dev, on a 16-byte boundary, must hold counts.workspace_bytes.  Pools and queries
  * of any alignment, head_dim up to 256.  Aligned rows (16 bytes) of a head_dim of 64, 128 or
@@ -588,10 +589,11 @@ typedef struct VaWeighCounts {
 VA_API int va_weigh_plan(const VaSubRequests* subs, const VaShape* shape, int32_t over_codes, int32_t num_pages,
                   int32_t window, int32_t* plan_host, int64_t plan_capacity_words, VaWeighCounts* counts);
 VA_API int va_weigh(const void* q_dev, int64_t q_row_stride, const void* k_pool_dev, int64_t pool_row_stride,
-             const int32_t* plan_dev, const int32_t* plan_header_host, const int64_t* sub_worker_dev,
-             const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride, const float* lse_dev, int32_t lse_base2,
-             const float* weights_in_dev, float* weights_out_dev, void* workspace_dev, int64_t workspace_bytes,
-             const VaShape* shape, const VaRope* rope, void* stream);
+             int32_t num_pages, const int32_t* plan_dev, const int32_t* plan_header_host,
+             const int64_t* sub_worker_dev, const int64_t* sub_loc_dev, int64_t sub_loc_axis_stride,
+             const float* lse_dev, int32_t lse_base2, const float* weights_in_dev, float* weights_out_dev,
+             void* workspace_dev, int64_t workspace_bytes, const VaShape* shape, const VaRope* rope,
+             void* stream);
 VA_API int va_weigh_q8(const void* q_dev, int64_t q_row_stride, const VaQuantPool* pool, const int32_t* plan_dev,
                 const int32_t* plan_header_host, const int64_t* sub_worker_dev, const int64_t* sub_loc_dev,
                 int64_t sub_loc_axis_stride, const float* lse_dev, int32_t lse_base2,
