@@ -55,6 +55,9 @@ def slots_meet(a: np.ndarray, b: np.ndarray) -> bool:
 class BlockKVOps:
     """``merge_blocks`` / ``append_block`` over a paged pool.
 
+    The right block's keys are turned to where they now are, which a table with a factor (``RotaryEmbedding.cos_sin_cache``
+    of a rotation with an attention factor) cannot do without making them longer: refused before anything is taken.
+
     ``kv_cache`` offers ``num_layers``, ``k_cache(layer)`` and ``v_cache(layer)``
     (contiguous ``[num_pages, page_size, kv_heads, head_dim]`` tensors on the
     GPU), or is the ``QuantizedKVCache`` of a ``QuantizedCacheAttention``, whose
@@ -87,6 +90,8 @@ class BlockKVOps:
         left_tokens, right_tokens = left.num_tokens, right.num_tokens
         left_span, right_span = left.mrope_span, right.mrope_span
         total_tokens = left_tokens + right_tokens
+        if right_tokens and left_span:
+            self.sc_attn._check_turns()
 
         merged = self.create_block()
         num_pages = -(-total_tokens // self.page_size)
@@ -111,6 +116,8 @@ class BlockKVOps:
         left_tokens, right_tokens = left.num_tokens, right.num_tokens
         left_span, right_span = left.mrope_span, right.mrope_span
         if right_tokens:
+            if left_span:
+                self.sc_attn._check_turns()
             # the source layout is taken before ``left`` grows: they may be the same object
             source_slots = token_slots(right)
             new_pages = self.page_allocator.alloc_pages(left.pages_needed(right_tokens))
@@ -143,7 +150,7 @@ class BlockKVOps:
         eviction = self._eviction
         eviction._check_weights(weights)
         if close_gaps:
-            eviction._check_turns()
+            self.sc_attn._check_turns()
         n = min(keep, block.num_tokens)
         result = self.create_block()
         if n:
@@ -239,6 +246,8 @@ class BlockKVOps:
     def _launch(self, source: np.ndarray, target: np.ndarray, position_shift: int) -> None:
         att = self.sc_attn
         n = source.size
+        if position_shift:
+            att._check_turns()
         host = torch.from_numpy(np.stack([source, target]))
         if self.device.type != "cuda":
             raise native.ViewAttnError("block copies run on the GPU only (HIP kernel, no CPU path)")

@@ -78,9 +78,6 @@ class CacheEviction:
         if self.num_slots > 2**31 - 1:
             raise ValueError(f"{self.num_pages} pages of {op.page_size} tokens are more slots than 32 bits address")
         self._weights_shape = (op.num_kv_heads, self.num_slots)
-        # what the rotation's table multiplies by where nothing turns: keys that are turned again must not grow
-        table = None if op.mrope_section is not None or op.rotary_dim == 0 else op.cos_sin_cache
-        self._table_factor = 1.0 if table is None or table.numel() == 0 else float(table[0, 0])
         self._key_addresses: Dict[int, int] = {}
         self._moved: Optional[list] = None
 
@@ -242,7 +239,7 @@ class CacheEviction:
         if weights is not None:
             self._check_weights(weights)
         if shifts is not None:
-            self._check_turns()
+            op._check_turns()
         source, target = source.contiguous(), target.contiguous()
         shifts = None if shifts is None else shifts.contiguous()
         rest = (source.data_ptr(), target.data_ptr(), None if shifts is None else shifts.data_ptr(), n)
@@ -257,11 +254,6 @@ class CacheEviction:
         for run in self._layers_at():
             native.call_on(device, native.lib.va_move_kv, *run, *rest, sums, shape, rope, stream)
             sums = None  # (moved with the first run)
-
-    def _check_turns(self) -> None:
-        if abs(self._table_factor - 1.0) > 1e-6:
-            raise ValueError(f"keys cannot be turned by a table that multiplies by {self._table_factor}: take one of unit length "
-                             f"(RotaryEmbedding.cos_sin_cache(unit=True))")
 
     def _layers_at(self) -> list:
         """Where the pool's layers lie, as the library takes them; found once where the pool is this package's own."""

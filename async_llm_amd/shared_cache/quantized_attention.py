@@ -244,12 +244,14 @@ class QuantizedCacheAttention(SharedCacheAttention):
     def copy_shifted(self, source: torch.Tensor, target: torch.Tensor, position_shift: int = 0) -> None:
         """Copy the tokens of slots ``source`` to slots ``target`` (int64 on the device, each target once, none of
         them a source of another token) in every layer, keys rotated by ``position_shift`` and quantised anew; values,
-        and keys where nothing rotates, move code for code."""
+        and keys where nothing rotates, move code for code.  A table with a factor turns no stored keys: refused."""
         for name, t in (("source", source), ("target", target)):
             native.require_device(t, name)
             if t.dim() != 1 or t.dtype != torch.int64 or t.device != self.device or t.numel() != source.numel():
                 raise ValueError(f"{name} must be one row of {source.numel()} int64 slots on {self.device}, got {t.dtype} "
                                  f"{tuple(t.shape)} on {t.device}")
+        if position_shift:
+            self._check_turns()
         pool, source, target = self.kv_cache, source.contiguous(), target.contiguous()
         if pool.num_layers:
             native.call_on(self.device, native.lib.va_copy_shift_kv_q8, pool.layer(0), pool.code_layer_bytes,

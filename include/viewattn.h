@@ -278,7 +278,8 @@ VA_API int va_plan_build_fixed(const VaSubRequests* subs, const VaShape* shape, 
  * v_pool_dev (num_layers = 1 for pools that are separate allocations), slots are
  * int64 on the device and the rotation uses position_shift on all three mRoPE
  * axes.  position_shift == 0 is a plain copy (rope may be NULL).  The keys are
- * rotated as fp32 copies and rounded once, as the reference does.  Source and
+ * rotated as fp32 copies and rounded once, as the reference does; a table has to be
+ * of unit length here, or they become longer by its factor.  Source and
  * destination slots must be disjoint sets: the reference gathers everything
  * before it scatters, this kernel does not.
  * Replaces session.py:470-528 (_copy_block, _copy_slots, _shift_keys_): per
@@ -535,7 +536,8 @@ VA_API int va_select_tokens(const float* weights_dev, int32_t num_heads, int64_t
  *   k[dst[i]] = round(R(shifts[i]) float(k[src[i]])),  v[dst[i]] = v[src[i]],
  * bit for bit where shifts[i] is 0 (shifts_dev NULL: everywhere), and
  * weights[h][dst[i]] = weights[h][src[i]] where weights_dev is not NULL.  Tokens with
- * a slot outside [0, num_slots) are skipped.  Destination slots must be distinct, and
+ * a slot outside [0, num_slots) are skipped.  A table has to be of unit length, or turned
+ * keys become longer by its factor.  Destination slots must be distinct, and
  * disjoint from the source slots or equal to them row by row.
  * va_move_kv_q8: the same over a quantised pool; turned keys are quantised anew.
  */
