@@ -194,7 +194,8 @@ class RotaryEmbedding:
         """The fp32 ``[max_position, rotary_dim]`` table of cosines and sines that ``SharedCacheAttention`` takes.  Its keys and
         queries are pairs ``(i, i + rotary_dim / 2)``: an interleaved rotation has no such table.  ``unit``: without
         ``attention_factor``, for caches whose keys are turned again when blocks are merged or tokens move, which would grow by it
-        each time; queries are then to be multiplied by its square."""
+        each time.  The factor belongs to what rotates, on both sides: the first ``rotary_dim`` elements of every query head are
+        then to be multiplied by its square before attention, those that pass through are not."""
         if self.interleaved:
             raise ValueError("the table's pairs are halves of a head: an interleaved rotation is applied to q and k only")
         if max_position <= 0:
