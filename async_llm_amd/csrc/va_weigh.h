@@ -2,8 +2,9 @@
 //
 // Attention walks a query row's tokens; weights want the sum over a token's rows.  So a plan turns the sub-request tables round:
 // runs of pages that the same sub-requests read at the same places ("spans") each get the packed list of those sub-requests'
-// rows, and a work item is a chunk of a span's tokens with a range of that list.  Every token lies in one span, so its keys are
-// read once however many rows look at it, and one workgroup a kv head owns its sum.
+// rows, and a work item is a chunk of a span's tokens with a range of that list.  Every token that somebody sees lies in one
+// span, so its keys are read once however many rows look at it, and one workgroup a kv head owns its sum.  The others lie in
+// none: tokens between single slots of a page that nobody sees split its span.
 #pragma once
 #include <stdint.h>
 

@@ -139,9 +139,10 @@ struct Planner {
     return true;
   }
 
+  // Tokens of a run that somebody sees, without a gap.
   struct Span {
     int64_t page_begin;
-    int32_t first, end;  // tokens that anybody sees
+    int32_t first, end;
     int64_t row_begin, row_end;  // packed
     int pairs;  // of a tile
   };
@@ -204,6 +205,7 @@ struct Planner {
     const bool halves = !rows32 && (shape.head_dim == 64 || shape.head_dim == 128 || shape.head_dim == 256);
     const size_t n = runs.size();
     std::vector<char> many(n, 0);
+    std::vector<std::pair<int32_t, int32_t>> seen_parts;
     for (size_t i = 0; i < n && halves; ++i) {
       int64_t rows = 0;
       rows_of_run(runs[i], [&](int32_t, int32_t, int32_t) { ++rows; });
@@ -215,15 +217,29 @@ struct Planner {
         if (many[i] != which) continue;
         const int64_t row_begin = (int64_t)sub_row.size();
         int32_t first = INT32_MAX, end = 0;
+        bool places = false;  // single tokens of a page: there may be some between them that nobody sees
         rows_of_run(runs[i], [&](int32_t row, int32_t from, int32_t to) {
           sub_row.push_back(row), lo.push_back(from), hi.push_back(to);
+          places = places || from > 0;
           first = std::min(first, from), end = std::max(end, to);
         });
         if ((int64_t)sub_row.size() == row_begin) continue;
         while (sub_row.size() % unit) sub_row.push_back(-1), lo.push_back(0), hi.push_back(0);
         if ((int64_t)sub_row.size() * G > INT32_MAX / 32)  // (a thread for each 16 elements of a row)
           return va_fail(VA_ERR_ARG, "too many query rows for one plan");
-        spans.push_back(Span{(int64_t)pages.size(), first, end, row_begin, (int64_t)sub_row.size(), pairs});
+        Span span{(int64_t)pages.size(), first, end, row_begin, (int64_t)sub_row.size(), pairs};
+        if (places) {  // a span for each part
+          seen_parts.clear();
+          for (size_t r = (size_t)row_begin; r < sub_row.size(); ++r)
+            if (sub_row[r] >= 0) seen_parts.emplace_back(lo[r], hi[r]);
+          std::sort(seen_parts.begin(), seen_parts.end());
+          span.end = first;
+          for (const auto& [from, to] : seen_parts) {
+            if (from > span.end) spans.push_back(span), span.first = from;
+            span.end = std::max(span.end, to);
+          }
+        }
+        spans.push_back(span);
         const int32_t* from = runs[i].list < 0 ? run_pages.data() : lists[(size_t)runs[i].list].at;
         pages.insert(pages.end(), from + runs[i].begin, from + runs[i].end);
       }

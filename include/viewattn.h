@@ -583,7 +583,7 @@ typedef struct VaWeighCounts {
   int32_t n_items;   /* work items, padding included                                         */
   int32_t n_rows;    /* query rows, once for every span that they see                        */
   int32_t n_joins;   /* chunks of tokens whose rows are split among items                    */
-  int32_t n_spans;   /* runs of pages with the same readers                                  */
+  int32_t n_spans;   /* runs of pages with the same readers, without gaps                    */
   int32_t plan_words;
   int64_t workspace_bytes;
 } VaWeighCounts;
