@@ -124,6 +124,21 @@ __global__ __launch_bounds__(1024) void move_kernel(MoveArgs a) {
   }
 }
 
+// A thread per token and head.
+__global__ __launch_bounds__(256) void move_weights_kernel(TokenWeights weights, const int64_t* src, const int64_t* dst, long long n) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long long s = src[i], d = dst[i];
+  if (s >= 0 && s < weights.slots && d >= 0 && d < weights.slots) move_weights(weights, (int)blockIdx.y + 1, s, d, (int)blockIdx.y, 1);
+}
+
+int launch_move_weights(const TokenWeights& w, int heads, const int64_t* src, const int64_t* dst, long long n, hipStream_t stream) {
+  if (heads > 65535 || n > 0x7fffffffLL * 256) return va_fail(VA_ERR_ARG, "too many tokens or heads for one launch");
+  hipLaunchKernelGGL(move_weights_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)heads), dim3(256), 0, stream, w, src, dst, n);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? VA_OK : va_fail(VA_ERR_HIP, "moving weights: %s", hipGetErrorString(e));
+}
+
 // A thread per slot and head: weights[h][slots[i]] = 0.
 __global__ __launch_bounds__(256) void clear_weights_kernel(TokenWeights weights, const int64_t* slots, long long n) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -165,14 +180,16 @@ extern "C" int va_move_kv(void* k_pool_dev, void* v_pool_dev, int64_t pool_row_s
                           int64_t n_tokens, float* weights_dev, const VaShape* shape, const VaRope* rope, void* stream) {
   if (!shape) return va_fail(VA_ERR_ARG, "null shape");
   if (n_tokens < 0 || num_layers < 0 || num_slots < 0) return va_fail(VA_ERR_ARG, "negative count");
-  if (n_tokens == 0 || num_layers == 0 || num_slots == 0) return VA_OK;
-  if (!k_pool_dev || !v_pool_dev || !src_slots_dev || !dst_slots_dev) return va_fail(VA_ERR_ARG, "null pointer");
+  if (n_tokens == 0 || num_slots == 0 || (num_layers == 0 && !weights_dev)) return VA_OK;
+  if ((num_layers && (!k_pool_dev || !v_pool_dev)) || !src_slots_dev || !dst_slots_dev) return va_fail(VA_ERR_ARG, "null pointer");
   if (shape->num_kv_heads <= 0 || shape->head_dim <= 0) return va_fail(VA_ERR_ARG, "bad shape");
+  const va::TokenWeights weights{weights_dev, (long long)num_slots};
+  if (num_layers == 0) return va::launch_move_weights(weights, shape->num_kv_heads, src_slots_dev, dst_slots_dev, n_tokens, (hipStream_t)stream);
   if (pool_row_stride < (int64_t)shape->num_kv_heads * shape->head_dim)
     return va_fail(VA_ERR_ARG, "pool rows overlap: stride %lld < %d elements", (long long)pool_row_stride,
                    shape->num_kv_heads * shape->head_dim);
   va::MoveArgs a{k_pool_dev, v_pool_dev, pool_row_stride, layer_stride, src_slots_dev, dst_slots_dev, nullptr, n_tokens, num_slots, 1,
-                 shape->num_kv_heads, shape->head_dim, va::RopeDev{}, va::TokenWeights{weights_dev, (long long)num_slots}};
+                 shape->num_kv_heads, shape->head_dim, va::RopeDev{}, weights};
   if (shifts_dev) {
     const int rc = va::make_rope(rope, shape->head_dim, &a.rope);
     if (rc) return rc;

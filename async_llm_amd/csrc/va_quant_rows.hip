@@ -545,13 +545,15 @@ extern "C" int va_move_kv_q8(const VaQuantPool* pool, int64_t code_layer_stride,
   int rc = va::check_quant_pool(pool, shape);
   if (rc) return rc;
   if (n_tokens < 0 || num_layers < 0) return va_fail(VA_ERR_ARG, "negative count");
-  if (n_tokens == 0 || num_layers == 0) return VA_OK;
+  if (n_tokens == 0 || (num_layers == 0 && !weights_dev)) return VA_OK;
   if (!src_slots_dev || !dst_slots_dev) return va_fail(VA_ERR_ARG, "null pointer");
   if (num_layers > 1 && code_layer_stride % 16) return va_fail(VA_ERR_ARG, "code arrays must start on 16-byte boundaries");
   const uint32_t slots = (uint32_t)pool->num_pages * (uint32_t)shape->page_size;
+  const va::TokenWeights weights{weights_dev, (long long)slots};
+  if (num_layers == 0) return va::launch_move_weights(weights, shape->num_kv_heads, src_slots_dev, dst_slots_dev, n_tokens, (hipStream_t)stream);
   va::QuantCopyArgs a{{(uint8_t*)pool->k_codes_dev, (uint8_t*)pool->v_codes_dev}, {pool->k_scales_dev, pool->v_scales_dev},
                       code_layer_stride, scale_layer_stride, src_slots_dev, dst_slots_dev, n_tokens, 0, slots, shape->num_kv_heads,
-                      va::page_map(shape->page_size), va::RopeDev{}, nullptr, va::TokenWeights{weights_dev, (long long)slots}};
+                      va::page_map(shape->page_size), va::RopeDev{}, nullptr, weights};
   if (shifts_dev) {
     rc = va::make_rope(rope, shape->head_dim, &a.rope);
     if (rc) return rc;

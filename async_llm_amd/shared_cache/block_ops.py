@@ -19,7 +19,7 @@ them.
 
 from __future__ import annotations
 
-from typing import Callable, Dict, Optional, Tuple
+from typing import Callable, Dict, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -128,10 +128,11 @@ class BlockKVOps:
         return left
 
     def evict_tokens(self, block: CacheBlock, weights: torch.Tensor, keep: int, first: int = 0, last: int = 0,
-                     close_gaps: bool = False) -> CacheBlock:
+                     close_gaps: bool = False, others: Sequence[torch.Tensor] = ()) -> CacheBlock:
         """Copy what stays of ``block`` into a new compact block: ``keep`` tokens, the first ``first`` and the last ``last`` among
-        them and the others by ``weights`` (``CacheEviction``), which move along.  ``block`` stays valid and unchanged; its pages
-        are the caller's to hand back.
+        them and the others by ``weights`` (``CacheEviction``), which move along.  Tokens leave all layers together: who keeps
+        weights for each layer chooses by one of them, or by their sum, and names the ``others``, which move along too.
+        ``block`` stays valid and unchanged; its pages are the caller's to hand back.
 
         Keys keep their positions and the new block spans as many as the old one; with ``close_gaps`` they are turned to
         the positions that the tokens have in the new block, which needs a block whose positions count its tokens.  A
@@ -148,7 +149,9 @@ class BlockKVOps:
         if self._eviction is None:
             self._eviction = CacheEviction(self.sc_attn)
         eviction = self._eviction
-        eviction._check_weights(weights)
+        moving = (weights, *others)
+        for w in moving:
+            eviction._check_weights(w)
         if close_gaps:
             self.sc_attn._check_turns()
         n = min(keep, block.num_tokens)
@@ -162,9 +165,10 @@ class BlockKVOps:
             host = torch.from_numpy(np.concatenate([source, room])).pin_memory()
             dev = host.to(self.device, non_blocking=True)
             self._refs = (host, dev)
-            eviction.clear(weights, dev[source.size:])
+            for w in moving:
+                eviction.clear(w, dev[source.size:])
             kept = eviction.select(weights, dev[: source.size], [source.size], n, first, last)
-            eviction.move(kept.slots, dev[source.size: source.size + n], kept.shifts if close_gaps else None, weights)
+            eviction.move(kept.slots, dev[source.size: source.size + n], kept.shifts if close_gaps else None, moving)
             if len(block.token_ids) == block.num_tokens:
                 result.token_ids = [block.token_ids[i] for i in kept.positions.tolist()]
         span = n if close_gaps else block.mrope_span

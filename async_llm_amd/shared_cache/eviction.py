@@ -225,9 +225,10 @@ class CacheEviction:
     # moving
     # ------------------------------------------------------------------
     def move(self, source: torch.Tensor, target: torch.Tensor, shifts: Optional[torch.Tensor] = None,
-             weights: Optional[torch.Tensor] = None) -> None:
+             weights: Union[None, torch.Tensor, Sequence[torch.Tensor]] = None) -> None:
         """Copy the tokens of slots ``source`` to slots ``target`` (int64 on the device, each target once, none of them a source of
-        another token) in every layer, keys rotated by ``shifts`` (int64; ``None``: as they are), and their ``weights``."""
+        another token) in every layer, keys rotated by ``shifts`` (int64; ``None``: as they are), and their ``weights`` (a tensor, or
+        several, as one for each layer)."""
         op, device, n = self.op, self.device, source.numel()
         for name, t in (("source", source), ("target", target), ("shifts", shifts)):
             if t is None and name == "shifts":
@@ -236,24 +237,26 @@ class CacheEviction:
                 native.require_device(t, name)
                 raise ValueError(f"{name} must be one row of {n} int64 numbers on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         native.require_device(source, "source")
-        if weights is not None:
-            self._check_weights(weights)
+        weights = () if weights is None else (weights,) if isinstance(weights, torch.Tensor) else tuple(weights)
+        for w in weights:
+            self._check_weights(w)
         if shifts is not None:
             op._check_turns()
         source, target = source.contiguous(), target.contiguous()
         shifts = None if shifts is None else shifts.contiguous()
         rest = (source.data_ptr(), target.data_ptr(), None if shifts is None else shifts.data_ptr(), n)
         shape, rope, stream = op._shape, None if shifts is None else op._rope_descriptor(), native.current_stream_ptr(device)
-        sums = None if weights is None else weights.data_ptr()
+        sums = [w.data_ptr() for w in weights]
         if self._coded:
             pool = self.kv_cache
             if pool.num_layers:
                 native.call_on(device, native.lib.va_move_kv_q8, pool.layer(0), pool.code_layer_bytes, pool.scale_layer_bytes,
-                               pool.num_layers, *rest, sums, shape, rope, stream)
-            return
-        for run in self._layers_at():
-            native.call_on(device, native.lib.va_move_kv, *run, *rest, sums, shape, rope, stream)
-            sums = None  # (moved with the first run)
+                               pool.num_layers, *rest, sums.pop(0) if sums else None, shape, rope, stream)
+        else:
+            for run in self._layers_at():
+                native.call_on(device, native.lib.va_move_kv, *run, *rest, sums.pop(0) if sums else None, shape, rope, stream)
+        for w in sums:
+            native.call_on(device, native.lib.va_move_kv, None, None, 0, 0, 0, self.num_slots, *rest, w, shape, None, stream)
 
     def _layers_at(self) -> list:
         """Where the pool's layers lie, as the library takes them; found once where the pool is this package's own."""

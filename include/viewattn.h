@@ -535,7 +535,8 @@ VA_API int va_select_tokens(const float* weights_dev, int32_t num_heads, int64_t
  * token i
  *   k[dst[i]] = round(R(shifts[i]) float(k[src[i]])),  v[dst[i]] = v[src[i]],
  * bit for bit where shifts[i] is 0 (shifts_dev NULL: everywhere), and
- * weights[h][dst[i]] = weights[h][src[i]] where weights_dev is not NULL.  Tokens with
+ * weights[h][dst[i]] = weights[h][src[i]] where weights_dev is not NULL; with
+ * num_layers = 0 the weights alone (further ones of the same pool).  Tokens with
  * a slot outside [0, num_slots) are skipped.  A table has to be of unit length, or turned
  * keys become longer by its factor.  Destination slots must be distinct, and
  * disjoint from the source slots or equal to them row by row.
