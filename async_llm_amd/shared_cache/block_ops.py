@@ -62,7 +62,8 @@ class BlockKVOps:
     (contiguous ``[num_pages, page_size, kv_heads, head_dim]`` tensors on the
     GPU), or is the ``QuantizedKVCache`` of a ``QuantizedCacheAttention``, whose
     shifted keys are quantised anew; ``sc_attn`` is the ``SharedCacheAttention`` whose rotation the keys were
-    stored with; ``page_allocator`` offers ``alloc_pages(n)``.
+    stored with; ``page_allocator`` offers ``alloc_pages(n)``, and ``free_pages(page_starts)`` where pages of an eviction that
+    fails are to go back to it.
     """
 
     def __init__(self, kv_cache, sc_attn, page_allocator,
@@ -156,26 +157,38 @@ class BlockKVOps:
             self.sc_attn._check_turns()
         n = min(keep, block.num_tokens)
         result = self.create_block()
-        if n:
-            source = token_slots(block)
-            result.page_starts = self.page_allocator.alloc_pages(-(-n // self.page_size)).tolist()
-            result.num_tokens = result.num_pages * self.page_size
-            room = token_slots(result)  # whole pages
-            result.num_tokens = n
-            host = torch.from_numpy(np.concatenate([source, room])).pin_memory()
-            dev = host.to(self.device, non_blocking=True)
-            self._refs = (host, dev)
-            for w in moving:
-                eviction.clear(w, dev[source.size:])
-            kept = eviction.select(weights, dev[: source.size], [source.size], n, first, last)
-            eviction.move(kept.slots, dev[source.size: source.size + n], kept.shifts if close_gaps else None, moving)
-            if len(block.token_ids) == block.num_tokens:
-                result.token_ids = [block.token_ids[i] for i in kept.positions.tolist()]
         span = n if close_gaps else block.mrope_span
         result.mrope_span_override = None if span == n else span
         result._replace_linear_states({i: (a.clone(), b.clone()) for i, (a, b) in block.linear_affine.items()},
                                       {i: s.clone() for i, s in block.linear_conv_state.items()})
+        if n:
+            pages = self.page_allocator.alloc_pages(-(-n // self.page_size))
+            try:
+                result.page_starts = pages.tolist()
+                self._fill_evicted(result, block, moving, n, first, last, close_gaps)
+            except BaseException:
+                # nobody else knows of these pages
+                hand_back = getattr(self.page_allocator, "free_pages", None)
+                if hand_back is not None:
+                    hand_back(pages)
+                raise
         return result
+
+    def _fill_evicted(self, result: CacheBlock, block: CacheBlock, weights: Sequence[torch.Tensor], n: int, first: int, last: int,
+                      close_gaps: bool) -> None:
+        eviction, source = self._eviction, token_slots(block)
+        result.num_tokens = result.num_pages * self.page_size
+        room = token_slots(result)  # whole pages
+        result.num_tokens = n
+        host = torch.from_numpy(np.concatenate([source, room])).pin_memory()
+        dev = host.to(self.device, non_blocking=True)
+        self._refs = (host, dev)
+        for w in weights:
+            eviction.clear(w, dev[source.size:])
+        kept = eviction.select(weights[0], dev[: source.size], [source.size], n, first, last)
+        eviction.move(kept.slots, dev[source.size: source.size + n], kept.shifts if close_gaps else None, weights)
+        if len(block.token_ids) == block.num_tokens:
+            result.token_ids = [block.token_ids[i] for i in kept.positions.tolist()]
 
     # ------------------------------------------------------------------
     def _finish_block_merge(self, *, destination: CacheBlock, left: CacheBlock, right: CacheBlock, left_span: int,
