@@ -139,7 +139,8 @@ __device__ __forceinline__ int row_exponent(float most) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// The row's other half: a row that is padding, or whose log-sum is -inf, adds exp2(-inf) = 0 to every token.
+// The row's other half: a row that is padding, or whose log-sum is -inf, adds exp2(-inf) = 0 to every token.  The log-sum in powers of
+// two is a 32-bit product, off by up to 1.3 * 2^-24 of it: an error that all of a row's weights share.
 __device__ __forceinline__ WeighRow row_beside(const WeighArgs& a, int row, bool counts, float lse, float scale) {
   if (!counts) return WeighRow{-INFINITY, 0.f, 0, 0x7fffffff};
   return WeighRow{a.lse_base2 ? -lse : -lse * kLog2e, scale, a.lo[row], a.hi[row]};
@@ -687,9 +688,9 @@ __device__ __forceinline__ void finish_sums(const WeighArgs& a, int page_begin, 
 }
 
 // What the keys of a pool are in the products of the tiles: float16 numbers, times 2^x for a token.  16-bit keys come within
-// float16's range by a power of two: with their row's largest element at 2^14 .. 2^15 what is over 2^-32 of it stays exact, and an error
-// of 2^-40 of it is the most.  Codes are float16 numbers as they are.  Two parts of a query instead of bf16's three: a third of
-// the products less.
+// float16's range by a power of two: with their row's largest element at 2^14 .. 2^15 what is over 2^-31 of it stays exact, and an error
+// of 2^-39 of it is the most.  Where one power serves 32 tokens a row may lie 2^8 lower: 2^-23 and 2^-31 of its largest.  Codes are float16
+// numbers as they are and stay exact either way.  Two parts of a query instead of bf16's three: a third of the products less.
 //   raw: 16 bytes of a row for every two operand pieces (codes) or one.  power: the token's x from those.  half: a piece of 8
 //   dims as float16, times 2^(power - x).
 template <typename C>
@@ -821,7 +822,9 @@ __device__ __forceinline__ void weigh_tiles(const WeighArgs& a, unsigned block) 
     for (int b = 0; b < kBlocks; ++b) {
       factor[b] = 1.f;
       if constexpr (K::kPowers) {
-        bool counts = power[b] < 128;  // (a row of 0, or one that is not finite, goes along with the others)
+        // A 16-bit row of 0, and one that is not finite, goes along with the others.  (Over codes a row of 0 has the least scale there
+        // is, which counts: beside rows of another size its wave takes the branch with a power for each token.)
+        bool counts = power[b] < 128;
         if constexpr (!K::kCodes) {
           uint32_t top = 0;  // magnitudes as whole numbers, which order them
 #pragma unroll

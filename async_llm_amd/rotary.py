@@ -13,9 +13,9 @@ longer than a model was trained on.
     yarn     f_i where a pair makes beta_fast turns and more within the original length, f_i / factor where it
              makes beta_slow and fewer, a ramp over the pairs in between; cosines and sines times a factor
 
-Frequencies, and products of position and frequency, are 64-bit numbers: far positions are as exact
-as near ones, and none is past the end of a table.  (A table of 32-bit products is off by up to
-position * 2^-24 in each angle.)
+Frequencies, and products of position and frequency, are 64-bit numbers: positions up to about 2^27 are
+as exact as near ones (farther angles lose 2^-52 of themselves), and none is past the end of a table.
+(A table of 32-bit products is off by up to position * 2^-24 in each angle.)
 """
 
 from __future__ import annotations

@@ -478,8 +478,9 @@ VA_API int va_attention_read_back_q8(const void* q_dev, int64_t q_row_stride, co
  * Positions: queries and keys rotated as a step makes them, for layers that call an
  * attention without a view (reference layers/rotary.py:24-51), and the cos|sin
  * table that VaRope takes.  The angle of pair i at position p is
- * p * quarters[i] * pi / 2, the product taken in 64 bits, so that far positions
- * lose nothing; cosines and sines are 32-bit numbers, times `factor`.
+ * p * quarters[i] * pi / 2, the product taken in 64 bits: angles up to about 2^27 are
+ * as good as small ones (2^-52 of an angle is lost); cosines and sines are 32-bit
+ * numbers, times `factor`.
  * ------------------------------------------------------------------------- */
 typedef struct VaTurns {
   int32_t rotary_dim;         /* leading head dims that rotate, even                           */
@@ -574,11 +575,11 @@ VA_API int va_clear_weights(float* weights_dev, int32_t num_heads, int64_t num_s
  * the size in counts.  plan_header_host is the start of the host plan (24 words);
  * workspace_dev, on a 16-byte boundary, must hold counts.workspace_bytes.  Pools and queries
  * of any alignment, head_dim up to 256.  Aligned rows (16 bytes) of a head_dim of 64, 128 or
- * 256 run on the matrix cores, others on the vector ALU.  There 16-bit keys and codes meet
- * queries as sums of three 16-bit numbers (an error of 2^-24 of the row's largest element), or of two
- * (2^-22: VA_F16 pools, and tokens that more than 16 (row, q head) pairs read); 32-bit
- * keys meet 32-bit queries.  A key that is not finite makes sums of its own token only
- * infinite or NaN.
+ * 256 run on the matrix cores, others on the vector ALU.  There VA_BF16 keys meet queries
+ * as sums of three 16-bit numbers (an error of 2^-24 of the row's largest element), VA_F16
+ * keys, codes, and keys of tokens that more than 16 (row, q head) pairs read meet sums of two
+ * (2^-22); 32-bit keys meet 32-bit queries.  The log-sum times log2(e) is rounded to 32 bits
+ * once for a row.  A key that is not finite makes sums of its own token only infinite or NaN.
  */
 typedef struct VaWeighCounts {
   int32_t n_items;   /* work items, padding included                                         */
