@@ -32,11 +32,11 @@ def test_merged_keys_are_those_of_their_new_positions(append):
     at, slots = torch.arange(50, device=dev), torch.from_numpy(token_slots(right)).to(dev)
     for layer in range(2):
         pool.k_cache(layer).view(-1, 2, 64)[slots] = plain(at, k[layer].to(dev))[0]
-    before, free = pool.k_cache(0).clone(), allocator.num_free_pages
+    before, free = pool.k_cache(0).view(torch.int32).clone(), allocator.num_free_pages  # (bits: nobody has written the other slots)
     for call in (refused.merge_blocks, refused.append_block):
         with pytest.raises(ValueError, match="unit"):
             call(left, right)
-    assert allocator.num_free_pages == free and torch.equal(pool.k_cache(0), before) and left.num_tokens == 61
+    assert allocator.num_free_pages == free and torch.equal(pool.k_cache(0).view(torch.int32), before) and left.num_tokens == 61
     result = (ops.append_block if append else ops.merge_blocks)(left, right)
     slots = torch.from_numpy(token_slots(result))[61:]
     angle = (2000 + torch.arange(50)).double()[:, None] * r.inv_freq.cpu()
