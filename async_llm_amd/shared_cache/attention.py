@@ -188,7 +188,9 @@ class SharedCacheAttention:
             assert rope_base is not None, "mrope_section needs rope_base"
             exponent = torch.arange(0, self.rotary_dim, 2, dtype=torch.float32, device=self.device) / self.rotary_dim
             self._mrope_inv_freq = (1.0 / (rope_base ** exponent)).contiguous()
-        self._table_factor = self._factor_of_table()  # (here: a first turn may be one that is recorded)
+        # (read here: a first turn may be one that is recorded, where nothing can be read)
+        recording = cos_sin_cache is not None and cos_sin_cache.is_cuda and torch.cuda.is_current_stream_capturing()
+        self._table_factor = None if recording else self._factor_of_table()
         kernel = kernel or os.environ.get("VIEWATTN_KERNEL", "auto")
         if kernel not in _KERNELS:
             raise ValueError(f"kernel must be one of {sorted(_KERNELS)}, got {kernel!r}")
@@ -258,11 +260,14 @@ class SharedCacheAttention:
         table = None if self.mrope_section is not None or self.rotary_dim == 0 else self.cos_sin_cache
         return 1.0 if table is None or table.numel() == 0 else float(table[0, 0])
 
+    def _turns_by_one(self) -> bool:
+        return self._table_factor is not None and abs(self._table_factor - 1.0) <= 1e-6
+
     def _check_turns(self) -> None:
         """Refuse to turn stored keys by a table with a factor (an attention factor, as yarn's): they would grow by it."""
-        if abs(self._table_factor - 1.0) > 1e-6:
+        if not self._turns_by_one():
             self._table_factor = self._factor_of_table()  # (it may have been filled since)
-        if abs(self._table_factor - 1.0) > 1e-6:
+        if not self._turns_by_one():
             raise ValueError(f"keys cannot be turned by a table that multiplies by {self._table_factor}: take one of unit length "
                              f"(RotaryEmbedding.cos_sin_cache(unit=True))")
 

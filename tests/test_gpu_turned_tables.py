@@ -9,6 +9,7 @@ from async_llm_amd.kvcache import MHAKVCache, PageAllocator
 from async_llm_amd.rotary import RotaryEmbedding
 from async_llm_amd.shared_cache import BlockKVOps, SharedCacheAttention, WorkerGroup
 from async_llm_amd.shared_cache.block_ops import token_slots
+from tests.eviction_util import fill, make_op
 
 pytestmark = pytest.mark.gpu
 YARN = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096}
@@ -101,3 +102,33 @@ def test_attention_over_a_unit_table_is_that_of_the_factor():
     # (what the bound is there to tell apart: the factor on all of a query)
     whole = torch.softmax(torch.einsum("hgd,nhd->hgn", torch.cat([x[..., :32], x[..., 32:] * r.attention_factor**2], -1), y) / D**0.5, -1)
     assert bool(((torch.einsum("hgn,nhd->hgd", whole, v.double()) - want).abs().amax(-1) > 4 * room.amax(-1)).all())
+
+
+def test_ops_and_turns_while_a_graph_is_recorded():
+    """A turn may be recorded first of all; an op that is made while recording looks at its table later."""
+    dev, gen = torch.device("cuda:0"), torch.Generator().manual_seed(14)
+    r = RotaryEmbedding(64, scaling=YARN, device=dev)
+    unit, scaled = r.cos_sin_cache(100, unit=True), r.cos_sin_cache(100)
+    op = make_op(dev, 4, 2, 64, 16, torch.bfloat16, 10, torch.int8)
+    fill(op, gen)
+    source, target = torch.arange(20, 50, device=dev), torch.arange(100, 130, device=dev)
+    graph, made, x = torch.cuda.CUDAGraph(), [], torch.zeros(4, device=dev)
+    torch.cuda.synchronize(dev)
+    with torch.cuda.graph(graph):
+        x += 1
+        op.copy_shifted(source, target, 7)
+        for table in (unit, scaled):
+            made.append(SharedCacheAttention(MHAKVCache(2, 1, 64, 4, 16, torch.bfloat16, dev), table, 4, 2, 64, 16, torch.bfloat16, dev))
+    made[0]._check_turns()
+    with pytest.raises(ValueError, match="unit"):
+        made[1]._check_turns()
+    codes = op.kv_cache.k_codes(0).view(torch.uint8)
+    for _ in range(3):
+        codes[6:].zero_()
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        got = codes.clone()
+        codes[6:].zero_()
+        op.copy_shifted(source, target, 7)
+        assert torch.equal(got, codes) and bool(codes[7].any())
+    assert float(x[0]) == 3.0

@@ -42,7 +42,7 @@ def two_blocks(ops, left, right):
 
 
 @pytest.mark.parametrize("codes", [None, torch.int8])
-@pytest.mark.parametrize("factor", [1.1386, 0.9, 0.0])
+@pytest.mark.parametrize("factor", [1.1386, 0.9, 0.0, float("nan")])
 def test_merges_and_appends_are_refused_before_anything_is_taken(factor, codes):
     op = made(factor, codes)
     ops = BlockKVOps(op.kv_cache, op, Pages())
